@@ -289,6 +289,62 @@ typedef struct pope_pad {
 int pope_pad_rows(const pope_pad* tensors, int n, void* stream);
 
 /*
+ * Paged cache of expanded key rows and values, and attention over it.  No counterpart in the reference
+ * (its cache is the caller's contiguous k / v).
+ *
+ * The cache holds, per slot and kv head, K_hat = [softplus(k) cos t | softplus(k) sin t | k_rest] with
+ * t = freqs + bias (D + R values, rounded once) and the value row: 16-bit elements of `dtype`, or, with
+ * `quantized`, e4m3 codes times 2^e with one e per row (the smallest with max |x| <= 448 2^e; the byte
+ * holds e + 127; a value that is not finite is stored as NaN).  Slots lie in pages of `page_size`; sequence
+ * b's position n is slot n % page_size of page page_table[b, n / page_size].  The bytes of a page are in the
+ * kernels' operand order (csrc/paged_index.hpp); pope_paged_read is the way to plain rows.
+ *
+ * New rows: a padded batch, B sequences of N rows, or packed (cu_seqlens given): N rows in one batch entry,
+ * sequence b owning rows cu_seqlens[b] <= r < cu_seqlens[b + 1].  Row i of a sequence's n stands at position
+ * lengths[b] - n + i: `lengths` counts the cached rows with the new ones.  Rows at negative positions, packed
+ * rows outside every sequence and rows on page numbers outside [0, pages) have no slot: a write skips them, a
+ * read gives zeros, and keys on such pages are not seen.  lengths beyond the page table's row are cut to it.
+ * cu_seqlens that decrease, and two rows of one call in the same slot, leave unspecified values (never an access
+ * out of bounds).
+ */
+typedef struct pope_paged {
+  int32_t pages, page_size;  /* page_size: a power of two, 32 .. 1024 */
+  int32_t Hk, D, R;          /* kv heads; 1 <= D <= 256, 0 <= R <= D, any values */
+  int32_t dtype;             /* enum pope_dtype of q, k, v, o: POPE_F16 or POPE_BF16 */
+  int32_t quantized;         /* 8-bit pages */
+  int32_t B, N, table_cols;  /* sequences; rows (above); columns of page_table */
+  int32_t Hq, causal;        /* attention: query heads (head h reads kv head h % Hk); a row sees positions <= its own */
+  float softmax_scale;
+  int64_t table_sb;          /* row stride of page_table */
+  int64_t q_s[3], k_s[3], v_s[3], o_s[3]; /* (b, h, n) element strides, unit feature stride, any alignment */
+  int64_t f_s[2], bias_sh;   /* freqs (b, n): a row of angles per new row; bias (1 or Hk, R) */
+} pope_paged;
+
+/* Bytes of the cache's three arrays: key pages, value pages, exponents (0 unless quantized).  The caller owns them,
+ * 16-byte aligned, zeroed once before the first use. */
+int pope_paged_cache_bytes(const pope_paged* desc, size_t bytes[3]);
+
+/* k, v (dtype, k_s / v_s) into their slots. */
+int pope_paged_write(const pope_paged* desc, const void* k, const void* v, const float* freqs, const float* bias,
+                     void* k_pages, void* v_pages, uint8_t* scales, const int32_t* page_table,
+                     const int32_t* lengths, const int32_t* cu_seqlens, void* stream);
+
+/* Rows out of their slots: k_hat (dtype, D + R columns, (cos, sin) pairs interleaved as pope_polar_fwd writes
+ * them, k_s) and v (D columns, v_s).  Every row of the call is written. */
+int pope_paged_read(const pope_paged* desc, const void* k_pages, const void* v_pages, const uint8_t* scales,
+                    const int32_t* page_table, const int32_t* lengths, const int32_t* cu_seqlens, void* k_hat,
+                    void* v, void* stream);
+
+/* Attention of the new rows' queries over their sequences' slots.  o (dtype, o_s); lse NULL or fp32 (batch, Hq, N)
+ * contiguous, natural log; rows that see no key give 0 and -inf.  Every row is written.  Workspace:
+ * pope_paged_workspace_bytes, 256-byte aligned (0: none), free again once the call's work is done. */
+int pope_paged_workspace_bytes(const pope_paged* desc, int packed, size_t* bytes);
+int pope_paged_attn(const pope_paged* desc, const void* q, const float* freqs, const void* k_pages,
+                    const void* v_pages, const uint8_t* scales, const int32_t* page_table,
+                    const int32_t* lengths, const int32_t* cu_seqlens, void* o, float* lse, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
+/*
  * Per-kernel timing.  No counterpart in the reference (its tests print only
  * parity diffs, tests/test_flash_attn.py:61,109).  While enabled, every kernel
  * launch of the library carries a pair of hipEvents that its dispatch stamps with

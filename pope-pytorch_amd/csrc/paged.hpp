@@ -1,0 +1,56 @@
+// Parameter blocks and launchers of the paged cache's kernels, shared with the C ABI.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "paged_index.hpp"
+#include "pope_kernels.hpp"
+
+namespace pope {
+
+// The cache and the call's view of it.
+struct PagedCache {
+  void* k; void* v; uint8_t* scales;   // pages; scales: 8-bit caches only
+  const int* table; int64_t table_sb;  // (B, columns) page numbers
+  PagedSeqs seqs;
+  int pages, blk_shift;                // blocks per page: 1 << blk_shift
+  int Hk, D, R, steps, tiles;          // tiles: V tiles of 16 columns (PagedSeqs knows the rows)
+  int64_t k_head, v_head;              // elements of one (page, head)
+};
+
+struct PagedRowsParams {               // write: k, v -> cache; read: cache -> k, v
+  PagedCache c;
+  void* k; void* v;                    // rows (b, h, n); read: k rows of D + R columns
+  const float* freqs; const float* bias;
+  int64_t k_s[3], v_s[3], f_s[2], bias_sh;
+  int k_vec, v_vec;                    // rows of whole 16-byte units
+  int64_t blocks;                      // grid.x: blocks of 32 slots over all sequences
+};
+hipError_t launch_paged_write(const PagedRowsParams& p, int dtype, bool q8, hipStream_t s);
+hipError_t launch_paged_read(const PagedRowsParams& p, int dtype, bool q8, hipStream_t s);
+
+struct PagedAttnParams {
+  PagedCache c;
+  const uint16_t* q; const float* freqs;
+  uint16_t* o; float* lse;             // lse may be null: (batch, Hq, rows) natural log
+  int Hq, G, causal, N;                // G = Hq / Hk; N: rows per batch entry (all of them when packed)
+  int splits, least;                   // splits of the key axis, the least blocks of one
+  int64_t tiles;                       // row tiles
+  float scale_log2, sign;              // |softmax scale| log2 e and its sign (0: scores are all 0)
+  int64_t q_s[3], o_s[3], f_s[2];
+  int o_vec;                           // output rows of whole 8-byte units
+  float* part_o; float* part_ml;       // splits > 1: (tile, head, split, row): 16 * tiles floats, and (m, l)
+};
+// Rows of a tile for a call with `rows` (query head of a key head, new token) rows per sequence on average.
+struct PagedPlan { int nq, wk; };      // column tiles of 16 rows per wave, waves that share a tile's rows
+PagedPlan paged_plan(int64_t rows, int tiles);
+inline int paged_tile_rows(PagedPlan p) { return 16 * p.nq * (4 / p.wk); }
+hipError_t launch_paged_attn(const PagedAttnParams& p, PagedPlan plan, int dtype, bool q8, hipStream_t s);
+
+// One translation unit each (paged_attn_*.hip).
+hipError_t launch_paged_attn_bf16(const PagedAttnParams& p, PagedPlan plan, hipStream_t s);
+hipError_t launch_paged_attn_f16(const PagedAttnParams& p, PagedPlan plan, hipStream_t s);
+hipError_t launch_paged_attn_bf16_8(const PagedAttnParams& p, PagedPlan plan, hipStream_t s);
+hipError_t launch_paged_attn_f16_8(const PagedAttnParams& p, PagedPlan plan, hipStream_t s);
+
+}  // namespace pope

@@ -1,0 +1,10 @@
+// Instances of the paged attention: 8-bit pages, fp16 queries.
+#include "paged_attn.hpp"
+
+namespace pope {
+
+hipError_t launch_paged_attn_f16_8(const PagedAttnParams& p, PagedPlan plan, hipStream_t s) {
+  return run_paged_shape<F16, true>(p, plan, s);
+}
+
+}  // namespace pope

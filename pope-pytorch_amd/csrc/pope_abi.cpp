@@ -10,6 +10,7 @@
 #include <cstring>
 #include <string>
 
+#include "paged.hpp"
 #include "pope_kernels.hpp"
 
 namespace {
@@ -1018,6 +1019,196 @@ int pope_polar_bwd(const pope_desc* d, const float* dq_hat, const float* dk_hat,
   if (e != hipSuccess) return hip_fail(e, "polar transform backward launch");
   e = det_reduce(*d, dp, dfreqs, dbias, false, s);
   if (e != hipSuccess) return hip_fail(e, "phase gradient reduction launch");
+  return POPE_OK;
+}
+
+}  // extern "C"
+
+namespace {
+
+// ---------------------------------------------------------------- paged cache
+
+int check_paged(const pope_paged* d) {
+  if (!d) return fail(POPE_ERR_INVALID, "descriptor is NULL");
+  if (d->pages < 1 || d->Hk < 1) return fail(POPE_ERR_INVALID, "pages, Hk must be >= 1 (got %d, %d)", d->pages, d->Hk);
+  if (d->page_size < 32 || d->page_size > 1024 || (d->page_size & (d->page_size - 1)))
+    return fail(POPE_ERR_INVALID, "page size %d must be a power of two in [32, 1024]", d->page_size);
+  if (d->D < 1 || d->D > 256) return fail(POPE_ERR_UNSUPPORTED, "paged cache covers head dims 1 to 256 (got %d)", d->D);
+  if (d->R < 0 || d->R > d->D) return fail(POPE_ERR_INVALID, "rotate dim %d must be in [0, head dim %d]", d->R, d->D);
+  if (d->dtype != POPE_F16 && d->dtype != POPE_BF16) return fail(POPE_ERR_INVALID, "paged cache takes fp16 or bf16 (dtype %d)", d->dtype);
+  return POPE_OK;
+}
+
+int check_strides(const char* name, const int64_t* s, int n) {
+  for (int i = 0; i < n; ++i)
+    if (s[i] < 0) return fail(POPE_ERR_INVALID, "%s stride[%d] = %lld is negative", name, i, (long long)s[i]);
+  return POPE_OK;
+}
+
+int check_paged_call(const pope_paged* d) {
+  const int rc = check_paged(d);
+  if (rc) return rc;
+  if (d->B < 1 || d->N < 0 || d->table_cols < 1)
+    return fail(POPE_ERR_INVALID, "B, table_cols must be >= 1 and N >= 0 (got %d, %d, %d)", d->B, d->table_cols, d->N);
+  // positions, with a block of 32 to spare on either side, are 32-bit numbers
+  if ((int64_t)d->table_cols * d->page_size > ((int64_t)1 << 31) - 4096 || d->N > (1 << 30))
+    return fail(POPE_ERR_UNSUPPORTED, "%d pages of %d slots in a page table row, %d rows: beyond 32-bit positions", d->table_cols,
+                d->page_size, d->N);
+  if (d->table_sb < 0 || d->bias_sh < 0) return fail(POPE_ERR_INVALID, "negative page table / bias stride");
+  return check_strides("freqs", d->f_s, 2);
+}
+
+int check_pages(const pope_paged* d, const void* k, const void* v, const void* scales, const int32_t* table, const int32_t* lengths) {
+  if (!k || !v || (d->quantized && !scales) || !table || !lengths)
+    return fail(POPE_ERR_INVALID, "k_pages, v_pages, page_table, lengths%s must be non-NULL", d->quantized ? ", scales" : "");
+  if (!aligned16(k) || !aligned16(v) || (d->quantized && !aligned16(scales))) return fail(POPE_ERR_INVALID, "pages must be 16-byte aligned");
+  return POPE_OK;
+}
+
+pope::PagedCache paged_cache(const pope_paged& d, const void* k, const void* v, const void* scales, const int32_t* table,
+                             const int32_t* lengths, const int32_t* cu) {
+  pope::PagedCache c;
+  std::memset(&c, 0, sizeof c);
+  c.k = const_cast<void*>(k);
+  c.v = const_cast<void*>(v);
+  c.scales = static_cast<uint8_t*>(const_cast<void*>(scales));
+  c.table = table;
+  c.table_sb = d.table_sb;
+  c.seqs = pope::PagedSeqs{lengths, cu, d.B, d.N, d.table_cols * d.page_size};
+  c.pages = d.pages;
+  while ((pope::kBlockKeys << c.blk_shift) < d.page_size) ++c.blk_shift;
+  c.Hk = d.Hk; c.D = d.D; c.R = d.R;
+  c.steps = pope::paged_k_steps(d.D, d.R);
+  c.tiles = pope::paged_v_tiles(d.D);
+  c.k_head = (int64_t)d.page_size * c.steps * 32;
+  c.v_head = (int64_t)d.page_size * c.tiles * 16;
+  return c;
+}
+
+// Split of the key axis: as many parts as bring the grid to kPagedGrid workgroups, of at least kPagedLeast blocks.
+constexpr int kPagedGrid = 1024, kPagedLeast = 16;
+
+struct PagedShape {
+  pope::PagedPlan plan;
+  int64_t tiles;
+  int splits;
+  size_t part_o, bytes;
+};
+
+PagedShape paged_shape(const pope_paged& d, bool packed) {
+  PagedShape s;
+  const int G = d.Hq / d.Hk, vt = pope::paged_v_tiles(d.D);
+  const int64_t avg = packed ? ((int64_t)d.N + d.B - 1) / d.B : d.N;
+  s.plan = pope::paged_plan(avg * G, vt);
+  const int rows = pope::paged_tile_rows(s.plan);
+  s.tiles = pope::paged_tiles(d.B, d.N, packed, G, rows, 1);
+  const int64_t wgs = std::max<int64_t>(s.tiles * d.Hk, 1);
+  const int64_t blocks = (int64_t)d.table_cols * d.page_size / pope::kBlockKeys;
+  s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kPagedGrid / wgs, blocks / kPagedLeast));
+  s.part_o = s.bytes = 0;
+  if (s.splits > 1) {
+    const size_t n = (size_t)wgs * s.splits * rows;
+    s.part_o = align_up(n * vt * 16 * sizeof(float));
+    s.bytes = s.part_o + align_up(n * 2 * sizeof(float));
+  }
+  return s;
+}
+
+int check_paged_heads(const pope_paged* d) {
+  if (d->Hq < 1 || d->Hq % d->Hk != 0) return fail(POPE_ERR_INVALID, "query heads %d must be a multiple of kv heads %d", d->Hq, d->Hk);
+  return POPE_OK;
+}
+
+int paged_rows(const pope_paged* d, void* k, void* v, const float* freqs, const float* bias, const void* k_pages, const void* v_pages,
+               const uint8_t* scales, const int32_t* table, const int32_t* lengths, const int32_t* cu, bool write, void* stream) {
+  int rc = check_paged_call(d);
+  if (rc) return rc;
+  if ((rc = check_strides("k", d->k_s, 3)) || (rc = check_strides("v", d->v_s, 3))) return rc;
+  if (d->N == 0) return POPE_OK;
+  if ((rc = check_pages(d, k_pages, v_pages, scales, table, lengths))) return rc;
+  if (!k || !v) return fail(POPE_ERR_INVALID, "k, v must be non-NULL");
+  if (write && d->R > 0 && (!freqs || !bias)) return fail(POPE_ERR_INVALID, "rotate dim %d > 0 needs freqs and bias", d->R);
+  pope::PagedRowsParams p;
+  std::memset(&p, 0, sizeof p);
+  p.c = paged_cache(*d, k_pages, v_pages, scales, table, lengths, cu);
+  p.k = k; p.v = v; p.freqs = freqs; p.bias = bias;
+  copy3(p.k_s, d->k_s); copy3(p.v_s, d->v_s);
+  p.f_s[0] = d->f_s[0]; p.f_s[1] = d->f_s[1];
+  p.bias_sh = d->bias_sh;
+  p.blocks = pope::paged_tiles(d->B, d->N, cu != nullptr, 1, pope::kBlockKeys, 2);
+  if (p.blocks >= ((int64_t)1 << 31) || d->Hk > 65535) return fail(POPE_ERR_UNSUPPORTED, "%lld blocks of rows x %d heads: too many workgroups", (long long)p.blocks, d->Hk);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const hipError_t e = write ? pope::launch_paged_write(p, d->dtype, d->quantized != 0, s) : pope::launch_paged_read(p, d->dtype, d->quantized != 0, s);
+  if (e != hipSuccess) return hip_fail(e, write ? "paged write launch" : "paged read launch");
+  return POPE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int pope_paged_cache_bytes(const pope_paged* d, size_t bytes[3]) {
+  const int rc = check_paged(d);
+  if (rc) return rc;
+  if (!bytes) return fail(POPE_ERR_INVALID, "bytes is NULL");
+  const size_t slots = (size_t)d->pages * d->Hk * d->page_size, e = d->quantized ? 1 : 2;
+  bytes[0] = slots * pope::paged_k_steps(d->D, d->R) * 32 * e;
+  bytes[1] = slots * pope::paged_v_tiles(d->D) * 16 * e;
+  bytes[2] = d->quantized ? slots * 2 : 0;
+  return POPE_OK;
+}
+
+int pope_paged_write(const pope_paged* d, const void* k, const void* v, const float* freqs, const float* bias, void* k_pages,
+                     void* v_pages, uint8_t* scales, const int32_t* table, const int32_t* lengths, const int32_t* cu, void* stream) {
+  return paged_rows(d, const_cast<void*>(k), const_cast<void*>(v), freqs, bias, k_pages, v_pages, scales, table, lengths, cu, true, stream);
+}
+
+int pope_paged_read(const pope_paged* d, const void* k_pages, const void* v_pages, const uint8_t* scales, const int32_t* table,
+                    const int32_t* lengths, const int32_t* cu, void* k_hat, void* v, void* stream) {
+  return paged_rows(d, k_hat, v, nullptr, nullptr, k_pages, v_pages, scales, table, lengths, cu, false, stream);
+}
+
+int pope_paged_workspace_bytes(const pope_paged* d, int packed, size_t* bytes) {
+  int rc = check_paged_call(d);
+  if (rc || (rc = check_paged_heads(d))) return rc;
+  if (!bytes) return fail(POPE_ERR_INVALID, "bytes is NULL");
+  *bytes = paged_shape(*d, packed != 0).bytes;
+  return POPE_OK;
+}
+
+int pope_paged_attn(const pope_paged* d, const void* q, const float* freqs, const void* k_pages, const void* v_pages, const uint8_t* scales,
+                    const int32_t* table, const int32_t* lengths, const int32_t* cu, void* o, float* lse, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+  int rc = check_paged_call(d);
+  if (rc || (rc = check_paged_heads(d))) return rc;
+  if ((rc = check_strides("q", d->q_s, 3)) || (rc = check_strides("o", d->o_s, 3))) return rc;
+  if (d->N == 0) return POPE_OK;
+  if ((rc = check_pages(d, k_pages, v_pages, scales, table, lengths))) return rc;
+  if (!q || !o) return fail(POPE_ERR_INVALID, "q, o must be non-NULL");
+  if (d->R > 0 && !freqs) return fail(POPE_ERR_INVALID, "rotate dim %d > 0 needs freqs", d->R);
+  const PagedShape sh = paged_shape(*d, cu != nullptr);
+  if ((rc = check_ws(sh.bytes, workspace, workspace_bytes))) return rc;
+  pope::PagedAttnParams p;
+  std::memset(&p, 0, sizeof p);
+  p.c = paged_cache(*d, k_pages, v_pages, scales, table, lengths, cu);
+  p.q = static_cast<const uint16_t*>(q);
+  p.freqs = freqs;
+  p.o = static_cast<uint16_t*>(o);
+  p.lse = lse;
+  p.Hq = d->Hq; p.G = d->Hq / d->Hk; p.causal = d->causal != 0; p.N = d->N;
+  p.splits = sh.splits; p.least = kPagedLeast;
+  p.tiles = sh.tiles;
+  const float sc = d->softmax_scale;
+  p.sign = sc > 0.f ? 1.f : sc < 0.f ? -1.f : 0.f;
+  p.scale_log2 = sc != 0.f ? (sc > 0.f ? sc : -sc) * 1.4426950408889634f : 1.f;
+  copy3(p.q_s, d->q_s); copy3(p.o_s, d->o_s);
+  p.f_s[0] = d->f_s[0]; p.f_s[1] = d->f_s[1];
+  p.o_vec = d->D % 4 == 0 && reinterpret_cast<uintptr_t>(o) % 8 == 0 && d->o_s[0] % 4 == 0 && d->o_s[1] % 4 == 0 && d->o_s[2] % 4 == 0;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + sh.part_o);
+  if (sh.tiles * d->Hk * sh.splits >= ((int64_t)1 << 31)) return fail(POPE_ERR_UNSUPPORTED, "%lld row tiles x %d heads: too many workgroups", (long long)sh.tiles, d->Hk);
+  const hipError_t e = pope::launch_paged_attn(p, sh.plan, d->dtype, d->quantized != 0, reinterpret_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "paged attention launch");
   return POPE_OK;
 }
 

@@ -8,6 +8,7 @@
 // workspaces, flags and entry points, under torch::autograd::Function.  Nothing is kept between calls.
 #include <torch/extension.h>
 
+#include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
@@ -693,6 +694,139 @@ std::pair<Tensor, Tensor> polar_padded(const Tensor& q, const Tensor& k, const T
   return {r[0], r[1]};
 }
 
+// ---------------------------------------------------------------- paged cache
+
+// The cache and the sequences of a call; the Python module has checked shapes and dtypes of everything else, what is
+// checked here keeps raw pointers in bounds for callers of the ops.
+struct Paged {
+  pope_paged d{};
+  void* k; void* v; uint8_t* scales;
+  const int32_t* table; const int32_t* lengths; const int32_t* cu;
+
+  Paged(const Tensor& k_pages, const Tensor& v_pages, const Tensor& sc, const Tensor& page_table, const Tensor& len, const Tensor& cu_seqlens,
+        int64_t page_size, int64_t D, int64_t R, int64_t rows, at::ScalarType dtype) {
+    check_device(k_pages, {&v_pages, &sc, &page_table, &len, &cu_seqlens});
+    for (const Tensor* t : {&page_table, &len, &cu_seqlens})
+      TORCH_CHECK_TYPE(!t->defined() || t->scalar_type() == at::kInt, "pope_amd paged cache: page_table, lengths and cu_seqlens are int32");
+    TORCH_CHECK_VALUE(k_pages.dim() == 4 && k_pages.is_contiguous() && v_pages.is_contiguous() && sc.is_contiguous(), "pope_amd paged cache: pages must be contiguous");
+    TORCH_CHECK_VALUE(page_table.dim() == 2 && page_table.stride(1) == 1 && len.dim() == 1 && len.size(0) == page_table.size(0) && len.is_contiguous() &&
+                          (!cu_seqlens.defined() || (cu_seqlens.dim() == 1 && cu_seqlens.size(0) == page_table.size(0) + 1 && cu_seqlens.is_contiguous())),
+                      "pope_amd paged cache: page_table ", page_table.sizes(), " and lengths ", len.sizes(), " do not fit");
+    const int64_t most = INT_MAX;
+    TORCH_CHECK_VALUE(page_table.size(0) < most && page_table.size(1) <= most && rows >= 0 && rows <= most && k_pages.size(0) <= most && k_pages.size(1) <= most &&
+                          page_size <= most && D <= most && R <= most, "pope_amd paged cache: too large");
+    d.pages = (int32_t)k_pages.size(0);
+    d.page_size = (int32_t)page_size;
+    d.Hk = (int32_t)k_pages.size(1);
+    d.D = (int32_t)D;
+    d.R = (int32_t)R;
+    d.dtype = dtype == at::kHalf ? POPE_F16 : POPE_BF16;
+    d.quantized = k_pages.scalar_type() == at::kByte;
+    d.B = (int32_t)page_table.size(0);
+    d.N = (int32_t)rows;
+    d.table_cols = (int32_t)page_table.size(1);
+    d.table_sb = page_table.stride(0);
+    d.Hq = d.Hk;
+    TORCH_CHECK_TYPE(dtype == at::kHalf || dtype == at::kBFloat16, "pope_amd paged cache: rows of dtype ", dtype);
+    TORCH_CHECK_TYPE((d.quantized || k_pages.scalar_type() == dtype) && v_pages.scalar_type() == k_pages.scalar_type() && sc.scalar_type() == at::kByte,
+                     "pope_amd paged cache: pages of dtype ", k_pages.scalar_type(), " next to rows of dtype ", dtype);
+    size_t bytes[3];
+    check(pope_paged_cache_bytes(&d, bytes), "paged cache");
+    TORCH_CHECK_VALUE(k_pages.nbytes() == bytes[0] && v_pages.nbytes() == bytes[1] && sc.nbytes() == bytes[2],
+                      "pope_amd paged cache: pages do not fit ", d.Hk, " heads of dim ", D, ", rotate dim ", R, ", page size ", page_size);
+    k = k_pages.data_ptr();
+    v = v_pages.data_ptr();
+    scales = d.quantized ? sc.data_ptr<uint8_t>() : nullptr;
+    table = page_table.data_ptr<int32_t>();
+    lengths = len.data_ptr<int32_t>();
+    cu = cu_seqlens.defined() ? cu_seqlens.data_ptr<int32_t>() : nullptr;
+  }
+
+  void rows(const Tensor& t, const Tensor& pages, int64_t heads, const char* name) const {
+    check_device(pages, {&t});
+    TORCH_CHECK_VALUE(t.dim() == 4 && t.size(0) == (cu ? 1 : d.B) && (heads < 0 || t.size(1) == heads) && t.size(2) == d.N && t.size(3) == d.D && t.stride(3) == 1,
+                      "pope_amd paged cache: ", name, " ", t.sizes(), " does not fit");
+  }
+
+  void angles(const Tensor& freqs, const Tensor& bias, const Tensor& pages, bool need_bias) {
+    check_device(pages, {&freqs, &bias});
+    if (!d.R) return;
+    const int64_t batch = cu ? 1 : d.B;
+    TORCH_CHECK_VALUE(freqs.defined() && freqs.scalar_type() == at::kFloat && freqs.dim() == 3 && (freqs.size(0) == 1 || freqs.size(0) == batch) &&
+                          freqs.size(1) == d.N && freqs.size(2) == d.R && freqs.stride(2) == 1, "pope_amd paged cache: freqs do not fit");
+    d.f_s[0] = freqs.size(0) > 1 ? freqs.stride(0) : 0;
+    d.f_s[1] = freqs.stride(1);
+    if (!need_bias) return;
+    TORCH_CHECK_VALUE(bias.defined() && bias.scalar_type() == at::kFloat && bias.dim() == 2 && (bias.size(0) == 1 || bias.size(0) == d.Hk) &&
+                          bias.size(1) == d.R && bias.stride(1) == 1, "pope_amd paged cache: bias does not fit");
+    d.bias_sh = bias.size(0) > 1 ? bias.stride(0) : 0;
+  }
+};
+
+int64_t width(const Tensor& freqs) { return freqs.defined() ? freqs.size(-1) : 0; }
+const float* floats(const Tensor& t) { return static_cast<const float*>(data(t)); }
+
+using OptTensor = const std::optional<Tensor>&;
+
+void paged_write(const Tensor& k, const Tensor& v, OptTensor freqs_, OptTensor bias_, const Tensor& k_pages, const Tensor& v_pages,
+                 const Tensor& scales, const Tensor& table, const Tensor& lengths, OptTensor cu_, int64_t page_size) {
+  const Tensor freqs = opt(freqs_), bias = opt(bias_), cu = opt(cu_);
+  TORCH_CHECK_VALUE(k.dim() == 4, "pope_amd paged cache: k ", k.sizes(), " must be 4-D");
+  TORCH_CHECK_TYPE(k.scalar_type() == v.scalar_type(), "pope_amd paged cache: v of dtype ", v.scalar_type(), " next to k of dtype ", k.scalar_type());
+  Paged p(k_pages, v_pages, scales, table, lengths, cu, page_size, k.size(3), width(freqs), k.size(2), k.scalar_type());
+  const c10::DeviceGuard guard(k_pages.device());
+  p.rows(k, k_pages, p.d.Hk, "k");
+  p.rows(v, k_pages, p.d.Hk, "v");
+  p.angles(freqs, bias, k_pages, true);
+  strides3(p.d.k_s, k);
+  strides3(p.d.v_s, v);
+  check(pope_paged_write(&p.d, k.data_ptr(), v.data_ptr(), floats(freqs), floats(bias), p.k, p.v, p.scales, p.table, p.lengths, p.cu, stream_of(k_pages)),
+        "paged write");
+}
+
+std::pair<Tensor, Tensor> paged_read(const Tensor& k_pages, const Tensor& v_pages, const Tensor& scales, const Tensor& table, const Tensor& lengths,
+                                     OptTensor cu_, int64_t n, int64_t D, int64_t R, int64_t page_size, bool half, bool head_first) {
+  const Tensor cu = opt(cu_);
+  const at::ScalarType dtype = half ? at::kHalf : at::kBFloat16;
+  Paged p(k_pages, v_pages, scales, table, lengths, cu, page_size, D, R, n, dtype);
+  const c10::DeviceGuard guard(k_pages.device());
+  const auto rows = [&](int64_t cols) {
+    const int64_t B = p.cu ? 1 : p.d.B, H = p.d.Hk;
+    const auto opt = k_pages.options().dtype(dtype).requires_grad(false);
+    return head_first ? at::empty({B, H, n, cols}, opt) : at::empty({B, n, H, cols}, opt).transpose(1, 2);
+  };
+  const Tensor k = rows(D + R), v = rows(D);
+  strides3(p.d.k_s, k);
+  strides3(p.d.v_s, v);
+  check(pope_paged_read(&p.d, p.k, p.v, p.scales, p.table, p.lengths, p.cu, k.data_ptr(), v.data_ptr(), stream_of(k_pages)), "paged read");
+  return {k, v};
+}
+
+std::pair<Tensor, Tensor> paged_attn(const Tensor& q, OptTensor freqs_, const Tensor& k_pages, const Tensor& v_pages, const Tensor& scales,
+                                     const Tensor& table, const Tensor& lengths, OptTensor cu_, int64_t page_size, bool causal, double softmax_scale,
+                                     bool with_lse) {
+  const Tensor freqs = opt(freqs_), cu = opt(cu_);
+  TORCH_CHECK_VALUE(q.dim() == 4, "pope_amd paged cache: q ", q.sizes(), " must be 4-D");
+  Paged p(k_pages, v_pages, scales, table, lengths, cu, page_size, q.size(3), width(freqs), q.size(2), q.scalar_type());
+  const c10::DeviceGuard guard(k_pages.device());
+  p.rows(q, k_pages, -1, "q");
+  p.angles(freqs, Tensor(), k_pages, false);
+  TORCH_CHECK_VALUE(q.size(1) <= INT_MAX, "pope_amd paged cache: too large");
+  p.d.Hq = (int32_t)q.size(1);
+  p.d.causal = causal;
+  p.d.softmax_scale = (float)softmax_scale;
+  const Tensor o = at::empty_like(q, q.options().requires_grad(false));
+  const Tensor lse = fp32_like(q, with_lse ? q.sizes().slice(0, 3) : at::IntArrayRef({0}));
+  strides3(p.d.q_s, q);
+  strides3(p.d.o_s, o);
+  size_t n = 0;
+  check(pope_paged_workspace_bytes(&p.d, p.cu != nullptr, &n), "workspace query");
+  const Tensor ws = bytes_like(q, n);
+  check(pope_paged_attn(&p.d, q.data_ptr(), floats(freqs), p.k, p.v, p.scales, p.table, p.lengths, p.cu, o.data_ptr(),
+                        with_lse ? static_cast<float*>(lse.data_ptr()) : nullptr, data(ws), n, stream_of(q)), "paged attention");
+  return {o, lse};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_pope_host, m) {
@@ -703,6 +837,9 @@ PYBIND11_MODULE(_pope_host, m) {
   m.def("sim_padded", &sim_padded, nogil);
   m.def("polar", &polar, nogil);
   m.def("polar_padded", &polar_padded, nogil);
+  m.def("paged_write", &paged_write, nogil);
+  m.def("paged_read", &paged_read, nogil);
+  m.def("paged_attn", &paged_attn, nogil);
   m.def("untraced", &untraced);
   m.def("last_bwd_prepared", [] { return g_last_bwd_prepared.load(); });
   m.def("abi_version", [] { return POPE_ABI_VERSION; });

@@ -47,10 +47,23 @@ class PopeCast(ctypes.Structure):
                 ("src_s", ctypes.c_int64 * 4), ("dst_s", ctypes.c_int64 * 4)]
 
 
+class PopePaged(ctypes.Structure):
+    """Mirror of ``struct pope_paged`` (include/pope_abi.h)."""
+
+    _fields_ = [
+        ("pages", ctypes.c_int32), ("page_size", ctypes.c_int32), ("Hk", ctypes.c_int32), ("D", ctypes.c_int32),
+        ("R", ctypes.c_int32), ("dtype", ctypes.c_int32), ("quantized", ctypes.c_int32), ("B", ctypes.c_int32),
+        ("N", ctypes.c_int32), ("table_cols", ctypes.c_int32), ("Hq", ctypes.c_int32), ("causal", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_float), ("table_sb", ctypes.c_int64), ("q_s", _I64x3), ("k_s", _I64x3),
+        ("v_s", _I64x3), ("o_s", _I64x3), ("f_s", ctypes.c_int64 * 2), ("bias_sh", ctypes.c_int64),
+    ]
+
+
 EXPORTS = (
     "pope_abi_version", "pope_last_error", "pope_workspace_bytes", "pope_sim_fwd", "pope_sim_bwd",
     "pope_flash_fwd", "pope_flash_fwd_split", "pope_flash_bwd", "pope_flash_bwd_split", "pope_flash_decode", "pope_flash_decode_noalloc", "pope_polar_fwd",
-    "pope_polar_bwd", "pope_cast_f16", "pope_pad_rows", "pope_profile_enable", "pope_profile_read", "pope_profile_reset",
+    "pope_polar_bwd", "pope_cast_f16", "pope_pad_rows", "pope_paged_cache_bytes",
+    "pope_paged_write", "pope_paged_read", "pope_paged_workspace_bytes", "pope_paged_attn", "pope_profile_enable", "pope_profile_read", "pope_profile_reset",
 )
 
 _lib = None
@@ -88,6 +101,17 @@ def _declare(lib):
     lib.pope_polar_bwd.argtypes = [dp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
     lib.pope_cast_f16.restype = i32
     lib.pope_cast_f16.argtypes = [ctypes.POINTER(PopeCast), i32, vp, vp]
+    gp = ctypes.POINTER(PopePaged)
+    lib.pope_paged_cache_bytes.restype = i32
+    lib.pope_paged_cache_bytes.argtypes = [gp, ctypes.POINTER(sz)]
+    lib.pope_paged_write.restype = i32
+    lib.pope_paged_write.argtypes = [gp] + [vp] * 11
+    lib.pope_paged_read.restype = i32
+    lib.pope_paged_read.argtypes = [gp] + [vp] * 9
+    lib.pope_paged_workspace_bytes.restype = i32
+    lib.pope_paged_workspace_bytes.argtypes = [gp, i32, ctypes.POINTER(sz)]
+    lib.pope_paged_attn.restype = i32
+    lib.pope_paged_attn.argtypes = [gp] + [vp] * 11 + [sz, vp]
     lib.pope_profile_enable.restype = i32
     lib.pope_profile_enable.argtypes = [i32]
     lib.pope_profile_read.restype = i32
