@@ -36,9 +36,11 @@ struct PagedAttnParams {
   int Hq, G, causal, N;                // G = Hq / Hk; N: rows per batch entry (all of them when packed)
   int splits, least;                   // splits of the key axis, the least blocks of one
   int64_t tiles;                       // row tiles
-  float scale_log2, sign;              // |softmax scale| log2 e and its sign (0: scores are all 0)
+  // Scores come out of the products in log2 units: Q_hat carries q_factor = softmax scale x log2 e.  fp16 does not hold
+  // every Q_hat times a factor above 1: the scores then take `late`, the factor's magnitude, and q_factor its sign.
+  float q_factor, late;
   int64_t q_s[3], o_s[3], f_s[2];
-  int o_vec;                           // output rows of whole 8-byte units
+  int q_vec, f_vec, o_vec;             // query rows: whole 16-byte units; angles likewise; output rows: 8-byte units
   float* part_o; float* part_ml;       // splits > 1: (tile, head, split, row): 16 * tiles floats, and (m, l)
 };
 // Rows of a tile for a call with `rows` (query head of a key head, new token) rows per sequence on average.

@@ -1,6 +1,6 @@
 // Attention of new tokens over the paged cache (gfx950): one kernel for single tokens and for chunks.
 //
-//   o_i = sum_j 2^(c s_ij - c m_i) v_j / sum_j 2^(c s_ij - c m_i),   s_ij = Q_hat_i . K_hat_j,  c = scale log2 e,
+//   o_i = sum_j 2^(s_ij - m_i) v_j / sum_j 2^(s_ij - m_i),   s_ij = scale log2 e  Q_hat_i . K_hat_j,
 // j < L, or j <= the row's position (causal).  K_hat rows come expanded from the cache, so there is no transform in the
 // loop; Q_hat = [softplus(q) cos F, softplus(q) sin F, q] is computed once per tile.
 //
@@ -19,7 +19,7 @@
 // rounded once, its error would appear in every score, about 0.4 of an output's own rounding); P is rounded to 16 bits
 // once (its errors are independent from key to key).
 #pragma once
-#include "paged_dev.hpp"
+#include "paged_rows.hpp"
 
 namespace pope {
 
@@ -32,27 +32,6 @@ struct PagedShared {
   static constexpr int kBytes = kQ > kJoin ? kQ : kJoin;
 };
 
-// Blocks of keys a tile's rows see, over all of them.
-__device__ __forceinline__ int paged_tile_blocks(const PagedSeg& g, int64_t local, int rows, int G, bool causal) {
-  const int64_t all = (int64_t)g.n * G, end = (local + 1) * rows;
-  const int64_t last = (end < all ? end : all) - 1;
-  const int limit = last < local * rows ? 0 : paged_limit(g.first + (int)(last / G), g.len, causal);
-  return (limit + kBlockKeys - 1) / kBlockKeys;
-}
-
-// x with the 16-bit (8-bit) elements j of which (keep >> j) & 1 is 0 cleared.
-__device__ __forceinline__ u32x4 keep16(u32x4 x, uint32_t keep) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] &= ((keep >> (2 * i)) & 1 ? 0xffffu : 0u) | ((keep >> (2 * i + 1)) & 1 ? 0xffff0000u : 0u);
-  return x;
-}
-
-template <typename T>
-__device__ __forceinline__ bool nonfinite16(uint32_t bits) {
-  constexpr uint32_t e = T::kCode == 2 ? 0x7f80u : 0x7c00u;
-  return (bits & e) == e;
-}
-
 template <typename T, bool Q8, int KS, int VT, int NQ, int WK>
 __global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnParams p) {
   using Sh = PagedShared<KS, VT, NQ, WK>;
@@ -63,11 +42,9 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnParams p) {
   const int group = wave / WK, wk = wave % WK;
   const int col = lane & 15, quad = lane >> 4;
 
-  int64_t id = blockIdx.x;
-  const int split = (int)(id % p.splits);
-  id /= p.splits;
-  const int64_t tile = id % p.tiles;
-  const int hk = (int)(id / p.tiles);
+  const PagedJob job = paged_job(p);
+  const int64_t tile = job.tile;
+  const int hk = job.hk, split = job.split;
   const PagedTile t = paged_tile(c.seqs, tile, p.G, kRows, 1);
   const PagedSeg& g = t.seg;
   const int64_t rows_all = (int64_t)g.n * p.G, r0 = t.local * kRows;
@@ -78,53 +55,29 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnParams p) {
   if (p.splits > 1 && range.begin >= range.end) return;   // the join knows which splits have blocks
 
   // ---- the lane's rows: column col of each of the wave's NQ column tiles -------------------------------------
+  const PagedRowMap map(r0, p.G);
+  const int count = (int)(rows_all - r0 < kRows ? rows_all - r0 : kRows), wx0 = group * 16 * NQ;
   int row_i[NQ], row_h[NQ], lim[NQ];
   bool live[NQ];
-  const int64_t wr0 = r0 + group * 16 * NQ;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    const int64_t r = wr0 + n * 16 + col;
-    live[n] = r < rows_all;
-    row_i[n] = live[n] ? (int)(r / p.G) : 0;
-    row_h[n] = (int)(r - (int64_t)row_i[n] * p.G) * c.Hk + hk;
+    const int x = wx0 + n * 16 + col;
+    live[n] = x < count;
+    row_i[n] = live[n] ? map.token(x) : 0;
+    row_h[n] = live[n] ? map.group(x) * c.Hk + hk : hk;
     lim[n] = live[n] ? paged_limit(g.first + row_i[n], g.len, causal) : 0;
   }
   // keys every live row of the wave sees
-  const int least_lim = wr0 < rows_all ? paged_limit(g.first + (int)(wr0 / p.G), g.len, causal) : 0;
+  const int least_lim = wx0 < count ? paged_limit(g.first + map.token(wx0), g.len, causal) : 0;
 
   // ---- Q_hat of the group's rows, 16 at a time, through LDS --------------------------------------------------
   uint16_t* qhi = reinterpret_cast<uint16_t*>(smem) + group * 2 * 16 * QST;
   uint16_t* qlo = qhi + 16 * QST;
   typename T::vec8 qh[NQ][KS], ql[NQ][KS];
-  const int E = c.D + c.R;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     if (n) __syncthreads();
-    constexpr int kTpr = 4 * WK;   // threads per row
-    const int tid = wk * 64 + lane, rr = tid / kTpr, tr = tid % kTpr;
-    const int64_t r = wr0 + n * 16 + rr;
-    const bool on = r < rows_all && p.sign != 0.f;
-    const int i = on ? (int)(r / p.G) : 0, h = on ? (int)(r - (int64_t)i * p.G) * c.Hk + hk : hk;
-    const uint16_t* src = p.q + (int64_t)g.batch * p.q_s[0] + (int64_t)h * p.q_s[1] + (int64_t)(g.row0 + i) * p.q_s[2];
-    const float* fr = p.freqs + (int64_t)g.batch * p.f_s[0] + (int64_t)(g.row0 + i) * p.f_s[1];
-    auto put = [&](int e, float x) {
-      const uint16_t hi = T::bits(x);
-      qhi[rr * QST + e] = hi;
-      qlo[rr * QST + e] = T::bits(x - T::to_float(hi));
-    };
-    for (int d = tr; d < c.D; d += kTpr) {
-      const float x = on ? T::to_float(src[d]) : 0.f;
-      if (d < c.R) {
-        float sn, cs;
-        sincos_rev(on ? fr[d] : 0.f, &sn, &cs);
-        const float a = on ? softplus_f(x) * p.sign : 0.f;
-        put(d, a * cs);
-        put(c.R + d, a * sn);
-      } else {
-        put(c.R + d, x * p.sign);
-      }
-    }
-    for (int e = E + tr; e < KS * 32; e += kTpr) put(e, 0.f);
+    paged_query_rows<T, 16, 4>(p, g, map, wx0 + n * 16, count, hk, wk * 64 + lane, 64 * WK, KS * 32, QST, qhi, qlo);
     __syncthreads();
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -201,7 +154,7 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnParams p) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         typename T::vec8 a;
-        if constexpr (Q8) a = as_vec8<typename T::vec8>(unpack_e4m3<T>(u32x2{kf[ks][2 * half], kf[ks][2 * half + 1]}));
+        if constexpr (Q8) a = as_vec8<typename T::vec8>(unpack_e4m3<T>(u32x2{kf[ks][2 * half], kf[ks][2 * half + 1]}, 1.f));
         else a = as_vec8<typename T::vec8>(kf[2 * ks + half]);
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
@@ -221,6 +174,12 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnParams p) {
           for (int n = 0; n < NQ; ++n) s[n][half][i] = __builtin_amdgcn_ldexpf(s[n][half][i], e);
         }
       }
+    }
+    if (T::kCode == 1 && p.late != 1.f) {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) s[n][half] *= p.late;
     }
     load_k(next_page, next);
 
@@ -250,13 +209,12 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnParams p) {
       mx = half_swap_max(mx);
       const float mn = fmaxf(m[n], mx);
       const float mu = mn == -INFINITY ? 0.f : mn;
-      const float alpha = __builtin_amdgcn_exp2f((m[n] - mu) * p.scale_log2);
-      const float base = -mu * p.scale_log2;
+      const float alpha = __builtin_amdgcn_exp2f(m[n] - mu);
       m[n] = mn;
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        pr[n][j] = __builtin_amdgcn_exp2f(fmaf(s[n][j >> 2][j & 3], p.scale_log2, base));
+        pr[n][j] = __builtin_amdgcn_exp2f(s[n][j >> 2][j & 3] - mu);
         sum += pr[n][j];
       }
       l[n] = fmaf(l[n], alpha, sum);
@@ -275,7 +233,7 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnParams p) {
     u32x4 va[VT];
 #pragma unroll
     for (int v = 0; v < VT; ++v) {
-      if constexpr (Q8) va[v] = unpack_e4m3<T>(u32x2{vf[v >> 1][2 * (v & 1)], vf[v >> 1][2 * (v & 1) + 1]});
+      if constexpr (Q8) va[v] = unpack_e4m3<T>(u32x2{vf[v >> 1][2 * (v & 1)], vf[v >> 1][2 * (v & 1) + 1]}, 1.f);
       else va[v] = vf[v];
     }
     if (edge) {
@@ -363,7 +321,7 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnParams p) {
         for (int n = 0; n < NQ; ++n) {
           const f32x4 ml = src[(n * (VT + 1) + VT) * 64];
           const float mn = fmaxf(m[n], ml[0]), mu = mn == -INFINITY ? 0.f : mn;
-          const float a = __builtin_amdgcn_exp2f((m[n] - mu) * p.scale_log2), b = __builtin_amdgcn_exp2f((ml[0] - mu) * p.scale_log2);
+          const float a = __builtin_amdgcn_exp2f(m[n] - mu), b = __builtin_amdgcn_exp2f(ml[0] - mu);
           m[n] = mn;
           l[n] = l[n] * a + ml[1] * b;
 #pragma unroll
@@ -402,7 +360,7 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnParams p) {
     }
     if (p.lse && quad == 0)
       p.lse[((int64_t)g.batch * p.Hq + row_h[n]) * p.N + g.row0 + row_i[n]] =
-          l[n] == 0.f ? -INFINITY : (m[n] * p.scale_log2 + __builtin_amdgcn_logf(l[n])) * kLn2;
+          l[n] == 0.f ? -INFINITY : (m[n] + __builtin_amdgcn_logf(l[n])) * kLn2;
   }
 }
 
@@ -432,7 +390,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p, int 
       const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + row * 2);
       const f32x4 x = *reinterpret_cast<const f32x4*>(p.part_o + row * (VT * 16) + d);
       const float mn = fmaxf(m, ml.x), mu = mn == -INFINITY ? 0.f : mn;
-      const float a = __builtin_amdgcn_exp2f((m - mu) * p.scale_log2), b = __builtin_amdgcn_exp2f((ml.x - mu) * p.scale_log2);
+      const float a = __builtin_amdgcn_exp2f(m - mu), b = __builtin_amdgcn_exp2f(ml.x - mu);
       m = mn;
       l = l * a + ml.y * b;
       o = o * a + x * b;
@@ -448,7 +406,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p, int 
         if (d + k < c.D) dst[k] = T::bits(o[k] * inv);
     }
     if (p.lse && d == 0)
-      p.lse[((int64_t)g.batch * p.Hq + h) * p.N + g.row0 + i] = l == 0.f ? -INFINITY : (m * p.scale_log2 + __builtin_amdgcn_logf(l)) * kLn2;
+      p.lse[((int64_t)g.batch * p.Hq + h) * p.N + g.row0 + i] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
   }
 }
 
@@ -456,7 +414,6 @@ template <typename T, bool Q8, int KS, int VT, int NQ, int WK>
 hipError_t run_paged_attn(const PagedAttnParams& p, hipStream_t s) {
   constexpr int rows = 16 * NQ * (4 / WK);
   const int64_t wgs = p.tiles * p.c.Hk * p.splits;
-  if (wgs >= ((int64_t)1 << 31)) return hipErrorInvalidConfiguration;
   hipError_t e = launch_named("paged_attn", paged_attn_kernel<T, Q8, KS, VT, NQ, WK>, dim3((unsigned)wgs), dim3(256), s, p);
   if (e != hipSuccess || p.splits == 1) return e;
   const int y = (rows * VT * 4 + 255) / 256;
@@ -464,10 +421,20 @@ hipError_t run_paged_attn(const PagedAttnParams& p, hipStream_t s) {
 }
 
 template <typename T, bool Q8, int KS, int VT>
+hipError_t run_paged_rows(const PagedAttnParams& p, hipStream_t s) {
+  constexpr int rows = PagedRows<Q8, KS, VT>::kRows, step = PagedRows<Q8, KS, VT>::kStep;
+  const int64_t wgs = p.tiles * p.c.Hk * p.splits;
+  const hipError_t e = launch_named("paged_rows", paged_rows_kernel<T, Q8, KS, VT>, dim3((unsigned)wgs), dim3(512), s, p);
+  if (e != hipSuccess || p.splits == 1) return e;
+  const int y = (rows * VT * 4 + 255) / 256;
+  return launch_named("paged_join", paged_join_kernel<T, VT>, dim3((unsigned)(p.tiles * p.c.Hk), y), dim3(256), s, p, rows, step);
+}
+
+template <typename T, bool Q8, int KS, int VT>
 hipError_t run_paged_plan(const PagedAttnParams& p, PagedPlan plan, hipStream_t s) {
   if (plan.wk == 4 && plan.nq == 1) return run_paged_attn<T, Q8, KS, VT, 1, 4>(p, s);
   if constexpr (VT > 8) return run_paged_attn<T, Q8, KS, VT, 1, 1>(p, s);   // paged_plan
-  else return plan.wk == 4 ? run_paged_attn<T, Q8, KS, VT, 2, 4>(p, s) : run_paged_attn<T, Q8, KS, VT, 2, 1>(p, s);
+  else return plan.wk == 4 ? run_paged_attn<T, Q8, KS, VT, 2, 4>(p, s) : run_paged_rows<T, Q8, KS, VT>(p, s);
 }
 
 // The instance of (steps, tiles): paged_k_steps and paged_v_tiles give no other.

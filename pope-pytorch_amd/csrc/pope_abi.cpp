@@ -1085,13 +1085,14 @@ pope::PagedCache paged_cache(const pope_paged& d, const void* k, const void* v, 
   return c;
 }
 
-// Split of the key axis: as many parts as bring the grid to kPagedGrid workgroups, of at least kPagedLeast blocks.
-constexpr int kPagedGrid = 1024, kPagedLeast = 16;
+// Split of the key axis where the row tiles are few: as many parts as bring the grid to kPagedGrid workgroups, of at
+// least paged_least blocks of keys.
+constexpr int kPagedGrid = 1024;
 
 struct PagedShape {
   pope::PagedPlan plan;
   int64_t tiles;
-  int splits;
+  int splits, least;
   size_t part_o, bytes;
 };
 
@@ -1104,7 +1105,8 @@ PagedShape paged_shape(const pope_paged& d, bool packed) {
   s.tiles = pope::paged_tiles(d.B, d.N, packed, G, rows, 1);
   const int64_t wgs = std::max<int64_t>(s.tiles * d.Hk, 1);
   const int64_t blocks = (int64_t)d.table_cols * d.page_size / pope::kBlockKeys;
-  s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kPagedGrid / wgs, blocks / kPagedLeast));
+  s.least = s.plan.wk == 4 ? 16 : 32;
+  s.splits = s.plan.wk != 4 && wgs >= 512 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(kPagedGrid / wgs, blocks / s.least));
   s.part_o = s.bytes = 0;
   if (s.splits > 1) {
     const size_t n = (size_t)wgs * s.splits * rows;
@@ -1196,13 +1198,19 @@ int pope_paged_attn(const pope_paged* d, const void* q, const float* freqs, cons
   p.o = static_cast<uint16_t*>(o);
   p.lse = lse;
   p.Hq = d->Hq; p.G = d->Hq / d->Hk; p.causal = d->causal != 0; p.N = d->N;
-  p.splits = sh.splits; p.least = kPagedLeast;
+  p.splits = sh.splits; p.least = sh.least;
   p.tiles = sh.tiles;
-  const float sc = d->softmax_scale;
-  p.sign = sc > 0.f ? 1.f : sc < 0.f ? -1.f : 0.f;
-  p.scale_log2 = sc != 0.f ? (sc > 0.f ? sc : -sc) * 1.4426950408889634f : 1.f;
+  const float factor = d->softmax_scale * 1.4426950408889634f;
+  p.q_factor = factor;
+  p.late = 1.f;
+  if (d->dtype == POPE_F16 && !(factor >= -1.f && factor <= 1.f)) {
+    p.q_factor = factor < 0.f ? -1.f : 1.f;
+    p.late = factor < 0.f ? -factor : factor;
+  }
   copy3(p.q_s, d->q_s); copy3(p.o_s, d->o_s);
   p.f_s[0] = d->f_s[0]; p.f_s[1] = d->f_s[1];
+  p.q_vec = d->D % 8 == 0 && aligned16(q) && d->q_s[0] % 8 == 0 && d->q_s[1] % 8 == 0 && d->q_s[2] % 8 == 0;
+  p.f_vec = d->R % 8 == 0 && aligned16(freqs) && d->f_s[0] % 4 == 0 && d->f_s[1] % 4 == 0;
   p.o_vec = d->D % 4 == 0 && reinterpret_cast<uintptr_t>(o) % 8 == 0 && d->o_s[0] % 4 == 0 && d->o_s[1] % 4 == 0 && d->o_s[2] % 4 == 0;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + sh.part_o);

@@ -15,11 +15,8 @@ using namespace pope;
 // paged_tile of the kernels: the last segment whose first tile is at or below `tile`
 static bool find_tile(const PagedSeqs& q, int64_t tile, int unit, int per, int extra, PagedSeg* g, int64_t* local) {
   if (!q.cu) {
-    const int64_t each = ((int64_t)q.N * unit + per - 1) / per + extra - 1;
-    const int b = (int)(tile / each);
-    CHECK(b >= 0 && b < q.B);
-    *g = paged_seg(q, b);
-    *local = tile - (int64_t)b * each;
+    *local = tile / q.B;   // the sequences' n-th tiles side by side
+    *g = paged_seg(q, (int)(tile - *local * q.B));
     return true;
   }
   int found = 0;
