@@ -33,7 +33,8 @@ struct PagedAttnParams {
   PagedCache c;
   const uint16_t* q; const float* freqs;
   uint16_t* o; float* lse;             // lse may be null: (batch, Hq, rows) natural log
-  int Hq, G, causal, N;                // G = Hq / Hk; N: rows per batch entry (all of them when packed)
+  PagedDiv G;                          // Hq / Hk
+  int Hq, causal, N;                   // N: rows per batch entry (all of them when packed)
   int splits, least;                   // splits of the key axis, the least blocks of one
   int64_t tiles;                       // row tiles
   // Scores come out of the products in log2 units: Q_hat carries q_factor = softmax scale x log2 e.  fp16 does not hold

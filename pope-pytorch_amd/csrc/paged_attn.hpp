@@ -43,20 +43,20 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnParams p) {
   const int col = lane & 15, quad = lane >> 4;
 
   const PagedJob job = paged_job(p);
-  const int64_t tile = job.tile;
-  const int hk = job.hk, split = job.split;
-  const PagedTile t = paged_tile(c.seqs, tile, p.G, kRows, 1);
+  const int tile = job.tile, hk = job.hk, split = job.split;
+  const PagedTile t = paged_tile(c.seqs, tile, p.G.d, kRows, 1);
   const PagedSeg& g = t.seg;
-  const int64_t rows_all = (int64_t)g.n * p.G, r0 = t.local * kRows;
+  const int rows_all = g.n * (int)p.G.d, r0 = t.local * kRows;
   if (r0 >= rows_all) return;
   const bool causal = p.causal != 0;
   const int blocks = paged_tile_blocks(g, t.local, kRows, p.G, causal);
   const PagedRange range = paged_range(blocks, p.splits, p.least, WK, split);
-  if (p.splits > 1 && range.begin >= range.end) return;   // the join knows which splits have blocks
+  if (split > 0 && range.begin >= range.end) return;   // the join knows which splits have blocks
+  const bool part = paged_parts(blocks, p.splits, p.least, WK) > 1;
 
   // ---- the lane's rows: column col of each of the wave's NQ column tiles -------------------------------------
   const PagedRowMap map(r0, p.G);
-  const int count = (int)(rows_all - r0 < kRows ? rows_all - r0 : kRows), wx0 = group * 16 * NQ;
+  const int count = min(rows_all - r0, kRows), wx0 = group * 16 * NQ;
   int row_i[NQ], row_h[NQ], lim[NQ];
   bool live[NQ];
 #pragma unroll
@@ -77,7 +77,10 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnParams p) {
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     if (n) __syncthreads();
-    paged_query_rows<T, 16, 4>(p, g, map, wx0 + n * 16, count, hk, wk * 64 + lane, 64 * WK, KS * 32, QST, qhi, qlo);
+    const int at = wk * 64 + lane;
+    for (int it = at; it < 32 * VT; it += 64 * WK)
+      paged_query_make<T>(p, paged_query_load<T>(p, g, map, wx0 + n * 16 + it % 16, count, hk, it / 16 * 8), it % 16, it / 16 * 8, QST, qhi, qlo);
+    paged_query_tail<16>(p, at, 64 * WK, KS * 32, QST, qhi, qlo);
     __syncthreads();
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -336,8 +339,8 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnParams p) {
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     if (!live[n]) continue;
-    if (p.splits > 1) {
-      const int64_t row = ((tile * c.Hk + hk) * p.splits + split) * kRows + group * 16 * NQ + n * 16 + col;
+    if (part) {
+      const int64_t row = (((int64_t)tile * c.Hk + hk) * p.splits + split) * kRows + group * 16 * NQ + n * 16 + col;
       float* dst = p.part_o + row * (VT * 16) + quad * 4;
 #pragma unroll
       for (int v = 0; v < VT; ++v) *reinterpret_cast<f32x4*>(dst + v * 16) = acc[n][v];
@@ -368,21 +371,20 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnParams p) {
 template <typename T, int VT>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p, int rows, int step) {
   const PagedCache& c = p.c;
-  const int64_t tile = blockIdx.x % p.tiles;
-  const int hk = (int)(blockIdx.x / p.tiles);
-  const PagedTile t = paged_tile(c.seqs, tile, p.G, rows, 1);
+  const int hk = blockIdx.x % c.Hk, tile = blockIdx.x / c.Hk;
+  const PagedTile t = paged_tile(c.seqs, tile, p.G.d, rows, 1);
   const PagedSeg& g = t.seg;
-  const int64_t rows_all = (int64_t)g.n * p.G, r0 = t.local * rows;
+  const int rows_all = g.n * (int)p.G.d, r0 = t.local * rows;
   if (r0 >= rows_all) return;
   const int blocks = paged_tile_blocks(g, t.local, rows, p.G, p.causal != 0);
-  const int per = paged_split_blocks(blocks, p.splits, p.least, step);
-  const int parts = (blocks + per - 1) / per;
+  const int parts = paged_parts(blocks, p.splits, p.least, step);
+  if (parts <= 1) return;   // written by the one that had it
   constexpr int kCols = VT * 4;   // threads per row
   for (int it = blockIdx.y * 256 + threadIdx.x; it < rows * kCols; it += gridDim.y * 256) {
     const int rr = it / kCols, d = it % kCols * 4;
-    const int64_t r = r0 + rr;
+    const int r = r0 + rr;
     if (r >= rows_all || d >= c.D) continue;
-    const int64_t first = (tile * c.Hk + hk) * p.splits * (int64_t)rows + rr;
+    const int64_t first = ((int64_t)tile * c.Hk + hk) * p.splits * (int64_t)rows + rr;
     float m = -INFINITY, l = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     for (int s = 0; s < parts; ++s) {
@@ -396,7 +398,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p, int 
       o = o * a + x * b;
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int i = (int)(r / p.G), h = (int)(r - (int64_t)i * p.G) * c.Hk + hk;
+    const int i = (int)p.G.of(r), h = (r - i * (int)p.G.d) * c.Hk + hk;
     uint16_t* dst = p.o + (int64_t)g.batch * p.o_s[0] + (int64_t)h * p.o_s[1] + (int64_t)(g.row0 + i) * p.o_s[2] + d;
     if (p.o_vec) {
       *reinterpret_cast<u32x2*>(dst) = u32x2{T::pack2(o[0] * inv, o[1] * inv), T::pack2(o[2] * inv, o[3] * inv)};
@@ -422,12 +424,12 @@ hipError_t run_paged_attn(const PagedAttnParams& p, hipStream_t s) {
 
 template <typename T, bool Q8, int KS, int VT>
 hipError_t run_paged_rows(const PagedAttnParams& p, hipStream_t s) {
-  constexpr int rows = PagedRows<Q8, KS, VT>::kRows, step = PagedRows<Q8, KS, VT>::kStep;
+  constexpr int rows = PagedRows<Q8, KS, VT>::kRows;
   const int64_t wgs = p.tiles * p.c.Hk * p.splits;
-  const hipError_t e = launch_named("paged_rows", paged_rows_kernel<T, Q8, KS, VT>, dim3((unsigned)wgs), dim3(512), s, p);
+  const hipError_t e = launch_named("paged_rows", paged_rows_kernel<T, Q8, KS, VT>, dim3((unsigned)wgs), dim3(256), s, p);
   if (e != hipSuccess || p.splits == 1) return e;
   const int y = (rows * VT * 4 + 255) / 256;
-  return launch_named("paged_join", paged_join_kernel<T, VT>, dim3((unsigned)(p.tiles * p.c.Hk), y), dim3(256), s, p, rows, step);
+  return launch_named("paged_join", paged_join_kernel<T, VT>, dim3((unsigned)(p.tiles * p.c.Hk), y), dim3(256), s, p, rows, 1);
 }
 
 template <typename T, bool Q8, int KS, int VT>

@@ -66,9 +66,9 @@ __device__ __forceinline__ Block find_block(const PagedCache& c, int64_t tile) {
   const PagedTile t = paged_tile(c.seqs, tile, 1, kBlockKeys, 2);
   b.seg = t.seg;
   const int first = floor_div(t.seg.first, kBlockKeys);
-  b.blk = first + (int)t.local;
+  b.blk = first + t.local;
   b.i0 = b.blk * kBlockKeys - t.seg.first;
-  b.any = t.local < ((int64_t)1 << 26) && b.i0 < t.seg.n;   // later tiles of the segment are empty
+  b.any = b.i0 < t.seg.n;   // later tiles of the segment are empty
   b.page = b.any && b.blk >= 0 && t.seg.b >= 0 ? paged_page(c, t.seg.b, b.blk) : -1;
   return b;
 }

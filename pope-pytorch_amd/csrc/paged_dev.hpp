@@ -8,12 +8,12 @@ namespace pope {
 // The segment that tile `tile` belongs to, and its tile within it; seg.n = 0 where there is none.  Packed calls: the
 // lanes of a wave test 64 segments' first tiles at a time, the last one at or below `tile` has it (with bounds that
 // decrease, any segment may come out, and paged_seg bounds it).  Padded calls: the sequences' n-th tiles side by side.
-struct PagedTile { PagedSeg seg; int64_t local; };
-__device__ __forceinline__ PagedTile paged_tile(const PagedSeqs& q, int64_t tile, int unit, int per, int extra) {
+struct PagedTile { PagedSeg seg; int local; };
+__device__ __forceinline__ PagedTile paged_tile(const PagedSeqs& q, int tile, int unit, int per, int extra) {
   PagedTile t;
   if (!q.cu) {
-    t.local = tile / q.B;
-    t.seg = paged_seg(q, (int)(tile - t.local * q.B));
+    t.local = (int)((unsigned)tile / (unsigned)q.B);
+    t.seg = paged_seg(q, tile - t.local * q.B);
     return t;
   }
   const int lane = threadIdx.x & 63, S = q.B + 2;
@@ -67,117 +67,117 @@ __device__ __forceinline__ u32x4 unpack_e4m3(u32x2 w, float unit) {
 
 // Workgroup -> (key head, row tile, split): heads fastest, so that a head's tiles, which read the same keys, run at once
 // on one XCD (ids are dealt round-robin to the 8 XCDs); later tiles first, which see the most keys when causal.
-struct PagedJob { int64_t tile; int hk, split; };
+struct PagedJob { int tile, hk, split; };
 __device__ __forceinline__ PagedJob paged_job(const PagedAttnParams& p) {
-  const int64_t id = blockIdx.x, rest = id / p.c.Hk;
-  return PagedJob{p.tiles - 1 - rest % p.tiles, (int)(id - rest * p.c.Hk), (int)(rest / p.tiles)};
+  const unsigned id = blockIdx.x, rest = id / (unsigned)p.c.Hk, n = (unsigned)p.tiles, split = rest / n, x = rest - split * n;
+  return PagedJob{(int)(n - 1 - x), (int)(id - rest * p.c.Hk), (int)split};
 }
 
 // Rows of a tile that starts at row r0 of its segment: row r0 + x is query head g Hk + hk of new token i, r = i G + g.
 struct PagedRowMap {
-  int i0, rem, G;
-  __device__ __forceinline__ PagedRowMap(int64_t r0, int g) : i0((int)(r0 / g)), rem((int)(r0 - (int64_t)i0 * g)), G(g) {}
-  __device__ __forceinline__ int token(int x) const { return i0 + (int)((unsigned)(rem + x) / (unsigned)G); }
-  __device__ __forceinline__ int group(int x) const { return (int)((unsigned)(rem + x) % (unsigned)G); }
+  unsigned i0, rem, G;
+  PagedDiv div;
+  __device__ __forceinline__ PagedRowMap(int r0, const PagedDiv& g) : i0(g.of(r0)), rem(r0 - i0 * g.d), G(g.d), div(g) {}
+  __device__ __forceinline__ int token(int x) const { return (int)(i0 + div.of(rem + x)); }
+  __device__ __forceinline__ int group(int x) const { return (int)(rem + x - div.of(rem + x) * G); }
 };
 
-// Q_hat of `ROWS` rows from x0 on (those below `live`; the others are zeros) by `n` threads, this one the `at`-th, times
-// `factor`, each value as the sum of two 16-bit parts; CH columns of a row per thread and turn, all loads independent.
-template <typename T, int ROWS, int CH>
-__device__ __forceinline__ void paged_query_rows(const PagedAttnParams& p, const PagedSeg& g, const PagedRowMap& map, int x0, int live, int hk,
-                                                 int at, int n, int cols, int stride, uint16_t* hi, uint16_t* lo) {
+// Q_hat of a tile's rows, eight columns of a row at a time: their inputs, loaded ahead; made and stored as the sum of two
+// 16-bit parts each; and the zeros behind a row.
+struct PagedQueryIn {
+  u32x4 x;        // the queries
+  f32x4 f[2];     // their angles
+};
+template <typename T>
+__device__ __forceinline__ PagedQueryIn paged_query_load(const PagedAttnParams& p, const PagedSeg& g, const PagedRowMap& map, int x, int count, int hk, int d0) {
   const PagedCache& c = p.c;
-  const int D = c.D, R = c.R, chunks = (D + CH - 1) / CH;
-  const bool whole = R % CH == 0;   // a chunk is all rotated or all not, and its columns start on a chunk
-  for (int it = at; it < ROWS * chunks; it += n) {
-    const int row = it % ROWS, d0 = it / ROWS * CH;
-    const bool on = x0 + row < live && p.q_factor != 0.f;
-    const int i = g.row0 + (on ? map.token(x0 + row) : 0), h = on ? map.group(x0 + row) * c.Hk + hk : hk;
-    const uint16_t* src = p.q + (int64_t)g.batch * p.q_s[0] + (int64_t)h * p.q_s[1] + (int64_t)i * p.q_s[2] + d0;
-    const float* fr = p.freqs + (int64_t)g.batch * p.f_s[0] + (int64_t)i * p.f_s[1] + d0;
-    float x[CH], f[CH];
-    if (p.q_vec) {   // D a multiple of 8, rows 16-byte aligned
-      if constexpr (CH == 8) {
-        unpack8<T>(on ? *reinterpret_cast<const u32x4*>(src) : u32x4{0, 0, 0, 0}, x);
-      } else {
-        const u32x2 w = on ? *reinterpret_cast<const u32x2*>(src) : u32x2{0, 0};
+  PagedQueryIn in;
+  in.x = u32x4{0, 0, 0, 0};
+  in.f[0] = in.f[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (x >= count || d0 >= c.D) return in;
+  const unsigned r = map.rem + x, i = map.div.of(r), gi = r - i * map.G;
+  const int64_t tok = g.row0 + (int)(map.i0 + i);
+  const uint16_t* src = p.q + (int64_t)g.batch * p.q_s[0] + (int64_t)(gi * c.Hk + hk) * p.q_s[1] + tok * p.q_s[2] + d0;
+  if (p.q_vec) {   // D a multiple of 8, rows 16-byte aligned
+    in.x = *reinterpret_cast<const u32x4*>(src);
+  } else {
 #pragma unroll
-        for (int k = 0; k < CH; ++k) x[k] = T::to_float((uint16_t)(w[k >> 1] >> (16 * (k & 1))));
-      }
+    for (int k = 0; k < 8; ++k)
+      if (d0 + k < c.D) in.x[k >> 1] |= (uint32_t)src[k] << (16 * (k & 1));
+  }
+  if (d0 < c.R) {
+    const float* fr = p.freqs + (int64_t)g.batch * p.f_s[0] + tok * p.f_s[1] + d0;
+    if (p.f_vec) {   // R a multiple of 8, rows 16-byte aligned
+      in.f[0] = *reinterpret_cast<const f32x4*>(fr);
+      in.f[1] = *reinterpret_cast<const f32x4*>(fr + 4);
     } else {
 #pragma unroll
-      for (int k = 0; k < CH; ++k) x[k] = on && d0 + k < D ? T::to_float(src[k]) : 0.f;
-    }
-    if (d0 < R) {
-      if (p.f_vec) {   // R a multiple of 8, rows 16-byte aligned
-#pragma unroll
-        for (int k = 0; k < CH; k += 4) {
-          const f32x4 w = on ? *reinterpret_cast<const f32x4*>(fr + k) : f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) f[k + e] = w[e];
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < CH; ++k) f[k] = on && d0 + k < R ? fr[k] : 0.f;
-      }
-    }
-    float a[CH], b[CH];   // a: cosine part, or the raw value; b: sine part
-#pragma unroll
-    for (int k = 0; k < CH; ++k) {
-      a[k] = x[k] * p.q_factor;
-      b[k] = 0.f;
-      if (d0 + k < R) {
-        float sn, cs;
-        sincos_rev(f[k], &sn, &cs);
-        const float m = on ? softplus_f(x[k]) * p.q_factor : 0.f;
-        a[k] = m * cs;
-        b[k] = m * sn;
-      }
-    }
-    auto store = [&](int e, const float* v) {   // CH columns from e on
-      uint32_t wh[CH / 2], wl[CH / 2];
-#pragma unroll
-      for (int k = 0; k < CH / 2; ++k) {
-        wh[k] = T::pack2(v[2 * k], v[2 * k + 1]);
-        wl[k] = T::pack2(v[2 * k] - T::to_float((uint16_t)wh[k]), v[2 * k + 1] - T::to_float((uint16_t)(wh[k] >> 16)));
-      }
-#pragma unroll
-      for (int k = 0; k < CH / 2; k += 2) {
-        *reinterpret_cast<u32x2*>(hi + row * stride + e + 2 * k) = u32x2{wh[k], wh[k + 1]};
-        *reinterpret_cast<u32x2*>(lo + row * stride + e + 2 * k) = u32x2{wl[k], wl[k + 1]};
-      }
-    };
-    if (whole) {
-      if (d0 < R) {
-        store(d0, a);
-        store(R + d0, b);
-      } else {
-        store(R + d0, a);
-      }
-    } else {
-      auto put = [&](int e, float v) {
-        const uint16_t w = T::bits(v);
-        hi[row * stride + e] = w;
-        lo[row * stride + e] = T::bits(v - T::to_float(w));
-      };
-#pragma unroll
-      for (int k = 0; k < CH; ++k) {
-        const int d = d0 + k;
-        if (d >= D) break;
-        put(d < R ? d : R + d, a[k]);
-        if (d < R) put(R + d, b[k]);
-      }
+      for (int k = 0; k < 8; ++k)
+        if (d0 + k < c.R) in.f[k >> 2][k & 3] = fr[k];
     }
   }
-  const int E = whole ? R + chunks * CH : D + R;
+  return in;
+}
+// Rows past the tile's are softplus(0) cos 0: finite values that nothing reads.
+template <typename T>
+__device__ __forceinline__ void paged_query_make(const PagedAttnParams& p, const PagedQueryIn& in, int row, int d0, int stride, uint16_t* hi, uint16_t* lo) {
+  const int D = p.c.D, R = p.c.R;
+  if (d0 >= D) return;
+  float x[8], a[8], b[8];   // a: cosine part, or the raw value; b: sine part
+  unpack8<T>(in.x, x);
+  const bool off = p.q_factor == 0.f;   // scores are 0, also of values that are not finite
+  if (d0 < R) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      float sn, cs;
+      sincos_rev(in.f[k >> 2][k & 3], &sn, &cs);
+      const float m = softplus_f(x[k]) * p.q_factor;
+      const bool rot = d0 + k < R;
+      a[k] = off ? 0.f : rot ? m * cs : x[k] * p.q_factor;
+      b[k] = off ? 0.f : m * sn;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) a[k] = off ? 0.f : x[k] * p.q_factor;
+  }
+  auto store = [&](int e, const float* v) {   // eight columns from e on
+    u32x4 wh, wl;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      wh[k] = T::pack2(v[2 * k], v[2 * k + 1]);
+      wl[k] = T::pack2(v[2 * k] - T::to_float((uint16_t)wh[k]), v[2 * k + 1] - T::to_float((uint16_t)(wh[k] >> 16)));
+    }
+    *reinterpret_cast<u32x4*>(hi + row * stride + e) = wh;
+    *reinterpret_cast<u32x4*>(lo + row * stride + e) = wl;
+  };
+  if (R % 8 == 0) {   // a chunk is all rotated or all not, and its columns start on a chunk
+    if (d0 < R) store(d0, a), store(R + d0, b);
+    else store(R + d0, a);
+  } else {
+    auto put = [&](int e, float v) {
+      const uint16_t w = T::bits(v);
+      hi[row * stride + e] = w;
+      lo[row * stride + e] = T::bits(v - T::to_float(w));
+    };
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int d = d0 + k;
+      if (d >= D) break;
+      put(d < R ? d : R + d, a[k]);
+      if (d < R) put(R + d, b[k]);
+    }
+  }
+}
+template <int ROWS>
+__device__ __forceinline__ void paged_query_tail(const PagedAttnParams& p, int at, int n, int cols, int stride, uint16_t* hi, uint16_t* lo) {
+  const int D = p.c.D, R = p.c.R, E = R % 8 == 0 ? R + (D + 7) / 8 * 8 : D + R;
   for (int it = at; it < ROWS * (cols - E); it += n) hi[it % ROWS * stride + E + it / ROWS] = lo[it % ROWS * stride + E + it / ROWS] = 0;
 }
 
 // Blocks of keys a tile's rows see, over all of them.
-__device__ __forceinline__ int paged_tile_blocks(const PagedSeg& g, int64_t local, int rows, int G, bool causal) {
-  const int64_t all = (int64_t)g.n * G, end = (local + 1) * rows;
-  const int64_t last = (end < all ? end : all) - 1;
-  const int limit = last < local * rows ? 0 : paged_limit(g.first + (int)(last / G), g.len, causal);
+__device__ __forceinline__ int paged_tile_blocks(const PagedSeg& g, int local, int rows, const PagedDiv& G, bool causal) {
+  const int last = min((local + 1) * rows, g.n * (int)G.d) - 1;
+  const int limit = last < local * rows ? 0 : paged_limit(g.first + (int)G.of(last), g.len, causal);
   return (limit + kBlockKeys - 1) / kBlockKeys;
 }
 

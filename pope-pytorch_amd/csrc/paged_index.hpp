@@ -27,6 +27,19 @@ constexpr int kBlockKeys = 32;   // keys per block: the k extent of one 16-bit M
 POPE_HD int clip(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
 POPE_HD int floor_div(int a, int b) { return a >= 0 ? a / b : -((b - 1 - a) / b); }
 
+// Division of numbers below 2^31 by d in [1, 2^30]: a product and a shift (with s = ceil(log2 d), m = ceil(2^(31 + s) / d) is too
+// large by less than d / d <= 1, which moves x m / 2^(31 + s) by less than 2^31 / 2^(31 + s) <= 1 / d).
+struct PagedDiv {
+  uint32_t d, m;
+  int shift;
+  POPE_HD uint32_t of(uint32_t x) const { return (uint32_t)(((uint64_t)x * m) >> shift); }
+};
+inline PagedDiv paged_div(uint32_t d) {
+  int s = 0;
+  while (((uint32_t)1 << s) < d) ++s;
+  return PagedDiv{d, (uint32_t)((((uint64_t)1 << (31 + s)) + d - 1) / d), 31 + s};
+}
+
 // What a call says about its sequences.
 struct PagedSeqs {
   const int* lengths;   // (B)
@@ -82,6 +95,10 @@ POPE_HD int paged_split_blocks(int blocks, int splits, int least, int step) {
   int per = (blocks + splits - 1) / splits;
   per = per < least ? least : per;
   return (per + step - 1) / step * step;
+}
+POPE_HD int paged_parts(int blocks, int splits, int least, int step) {   // splits that have blocks; 0: there are none
+  const int per = paged_split_blocks(blocks, splits, least, step);
+  return (blocks + per - 1) / per;
 }
 POPE_HD PagedRange paged_range(int blocks, int splits, int least, int step, int s) {
   const int per = paged_split_blocks(blocks, splits, least, step);

@@ -1,11 +1,11 @@
 // Attention over the paged cache for many rows (gfx950): chunks and whole prompts.
 //
-// One workgroup = 8 waves = 128 rows of one key head.  Waves 0-3 and 4-7 have the same rows, 32 each, and take turns
-// with the key blocks; at the end the second group hands its (m, l, O) to the first through LDS.  Two waves per SIMD:
-// one's softmax runs under the other's products.
+// One workgroup = 4 waves = 128 rows of one key head, 32 per wave; two workgroups per CU (registers and half of the LDS),
+// each with its own barriers: what one does between its products runs under the other's.  (One workgroup of 8 waves,
+// two groups of 4 that took turns with the key blocks: 4,096-token prompts, 2 x 8 heads, D 64, R 32, @A us against @B.)
 //
-// Blocks of K and V go to LDS as they lie in the pages (direct loads, no registers), into a ring of stages: while step t
-// is in use, t + 1 has landed and t + 2 (t + 3 where four stages fit) is on its way.  Pages hold operands of 16x16
+// Blocks of K and V go to LDS as they lie in the pages (direct loads, no registers), into a ring of three to eight
+// stages: while step t is in use and t + 1 has landed, the others are on their way.  Pages hold operands of 16x16
 // MFMAs in units of 8 elements, and a unit is 8 consecutive k elements of one row: the 32x32x16 products here read the
 // same units in another order.  S^T row x of the product is key 16 (x / 8 % 2) + 8 (x / 16) + x % 8 of the block, so that
 // a lane's scores 8 s .. 8 s + 7 belong, in order, to the eight keys of the V unit of group 2 s + lane / 32, and P goes
@@ -29,56 +29,54 @@ struct PagedRows {
   static constexpr int kBlock = kKB + kVB;
   static constexpr int kRegs = KS * 16 + VT * 8;                     // of Q_hat (two parts) and O
   static constexpr bool kPipe = kRegs + 40 <= 170;                   // scores of two steps at once
-  static constexpr int BG = 4 * kBlock * 4 <= 160 * 1024 && kRegs + (kPipe ? 64 : 32) <= 150 ? 2 : 1;   // blocks per group and step
-  static constexpr int kStep = 2 * BG;                               // blocks per step
-  static constexpr int kStage = kStep * (kBlock + (Q8 ? 64 : 0));    // 8-bit: the blocks' exponents behind them
-  static constexpr int kSlots = 4 * kStage <= 160 * 1024 - 128 ? 4 : 3;
+  static constexpr int BG = 2 * kBlock * 3 <= 79 * 1024 && kRegs + (kPipe ? 64 : 32) <= 150 ? 2 : 1;   // blocks per step
+  static constexpr int kStage = BG * (kBlock + (Q8 ? 64 : 0));    // 8-bit: the blocks' exponents behind them
+  static constexpr int kFit = (80 * 1024 - 128) / kStage, kSlots = kFit < 8 ? kFit : 8;
   static constexpr int QST = KS * 32 + 8;
   // rows of Q_hat made at a time
   static constexpr int kQRows = 128 * QST * 4 <= kStage ? 128 : 64 * QST * 4 <= kStage ? 64 : 32;
-  static constexpr int kJoin = 4 * 64 * (VT / 2 * 16 + 4) * 4;
-  static constexpr int kMost = kQRows * QST * 4 > kStage ? (kSlots - 1) * kStage + kQRows * QST * 4 : kSlots * kStage;
-  static constexpr int kBytes = kMost > kJoin ? kMost : kJoin;
-  static_assert(kBytes + 128 <= 160 * 1024, "LDS");
+  static constexpr int kBytes = kSlots * kStage;
+  // stages that load while Q_hat is made behind them
+  static constexpr int kEarly = (kBytes - kQRows * QST * 4) / kStage < kSlots - 1 ? (kBytes - kQRows * QST * 4) / kStage : kSlots - 1;
+  static_assert(kSlots >= 3 && kEarly >= 1 && kBytes + 128 <= 80 * 1024, "LDS of two workgroups");
 };
 
 template <typename T, bool Q8, int KS, int VT>
-__global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedAttnParams p) {
+__global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedAttnParams p) {
   using C = PagedRows<Q8, KS, VT>;
   typedef typename T::vec8 vec8;
-  constexpr int BG = C::BG, kStep = C::kStep, NDB = VT / 2, K16 = 2 * KS, kRows = C::kRows;
+  constexpr int BG = C::BG, NDB = VT / 2, K16 = 2 * KS, kRows = C::kRows;
   __shared__ __attribute__((aligned(16))) char smem[C::kBytes];
   // Per (step % 8, block of the step): keys of values that are not finite.  Never cleared: add_seen looks at the value again.
   __shared__ uint32_t odd[32];
   const PagedCache& c = p.c;
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), lr = lane & 31, hf = lane >> 5;
-  const int grp = wave >> 2, wq = wave & 3;
 
   const PagedJob job = paged_job(p);
   const int hk = job.hk;
-  const PagedTile t = paged_tile(c.seqs, job.tile, p.G, kRows, 1);
+  const PagedTile t = paged_tile(c.seqs, job.tile, p.G.d, kRows, 1);
   const PagedSeg& g = t.seg;
-  const int64_t rows_all = (int64_t)g.n * p.G, r0 = t.local * kRows;
+  const int rows_all = g.n * (int)p.G.d, r0 = t.local * kRows;
   if (r0 >= rows_all) return;
   const bool causal = p.causal != 0;
   const int blocks = paged_tile_blocks(g, t.local, kRows, p.G, causal);
-  const PagedRange range = paged_range(blocks, p.splits, p.least, kStep, job.split);
-  if (p.splits > 1 && range.begin >= range.end) return;
+  const PagedRange range = paged_range(blocks, p.splits, p.least, 1, job.split);
+  if (job.split > 0 && range.begin >= range.end) return;
 
   // ---- the lane's row, and the keys that all of the wave's (of the tile's) rows see -----------------------------
   const PagedRowMap map(r0, p.G);
-  const int count = (int)(rows_all - r0 < kRows ? rows_all - r0 : kRows), x = wq * 32 + lr;   // the lane's row of the tile
+  const int count = min(rows_all - r0, kRows), x = wave * 32 + lr;   // the lane's row of the tile
   const bool live = x < count;
   const int row_i = live ? map.token(x) : 0, row_h = live ? map.group(x) * c.Hk + hk : hk;
   const int lim = live ? paged_limit(g.first + row_i, g.len, causal) : 0;
-  const int least_lim = wq * 32 < count ? paged_limit(g.first + map.token(wq * 32), g.len, causal) : 0;
+  const int least_lim = wave * 32 < count ? paged_limit(g.first + map.token(wave * 32), g.len, causal) : 0;
   const int tile_lim = paged_limit(g.first + map.i0, g.len, causal);   // the first row sees the fewest keys
 
   // ---- staging -------------------------------------------------------------------------------------------------
-  // A step's blocks are dealt to the waves, 8 / kStep waves per block, so that a wave finds one page per step.  Page numbers
+  // A step's blocks are dealt to the waves, 4 / BG waves per block, so that a wave finds one page per step.  Page numbers
   // of 64 pages at a time, one per lane; `lost`: some page was outside the cache (then gone_of looks closer).
-  const int steps = (range.end - range.begin + kStep - 1) / kStep;
-  constexpr int kPer = C::kBlock / 1024, kShare = 8 / kStep;   // a block's units of 64 x 16 bytes; waves per block
+  const int steps = (range.end - range.begin + BG - 1) / BG;
+  constexpr int kPer = C::kBlock / 1024, kShare = 4 / BG;   // a block's units of 64 x 16 bytes; waves per block
   constexpr int kWaveUnits = (kPer + kShare - 1) / kShare, kLeast = kPer / kShare;   // units a wave has at most / at least
   constexpr int kE = Q8 ? 1 : 2;
   const int my_block = wave / kShare, my_part = wave % kShare;
@@ -96,8 +94,8 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedAttnParams p) {
   const char* k_at = static_cast<const char*>(c.k) + hk * c.k_head * kE + my_part * 1024;
   const char* v_at = static_cast<const char*>(c.v) + hk * c.v_head * kE + (my_part * 1024 - C::kKB);
   auto issue = [&](int step, int slot) {   // slot: byte offset of the stage
-    const int first = range.begin + step * kStep, blk = min(first + my_block, range.end - 1), pg = blk >> c.blk_shift, sub = blk - (pg << c.blk_shift);
-    if ((first >> c.blk_shift) + kStep - page_base > 64) {   // the same for all waves: `lost` has to be
+    const int first = range.begin + step * BG, blk = min(first + my_block, range.end - 1), pg = blk >> c.blk_shift, sub = blk - (pg << c.blk_shift);
+    if ((first >> c.blk_shift) + BG - page_base > 64) {   // the same for all waves: `lost` has to be
       POPE_COLD_PATH();
       page_base = first >> c.blk_shift;
       window();
@@ -114,7 +112,7 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedAttnParams p) {
       load_lds16((key ? k_src : v_src) + x * 1024, lane * 16, dst + x * 1024);
     }
     if (Q8 && my_part == 0 && lane < 4)   // the block's 64 bytes of exponents
-      load_lds16(c.scales + (((((int64_t)page * c.Hk + hk) << c.blk_shift) + sub) * 64 + lane * 16), lds_addr(smem) + slot + kStep * C::kBlock + my_block * 64);
+      load_lds16(c.scales + (((((int64_t)page * c.Hk + hk) << c.blk_shift) + sub) * 64 + lane * 16), lds_addr(smem) + slot + BG * C::kBlock + my_block * 64);
   };
 
   // ---- the loop --------------------------------------------------------------------------------------------------
@@ -138,9 +136,9 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedAttnParams p) {
   // the lane's key of score x, less 4 hf
   auto key_of = [](int x) { return 16 * ((x >> 2) & 1) + 8 * (x >> 3) + (x & 3); };
   // the group's blocks of a step; `slot`: byte offset of its stage
-  auto stage_of = [&](int slot) -> const char* { return smem + slot + grp * BG * C::kBlock; };
-  auto scales_of = [&](int slot, int b) -> const uint8_t* { return reinterpret_cast<const uint8_t*>(smem + slot + kStep * C::kBlock + (grp * BG + b) * 64); };
-  auto first_block = [&](int st) { return range.begin + st * kStep + grp * BG; };
+  auto stage_of = [&](int slot) -> const char* { return smem + slot; };
+  auto scales_of = [&](int slot, int b) -> const uint8_t* { return reinterpret_cast<const uint8_t*>(smem + slot + BG * C::kBlock + b * 64); };
+  auto first_block = [&](int st) { return range.begin + st * BG; };
   auto gone = [&](int blk) { return lost && (g.b < 0 || paged_page(c, g.b, min(blk, range.end - 1)) < 0); };
   // whether some block of the step has keys that some row of the wave (of the tile) does not see
   const int free_blocks = min(least_lim / kBlockKeys, range.end), tile_blocks = min(tile_lim / kBlockKeys, range.end);
@@ -291,13 +289,20 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedAttnParams p) {
   // Blocks with keys that some row of the tile does not see: 0 x NaN must not count.  Slots from len on, and pages outside
   // the cache, hold whatever was there and become zeros in the stage; values that are not finite do too, and their keys are
   // noted, for `add_seen` to add them outside the product where they are seen.
-  auto tile_edge = [&](int st) { return range.begin + (st + 1) * kStep > tile_blocks || lost; };
+  auto tile_edge = [&](int st) { return range.begin + (st + 1) * BG > tile_blocks || lost; };
   auto sanitize = [&](int st, int slot) {
     char* stage = smem + slot;
-    for (int u = tid; u < kStep * (C::kVB / 16); u += 512) {
-      const int b = u / (C::kVB / 16), x = u % (C::kVB / 16), blk = range.begin + st * kStep + b;
+    for (int u = tid; u < BG * (C::kVB / 16); u += 256) {
+      const int b = u / (C::kVB / 16), x = u % (C::kVB / 16), blk = range.begin + st * BG + b;
       const int have = gone(blk) ? 0 : g.len - blk * kBlockKeys - 4 * ((x & 63) >> 4);
       uint32_t* w = reinterpret_cast<uint32_t*>(stage + b * C::kBlock + C::kKB + x * 16);
+      // an element with all exponent bits set (8-bit: a NaN code) carries into its sign bit
+      const u32x4 v4 = *reinterpret_cast<const u32x4*>(w);
+      constexpr uint32_t kMag = Q8 ? 0x7f7f7f7fu : 0x7fff7fffu, kOne = Q8 ? 0x01010101u : T::kCode == 2 ? 0x00800080u : 0x04000400u;
+      uint32_t carry = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) carry |= ((v4[i] & kMag) + kOne) & ~kMag;
+      if (!carry && have >= 20) continue;   // all 8 keys, 16 (j / 4) + j % 4, are there
       uint32_t noted = 0;
 #pragma unroll 1
       for (int i = 0; i < 4; ++i) {
@@ -318,7 +323,7 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedAttnParams p) {
   auto add_seen = [&](int st, const f32x16* s) {
 #pragma unroll
     for (int b = 0; b < BG; ++b) {
-      uint32_t keys = __builtin_amdgcn_readfirstlane(odd[(st & 7) * 4 + grp * BG + b]);
+      uint32_t keys = __builtin_amdgcn_readfirstlane(odd[(st & 7) * 4 + b]);
       const int blk = first_block(st) + b;
       if (keys && blk < range.end) {
         POPE_COLD_PATH();
@@ -347,25 +352,33 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedAttnParams p) {
   };
 
   if (tid < 32) odd[tid] = 0;
-  settle_vector_loads();
+  constexpr int RB = C::kQRows, kTurns = (RB * VT * 2 + 255) / 256;   // rows at a time, chunks per thread
+  PagedQueryIn in[kRows / RB][kTurns];
+#pragma unroll
+  for (int b = 0; b < kRows / RB; ++b)
+#pragma unroll
+    for (int k = 0; k < kTurns; ++k) in[b][k] = paged_query_load<T>(p, g, map, b * RB + (tid + 256 * k) % RB, count, hk, (tid + 256 * k) / RB * 8);
+  __builtin_amdgcn_sched_barrier(0);
   auto next_slot = [](int slot) { return slot + C::kStage == C::kSlots * C::kStage ? 0 : slot + C::kStage; };
   int put = 0;   // stage of the next step to issue
 #pragma unroll
-  for (int st = 0; st < C::kSlots - 1; ++st) {
+  for (int st = 0; st < C::kEarly; ++st) {
     if (st < steps) issue(st, put);
     put += C::kStage;
   }
-  // ---- Q_hat, through the stage that is issued last, while the first ones load ---------------------------------
+  // ---- Q_hat, through the stages behind, while the first ones load ---------------------------------------------
   {
-    constexpr int RB = C::kQRows;   // rows at a time
-    uint16_t* hi = reinterpret_cast<uint16_t*>(smem + (C::kSlots - 1) * C::kStage);
+    uint16_t* hi = reinterpret_cast<uint16_t*>(smem + C::kEarly * C::kStage);
     uint16_t* lo = hi + RB * C::QST;
 #pragma unroll
     for (int x0 = 0; x0 < kRows; x0 += RB) {
       if (x0) __syncthreads();
-      paged_query_rows<T, RB, 8>(p, g, map, x0, count, hk, tid, 512, KS * 32, C::QST, hi, lo);
+#pragma unroll
+      for (int k = 0; k < kTurns; ++k)
+        paged_query_make<T>(p, in[x0 / RB][k], (tid + 256 * k) % RB, (tid + 256 * k) / RB * 8, C::QST, hi, lo);
+      paged_query_tail<RB>(p, tid, 256, KS * 32, C::QST, hi, lo);
       __syncthreads();
-      if (wq * 32 >= x0 && wq * 32 < x0 + RB) {
+      if (wave * 32 >= x0 && wave * 32 < x0 + RB) {
         const int at = (x - x0) * C::QST + 8 * hf;
 #pragma unroll
         for (int k = 0; k < K16; ++k) {
@@ -375,12 +388,18 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedAttnParams p) {
       }
     }
   }
+  if constexpr (C::kEarly < C::kSlots - 1) {
+    __syncthreads();   // the last rows of Q_hat have been read
+    for (int st = C::kEarly; st < C::kSlots - 1; ++st) {
+      if (st < steps) issue(st, put);
+      put += C::kStage;
+    }
+  }
   // Loads of steps up to `st` have landed; later ones, with at least kLeast loads of this wave each, may be in flight.
   auto landed = [&](int st) {
-    const int ahead = min(steps - 1 - st, C::kSlots - 2 - (C::kPipe ? 1 : 0));
-    if (ahead >= 2) wait_vmcnt<2 * kLeast>();
-    else if (ahead == 1) wait_vmcnt<kLeast>();
-    else wait_vmcnt<0>();
+    constexpr int most = C::kSlots - 2 - (C::kPipe ? 1 : 0);
+    if (steps - 1 - st >= most) wait_vmcnt<most * kLeast>();
+    else wait_vmcnt<0>();   // the last steps were issued long ago
   };
   auto refill = [&](int st) {   // behind the barrier that ends the use of stage st - 1
     if (st + C::kSlots - 1 < steps) issue(st + C::kSlots - 1, put);
@@ -392,8 +411,7 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedAttnParams p) {
   if constexpr (C::kPipe) {
     float mx = -INFINITY;
     if (steps > 0) {
-      if (steps > 2 && C::kSlots > 3) wait_vmcnt<2 * kLeast>();
-      else if (steps > 1) wait_vmcnt<kLeast>();
+      if (steps >= C::kSlots - 1) wait_vmcnt<(C::kSlots - 2) * kLeast>();
       else wait_vmcnt<0>();
       __syncthreads();
       if (tile_edge(0)) {
@@ -489,36 +507,21 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedAttnParams p) {
   }
   l += wave_shfl_xor(l, 32);
 
-  // ---- the second group's state joins the first's -------------------------------------------------------------
-  __syncthreads();
-  f32x4* join = reinterpret_cast<f32x4*>(smem) + wq * (VT / 2 * 4 + 1) * 64 + lane;
-  if (grp == 1) {
-#pragma unroll
-    for (int d = 0; d < NDB; ++d)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) join[(d * 4 + q) * 64] = f32x4{acc[d][4 * q], acc[d][4 * q + 1], acc[d][4 * q + 2], acc[d][4 * q + 3]};
-    join[NDB * 4 * 64] = f32x4{set ? m : -INFINITY, l, 0.f, 0.f};
-  }
-  __syncthreads();
-  if (grp == 1 || !live) return;
-  const f32x4 ml = join[NDB * 4 * 64];
+  // ---- output, or this split's part -----------------------------------------------------------------------------
+  if (!live) return;
   if (!set) m = -INFINITY;
-  const float mn = fmaxf(m, ml[0]), mu = mn == -INFINITY ? 0.f : mn;
-  const float a = __builtin_amdgcn_exp2f(m - mu), b = __builtin_amdgcn_exp2f(ml[0] - mu);
-  l = l * a + ml[1] * b;
-  const bool part = p.splits > 1;
+  const bool part = paged_parts(blocks, p.splits, p.least, 1) > 1;
   const float f = part ? 1.f : l == 0.f ? 0.f : 1.f / l;
-  const int64_t row = part ? ((job.tile * c.Hk + hk) * p.splits + job.split) * kRows + wq * 32 + lr : 0;
+  const int64_t row = part ? (((int64_t)job.tile * c.Hk + hk) * p.splits + job.split) * kRows + wave * 32 + lr : 0;
   uint16_t* dst = p.o + (int64_t)g.batch * p.o_s[0] + (int64_t)row_h * p.o_s[1] + (int64_t)(g.row0 + row_i) * p.o_s[2];
 #pragma unroll
   for (int d = 0; d < NDB; ++d)
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int col = 32 * d + 8 * q + 4 * hf;
-      const f32x4 o = join[(d * 4 + q) * 64];
       f32x4 x;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = (acc[d][4 * q + i] * a + o[i] * b) * f;
+      for (int i = 0; i < 4; ++i) x[i] = acc[d][4 * q + i] * f;
       if (part) {
         *reinterpret_cast<f32x4*>(p.part_o + row * (VT * 16) + col) = x;
       } else if (p.o_vec) {
@@ -530,9 +533,9 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedAttnParams p) {
       }
     }
   if (hf == 0) {
-    if (part) *reinterpret_cast<float2*>(p.part_ml + row * 2) = make_float2(mn, l);
+    if (part) *reinterpret_cast<float2*>(p.part_ml + row * 2) = make_float2(m, l);
     else if (p.lse)
-      p.lse[((int64_t)g.batch * p.Hq + row_h) * p.N + g.row0 + row_i] = l == 0.f ? -INFINITY : (mn + __builtin_amdgcn_logf(l)) * kLn2;
+      p.lse[((int64_t)g.batch * p.Hq + row_h) * p.N + g.row0 + row_i] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
   }
 }
 

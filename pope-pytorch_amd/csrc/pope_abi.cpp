@@ -1085,9 +1085,11 @@ pope::PagedCache paged_cache(const pope_paged& d, const void* k, const void* v, 
   return c;
 }
 
-// Split of the key axis where the row tiles are few: as many parts as bring the grid to kPagedGrid workgroups, of at
-// least paged_least blocks of keys.
-constexpr int kPagedGrid = 1024;
+// Splits of the key axis.  A tile's blocks of keys go to as many workgroups as they have parts of `least` blocks (at most
+// `splits`, the grid's); tiles of one part write their output themselves.
+//   few rows   parts of 16 blocks (512 keys) while they bring the grid to kPagedGrid workgroups
+//   many rows  the chip holds kPagedSlots workgroups; a part is at most the blocks one of these places gets
+constexpr int kPagedGrid = 1024, kPagedSlots = 512;
 
 struct PagedShape {
   pope::PagedPlan plan;
@@ -1105,8 +1107,13 @@ PagedShape paged_shape(const pope_paged& d, bool packed) {
   s.tiles = pope::paged_tiles(d.B, d.N, packed, G, rows, 1);
   const int64_t wgs = std::max<int64_t>(s.tiles * d.Hk, 1);
   const int64_t blocks = (int64_t)d.table_cols * d.page_size / pope::kBlockKeys;
-  s.least = s.plan.wk == 4 ? 16 : 32;
-  s.splits = s.plan.wk != 4 && wgs >= 512 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(kPagedGrid / wgs, blocks / s.least));
+  if (s.plan.wk == 4) {
+    s.least = 16;
+    s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kPagedGrid / wgs, blocks / s.least));
+  } else {
+    s.least = (int)std::max<int64_t>(16, std::min<int64_t>(blocks, wgs * blocks / kPagedSlots));
+    s.splits = (int)((blocks + s.least - 1) / s.least);
+  }
   s.part_o = s.bytes = 0;
   if (s.splits > 1) {
     const size_t n = (size_t)wgs * s.splits * rows;
@@ -1197,7 +1204,7 @@ int pope_paged_attn(const pope_paged* d, const void* q, const float* freqs, cons
   p.freqs = freqs;
   p.o = static_cast<uint16_t*>(o);
   p.lse = lse;
-  p.Hq = d->Hq; p.G = d->Hq / d->Hk; p.causal = d->causal != 0; p.N = d->N;
+  p.Hq = d->Hq; p.G = pope::paged_div(d->Hq / d->Hk); p.causal = d->causal != 0; p.N = d->N;
   p.splits = sh.splits; p.least = sh.least;
   p.tiles = sh.tiles;
   const float factor = d->softmax_scale * 1.4426950408889634f;
@@ -1214,7 +1221,7 @@ int pope_paged_attn(const pope_paged* d, const void* q, const float* freqs, cons
   p.o_vec = d->D % 4 == 0 && reinterpret_cast<uintptr_t>(o) % 8 == 0 && d->o_s[0] % 4 == 0 && d->o_s[1] % 4 == 0 && d->o_s[2] % 4 == 0;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + sh.part_o);
-  if (sh.tiles * d->Hk * sh.splits >= ((int64_t)1 << 31)) return fail(POPE_ERR_UNSUPPORTED, "%lld row tiles x %d heads: too many workgroups", (long long)sh.tiles, d->Hk);
+  if ((int64_t)d->N * (d->Hq / d->Hk) > ((int64_t)1 << 30) || sh.tiles * d->Hk * sh.splits >= ((int64_t)1 << 31)) return fail(POPE_ERR_UNSUPPORTED, "%lld row tiles x %d heads: too many workgroups", (long long)sh.tiles, d->Hk);
   const hipError_t e = pope::launch_paged_attn(p, sh.plan, d->dtype, d->quantized != 0, reinterpret_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "paged attention launch");
   return POPE_OK;

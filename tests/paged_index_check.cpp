@@ -101,10 +101,17 @@ int main() {
     for (int s = 0; s < splits; ++s) {
       const PagedRange r = paged_range(nb, splits, least, step, s);
       CHECK(r.begin >= 0 && r.begin <= r.end && r.end <= nb);
-      CHECK((r.begin < r.end) == (s < (nb + per - 1) / per));   // the join counts the same splits
+      CHECK((r.begin < r.end) == (s < paged_parts(nb, splits, least, step)));   // the join counts the same splits
       for (int b = r.begin; b < r.end; ++b) ++part[b];
     }
     for (int x : part) CHECK(x == 1);
+  }
+  for (uint32_t d : {1u, 2u, 3u, 5u, 7u, 8u, 20u, 31u, 127u, 1000u, 65535u, 65537u, 1u << 30}) {
+    const PagedDiv div = paged_div(d);
+    for (int k = 0; k < 20000; ++k) {
+      const uint32_t x = k < 200 ? k : k < 400 ? 0x7fffffffu - (k - 200) : (rng() & 0x7fffffffu) / d * d + (k & 1 ? d - 1 : 0);
+      if (x <= 0x7fffffffu) CHECK(div.of(x) == x / d);
+    }
   }
   for (bool q8 : {false, true}) {
     for (int steps = 1; steps <= 16; ++steps) {
