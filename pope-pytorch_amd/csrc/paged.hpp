@@ -23,7 +23,7 @@ struct PagedRowsParams {               // write: k, v -> cache; read: cache -> k
   void* k; void* v;                    // rows (b, h, n); read: k rows of D + R columns
   const float* freqs; const float* bias;
   int64_t k_s[3], v_s[3], f_s[2], bias_sh;
-  int k_vec, v_vec;                    // rows of whole 16-byte units
+  int k_vec, v_vec, f_vec;             // rows of whole 16-byte units (f: of angles and bias)
   int64_t blocks;                      // grid.x: blocks of 32 slots over all sequences
 };
 hipError_t launch_paged_write(const PagedRowsParams& p, int dtype, bool q8, hipStream_t s);

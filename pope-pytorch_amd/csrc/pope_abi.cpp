@@ -1144,6 +1144,12 @@ int paged_rows(const pope_paged* d, void* k, void* v, const float* freqs, const 
   copy3(p.k_s, d->k_s); copy3(p.v_s, d->v_s);
   p.f_s[0] = d->f_s[0]; p.f_s[1] = d->f_s[1];
   p.bias_sh = d->bias_sh;
+  const auto whole = [&](const void* t, const int64_t* st, int cols) {
+    return cols % 8 == 0 && aligned16(t) && st[0] % 8 == 0 && st[1] % 8 == 0 && st[2] % 8 == 0;
+  };
+  p.k_vec = whole(k, d->k_s, write ? d->D : d->D + d->R);
+  p.v_vec = whole(v, d->v_s, d->D);
+  p.f_vec = d->R % 8 == 0 && aligned16(freqs) && aligned16(bias) && d->f_s[0] % 4 == 0 && d->f_s[1] % 4 == 0 && d->bias_sh % 4 == 0;
   p.blocks = pope::paged_tiles(d->B, d->N, cu != nullptr, 1, pope::kBlockKeys, 2);
   if (p.blocks >= ((int64_t)1 << 31) || d->Hk > 65535) return fail(POPE_ERR_UNSUPPORTED, "%lld blocks of rows x %d heads: too many workgroups", (long long)p.blocks, d->Hk);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
