@@ -827,6 +827,108 @@ std::pair<Tensor, Tensor> paged_attn(const Tensor& q, OptTensor freqs_, const Te
   return {o, lse};
 }
 
+// The eager calls' way in: everything a call has, checked and launched here when it needs no conversion and has nothing
+// wrong; false (nothing) otherwise, and the Python module converts or says what is wrong.  A serving step is a few
+// calls of a few microseconds each: their checks took 8-12 us in Python.
+struct PagedCall {
+  const Tensor &k_pages, &v_pages, &scales, &table, &lengths;
+  Tensor freqs, bias, cu;
+  int64_t page_size, heads, D, R;
+  at::ScalarType dtype;
+  int h, n;   // dims of heads and rows
+
+  PagedCall(const Tensor& kp, const Tensor& vp, const Tensor& sc, const Tensor& tb, const Tensor& ln, OptTensor f, OptTensor b, OptTensor c, int64_t ps,
+            int64_t D_, int64_t R_, bool half, bool head_first)
+      : k_pages(kp), v_pages(vp), scales(sc), table(tb), lengths(ln), freqs(opt(f)), bias(opt(b)), cu(opt(c)), page_size(ps), heads(kp.size(1)), D(D_), R(R_),
+        dtype(half ? at::kHalf : at::kBFloat16), h(head_first ? 1 : 2), n(head_first ? 2 : 1) {}
+
+  int64_t batch() const { return cu.defined() ? 1 : table.size(0); }
+  bool here(const Tensor& t) const { return t.device() == k_pages.device(); }
+  bool tracked(const Tensor& t) const { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
+  bool seqs() const {
+    const auto ints = [&](const Tensor& t, int64_t dim) { return t.scalar_type() == at::kInt && here(t) && t.dim() == dim && t.stride(-1) == 1; };
+    return k_pages.is_cuda() && ints(table, 2) && table.size(0) > 0 && table.size(1) > 0 && ints(lengths, 1) && lengths.size(0) == table.size(0) &&
+           (!cu.defined() || (ints(cu, 1) && cu.size(0) == table.size(0) + 1));
+  }
+  bool rows(const Tensor& t, int64_t want) const {
+    return t.scalar_type() == dtype && here(t) && t.dim() == 4 && t.size(0) == batch() && t.size(3) == D && t.stride(3) == 1 && !tracked(t) &&
+           (want ? t.size(h) == want : t.size(h) > 0 && t.size(h) % heads == 0);
+  }
+  bool angles(int64_t rows, bool need_bias) const {
+    if (!R) return !freqs.defined() && !bias.defined();
+    if (!freqs.defined() || freqs.scalar_type() != at::kFloat || !here(freqs) || freqs.dim() < 2 || freqs.dim() > 3 || freqs.size(-1) != R || freqs.size(-2) != rows ||
+        freqs.stride(-1) != 1 || (freqs.dim() == 3 && freqs.size(0) != 1 && freqs.size(0) != batch()) || tracked(freqs))
+      return false;
+    return !need_bias || (bias.defined() && bias.scalar_type() == at::kFloat && here(bias) && bias.dim() == 2 && bias.size(1) == R && bias.stride(1) == 1 &&
+                          (bias.size(0) == 1 || bias.size(0) == heads) && !tracked(bias));
+  }
+  Paged desc(int64_t rows) const {
+    Paged p(k_pages, v_pages, scales, table, lengths, cu, page_size, D, R, rows, dtype);
+    if (R) {
+      p.d.f_s[0] = freqs.dim() == 3 && freqs.size(0) > 1 ? freqs.stride(0) : 0;
+      p.d.f_s[1] = freqs.stride(-2);
+      if (bias.defined()) p.d.bias_sh = bias.size(0) > 1 ? bias.stride(0) : 0;
+    }
+    return p;
+  }
+  void strides(int64_t* s, const Tensor& t) const { s[0] = t.stride(0), s[1] = t.stride(h), s[2] = t.stride(n); }
+};
+
+bool paged_write_eager(const Tensor& k, const Tensor& v, OptTensor freqs, OptTensor bias, const Tensor& k_pages, const Tensor& v_pages, const Tensor& scales,
+                       const Tensor& table, const Tensor& lengths, OptTensor cu, int64_t page_size, int64_t D, int64_t R, bool half, bool head_first) {
+  const PagedCall c(k_pages, v_pages, scales, table, lengths, freqs, bias, cu, page_size, D, R, half, head_first);
+  if (!c.seqs() || !c.rows(k, c.heads) || !c.rows(v, c.heads) || v.size(c.n) != k.size(c.n) || !c.angles(k.size(c.n), true)) return false;
+  Paged p = c.desc(k.size(c.n));
+  const c10::DeviceGuard guard(k_pages.device());
+  c.strides(p.d.k_s, k);
+  c.strides(p.d.v_s, v);
+  check(pope_paged_write(&p.d, k.data_ptr(), v.data_ptr(), floats(c.freqs), floats(c.bias), p.k, p.v, p.scales, p.table, p.lengths, p.cu, stream_of(k_pages)),
+        "paged write");
+  return true;
+}
+
+std::optional<std::pair<Tensor, Tensor>> paged_read_eager(const Tensor& k_pages, const Tensor& v_pages, const Tensor& scales, const Tensor& table,
+                                                          const Tensor& lengths, OptTensor cu, int64_t rows, int64_t D, int64_t R, int64_t page_size, bool half,
+                                                          bool head_first) {
+  const PagedCall c(k_pages, v_pages, scales, table, lengths, std::nullopt, std::nullopt, cu, page_size, D, R, half, head_first);
+  if (!c.seqs() || rows < 0) return std::nullopt;
+  Paged p(k_pages, v_pages, scales, table, lengths, c.cu, page_size, D, R, rows, c.dtype);
+  const c10::DeviceGuard guard(k_pages.device());
+  const auto make = [&](int64_t cols) {
+    const auto o = k_pages.options().dtype(c.dtype).requires_grad(false);
+    return head_first ? at::empty({c.batch(), c.heads, rows, cols}, o) : at::empty({c.batch(), rows, c.heads, cols}, o);
+  };
+  const Tensor k = make(D + R), v = make(D);
+  c.strides(p.d.k_s, k);
+  c.strides(p.d.v_s, v);
+  check(pope_paged_read(&p.d, p.k, p.v, p.scales, p.table, p.lengths, p.cu, k.data_ptr(), v.data_ptr(), stream_of(k_pages)), "paged read");
+  return std::make_pair(k, v);
+}
+
+std::optional<std::pair<Tensor, Tensor>> paged_attn_eager(const Tensor& q, OptTensor freqs, const Tensor& k_pages, const Tensor& v_pages, const Tensor& scales,
+                                                          const Tensor& table, const Tensor& lengths, OptTensor cu, int64_t page_size, int64_t D, int64_t R, bool half,
+                                                          bool head_first, bool causal, double softmax_scale, bool with_lse) {
+  const PagedCall c(k_pages, v_pages, scales, table, lengths, freqs, std::nullopt, cu, page_size, D, R, half, head_first);
+  if (!c.seqs() || !c.rows(q, 0) || !c.angles(q.size(c.n), false)) return std::nullopt;
+  Paged p = c.desc(q.size(c.n));
+  const c10::DeviceGuard guard(k_pages.device());
+  TORCH_CHECK_VALUE(q.size(c.h) <= INT_MAX, "pope_amd paged cache: too large");
+  p.d.Hq = (int32_t)q.size(c.h);
+  p.d.causal = causal;
+  p.d.softmax_scale = (float)softmax_scale;
+  const Tensor o = at::empty_like(q, q.options().requires_grad(false));
+  Tensor lse;
+  if (with_lse) lse = fp32_like(q, {q.size(0), q.size(c.h), q.size(c.n)});
+  c.strides(p.d.q_s, q);
+  c.strides(p.d.o_s, o);
+  size_t n = 0;
+  check(pope_paged_workspace_bytes(&p.d, p.cu != nullptr, &n), "workspace query");
+  const Tensor ws = bytes_like(q, n);
+  check(pope_paged_attn(&p.d, q.data_ptr(), floats(c.freqs), p.k, p.v, p.scales, p.table, p.lengths, p.cu, o.data_ptr(), static_cast<float*>(data(lse)), data(ws), n,
+                        stream_of(q)), "paged attention");
+  return std::make_pair(o, lse);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_pope_host, m) {
@@ -840,6 +942,9 @@ PYBIND11_MODULE(_pope_host, m) {
   m.def("paged_write", &paged_write, nogil);
   m.def("paged_read", &paged_read, nogil);
   m.def("paged_attn", &paged_attn, nogil);
+  m.def("paged_write_eager", &paged_write_eager, nogil);
+  m.def("paged_read_eager", &paged_read_eager, nogil);
+  m.def("paged_attn_eager", &paged_attn_eager, nogil);
   m.def("untraced", &untraced);
   m.def("last_bwd_prepared", [] { return g_last_bwd_prepared.load(); });
   m.def("abi_version", [] { return POPE_ABI_VERSION; });

@@ -219,6 +219,13 @@ def paged_cache_write(cache: PagedPoPECache, k: Tensor, v: Tensor, pos_emb, page
     ``pos_emb``: (freqs, bias) of the new rows, ``pope(positions)``, or None for a cache without rotated dims.
     ``page_table`` (sequences, pages), ``lengths`` (sequences,) with the new rows counted.  Slots of other tokens are
     not touched.  Two rows must not share a slot."""
+    on_gpu = cache.k_pages.is_cuda
+    freqs, bias = pos_emb if exists(pos_emb) else (None, None)
+    eager = on_gpu and _lib.eager(k, v, freqs, bias, cache.k_pages, page_table, lengths, cu_seqlens)
+    if eager and _lib.host().paged_write_eager(k, v, freqs, bias, cache.k_pages, cache.v_pages, cache.scales, page_table, lengths, cu_seqlens,
+                                               cache.page_size, cache.dim, cache.rotate_dim, cache.dtype == torch.float16, head_dimension_at_first):
+        return
+    # conversions, what is wrong with the call, tracing
     if not head_dimension_at_first:
         k, v = k.transpose(1, 2), v.transpose(1, 2)
     packed = exists(cu_seqlens)
@@ -232,10 +239,10 @@ def paged_cache_write(cache: PagedPoPECache, k: Tensor, v: Tensor, pos_emb, page
     if exists(freqs) and not exists(bias):
         raise ValueError("pos_emb needs its bias: keys are stored with it")
     _no_grad(k, v, freqs, bias)
-    if cache.device.type != "cuda":
+    if not on_gpu:
         return _write_torch(cache, k, v, freqs, bias, page_table, lengths, cu_seqlens)
     args = (k, v, freqs, bias, cache.k_pages, cache.v_pages, cache.scales, page_table, lengths, cu_seqlens, cache.page_size)
-    if _lib.eager(k, v, freqs, bias, cache.k_pages, page_table, lengths, cu_seqlens):
+    if eager:
         _lib.host().paged_write(*args)
     else:
         paged_write_op(*args)
@@ -246,15 +253,21 @@ def paged_cache_read(cache: PagedPoPECache, page_table: Tensor, lengths: Tensor,
     """The last n cached rows of every sequence, (k_hat, v) of (batch, heads, n, dim + rotate_dim) and (.., dim) in the
     cache's dtype; packed: n rows in all, of sequence b its last cu_seqlens[b + 1] - cu_seqlens[b].  k_hat has the
     column order of ``apply_pope_to_qk``.  Rows without a slot are zeros."""
+    on_gpu = cache.k_pages.is_cuda
+    eager = on_gpu and _lib.eager(cache.k_pages, page_table, lengths, cu_seqlens)
+    if eager:
+        r = _lib.host().paged_read_eager(cache.k_pages, cache.v_pages, cache.scales, page_table, lengths, cu_seqlens, n, cache.dim, cache.rotate_dim,
+                                         cache.page_size, cache.dtype == torch.float16, head_dimension_at_first)
+        if exists(r):
+            return r
     page_table, lengths, cu_seqlens = _check_seqs(cache, page_table, lengths, cu_seqlens)
     if n < 0:
         raise ValueError(f"n must not be negative, got {n}")
-    if cache.device.type != "cuda":
+    if not on_gpu:
         k, v = _read_torch(cache, page_table, lengths, cu_seqlens, n)
     else:
         args = (cache.k_pages, cache.v_pages, cache.scales, page_table, lengths, cu_seqlens, n, cache.dim, cache.rotate_dim,
                 cache.page_size, cache.dtype == torch.float16, head_dimension_at_first)
-        eager = _lib.eager(cache.k_pages, page_table, lengths, cu_seqlens)
         k, v = _lib.host().paged_read(*args) if eager else paged_read_op(*args)
     return (k, v) if head_dimension_at_first else (k.transpose(1, 2), v.transpose(1, 2))
 
@@ -266,6 +279,15 @@ def paged_flash_attn_with_pope(q: Tensor, cache: PagedPoPECache, pos_emb, page_t
     (they are written before).  Query head h reads kv head h % heads.  ``causal``: a row sees positions up to its own
     (bottom-right aligned: the last row sees everything), otherwise all of its sequence.  ``pos_emb``: the new rows'
     (freqs, bias); bias is not read.  ``return_lse``: also the scores' log-sum-exp, fp32 (batch, query heads, n)."""
+    on_gpu = cache.k_pages.is_cuda
+    scale = cache.dim ** -0.5 if softmax_scale is None else float(softmax_scale)
+    freqs = pos_emb[0] if exists(pos_emb) else None
+    eager = on_gpu and _lib.eager(q, freqs, cache.k_pages, page_table, lengths, cu_seqlens)
+    if eager:
+        r = _lib.host().paged_attn_eager(q, freqs, cache.k_pages, cache.v_pages, cache.scales, page_table, lengths, cu_seqlens, cache.page_size,
+                                         cache.dim, cache.rotate_dim, cache.dtype == torch.float16, head_dimension_at_first, causal, scale, return_lse)
+        if exists(r):
+            return r if return_lse else r[0]
     if not head_dimension_at_first:
         q = q.transpose(1, 2)
     packed = exists(cu_seqlens)
@@ -275,13 +297,11 @@ def paged_flash_attn_with_pope(q: Tensor, cache: PagedPoPECache, pos_emb, page_t
         raise ValueError(f"{q.shape[1]} query heads must be a multiple of the cache's {cache.heads}")
     freqs, _ = _check_pos_emb(cache, pos_emb, q.shape[0], q.shape[2])
     _no_grad(q, freqs)
-    scale = cache.dim ** -0.5 if softmax_scale is None else float(softmax_scale)
-    if cache.device.type != "cuda":
+    if not on_gpu:
         o, lse = _attend_torch(cache, q, freqs, page_table, lengths, cu_seqlens, causal, scale)
     else:
         args = (q, freqs, cache.k_pages, cache.v_pages, cache.scales, page_table, lengths, cu_seqlens, cache.page_size, bool(causal),
                 scale, bool(return_lse))
-        eager = _lib.eager(q, freqs, cache.k_pages, page_table, lengths, cu_seqlens)
         o, lse = _lib.host().paged_attn(*args) if eager else paged_attn_op(*args)
     if not head_dimension_at_first:
         o = o.transpose(1, 2)
