@@ -42,18 +42,16 @@ struct PagedAttnParams {
   float q_factor, late;
   int64_t q_s[3], o_s[3], f_s[2];
   int q_vec, f_vec, o_vec;             // query rows: whole 16-byte units; angles likewise; output rows: 8-byte units
-  float* part_o; float* part_ml;       // splits > 1: (tile, head, split, row): 16 * tiles floats, and (m, l)
+  float* part_o; float* part_ml;       // splits > 1: (tile, head, row, split): 16 * tiles floats, and (m, l)
 };
-// Rows of a tile for a call with `rows` (query head of a key head, new token) rows per sequence on average.
-struct PagedPlan { int nq, wk; };      // column tiles of 16 rows per wave, waves that share a tile's rows
-PagedPlan paged_plan(int64_t rows, int tiles);
-inline int paged_tile_rows(PagedPlan p) { return 16 * p.nq * (4 / p.wk); }
-hipError_t launch_paged_attn(const PagedAttnParams& p, PagedPlan plan, int dtype, bool q8, hipStream_t s);
+// Rows of a tile: 16 where a sequence has at most as many (query head of a key head, new token) rows on average, else 128.
+constexpr int kPagedFewRows = 16, kPagedManyRows = 128;
+hipError_t launch_paged_attn(const PagedAttnParams& p, bool few, int dtype, bool q8, hipStream_t s);
 
 // One translation unit each (paged_attn_*.hip).
-hipError_t launch_paged_attn_bf16(const PagedAttnParams& p, PagedPlan plan, hipStream_t s);
-hipError_t launch_paged_attn_f16(const PagedAttnParams& p, PagedPlan plan, hipStream_t s);
-hipError_t launch_paged_attn_bf16_8(const PagedAttnParams& p, PagedPlan plan, hipStream_t s);
-hipError_t launch_paged_attn_f16_8(const PagedAttnParams& p, PagedPlan plan, hipStream_t s);
+hipError_t launch_paged_attn_bf16(const PagedAttnParams& p, bool few, hipStream_t s);
+hipError_t launch_paged_attn_f16(const PagedAttnParams& p, bool few, hipStream_t s);
+hipError_t launch_paged_attn_bf16_8(const PagedAttnParams& p, bool few, hipStream_t s);
+hipError_t launch_paged_attn_f16_8(const PagedAttnParams& p, bool few, hipStream_t s);
 
 }  // namespace pope

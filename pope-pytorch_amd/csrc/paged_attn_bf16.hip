@@ -3,8 +3,8 @@
 
 namespace pope {
 
-hipError_t launch_paged_attn_bf16(const PagedAttnParams& p, PagedPlan plan, hipStream_t s) {
-  return run_paged_shape<BF16, false>(p, plan, s);
+hipError_t launch_paged_attn_bf16(const PagedAttnParams& p, bool few, hipStream_t s) {
+  return run_paged_shape<BF16, false>(p, few, s);
 }
 
 }  // namespace pope

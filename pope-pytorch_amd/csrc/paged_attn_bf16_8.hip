@@ -3,8 +3,8 @@
 
 namespace pope {
 
-hipError_t launch_paged_attn_bf16_8(const PagedAttnParams& p, PagedPlan plan, hipStream_t s) {
-  return run_paged_shape<BF16, true>(p, plan, s);
+hipError_t launch_paged_attn_bf16_8(const PagedAttnParams& p, bool few, hipStream_t s) {
+  return run_paged_shape<BF16, true>(p, few, s);
 }
 
 }  // namespace pope

@@ -1,7 +1,7 @@
 // Attention over the paged cache for many rows (gfx950): chunks and whole prompts.
 //
-// One workgroup = 4 waves = 128 rows of one key head, 32 per wave; two workgroups per CU (registers and half of the LDS),
-// each with its own barriers: what one does between its products runs under the other's.  (One workgroup of 8 waves,
+// One workgroup = 4 waves = 128 rows of one key head, 32 per wave; two workgroups per CU (registers and half of the LDS; one
+// where values are wider than 128 columns), each with its own barriers: what one does between its products runs under the other's.  (One workgroup of 8 waves,
 // two groups of 4 that took turns with the key blocks: 4,096-token prompts, 2 x 8 heads, D 64, R 32, @A us against @B.)
 //
 // Blocks of K and V go to LDS as they lie in the pages (direct loads, no registers), into a ring of three to eight
@@ -29,20 +29,20 @@ struct PagedRows {
   static constexpr int kBlock = kKB + kVB;
   static constexpr int kRegs = KS * 16 + VT * 8;                     // of Q_hat (two parts) and O
   static constexpr bool kPipe = kRegs + 40 <= 170;                   // scores of two steps at once
-  static constexpr int BG = 2 * kBlock * 3 <= 79 * 1024 && kRegs + (kPipe ? 64 : 32) <= 150 ? 2 : 1;   // blocks per step
+  static constexpr int BG = 2 * kBlock * 3 <= 79 * 1024 && VT <= 8 && kRegs + (kPipe ? 64 : 32) <= 150 ? 2 : 1;   // blocks per step
   static constexpr int kStage = BG * (kBlock + (Q8 ? 64 : 0));    // 8-bit: the blocks' exponents behind them
-  static constexpr int kFit = (80 * 1024 - 128) / kStage, kSlots = kFit < 8 ? kFit : 8;
+  static constexpr int kLds = (VT <= 8 ? 80 : 160) * 1024, kFit = (kLds - 128) / kStage, kSlots = kFit < 8 ? kFit : 8;
   static constexpr int QST = KS * 32 + 8;
   // rows of Q_hat made at a time
   static constexpr int kQRows = 128 * QST * 4 <= kStage ? 128 : 64 * QST * 4 <= kStage ? 64 : 32;
   static constexpr int kBytes = kSlots * kStage;
   // stages that load while Q_hat is made behind them
   static constexpr int kEarly = (kBytes - kQRows * QST * 4) / kStage < kSlots - 1 ? (kBytes - kQRows * QST * 4) / kStage : kSlots - 1;
-  static_assert(kSlots >= 3 && kEarly >= 1 && kBytes + 128 <= 80 * 1024, "LDS of two workgroups");
+  static_assert(kSlots >= 3 && kEarly >= 1 && kBytes + 128 <= kLds, "LDS");
 };
 
 template <typename T, bool Q8, int KS, int VT>
-__global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedAttnParams p) {
+__global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_rows_kernel(PagedAttnParams p) {
   using C = PagedRows<Q8, KS, VT>;
   typedef typename T::vec8 vec8;
   constexpr int BG = C::BG, NDB = VT / 2, K16 = 2 * KS, kRows = C::kRows;
@@ -405,6 +405,36 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedAttnParams p) {
     if (st + C::kSlots - 1 < steps) issue(st + C::kSlots - 1, put);
     put = next_slot(put);
   };
+  if (wave * 32 >= count) {   // a wave without rows: the others' loads and barriers
+    int at = 0;
+    if constexpr (C::kPipe) {
+      if (steps > 0) {
+        wait_vmcnt<0>();
+        __syncthreads();
+        if (tile_edge(0)) sanitize(0, 0);
+        for (int st = 0; st + 1 < steps; ++st) {
+          landed(st + 1);
+          __syncthreads();
+          refill(st);
+          at = next_slot(at);
+          if (tile_edge(st + 1)) sanitize(st + 1, at);
+        }
+        __syncthreads();
+      }
+    } else {
+      for (int st = 0; st < steps; ++st) {
+        landed(st);
+        __syncthreads();
+        refill(st);
+        if (tile_edge(st)) {
+          sanitize(st, at);
+          __syncthreads();
+        }
+        at = next_slot(at);
+      }
+    }
+    return;
+  }
   f32x16 sa[BG], sb[C::kPipe ? BG : 1];
   u32x4 pw[BG][2];
   int slot = 0;   // stage of the current step
@@ -459,8 +489,8 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedAttnParams p) {
       slot = ahead;
     };
     auto last = [&](int st, f32x16* cur) {
-      rescale(mx, cur);
       __syncthreads();   // the values of stage st are clean
+      rescale(mx, cur);
       probs(slot, cur, pw);
       products(slot, pw, nothing);
       if (tile_edge(st)) {
@@ -512,7 +542,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedAttnParams p) {
   if (!set) m = -INFINITY;
   const bool part = paged_parts(blocks, p.splits, p.least, 1) > 1;
   const float f = part ? 1.f : l == 0.f ? 0.f : 1.f / l;
-  const int64_t row = part ? (((int64_t)job.tile * c.Hk + hk) * p.splits + job.split) * kRows + wave * 32 + lr : 0;
+  const int64_t row = part ? (((int64_t)job.tile * c.Hk + hk) * kRows + x) * p.splits + job.split : 0;
   uint16_t* dst = p.o + (int64_t)g.batch * p.o_s[0] + (int64_t)row_h * p.o_s[1] + (int64_t)(g.row0 + row_i) * p.o_s[2];
 #pragma unroll
   for (int d = 0; d < NDB; ++d)

@@ -1085,14 +1085,15 @@ pope::PagedCache paged_cache(const pope_paged& d, const void* k, const void* v, 
   return c;
 }
 
-// Splits of the key axis.  A tile's blocks of keys go to as many workgroups as they have parts of `least` blocks (at most
-// `splits`, the grid's); tiles of one part write their output themselves.
-//   few rows   parts of 16 blocks (512 keys) while they bring the grid to kPagedGrid workgroups
+// Parts of the key axis.  A tile's blocks of keys go to as many workgroups as they have parts (at most `splits`, the
+// grid's) of at least `least` blocks; tiles of one part write their output themselves, the others a second launch joins.
+//   few rows   as many parts as bring the grid to kPagedGrid workgroups, of 16 blocks (512 keys) or more, and of at most
+//              kPagedPart blocks: sequences differ in length, and what the longest parts leave to do alone is lost
 //   many rows  the chip holds kPagedSlots workgroups; a part is at most the blocks one of these places gets
-constexpr int kPagedGrid = 1024, kPagedSlots = 512;
+constexpr int kPagedGrid = 1024, kPagedSlots = 512, kPagedPart = 64;
 
 struct PagedShape {
-  pope::PagedPlan plan;
+  bool few;       // tiles of 16 rows, else of 128
   int64_t tiles;
   int splits, least;
   size_t part_o, bytes;
@@ -1102,14 +1103,14 @@ PagedShape paged_shape(const pope_paged& d, bool packed) {
   PagedShape s;
   const int G = d.Hq / d.Hk, vt = pope::paged_v_tiles(d.D);
   const int64_t avg = packed ? ((int64_t)d.N + d.B - 1) / d.B : d.N;
-  s.plan = pope::paged_plan(avg * G, vt);
-  const int rows = pope::paged_tile_rows(s.plan);
+  s.few = avg * G <= pope::kPagedFewRows;
+  const int rows = s.few ? pope::kPagedFewRows : pope::kPagedManyRows;
   s.tiles = pope::paged_tiles(d.B, d.N, packed, G, rows, 1);
   const int64_t wgs = std::max<int64_t>(s.tiles * d.Hk, 1);
   const int64_t blocks = (int64_t)d.table_cols * d.page_size / pope::kBlockKeys;
-  if (s.plan.wk == 4) {
+  if (s.few) {
     s.least = 16;
-    s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kPagedGrid / wgs, blocks / s.least));
+    s.splits = (int)std::max<int64_t>({(int64_t)1, std::min<int64_t>(kPagedGrid / wgs, blocks / s.least), (blocks + kPagedPart - 1) / kPagedPart});
   } else {
     s.least = (int)std::max<int64_t>(16, std::min<int64_t>(blocks, wgs * blocks / kPagedSlots));
     s.splits = (int)((blocks + s.least - 1) / s.least);
@@ -1228,7 +1229,7 @@ int pope_paged_attn(const pope_paged* d, const void* q, const float* freqs, cons
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + sh.part_o);
   if ((int64_t)d->N * (d->Hq / d->Hk) > ((int64_t)1 << 30) || sh.tiles * d->Hk * sh.splits >= ((int64_t)1 << 31)) return fail(POPE_ERR_UNSUPPORTED, "%lld row tiles x %d heads: too many workgroups", (long long)sh.tiles, d->Hk);
-  const hipError_t e = pope::launch_paged_attn(p, sh.plan, d->dtype, d->quantized != 0, reinterpret_cast<hipStream_t>(stream));
+  const hipError_t e = pope::launch_paged_attn(p, sh.few, d->dtype, d->quantized != 0, reinterpret_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "paged attention launch");
   return POPE_OK;
 }
