@@ -123,14 +123,16 @@ __global__ __launch_bounds__(kThreads) void paged_write_kernel(PagedRowsParams p
   const int D = c.D, R = c.R, KE = c.steps * 32;
   const bool whole = R % 8 == 0;
 
+  // A thread's chunks: four side by side in a row, 32 rows, then the next four: a wave's are all rotated or mostly not, and a
+  // chunk's sine, cosine and softplus are most of the work (rows' chunks side by side: both branches in every wave).
   u32x4 kin[kTurns], vin[kTurns];
   f32x4 fin[kTurns][2], bin[kTurns][2];
 #pragma unroll
   for (int u = 0; u < kTurns; ++u) {
-    const int it = tid + u * kThreads, t = it / (2 * VT), d0 = it % (2 * VT) * 8;   // a row's chunks side by side
+    const int t = (tid >> 2) % kBlockKeys, d0 = ((tid & 3) + 4 * (tid / 128 + 2 * u)) * 8;
     kin[u] = vin[u] = u32x4{0, 0, 0, 0};
     fin[u][0] = fin[u][1] = bin[u][0] = bin[u][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (t >= kBlockKeys || !live(t) || d0 >= D) continue;
+    if (!live(t) || d0 >= D) continue;
     const int64_t n = b.seg.row0 + b.i0 + t;
     kin[u] = load_row8(static_cast<const uint16_t*>(p.k) + b.seg.batch * p.k_s[0] + hk * p.k_s[1] + n * p.k_s[2], d0, D, p.k_vec);
     vin[u] = load_row8(static_cast<const uint16_t*>(p.v) + b.seg.batch * p.v_s[0] + hk * p.v_s[1] + n * p.v_s[2], d0, D, p.v_vec);
@@ -163,7 +165,7 @@ __global__ __launch_bounds__(kThreads) void paged_write_kernel(PagedRowsParams p
   float ka[kTurns][8], kb[kTurns][8];   // cosine part or raw value, sine part
 #pragma unroll
   for (int u = 0; u < kTurns; ++u) {
-    const int it = tid + u * kThreads, t = it / (2 * VT), d0 = it % (2 * VT) * 8;   // a row's chunks side by side
+    const int t = (tid >> 2) % kBlockKeys, d0 = ((tid & 3) + 4 * (tid / 128 + 2 * u)) * 8;
     unpack8<T>(kin[u], ka[u]);
     if (d0 < R) {
 #pragma unroll
@@ -176,7 +178,7 @@ __global__ __launch_bounds__(kThreads) void paged_write_kernel(PagedRowsParams p
         ka[u][k] = rot ? m * cs : ka[u][k];
       }
     }
-    if (Q8 && t < kBlockKeys && live(t) && d0 < D) {
+    if (Q8 && live(t) && d0 < D) {
       float mk = 0.f, mv = 0.f, v[8];
       unpack8<T>(vin[u], v);
 #pragma unroll
@@ -199,8 +201,8 @@ __global__ __launch_bounds__(kThreads) void paged_write_kernel(PagedRowsParams p
   }
 #pragma unroll
   for (int u = 0; u < kTurns; ++u) {
-    const int it = tid + u * kThreads, t = it / (2 * VT), d0 = it % (2 * VT) * 8;   // a row's chunks side by side
-    if (t >= kBlockKeys || d0 >= D) continue;
+    const int t = (tid >> 2) % kBlockKeys, d0 = ((tid & 3) + 4 * (tid / 128 + 2 * u)) * 8;
+    if (d0 >= D) continue;
     float v[8];
     unpack8<T>(vin[u], v);
     // eight columns from e on, whole or one by one
@@ -301,8 +303,8 @@ __device__ __forceinline__ uint16_t value_bits(float x) {
 
 template <typename T, bool Q8, int VT>
 __global__ __launch_bounds__(kThreads) void paged_read_kernel(PagedRowsParams p) {
-  constexpr int ST = VT * 32 + 2;
-  __shared__ uint16_t rows[kBlockKeys * ST];
+  constexpr int ST = VT * 32 + 8;   // an odd number of 16-byte units
+  __shared__ __attribute__((aligned(16))) uint16_t rows[kBlockKeys * ST];
   const PagedCache& c = p.c;
   const int hk = blockIdx.y, lane = threadIdx.x & 63, wave = wave_id();
   const Block b = find_block(c, blockIdx.x);
@@ -327,12 +329,12 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(PagedRowsParams p)
             const u32x2 w = *reinterpret_cast<const u32x2*>(src + u * 8);
             const int e = scale(t, 0);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) rows[t * ST + e0 + j] = value_bits<T>(__builtin_amdgcn_ldexpf(code_at(w, j), e));
+            for (int j = 0; j < 8; j += 2)
+              *reinterpret_cast<uint32_t*>(rows + t * ST + e0 + j) = value_bits<T>(__builtin_amdgcn_ldexpf(code_at(w, j), e)) |
+                                                                    (uint32_t)value_bits<T>(__builtin_amdgcn_ldexpf(code_at(w, j + 1), e)) << 16;
           } else {
             const int ln = u & 63, half = (u >> 6) & 1, st = u >> 7, t = half * 16 + (ln & 15), e0 = st * 32 + 8 * (ln >> 4);
-            const u32x4 w = *reinterpret_cast<const u32x4*>(src + u * 16);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) *reinterpret_cast<uint32_t*>(rows + t * ST + e0 + 2 * j) = w[j];
+            *reinterpret_cast<u32x4*>(rows + t * ST + e0) = *reinterpret_cast<const u32x4*>(src + u * 16);
           }
         }
       } else {
@@ -356,18 +358,37 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(PagedRowsParams p)
       }
     }
     __syncthreads();
-    for (int t = wave; t < kBlockKeys; t += kThreads / 64) {
-      if (!live(t)) continue;
-      const int64_t n = b.seg.row0 + b.i0 + t;
-      if (!which) {
-        uint16_t* dst = static_cast<uint16_t*>(p.k) + b.seg.batch * p.k_s[0] + hk * p.k_s[1] + n * p.k_s[2];
-        for (int x = lane; x < E; x += 64) {
-          const int e = x >= 2 * R ? x : (x & 1) * R + (x >> 1);
+    const int cols = which ? D : E;
+    if (which ? p.v_vec : p.k_vec && R % 4 == 0) {   // 16 bytes at a time: eight columns, or four (cos, sin) pairs
+      for (int u = threadIdx.x; u < kBlockKeys * (VT * (which ? 2 : 4)); u += kThreads) {
+        const int t = u / (VT * (which ? 2 : 4)), x = u % (VT * (which ? 2 : 4)) * 8;
+        if (!live(t) || x >= cols) continue;
+        const int64_t n = b.seg.row0 + b.i0 + t;
+        const uint16_t* row = rows + t * ST;
+        u32x4 w = {0, 0, 0, 0};
+        if (b.page >= 0) {
+          if (which || x >= 2 * R) {
+            w = *reinterpret_cast<const u32x4*>(row + x);
+          } else {
+            const u32x2 cs = *reinterpret_cast<const u32x2*>(row + x / 2), sn = *reinterpret_cast<const u32x2*>(row + R + x / 2);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = ((cs[k >> 1] >> (16 * (k & 1))) & 0xffffu) | (sn[k >> 1] >> (16 * (k & 1))) << 16;
+          }
+        }
+        uint16_t* dst = which ? static_cast<uint16_t*>(p.v) + b.seg.batch * p.v_s[0] + hk * p.v_s[1] + n * p.v_s[2]
+                              : static_cast<uint16_t*>(p.k) + b.seg.batch * p.k_s[0] + hk * p.k_s[1] + n * p.k_s[2];
+        *reinterpret_cast<u32x4*>(dst + x) = w;
+      }
+    } else {
+      for (int t = wave; t < kBlockKeys; t += kThreads / 64) {
+        if (!live(t)) continue;
+        const int64_t n = b.seg.row0 + b.i0 + t;
+        uint16_t* dst = which ? static_cast<uint16_t*>(p.v) + b.seg.batch * p.v_s[0] + hk * p.v_s[1] + n * p.v_s[2]
+                              : static_cast<uint16_t*>(p.k) + b.seg.batch * p.k_s[0] + hk * p.k_s[1] + n * p.k_s[2];
+        for (int x = lane; x < cols; x += 64) {
+          const int e = which || x >= 2 * R ? x : (x & 1) * R + (x >> 1);
           dst[x] = b.page >= 0 ? rows[t * ST + e] : (uint16_t)0;
         }
-      } else {
-        uint16_t* dst = static_cast<uint16_t*>(p.v) + b.seg.batch * p.v_s[0] + hk * p.v_s[1] + n * p.v_s[2];
-        for (int x = lane; x < D; x += 64) dst[x] = b.page >= 0 ? rows[t * ST + x] : (uint16_t)0;
       }
     }
   }
