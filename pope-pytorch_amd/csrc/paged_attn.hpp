@@ -37,6 +37,7 @@ template <typename T, bool Q8, int KS, int VT>
 __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_few_kernel(PagedAttnParams p) {
   using C = PagedFew<KS, VT>;
   typedef typename T::vec8 vec8;
+  typedef std::conditional_t<Q8, BF16, T> V;   // the second product's: P x 2^e leaves fp16's range where values are far from 1
   constexpr int kRows = C::kRows, WK = C::kWaves, QST = C::QST;
   __shared__ __attribute__((aligned(16))) char smem[C::kBytes];
   const PagedCache& c = p.c;
@@ -206,19 +207,19 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_few_kernel(PagedAt
     u32x4 ph, pl;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      ph[i] = T::pack2(pr[2 * i], pr[2 * i + 1]);
-      pl[i] = T::pack2(pr[2 * i] - T::to_float((uint16_t)ph[i]), pr[2 * i + 1] - T::to_float((uint16_t)(ph[i] >> 16)));
+      ph[i] = V::pack2(pr[2 * i], pr[2 * i + 1]);
+      pl[i] = V::pack2(pr[2 * i] - V::to_float((uint16_t)ph[i]), pr[2 * i + 1] - V::to_float((uint16_t)(ph[i] >> 16)));
     }
 
     // O^T += V^T P^T
 #pragma unroll
     for (int v = 0; v < VT; ++v) {
-      vec8 a;
-      if constexpr (Q8) a = as_vec8<vec8>(unpack_e4m3<T>(u32x2{vf[v >> 1][2 * (v & 1)], vf[v >> 1][2 * (v & 1) + 1]}, 1.f));
-      else a = as_vec8<vec8>(vf[v]);
+      typename V::vec8 a;
+      if constexpr (Q8) a = as_vec8<typename V::vec8>(unpack_e4m3<V>(u32x2{vf[v >> 1][2 * (v & 1)], vf[v >> 1][2 * (v & 1) + 1]}, 1.f));
+      else a = as_vec8<typename V::vec8>(vf[v]);
       acc[v] *= alpha;
-      acc[v] = T::mfma16(a, as_vec8<vec8>(ph), acc[v]);
-      acc[v] = T::mfma16(a, as_vec8<vec8>(pl), acc[v]);
+      acc[v] = V::mfma16(a, as_vec8<typename V::vec8>(ph), acc[v]);
+      acc[v] = V::mfma16(a, as_vec8<typename V::vec8>(pl), acc[v]);
     }
     load_v(next_page, next);
     if (edge && __any(odd != 0)) {

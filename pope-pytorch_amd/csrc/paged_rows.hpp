@@ -45,6 +45,11 @@ template <typename T, bool Q8, int KS, int VT>
 __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_rows_kernel(PagedAttnParams p) {
   using C = PagedRows<Q8, KS, VT>;
   typedef typename T::vec8 vec8;
+  // The second product's type: P x 2^e (8-bit values' scales) leaves fp16's range where values are far from 1.  fp16 outputs
+  // then take P as two bf16 parts.
+  typedef std::conditional_t<Q8, BF16, T> V;
+  typedef typename V::vec8 vvec8;
+  constexpr int kParts = Q8 && T::kCode == 1 ? 2 : 1;
   constexpr int BG = C::BG, NDB = VT / 2, K16 = 2 * KS, kRows = C::kRows;
   __shared__ __attribute__((aligned(16))) char smem[C::kBytes];
   // Per (step % 8, block of the step): keys of values that are not finite.  Never cleared: add_seen looks at the value again.
@@ -154,6 +159,10 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_rows_kernel(PagedA
     if constexpr (Q8) return as_vec8<vec8>(unpack_e4m3<T>(w, unit));
     else return as_vec8<vec8>(w);
   };
+  auto v_operand = [&](Raw w) -> vvec8 {
+    if constexpr (Q8) return as_vec8<vvec8>(unpack_e4m3<V>(w, 1.f));
+    else return as_vec8<vvec8>(w);
+  };
   auto power = [](uint32_t w, int i) { return __uint_as_float(((w >> (8 * i)) & 0xffu) << 23); };   // 2^(byte i - 127)
   // S of a step.  8-bit: bf16 holds code x 2^e, so the scale goes into the unpacking; fp16 does not, the scores take it.
   constexpr bool kUnpackScale = Q8 && T::kCode == 2, kLate = T::kCode == 1;
@@ -247,7 +256,7 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_rows_kernel(PagedA
     }
   };
   // Unit u of BG x 8: two probabilities, their share of the sum, packed (8-bit: times the values' scales).
-  auto prob = [&](int slot, f32x16* s, u32x4 (*pw)[2], int u) {
+  auto prob = [&](int slot, f32x16* s, u32x4 (*pw)[2 * kParts], int u) {
     const int b = u / 8, q = u % 8;
     float x[2];
 #pragma unroll
@@ -260,16 +269,20 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_rows_kernel(PagedA
 #pragma unroll
       for (int k = 0; k < 2; ++k) x[k] *= power(w, 2 * (q & 1) + k);
     }
-    pw[b][q >> 2][q & 3] = T::pack2(x[0], x[1]);
+    pw[b][q >> 2][q & 3] = V::pack2(x[0], x[1]);
+    if constexpr (kParts == 2) {
+      const uint32_t w = pw[b][q >> 2][q & 3];
+      pw[b][2 + (q >> 2)][q & 3] = V::pack2(x[0] - V::to_float((uint16_t)w), x[1] - V::to_float((uint16_t)(w >> 16)));
+    }
     if constexpr (C::kPipe) asm volatile("" : "+v"(pw[b][q >> 2][q & 3]), "+v"(l));   // stays between its fences
     s[b][2 * q] = x[0];
     s[b][2 * q + 1] = x[1];
   };
-  auto probs = [&](int slot, f32x16* s, u32x4 (*pw)[2]) {
+  auto probs = [&](int slot, f32x16* s, u32x4 (*pw)[2 * kParts]) {
 #pragma unroll
     for (int u = 0; u < 8 * BG; ++u) prob(slot, s, pw, u);
   };
-  auto products = [&](int slot, const u32x4 (*pw)[2], auto&& between) {
+  auto products = [&](int slot, const u32x4 (*pw)[2 * kParts], auto&& between) {
     const char* stage = stage_of(slot);
     constexpr int n = BG * 2 * NDB, ahead = n < 4 ? n : 4;
     Raw w[n];
@@ -279,7 +292,9 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_rows_kernel(PagedA
 #pragma unroll
     for (int i = 0; i < n; ++i) {
       const int b = i / (2 * NDB), h = i / NDB % 2, d = i % NDB;
-      acc[d] = T::mfma32(operand(w[i], 1.f), as_vec8<vec8>(pw[b][h]), acc[d]);
+      const vvec8 a = v_operand(w[i]);
+      acc[d] = V::mfma32(a, as_vec8<vvec8>(pw[b][h]), acc[d]);
+      if constexpr (kParts == 2) acc[d] = V::mfma32(a, as_vec8<vvec8>(pw[b][2 + h]), acc[d]);
       if (i + ahead < n) w[i + ahead] = v_read(stage, (i + ahead) / (2 * NDB), (i + ahead) % NDB, (i + ahead) / NDB % 2);
       between(i, n);
       __builtin_amdgcn_sched_barrier(0);
@@ -436,7 +451,7 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_rows_kernel(PagedA
     return;
   }
   f32x16 sa[BG], sb[C::kPipe ? BG : 1];
-  u32x4 pw[BG][2];
+  u32x4 pw[BG][2 * kParts];
   int slot = 0;   // stage of the current step
   if constexpr (C::kPipe) {
     float mx = -INFINITY;

@@ -1088,9 +1088,10 @@ pope::PagedCache paged_cache(const pope_paged& d, const void* k, const void* v, 
 // Parts of the key axis.  A tile's blocks of keys go to as many workgroups as they have parts (at most `splits`, the
 // grid's) of at least `least` blocks; tiles of one part write their output themselves, the others a second launch joins.
 //   few rows   as many parts as bring the grid to kPagedGrid workgroups, of 16 blocks (512 keys) or more, and of at most
-//              kPagedPart blocks: sequences differ in length, and what the longest parts leave to do alone is lost
+//              kPagedPart blocks (sequences differ in length, and what the longest parts leave to do alone is lost)
+//              within kPagedMost workgroups, which bounds the workspace of wide page tables
 //   many rows  the chip holds kPagedSlots workgroups; a part is at most the blocks one of these places gets
-constexpr int kPagedGrid = 1024, kPagedSlots = 512, kPagedPart = 64;
+constexpr int kPagedGrid = 1024, kPagedSlots = 512, kPagedPart = 64, kPagedMost = 8192;
 
 struct PagedShape {
   bool few;       // tiles of 16 rows, else of 128
@@ -1110,7 +1111,8 @@ PagedShape paged_shape(const pope_paged& d, bool packed) {
   const int64_t blocks = (int64_t)d.table_cols * d.page_size / pope::kBlockKeys;
   if (s.few) {
     s.least = 16;
-    s.splits = (int)std::max<int64_t>({(int64_t)1, std::min<int64_t>(kPagedGrid / wgs, blocks / s.least), (blocks + kPagedPart - 1) / kPagedPart});
+    const int64_t want = std::max(std::min<int64_t>(kPagedGrid / wgs, blocks / s.least), (blocks + kPagedPart - 1) / kPagedPart);
+    s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, kPagedMost / wgs));
   } else {
     s.least = (int)std::max<int64_t>(16, std::min<int64_t>(blocks, wgs * blocks / kPagedSlots));
     s.splits = (int)((blocks + s.least - 1) / s.least);

@@ -43,6 +43,11 @@ def exists(v):
     return v is not None
 
 
+def _unit(t: Tensor) -> Tensor:
+    """The tensor with unit stride in its last dim (contiguous() keeps odd strides of extents of 1)."""
+    return t if t.stride(-1) == 1 else t.clone(memory_format=torch.contiguous_format)
+
+
 def _v_tiles(D: int) -> int:
     """Value columns held, in tiles of 16: 32, 64, 96, 128 or 256."""
     return next(t for t, most in ((2, 32), (4, 64), (6, 96), (8, 128), (16, 256)) if D <= most)
@@ -115,8 +120,7 @@ def _check_seqs(cache: PagedPoPECache, page_table: Tensor, lengths: Tensor, cu_s
             if t.dtype != torch.int32:
                 # out of range is no slot, never another one: what int32 cannot hold stays out of range
                 t = t.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
-            if t.stride(-1) != 1:
-                t = t.contiguous()
+            t = _unit(t)
         out.append(t)
     return out
 
@@ -132,7 +136,7 @@ def _check_rows(cache: PagedPoPECache, t: Tensor, name: str, B: int, heads: Opti
         raise ValueError(f"{name} {tuple(t.shape)} must have batch {1 if packed else B}" + (" (cu_seqlens: packed rows)" if packed else ""))
     if t.shape[3] != cache.dim or (heads is not None and t.shape[1] != heads):
         raise ValueError(f"{name} {tuple(t.shape)} (batch, heads, n, dim) does not fit a cache of {cache.heads} heads of dim {cache.dim}")
-    return t if t.stride(-1) == 1 else t.contiguous()
+    return _unit(t)
 
 
 def _check_pos_emb(cache: PagedPoPECache, pos_emb, batch: int, n: int):
@@ -159,8 +163,7 @@ def _check_pos_emb(cache: PagedPoPECache, pos_emb, batch: int, n: int):
         if exists(t):
             if t.device != cache.device:
                 raise RuntimeError(f"pope_amd paged cache: {name} on {t.device}, the cache on {cache.device}")
-            t = t.float()
-            t = t if t.stride(-1) == 1 else t.contiguous()
+            t = _unit(t.float())
         out.append(t)
     return out
 

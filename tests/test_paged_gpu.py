@@ -269,6 +269,29 @@ def test_softmax_scales(cuda, scale):
         attend_and_check(B, [3, 3], packed=False, scale=scale)
 
 
+@pytest.mark.parametrize("size", [1e-6, 1e-3, 60.0, 2e4])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("q8", [False, True], ids=["16bit", "8bit"])
+def test_values_far_from_one(cuda, size, dtype, q8):
+    """Tiny and large values: the second product's operands carry the 8-bit values' scales.  Keys are small, so that every
+    key counts."""
+    B = Batch([700, 64], heads=2, dtype=dtype, q8=q8)
+    B.k, B.v = B.k * 0.25, (B.v.float() * size).clamp(-65000, 65000).to(dtype)
+    paged_cache_write(B.cache, B.k, B.v, B.emb(B.pos), B.table, B.lengths, cu_seqlens=B.cu)
+    for new in ([1, 1], [64, 64]):
+        q = B.rand(1, 2, sum(new), 64)
+        cu = torch.tensor([0, new[0], sum(new)], dtype=I32, device="cuda")
+        pos = torch.cat([torch.arange(t - n, t, device="cuda") for t, n in zip(B.total, new)])
+        o = paged_flash_attn_with_pope(q, B.cache, B.emb(pos), B.table, B.lengths, cu_seqlens=cu)
+        for b in range(2):
+            s = slice(int(cu[b]), int(cu[b + 1]))
+            k, v = B.rows(b)
+            want, _, tol, _ = reference(q[0, :, s], angles(pos[s], 32), k, v, 32, 0.125, True, dtype)
+            # the reference's absolute term is for values of about 1; outputs below fp16's normal range have its spacing
+            tol = tol - 2.0 ** -25 + (2.0 ** -25 if dtype == torch.float16 else 0.0)
+            assert ((o[0, :, s].double() - want).abs() <= tol).all()
+
+
 def test_layouts_and_strides(cuda):
     """Views with any strides and odd offsets, broadcast angles and one bias row, int64 tables: the same bits."""
     B = Batch([90, 90], heads=2, G=2, D=40, R=20)
@@ -531,6 +554,22 @@ def test_ops_trace(cuda):
     paged_cache_write(c, B.k, B.v, B.emb(B.pos), B.table, B.lengths, cu_seqlens=B.cu)
     got = torch.compile(step, backend="aot_eager", fullgraph=True)(q, k, v, freqs, bias, B.table, B.lengths)
     assert torch.equal(got, want) and torch.equal(c.k_pages, pages)
+
+
+def test_extents_of_one(cuda):
+    """Dims of extent 1 may have any stride: one page, one sequence, one column, one rotated dim."""
+    c = PagedPoPECache(2, heads=1, dim=1, rotate_dim=1, page_size=32, device="cuda")
+    odd = lambda t: t.as_strided(t.shape, [7 if n == 1 else s for n, s in zip(t.shape, t.stride())])
+    table, lens = torch.ones(1, 1, dtype=I32, device="cuda"), torch.full((1,), 3, dtype=I32, device="cuda")
+    k = torch.randn(1, 1, 3, 1, device="cuda").bfloat16()
+    emb = (torch.rand(3, 1, device="cuda"), torch.zeros(1, 1, device="cuda"))
+    paged_cache_write(c, k, k, emb, table, lens)
+    want = paged_flash_attn_with_pope(k, c, emb, table, lens), *paged_cache_read(c, table, lens, 3)
+    c.k_pages.zero_(), c.v_pages.zero_()
+    emb = tuple(odd(t) for t in emb)
+    paged_cache_write(c, odd(k), odd(k), emb, odd(table), odd(lens))
+    got = paged_flash_attn_with_pope(odd(k), c, emb, odd(table), odd(lens)), *paged_cache_read(c, odd(table), odd(lens), 3)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and got[1].any()
 
 
 def test_refusals_on_the_gpu(cuda):
