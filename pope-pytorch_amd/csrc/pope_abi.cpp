@@ -1090,7 +1090,8 @@ pope::PagedCache paged_cache(const pope_paged& d, const void* k, const void* v, 
 //   few rows   as many parts as bring the grid to kPagedGrid workgroups, of 16 blocks (512 keys) or more, and of at most
 //              kPagedPart blocks (sequences differ in length, and what the longest parts leave to do alone is lost)
 //              within kPagedMost workgroups, which bounds the workspace of wide page tables
-//   many rows  the chip holds kPagedSlots workgroups; a part is at most the blocks one of these places gets
+//   many rows  the chip holds kPagedSlots workgroups (half where values are wider than 128 columns); a part is at most the
+//              blocks that one of these places gets
 constexpr int kPagedGrid = 1024, kPagedSlots = 512, kPagedPart = 64, kPagedMost = 8192;
 
 struct PagedShape {
@@ -1114,7 +1115,7 @@ PagedShape paged_shape(const pope_paged& d, bool packed) {
     const int64_t want = std::max(std::min<int64_t>(kPagedGrid / wgs, blocks / s.least), (blocks + kPagedPart - 1) / kPagedPart);
     s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, kPagedMost / wgs));
   } else {
-    s.least = (int)std::max<int64_t>(16, std::min<int64_t>(blocks, wgs * blocks / kPagedSlots));
+    s.least = (int)std::max<int64_t>(16, std::min<int64_t>(blocks, wgs * blocks / (vt <= 8 ? kPagedSlots : kPagedSlots / 2)));
     s.splits = (int)((blocks + s.least - 1) / s.least);
   }
   s.part_o = s.bytes = 0;
