@@ -315,46 +315,50 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p, int 
   if ((int)blockIdx.y * RPW >= count) return;
   const int parts = paged_parts(paged_tile_blocks(g, t.local, rows, p.G, p.causal != 0), p.splits, p.least, step);
   if (parts <= 1) return;   // written by the one that had it
-  const int d = tid % kQuads * 4, rr = blockIdx.y * RPW + tid / kQuads % RPW, group = tid / (kQuads * RPW);
-  const bool on = group < kGroups && rr < count && d < c.D;
-  float m = -INFINITY, l = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  // a part whose scores are all NaN has m = -inf, as one without a visible key, but l = NaN, and its row becomes NaN
-  auto fold = [&](float2 ml, f32x4 x) {
-    const float mn = fmaxf(m, ml.x), mu = mn == -INFINITY ? 0.f : mn;
-    const float a = __builtin_amdgcn_exp2f(m - mu), b = __builtin_amdgcn_exp2f(ml.x - mu);
-    m = mn;
-    l = l * a + ml.y * b;
-    o = o * a + x * b;
-  };
-  if (on) {
-    const int64_t first = (((int64_t)tile * c.Hk + hk) * rows + rr) * p.splits;
+  const int d = tid % kQuads * 4, group = tid / (kQuads * RPW);
+  for (int r0 = blockIdx.y * RPW; r0 < count; r0 += gridDim.y * RPW) {
+    const int rr = r0 + tid / kQuads % RPW;
+    const bool on = group < kGroups && rr < count && d < c.D;
+    float m = -INFINITY, l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    // a part whose scores are all NaN has m = -inf, as one without a visible key, but l = NaN, and its row becomes NaN
+    auto fold = [&](float2 ml, f32x4 x) {
+      const float mn = fmaxf(m, ml.x), mu = mn == -INFINITY ? 0.f : mn;
+      const float a = __builtin_amdgcn_exp2f(m - mu), b = __builtin_amdgcn_exp2f(ml.x - mu);
+      m = mn;
+      l = l * a + ml.y * b;
+      o = o * a + x * b;
+    };
+    if (on) {
+      const int64_t first = (((int64_t)tile * c.Hk + hk) * rows + rr) * p.splits;
 #pragma unroll 4
-    for (int s = group; s < parts; s += kGroups)
-      fold(*reinterpret_cast<const float2*>(p.part_ml + (first + s) * 2), *reinterpret_cast<const f32x4*>(p.part_o + (first + s) * (VT * 16) + d));
-  }
-  if constexpr (kGroups > 1) {
-    o_s[tid] = o;
-    ml_s[tid] = make_float2(m, l);
-    __syncthreads();
-    if (on && group == 0) {
-#pragma unroll
-      for (int k = 1; k < kGroups; ++k) fold(ml_s[tid + k * kQuads * RPW], o_s[tid + k * kQuads * RPW]);
+      for (int s = group; s < parts; s += kGroups)
+        fold(*reinterpret_cast<const float2*>(p.part_ml + (first + s) * 2), *reinterpret_cast<const f32x4*>(p.part_o + (first + s) * (VT * 16) + d));
     }
-  }
-  if (!on || group) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int r = t.local * rows + rr, i = (int)p.G.of(r), h = (r - i * (int)p.G.d) * c.Hk + hk;
-  uint16_t* dst = p.o + (int64_t)g.batch * p.o_s[0] + (int64_t)h * p.o_s[1] + (int64_t)(g.row0 + i) * p.o_s[2] + d;
-  if (p.o_vec) {
-    *reinterpret_cast<u32x2*>(dst) = u32x2{T::pack2(o[0] * inv, o[1] * inv), T::pack2(o[2] * inv, o[3] * inv)};
-  } else {
+    if constexpr (kGroups > 1) {
+      __syncthreads();   // the rows before have been read
+      o_s[tid] = o;
+      ml_s[tid] = make_float2(m, l);
+      __syncthreads();
+      if (on && group == 0) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (d + k < c.D) dst[k] = T::bits(o[k] * inv);
+        for (int k = 1; k < kGroups; ++k) fold(ml_s[tid + k * kQuads * RPW], o_s[tid + k * kQuads * RPW]);
+      }
+    }
+    if (!on || group) continue;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int r = t.local * rows + rr, i = (int)p.G.of(r), h = (r - i * (int)p.G.d) * c.Hk + hk;
+    uint16_t* dst = p.o + (int64_t)g.batch * p.o_s[0] + (int64_t)h * p.o_s[1] + (int64_t)(g.row0 + i) * p.o_s[2] + d;
+    if (p.o_vec) {
+      *reinterpret_cast<u32x2*>(dst) = u32x2{T::pack2(o[0] * inv, o[1] * inv), T::pack2(o[2] * inv, o[3] * inv)};
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (d + k < c.D) dst[k] = T::bits(o[k] * inv);
+    }
+    if (p.lse && d == 0)
+      p.lse[((int64_t)g.batch * p.Hq + h) * p.N + g.row0 + i] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
   }
-  if (p.lse && d == 0)
-    p.lse[((int64_t)g.batch * p.Hq + h) * p.N + g.row0 + i] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 template <typename T, bool Q8, int KS, int VT>
@@ -365,11 +369,13 @@ hipError_t run_paged_plan(const PagedAttnParams& p, bool few, hipStream_t s) {
   const hipError_t e = few ? launch_named("paged_few", paged_few_kernel<T, Q8, KS, VT>, grid, dim3(256), s, p)
                            : launch_named("paged_rows", paged_rows_kernel<T, Q8, KS, VT>, grid, dim3(256), s, p);
   if (e != hipSuccess || p.splits == 1) return e;
-  // rows per workgroup: few workgroups where a row's threads are many anyway
+  // Rows at a time, and workgroups per tile: about 2,048 in all, since finding the tile costs one as much as its rows do
+  // (4,096-token prompts, 2 x 8 heads: 16,384 workgroups of 4 rows took 20 us).
   constexpr int few_rpw = VT <= 8 ? 4 : 1, many_rpw = VT < 8 ? 4 : VT == 8 ? 8 : 4;
-  const unsigned heads = (unsigned)(p.tiles * p.c.Hk);
-  if (few) return launch_named("paged_join", paged_join_kernel<T, VT, few_rpw>, dim3(heads, least_rows / few_rpw), dim3(256), s, p, least_rows, PagedFew<KS, VT>::kWaves);
-  return launch_named("paged_join", paged_join_kernel<T, VT, many_rpw>, dim3(heads, most_rows / many_rpw), dim3(256), s, p, most_rows, 1);
+  const int64_t heads = p.tiles * p.c.Hk, each = 2048 / heads;
+  const auto y = [&](int most) { return (unsigned)(each < 1 ? 1 : each < most ? each : most); };
+  if (few) return launch_named("paged_join", paged_join_kernel<T, VT, few_rpw>, dim3((unsigned)heads, y(least_rows / few_rpw)), dim3(256), s, p, least_rows, PagedFew<KS, VT>::kWaves);
+  return launch_named("paged_join", paged_join_kernel<T, VT, many_rpw>, dim3((unsigned)heads, y(most_rows / many_rpw)), dim3(256), s, p, most_rows, 1);
 }
 
 // The instance of (steps, tiles): paged_k_steps and paged_v_tiles give no other.

@@ -1091,7 +1091,12 @@ pope::PagedCache paged_cache(const pope_paged& d, const void* k, const void* v, 
 //              kPagedPart blocks (sequences differ in length, and what the longest parts leave to do alone is lost)
 //              within kPagedMost workgroups, which bounds the workspace of wide page tables
 //   many rows  the chip holds kPagedSlots workgroups (half where values are wider than 128 columns); a part is at most the
-//              blocks that one of these places gets
+//              blocks that one of these places gets, less a quarter of what causality takes from the first rows of a
+//              prompt: its heaviest tile has twice the mean's blocks and would end alone (prompts of 4,096 tokens x 8
+//              heads, D 64: 63 us so, 71 without; 8,192 x 8, D 128: 268 / 309; 2 x 2,048 x 8, D 256: 139 / 161).  Taken
+//              off calls whose rows see nearly all keys it leaves a second turn of a few workgroups (16 x 64 rows over
+//              6,100 keys: 67 against 57).  Parts of 48 blocks or more where the tiles alone fill half the chip: the
+//              join costs more than it gives (8 x 1,024 tokens x 8 heads: 33 us, 59 with parts of 24)
 constexpr int kPagedGrid = 1024, kPagedSlots = 512, kPagedPart = 64, kPagedMost = 8192;
 
 struct PagedShape {
@@ -1115,7 +1120,8 @@ PagedShape paged_shape(const pope_paged& d, bool packed) {
     const int64_t want = std::max(std::min<int64_t>(kPagedGrid / wgs, blocks / s.least), (blocks + kPagedPart - 1) / kPagedPart);
     s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, kPagedMost / wgs));
   } else {
-    s.least = (int)std::max<int64_t>(16, std::min<int64_t>(blocks, wgs * blocks / (vt <= 8 ? kPagedSlots : kPagedSlots / 2)));
+    const int64_t slots = vt <= 8 ? kPagedSlots : kPagedSlots / 2, unseen = d.causal ? std::min(avg / pope::kBlockKeys, blocks) / 4 : 0;
+    s.least = (int)std::max<int64_t>(2 * wgs < slots ? 16 : 48, std::min(blocks, wgs * (blocks - unseen) / slots));
     s.splits = (int)((blocks + s.least - 1) / s.least);
   }
   s.part_o = s.bytes = 0;
