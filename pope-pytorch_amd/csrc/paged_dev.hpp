@@ -181,13 +181,6 @@ __device__ __forceinline__ int paged_tile_blocks(const PagedSeg& g, int local, i
   return (limit + kBlockKeys - 1) / kBlockKeys;
 }
 
-// x with the 16-bit (8-bit) elements j of which (keep >> j) & 1 is 0 cleared.
-__device__ __forceinline__ u32x4 keep16(u32x4 x, uint32_t keep) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] &= ((keep >> (2 * i)) & 1 ? 0xffffu : 0u) | ((keep >> (2 * i + 1)) & 1 ? 0xffff0000u : 0u);
-  return x;
-}
-
 template <typename T>
 __device__ __forceinline__ bool nonfinite16(uint32_t bits) {
   constexpr uint32_t e = T::kCode == 2 ? 0x7f80u : 0x7c00u;

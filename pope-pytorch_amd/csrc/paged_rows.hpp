@@ -1,8 +1,16 @@
 // Attention over the paged cache for many rows (gfx950): chunks and whole prompts.
 //
-// One workgroup = 4 waves = 128 rows of one key head, 32 per wave; two workgroups per CU (registers and half of the LDS; one
-// where values are wider than 128 columns), each with its own barriers: what one does between its products runs under the other's.  (One workgroup of 8 waves,
-// two groups of 4 that took turns with the key blocks: 4,096-token prompts, 2 x 8 heads, D 64, R 32, @A us against @B.)
+// One workgroup = 4 waves = 128 rows of one key head, 32 per wave; two workgroups per CU (registers and half of the LDS;
+// one where values are wider than 128 columns), each with its own barriers: what one does between its products runs under
+// the other's.  (4 x 1,024 rows x 8 heads over 8,024 keys: D 64, R 32 126 us, D 128, R 64 239; as one workgroup of 8 waves,
+// two groups of 4 that took turns with the key blocks, 151 and 273.)
+//
+// Bound by the matrix cores where the chip is full, and by the heaviest tiles where it is not.  Measured: prompts of 4,096
+// tokens x 8 heads, 2 of them, D 64, R 32: 78 us with the join, 550 TFLOP/s of what the formula has and 890 with the second
+// part of Q_hat; the matrix cores are busy 31 % of the cycles, a CU has on average 57 % of its waves (causal tiles end
+// at different times).  130 rows over 16,000 keys, 8 heads, D 64, R 64: 35 us with the join; 46 MB, in 512 parts of 16 blocks whose
+// start and end cost as much as their keys.  20 rows (5 tokens x 4 query heads) of 16 sequences of up to 4,101 keys, 8 key
+// heads, D 128, R 64, 190 MB: 55 us, 3.4 TB/s.
 //
 // Blocks of K and V go to LDS as they lie in the pages (direct loads, no registers), into a ring of three to eight
 // stages: while step t is in use and t + 1 has landed, the others are on their way.  Pages hold operands of 16x16
@@ -169,7 +177,7 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_rows_kernel(PagedA
   // The loop's two bursts of products, in an explicit order (a fence behind each operand's products): operand reads run
   // kAhead operands in front, and every product is followed by its share of the vector work that the burst covers.  Left
   // to the compiler, each read stood right before its product and the vector work in front of or behind them all, and a
-  // step took the sum of both, 3,700 cycles at D 64, R 32, instead of little more than the products' 2,048.
+  // step of two workgroups took the sum of both, 3,700 cycles at D 64, R 32; it takes 2,860 so (the products alone: 2,048).
   constexpr int kAhead = Q8 || VT < 8 ? 6 : 4;
   auto scores = [&](int slot, f32x16* s, auto&& between) {
     const char* stage = stage_of(slot);

@@ -12,8 +12,8 @@ angles only.  ``quantized`` caches hold e4m3 codes times a power of two per (tok
                                sequences have cached, the new rows included
 
 New rows are (batch, heads, n, dim), or (batch, n, heads, dim) with ``head_dimension_at_first=False``: sequence b's
-are batch entry b.  Packed calls have batch 1 and ``cu_seqlens`` (batch + 1 numbers, from 0): rows cu_seqlens[b] ..
-cu_seqlens[b + 1] - 1 belong to sequence b.  ``lengths`` counts a sequence's tokens with the new ones; row i of n
+are batch entry b.  Packed calls have batch 1 and ``cu_seqlens`` (batch + 1 ascending numbers; of rows that numbers
+which descend leave out or count twice nothing is said): rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 belong to sequence b.  ``lengths`` counts a sequence's tokens with the new ones; row i of n
 stands at position lengths - n + i, and ``pos_emb`` has one row of angles per new row, ``pope(positions)``.  A serving
 step is a write and an attention call with the same page table, lengths and cu_seqlens.
 

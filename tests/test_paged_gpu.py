@@ -262,6 +262,37 @@ def test_attention_ragged(cuda, page, q8):
     attend_and_check(B, [0] * 4 + [2048] + [0] * 72, packed=True, causal=False)
 
 
+@pytest.mark.parametrize("D,R", [(64, 32), (128, 64), (200, 40)])
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "all"])
+def test_prompts_in_parts(cuda, D, R, causal):
+    """More row tiles than the join has workgroups for, their keys in parts, the first tiles of a prompt in one."""
+    attend_and_check(Batch([2300], heads=8, D=D, R=R, dtype=torch.float16), [2300], packed=False, causal=causal)
+
+
+def test_shared_pages_in_parts(cuda):
+    """One page table row for all sequences, of different lengths, single tokens, in parts of the key axis."""
+    B = Batch([2500], heads=16, D=32, R=16)
+    k, v = B.rows(0)
+    lens = torch.arange(2500, 2500 - 40 * 60, -60, dtype=I32, device="cuda")
+    pos = lens[:, None].long() - 1
+    q = B.rand(40, 16, 1, 32)
+    o = paged_flash_attn_with_pope(q, B.cache, B.emb(pos), B.table.expand(40, -1), lens)
+    for b, L in enumerate(lens.tolist()):
+        want, _, tol, _ = reference(q[b], angles(pos[b], 16), k[:, :L], v[:, :L], 16, 32 ** -0.5, True, B.dtype)
+        assert ((o[b].double() - want).abs() <= tol).all(), L
+
+
+@pytest.mark.parametrize("n", [1, 70])
+def test_wide_page_tables(cuda, n):
+    """A page table far wider than the sequences are long: within the same bounds, behind them bad page numbers."""
+    B = Batch([300, 77], heads=2, G=2)
+    table = torch.full((2, 5000), 2 ** 31 - 1, dtype=I32, device="cuda")
+    table[:, :B.table.shape[1]] = B.table
+    B.table = table
+    attend_and_check(B, [n, n], packed=False)
+    attend_and_check(B, [n, min(n, 50)], packed=True, gap=3)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.2, 1.0, 40.0])
 def test_softmax_scales(cuda, scale):
     for dtype in (torch.bfloat16, torch.float16):
@@ -531,6 +562,34 @@ def test_graph_of_a_serving_step(cuda):
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
         assert want.any()
+
+
+def test_graph_of_packed_chunks(cuda):
+    """A captured call of packed chunks replays with other bounds, lengths and pages."""
+    B = Batch([2100, 700, 64], heads=2, G=2)
+    q = B.rand(1, 4, 150, 64)
+    cu = torch.tensor([0, 90, 140, 150], dtype=I32, device="cuda")
+    freqs = B.emb(torch.zeros(150, device="cuda"))[0]
+    run = lambda: paged_flash_attn_with_pope(q, B.cache, (freqs, B.bias), B.table, B.lengths, cu_seqlens=cu)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = run()
+    for bounds, lens in (([0, 90, 140, 150], [2100, 700, 64]), ([0, 0, 150, 150], [5, 690, 0]), ([20, 100, 100, 130], [2000, 64, 40]), ([0, 1, 2, 3], [2100, 1, 64])):
+        cu.copy_(torch.tensor(bounds, dtype=I32, device="cuda"))
+        B.lengths.copy_(torch.tensor(lens, dtype=I32, device="cuda"))
+        q.copy_(B.rand(*q.shape))
+        freqs.copy_(angles(torch.randint(0, 2100, (150,), generator=B.g, device="cuda"), 32))
+        B.table.copy_(B.table[[0, 1, 2]].roll(1, 1).where(torch.tensor([[True], [False], [True]], device="cuda"), B.table))
+        want = run()
+        out.fill_(NAN)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and want.any()
 
 
 def test_ops_trace(cuda):
