@@ -36,6 +36,7 @@ struct PagedAttnParams {
   PagedDiv G;                          // Hq / Hk
   int Hq, causal, N;                   // N: rows per batch entry (all of them when packed)
   int splits, least;                   // splits of the key axis, the least blocks of one
+  int slots;                           // workgroups that the chip holds: paged_balance raises `least`; 0: `least` stands
   int64_t tiles;                       // row tiles
   // Scores come out of the products in log2 units: Q_hat carries q_factor = softmax scale x log2 e.  fp16 does not hold
   // every Q_hat times a factor above 1: the scores then take `late`, the factor's magnitude, and q_factor its sign.
@@ -43,6 +44,7 @@ struct PagedAttnParams {
   int64_t q_s[3], o_s[3], f_s[2];
   int q_vec, f_vec, o_vec;             // query rows: whole 16-byte units; angles likewise; output rows: 8-byte units
   float* part_o; float* part_ml;       // splits > 1: (tile, head, row, split): 16 * tiles floats, and (m, l)
+  int* parts;                          // splits > 1: (tile, head): splits that have keys
 };
 // Rows of a tile: 16 where a sequence has at most as many (query head of a key head, new token) rows on average, else 128.
 constexpr int kPagedFewRows = 16, kPagedManyRows = 128;

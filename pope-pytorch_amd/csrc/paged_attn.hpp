@@ -45,17 +45,19 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_few_kernel(PagedAt
   const PagedCache& c = p.c;
   const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15, quad = lane >> 4;
 
-  const PagedJob job = paged_job(p);
+  const PagedPlan job = paged_plan(p, kRows);
   const int hk = job.hk;
-  const PagedTile t = paged_tile(c.seqs, job.tile, p.G.d, kRows, 1);
+  const PagedTile& t = job.t;
   const PagedSeg& g = t.seg;
   const int rows_all = g.n * (int)p.G.d, r0 = t.local * kRows;
   if (r0 >= rows_all) return;
   const bool causal = p.causal != 0;
   const int blocks = paged_tile_blocks(g, t.local, kRows, p.G, causal);
-  const PagedRange range = paged_range(blocks, p.splits, p.least, WK, job.split);
-  if (job.split > 0 && range.begin >= range.end) return;   // the join knows which splits have blocks
-  const bool part = paged_parts(blocks, p.splits, p.least, WK) > 1;
+  const PagedRange range = paged_range(blocks, p.splits, job.least, WK, job.split);
+  const int parts = paged_parts(blocks, p.splits, job.least, WK);
+  if (job.split > 0 && range.begin >= range.end) return;
+  if (p.splits > 1 && job.split == 0 && threadIdx.x == 0) p.parts[(int64_t)job.tile * c.Hk + hk] = parts;
+  const bool part = parts > 1;
 
   // ---- the first block's loads ---------------------------------------------------------------------------------
   constexpr int kKL = Q8 ? KS : 2 * KS, kVL = Q8 ? VT / 2 : VT, kE = Q8 ? 1 : 2;   // 16-byte loads per lane and block; bytes
@@ -305,7 +307,7 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_few_kernel(PagedAt
 // The parts of a tile's rows joined, RPW rows per workgroup.  A thread has four columns of a row and every kGroups-th of its
 // parts, of which it keeps a running (m, l, o); the groups join through LDS.  A row's parts lie side by side.
 template <typename T, int VT, int RPW>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p, int rows, int step) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p, int rows) {
   constexpr int kQuads = VT * 4, kGroups = 256 / (RPW * kQuads);
   __shared__ f32x4 o_s[256];
   __shared__ float2 ml_s[256];
@@ -315,7 +317,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p, int 
   const PagedSeg& g = t.seg;
   const int count = min(g.n * (int)p.G.d - t.local * rows, rows);
   if ((int)blockIdx.y * RPW >= count) return;
-  const int parts = paged_parts(paged_tile_blocks(g, t.local, rows, p.G, p.causal != 0), p.splits, p.least, step);
+  const int parts = p.parts[blockIdx.x];
   if (parts <= 1) return;   // written by the one that had it
   const int d = tid % kQuads * 4, group = tid / (kQuads * RPW);
   for (int r0 = blockIdx.y * RPW; r0 < count; r0 += gridDim.y * RPW) {
@@ -376,8 +378,8 @@ hipError_t run_paged_plan(const PagedAttnParams& p, bool few, hipStream_t s) {
   constexpr int few_rpw = VT <= 8 ? 4 : 1, many_rpw = VT < 8 ? 4 : VT == 8 ? 8 : 4;
   const int64_t heads = p.tiles * p.c.Hk, each = 2048 / heads;
   const auto y = [&](int most) { return (unsigned)(each < 1 ? 1 : each < most ? each : most); };
-  if (few) return launch_named("paged_join", paged_join_kernel<T, VT, few_rpw>, dim3((unsigned)heads, y(least_rows / few_rpw)), dim3(256), s, p, least_rows, PagedFew<KS, VT>::kWaves);
-  return launch_named("paged_join", paged_join_kernel<T, VT, many_rpw>, dim3((unsigned)heads, y(most_rows / many_rpw)), dim3(256), s, p, most_rows, 1);
+  if (few) return launch_named("paged_join", paged_join_kernel<T, VT, few_rpw>, dim3((unsigned)heads, y(least_rows / few_rpw)), dim3(256), s, p, least_rows);
+  return launch_named("paged_join", paged_join_kernel<T, VT, many_rpw>, dim3((unsigned)heads, y(most_rows / many_rpw)), dim3(256), s, p, most_rows);
 }
 
 // The instance of (steps, tiles): paged_k_steps and paged_v_tiles give no other.

@@ -73,6 +73,74 @@ __device__ __forceinline__ PagedJob paged_job(const PagedAttnParams& p) {
   return PagedJob{(int)(n - 1 - x), (int)(id - rest * p.c.Hk), (int)split};
 }
 
+// A workgroup's tile, part of the key axis, and the least blocks of a part.
+//
+// Many rows, at most 64 segments (`slots`, the workgroups that the chip holds, is not 0): parts are cut by what the sequences
+// have, as few blocks as these workgroups get of all tiles' blocks, or more where the tiles' parts would then be more
+// than the workgroups.  A quarter of what causality takes from a prompt's first rows is left out: its heaviest tile has
+// twice the mean's blocks and would end alone (prompts of 4,096 tokens x 8 heads, D 64: 62 us so, 71 without; 8,192 x 8,
+// D 128: 270 / 309; 2 x 2,048 x 8, D 256: 139 / 161).
+// Parts that all fit then go to the first workgroups: with empty ones in between, the shader engines, which are dealt
+// workgroups in turn, get unequal work (20 rows of 16 sequences x 8 heads, D 128, every other one 64 tokens long, the
+// others 4,096: 38 us, 58 with empty ones in between).  Tiles of prompts keep paged_job's order instead, heaviest first
+// over all sequences (2 x 4,096 tokens: 89 us, 101 sequence by sequence).
+// Every workgroup computes the same sums in the same order.
+struct PagedPlan { PagedTile t; int tile, hk, split, least; };
+__device__ __forceinline__ PagedPlan paged_plan(const PagedAttnParams& p, int rows) {
+  const PagedSeqs& q = p.c.seqs;
+  const PagedJob job = paged_job(p);
+  PagedPlan r;
+  r.tile = job.tile;
+  r.hk = job.hk;
+  r.split = job.split;
+  r.least = p.least;
+  if (p.slots) {
+    const int s = threadIdx.x & 63;
+    PagedSeg g = {};
+    int tiles = 0, blocks = 0, unseen = 0;
+    if (s < (q.cu ? q.B + 2 : q.B)) {
+      g = paged_seg(q, s);
+      tiles = (int)(((int64_t)g.n * p.G.d + rows - 1) / rows);
+      blocks = (g.len + kBlockKeys - 1) / kBlockKeys;
+      unseen = p.causal ? min(g.n / kBlockKeys, blocks) / 4 : 0;
+    }
+    auto sum = [](float x) {
+#pragma unroll
+      for (int i = 1; i < 64; i *= 2) x += wave_shfl_xor(x, i);
+      return x;
+    };
+    const float slots = (float)p.slots / (float)p.c.Hk, n = (float)tiles, each = (float)(blocks - unseen);
+    int least = max(p.least, (int)__builtin_ceilf(sum(n * each) / slots));
+    bool fits = false;
+    for (int i = 0; i < 16 && !fits; ++i) {
+      fits = sum(n * fmaxf(1.f, __builtin_ceilf(each / (float)least))) <= slots;
+      if (!fits) least += max(1, least / 16);
+    }
+    r.least = __builtin_amdgcn_readfirstlane(least);
+    if (__builtin_amdgcn_readfirstlane(fits) && !__any(tiles > 1 && 8 * unseen >= blocks)) {
+      const int mine = tiles * max(1, min(p.splits, (blocks + r.least - 1) / r.least));
+      int upto = mine;
+#pragma unroll
+      for (int i = 1; i < 64; i *= 2) {
+        const int x = __shfl_up(upto, i, 64);
+        upto += s >= i ? x : 0;
+      }
+      const int at = (int)(blockIdx.x / (unsigned)p.c.Hk);
+      const uint64_t behind = __ballot(upto > at);
+      const int f = behind ? __builtin_ctzll(behind) : 0;
+      auto of = [&](int x) { return __builtin_amdgcn_readlane(x, f); };
+      r.t.seg = PagedSeg{of(g.b), of(g.batch), of(g.row0), behind ? of(g.n) : 0, of(g.len), of(g.first)};
+      const int count = max(of(tiles), 1), k = at - (of(upto) - of(mine));
+      r.split = behind ? k / count : 0;
+      r.t.local = behind ? count - 1 - (k - r.split * count) : 0;
+      r.tile = q.cu ? (int)paged_first_tile(q, f, p.G.d, rows, 1) + r.t.local : r.t.local * q.B + f;
+      return r;
+    }
+  }
+  r.t = paged_tile(q, job.tile, p.G.d, rows, 1);
+  return r;
+}
+
 // Rows of a tile that starts at row r0 of its segment: row r0 + x is query head g Hk + hk of new token i, r = i G + g.
 struct PagedRowMap {
   unsigned i0, rem, G;

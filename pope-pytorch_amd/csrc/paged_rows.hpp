@@ -65,16 +65,18 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_rows_kernel(PagedA
   const PagedCache& c = p.c;
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), lr = lane & 31, hf = lane >> 5;
 
-  const PagedJob job = paged_job(p);
+  const PagedPlan job = paged_plan(p, kRows);
   const int hk = job.hk;
-  const PagedTile t = paged_tile(c.seqs, job.tile, p.G.d, kRows, 1);
+  const PagedTile& t = job.t;
   const PagedSeg& g = t.seg;
   const int rows_all = g.n * (int)p.G.d, r0 = t.local * kRows;
   if (r0 >= rows_all) return;
   const bool causal = p.causal != 0;
   const int blocks = paged_tile_blocks(g, t.local, kRows, p.G, causal);
-  const PagedRange range = paged_range(blocks, p.splits, p.least, 1, job.split);
+  const int parts = paged_parts(blocks, p.splits, job.least, 1);
+  const PagedRange range = paged_range(blocks, p.splits, job.least, 1, job.split);
   if (job.split > 0 && range.begin >= range.end) return;
+  if (p.splits > 1 && job.split == 0 && tid == 0) p.parts[(int64_t)job.tile * c.Hk + hk] = parts;
 
   // ---- the lane's row, and the keys that all of the wave's (of the tile's) rows see -----------------------------
   const PagedRowMap map(r0, p.G);
@@ -563,7 +565,7 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_rows_kernel(PagedA
   // ---- output, or this split's part -----------------------------------------------------------------------------
   if (!live) return;
   if (!set) m = -INFINITY;
-  const bool part = paged_parts(blocks, p.splits, p.least, 1) > 1;
+  const bool part = parts > 1;
   const float f = part ? 1.f : l == 0.f ? 0.f : 1.f / l;
   const int64_t row = part ? (((int64_t)job.tile * c.Hk + hk) * kRows + x) * p.splits + job.split : 0;
   uint16_t* dst = p.o + (int64_t)g.batch * p.o_s[0] + (int64_t)row_h * p.o_s[1] + (int64_t)(g.row0 + row_i) * p.o_s[2];

@@ -1090,20 +1090,19 @@ pope::PagedCache paged_cache(const pope_paged& d, const void* k, const void* v, 
 //   few rows   as many parts as bring the grid to kPagedGrid workgroups, of 16 blocks (512 keys) or more, and of at most
 //              kPagedPart blocks (sequences differ in length, and what the longest parts leave to do alone is lost)
 //              within kPagedMost workgroups, which bounds the workspace of wide page tables
-//   many rows  the chip holds kPagedSlots workgroups (half where values are wider than 128 columns); a part is at most the
-//              blocks that one of these places gets, less a quarter of what causality takes from the first rows of a
-//              prompt: its heaviest tile has twice the mean's blocks and would end alone (prompts of 4,096 tokens x 8
-//              heads, D 64: 63 us so, 71 without; 8,192 x 8, D 128: 268 / 309; 2 x 2,048 x 8, D 256: 139 / 161).  Taken
-//              off calls whose rows see nearly all keys it leaves a second turn of a few workgroups (16 x 64 rows over
-//              6,100 keys: 67 against 57).  Parts of 48 blocks or more where the tiles alone fill half the chip: the
-//              join costs more than it gives (8 x 1,024 tokens x 8 heads: 33 us, 59 with parts of 24)
+//   many rows  the chip holds kPagedSlots workgroups (half where values are wider than 128 columns).  The kernel cuts parts
+//              by the sequences' lengths so that these places get equal work (paged_plan), up to two parts per place; with
+//              more than 64 segments, which it does not look at, by the page table's width.  By the width, tokens of 16
+//              sequences of 2,000 in tables four times as wide took 73 us instead of 38 (20 rows, 8 heads, D 128).
+//              Parts of 16 blocks or more, of 48 where the tiles alone fill half the chip: the join costs more than it
+//              gives (8 x 1,024 tokens x 8 heads: 33 us, 59 with parts of 24)
 constexpr int kPagedGrid = 1024, kPagedSlots = 512, kPagedPart = 64, kPagedMost = 8192;
 
 struct PagedShape {
   bool few;       // tiles of 16 rows, else of 128
   int64_t tiles;
-  int splits, least;
-  size_t part_o, bytes;
+  int splits, least, slots;
+  size_t part_o, part_ml, bytes;
 };
 
 PagedShape paged_shape(const pope_paged& d, bool packed) {
@@ -1115,20 +1114,26 @@ PagedShape paged_shape(const pope_paged& d, bool packed) {
   s.tiles = pope::paged_tiles(d.B, d.N, packed, G, rows, 1);
   const int64_t wgs = std::max<int64_t>(s.tiles * d.Hk, 1);
   const int64_t blocks = (int64_t)d.table_cols * d.page_size / pope::kBlockKeys;
+  s.slots = 0;
   if (s.few) {
     s.least = 16;
     const int64_t want = std::max(std::min<int64_t>(kPagedGrid / wgs, blocks / s.least), (blocks + kPagedPart - 1) / kPagedPart);
     s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, kPagedMost / wgs));
   } else {
-    const int64_t slots = vt <= 8 ? kPagedSlots : kPagedSlots / 2, unseen = d.causal ? std::min(avg / pope::kBlockKeys, blocks) / 4 : 0;
-    s.least = (int)std::max<int64_t>(2 * wgs < slots ? 16 : 48, std::min(blocks, wgs * (blocks - unseen) / slots));
-    s.splits = (int)((blocks + s.least - 1) / s.least);
+    const int64_t slots = vt <= 8 ? kPagedSlots : kPagedSlots / 2;
+    s.least = 2 * wgs < slots ? 16 : 48;
+    s.splits = (int)std::max<int64_t>(1, std::min((blocks + s.least - 1) / s.least, 2 * slots / wgs));
+    if (s.splits > 1) {
+      if (d.B + (packed ? 2 : 0) <= 64) s.slots = (int)slots;
+      else s.least = (int)std::max<int64_t>(s.least, std::min(blocks, wgs * blocks / slots));
+    }
   }
-  s.part_o = s.bytes = 0;
+  s.part_o = s.part_ml = s.bytes = 0;
   if (s.splits > 1) {
     const size_t n = (size_t)wgs * s.splits * rows;
     s.part_o = align_up(n * vt * 16 * sizeof(float));
-    s.bytes = s.part_o + align_up(n * 2 * sizeof(float));
+    s.part_ml = align_up(n * 2 * sizeof(float));
+    s.bytes = s.part_o + s.part_ml + align_up((size_t)wgs * sizeof(int));
   }
   return s;
 }
@@ -1221,7 +1226,7 @@ int pope_paged_attn(const pope_paged* d, const void* q, const float* freqs, cons
   p.o = static_cast<uint16_t*>(o);
   p.lse = lse;
   p.Hq = d->Hq; p.G = pope::paged_div(d->Hq / d->Hk); p.causal = d->causal != 0; p.N = d->N;
-  p.splits = sh.splits; p.least = sh.least;
+  p.splits = sh.splits; p.least = sh.least; p.slots = sh.slots;
   p.tiles = sh.tiles;
   const float factor = d->softmax_scale * 1.4426950408889634f;
   p.q_factor = factor;
@@ -1237,6 +1242,7 @@ int pope_paged_attn(const pope_paged* d, const void* q, const float* freqs, cons
   p.o_vec = d->D % 4 == 0 && reinterpret_cast<uintptr_t>(o) % 8 == 0 && d->o_s[0] % 4 == 0 && d->o_s[1] % 4 == 0 && d->o_s[2] % 4 == 0;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + sh.part_o);
+  p.parts = reinterpret_cast<int*>(static_cast<char*>(workspace) + sh.part_o + sh.part_ml);
   if ((int64_t)d->N * (d->Hq / d->Hk) > ((int64_t)1 << 30) || sh.tiles * d->Hk * sh.splits >= ((int64_t)1 << 31)) return fail(POPE_ERR_UNSUPPORTED, "%lld row tiles x %d heads: too many workgroups", (long long)sh.tiles, d->Hk);
   const hipError_t e = pope::launch_paged_attn(p, sh.few, d->dtype, d->quantized != 0, reinterpret_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "paged attention launch");

@@ -282,6 +282,15 @@ def test_shared_pages_in_parts(cuda):
         assert ((o[b].double() - want).abs() <= tol).all(), L
 
 
+@pytest.mark.parametrize("q8", [False, True], ids=["16bit", "8bit"])
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "all"])
+def test_parts_by_length(cuda, q8, causal):
+    """Long sequences between short and empty ones, their keys in parts; packed with empty segments and rows behind."""
+    B = Batch([1900, 40, 0, 1200] * 5, heads=2, G=4, D=96, R=48, page=32, q8=q8)
+    attend_and_check(B, [30] * 20, packed=False, causal=causal)
+    attend_and_check(B, [70, 33, 0, 5, 300, 0, 0, 100, 1, 40, 0, 0] + [9, 8, 0, 64] * 2, packed=True, causal=causal, gap=150)
+
+
 @pytest.mark.parametrize("n", [1, 70])
 def test_wide_page_tables(cuda, n):
     """A page table far wider than the sequences are long: within the same bounds, behind them bad page numbers."""
