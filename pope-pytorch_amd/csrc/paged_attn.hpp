@@ -118,7 +118,7 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_few_kernel(PagedAt
     uint16_t* hi = reinterpret_cast<uint16_t*>(smem);
     uint16_t* lo = hi + kRows * QST;
 #pragma unroll
-    for (int k = 0; k < (VT + 7) / 8; ++k) paged_query_make<T>(p, in[k], (threadIdx.x + 256 * k) % kRows, (threadIdx.x + 256 * k) / kRows * 8, QST, hi, lo);
+    for (int k = 0; k < (VT + 7) / 8; ++k) paged_query_make<T>(p, in[k], true, (threadIdx.x + 256 * k) % kRows, (threadIdx.x + 256 * k) / kRows * 8, QST, hi, lo);
     paged_query_tail<kRows>(p, threadIdx.x, 256, KS * 32, QST, hi, lo);
     __syncthreads();
 #pragma unroll

@@ -118,7 +118,7 @@ __device__ __forceinline__ PagedPlan paged_plan(const PagedAttnParams& p, int ro
     }
     r.least = __builtin_amdgcn_readfirstlane(least);
     if (__builtin_amdgcn_readfirstlane(fits) && !__any(tiles > 1 && 8 * unseen >= blocks)) {
-      const int mine = tiles * max(1, min(p.splits, (blocks + r.least - 1) / r.least));
+      const int parts = max(1, min(p.splits, (blocks + r.least - 1) / r.least)), mine = tiles * parts;
       int upto = mine;
 #pragma unroll
       for (int i = 1; i < 64; i *= 2) {
@@ -133,6 +133,7 @@ __device__ __forceinline__ PagedPlan paged_plan(const PagedAttnParams& p, int ro
       const int count = max(of(tiles), 1), k = at - (of(upto) - of(mine));
       r.split = behind ? k / count : 0;
       r.t.local = behind ? count - 1 - (k - r.split * count) : 0;
+      r.least = max(1, of((blocks + parts - 1) / parts));   // a sequence's parts alike
       r.tile = q.cu ? (int)paged_first_tile(q, f, p.G.d, rows, 1) + r.t.local : r.t.local * q.B + f;
       return r;
     }
@@ -186,15 +187,18 @@ __device__ __forceinline__ PagedQueryIn paged_query_load(const PagedAttnParams& 
   }
   return in;
 }
-// Rows past the tile's are softplus(0) cos 0: finite values that nothing reads.
+// Rows past the tile's are softplus(0) cos 0, or zeros where all of a wave's are (`live`): finite values that nothing reads.
 template <typename T>
-__device__ __forceinline__ void paged_query_make(const PagedAttnParams& p, const PagedQueryIn& in, int row, int d0, int stride, uint16_t* hi, uint16_t* lo) {
+__device__ __forceinline__ void paged_query_make(const PagedAttnParams& p, const PagedQueryIn& in, bool live, int row, int d0, int stride, uint16_t* hi, uint16_t* lo) {
   const int D = p.c.D, R = p.c.R;
   if (d0 >= D) return;
   float x[8], a[8], b[8];   // a: cosine part, or the raw value; b: sine part
   unpack8<T>(in.x, x);
   const bool off = p.q_factor == 0.f;   // scores are 0, also of values that are not finite
-  if (d0 < R) {
+  if (!live) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) a[k] = b[k] = 0.f;
+  } else if (d0 < R) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       float sn, cs;

@@ -400,7 +400,7 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_rows_kernel(PagedA
       if (x0) __syncthreads();
 #pragma unroll
       for (int k = 0; k < kTurns; ++k)
-        paged_query_make<T>(p, in[x0 / RB][k], (tid + 256 * k) % RB, (tid + 256 * k) / RB * 8, C::QST, hi, lo);
+        paged_query_make<T>(p, in[x0 / RB][k], __any(x0 + (tid + 256 * k) % RB < count), (tid + 256 * k) % RB, (tid + 256 * k) / RB * 8, C::QST, hi, lo);
       paged_query_tail<RB>(p, tid, 256, KS * 32, C::QST, hi, lo);
       __syncthreads();
       if (wave * 32 >= x0 && wave * 32 < x0 + RB) {
