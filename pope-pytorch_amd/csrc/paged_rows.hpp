@@ -6,11 +6,11 @@
 // two groups of 4 that took turns with the key blocks, 151 and 273.)
 //
 // Bound by the matrix cores where the chip is full, and by the heaviest tiles where it is not.  Measured: prompts of 4,096
-// tokens x 8 heads, 2 of them, D 64, R 32: 78 us with the join, 550 TFLOP/s of what the formula has and 890 with the second
-// part of Q_hat; the matrix cores are busy 31 % of the cycles, a CU has on average 57 % of its waves (causal tiles end
-// at different times).  130 rows over 16,000 keys, 8 heads, D 64, R 64: 35 us with the join; 46 MB, in 512 parts of 16 blocks whose
+// tokens x 8 heads, 2 of them, D 64, R 32: 80 us and 9 for the join, 540 TFLOP/s of what the formula has and 860 with the
+// second part of Q_hat; the matrix cores are busy 38 % of the cycles, 1.55 of 2 waves per SIMD alive (causal tiles end at
+// different times).  130 rows over 16,000 keys, 8 heads, D 64, R 64: 32 us and 4; 46 MB, in 512 parts of 16 blocks whose
 // start and end cost as much as their keys.  20 rows (5 tokens x 4 query heads) of 16 sequences of up to 4,101 keys, 8 key
-// heads, D 128, R 64, 190 MB: 55 us, 3.4 TB/s.
+// heads, D 128, R 64, 200 MB: 48 us and 4.5, 4.2 TB/s.
 //
 // Blocks of K and V go to LDS as they lie in the pages (direct loads, no registers), into a ring of three to eight
 // stages: while step t is in use and t + 1 has landed, the others are on their way.  Pages hold operands of 16x16
