@@ -36,7 +36,7 @@ struct PagedAttnParams {
   PagedDiv G;                          // Hq / Hk
   int Hq, causal, N;                   // N: rows per batch entry (all of them when packed)
   int splits, least;                   // splits of the key axis, the least blocks of one
-  int slots;                           // workgroups that the chip holds: paged_balance raises `least`; 0: `least` stands
+  int slots;                           // workgroups that the chip holds: paged_plan raises `least` (many rows); 0: `least` stands
   int64_t tiles;                       // row tiles
   // Scores come out of the products in log2 units: Q_hat carries q_factor = softmax scale x log2 e.  fp16 does not hold
   // every Q_hat times a factor above 1: the scores then take `late`, the factor's magnitude, and q_factor its sign.

@@ -45,16 +45,16 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_few_kernel(PagedAt
   const PagedCache& c = p.c;
   const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15, quad = lane >> 4;
 
-  const PagedPlan job = paged_plan(p, kRows);
+  const PagedJob job = paged_job(p);
   const int hk = job.hk;
-  const PagedTile& t = job.t;
+  const PagedTile t = paged_tile(c.seqs, job.tile, p.G.d, kRows, 1);
   const PagedSeg& g = t.seg;
   const int rows_all = g.n * (int)p.G.d, r0 = t.local * kRows;
   if (r0 >= rows_all) return;
   const bool causal = p.causal != 0;
   const int blocks = paged_tile_blocks(g, t.local, kRows, p.G, causal);
-  const PagedRange range = paged_range(blocks, p.splits, job.least, WK, job.split);
-  const int parts = paged_parts(blocks, p.splits, job.least, WK);
+  const PagedRange range = paged_range(blocks, p.splits, p.least, WK, job.split);
+  const int parts = paged_parts(blocks, p.splits, p.least, WK);
   if (job.split > 0 && range.begin >= range.end) return;
   if (p.splits > 1 && job.split == 0 && threadIdx.x == 0) p.parts[(int64_t)job.tile * c.Hk + hk] = parts;
   const bool part = parts > 1;
