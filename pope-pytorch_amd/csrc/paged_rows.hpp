@@ -551,8 +551,13 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_rows_kernel(PagedA
         mask(st, sa);
       }
       rescale(row_max(sa), sa);
-      probs(slot, sa, pw);
-      products(slot, pw, nothing);
+      // the first half of the keys' probabilities, the second half's under the first half's products
+#pragma unroll
+      for (int u = 0; u < 4; ++u) prob(slot, sa, pw, u);
+      products(slot, pw, [&](int i, int) {
+#pragma unroll
+        for (int u = 4 + 4 * i / NDB; u < 8 && u < 4 + 4 * (i + 1) / NDB; ++u) prob(slot, sa, pw, u);
+      });
       if (edge) {
         POPE_COLD_PATH();
         add_seen(st, sa);
