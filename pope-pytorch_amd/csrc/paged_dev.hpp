@@ -110,7 +110,7 @@ __device__ __forceinline__ PagedPlan paged_plan(const PagedAttnParams& p, int ro
       return x;
     };
     const float slots = (float)p.slots / (float)p.c.Hk, n = (float)tiles, each = (float)(blocks - unseen);
-    int least = max(p.least, (int)__builtin_ceilf(sum(n * each) / slots));
+    int least = max(p.least, (int)fminf(__builtin_ceilf(sum(n * each) / slots), 67108864.f));   // 2^26 blocks: all positions
     bool fits = false;
     for (int i = 0; i < 16 && !fits; ++i) {
       fits = sum(n * fmaxf(1.f, __builtin_ceilf(each / (float)least))) <= slots;
