@@ -17,7 +17,7 @@
 // leave the chip idle, workgroups take parts of the key axis, and a second launch joins those that had several.
 // Measured: 8 sequences of 4,096 .. 32,768 tokens, 16 heads, D 64, R 64, 16 bits, 906 MB: 165 us with the join, 5.5 TB/s
 // (a copy: 4.7, half of it writes); 32 of 1,000 .. 16,384, 8 key heads of 4 query heads, D 128, R 64, 8 bits, 717 MB: 155 us,
-// 4.6 TB/s.  One sequence of 4,000 tokens, 18 MB: 14 us, two launches and a wave's chain of a few blocks.
+// 4.6 TB/s.  One sequence of 4,000 tokens, 18 MB: 13 us, two launches and a wave's chain of a few blocks.
 //
 // Precision: S, the maxima, sums and O in fp32.  Q_hat is the sum of two 16-bit parts (twice the S products: rounded once, its
 // error would appear in every score, about 0.8 of an output's own rounding at N(0, 1) inputs), and so is P here, where
