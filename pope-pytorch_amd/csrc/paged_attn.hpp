@@ -317,7 +317,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p, int 
   const PagedSeg& g = t.seg;
   const int count = min(g.n * (int)p.G.d - t.local * rows, rows);
   if ((int)blockIdx.y * RPW >= count) return;
-  const int parts = p.parts[blockIdx.x];
+  // bounded: lengths that another stream changes between the launches must not lead out of the workspace
+  const int parts = min(p.parts[blockIdx.x], p.splits);
   if (parts <= 1) return;   // written by the one that had it
   const int d = tid % kQuads * 4, group = tid / (kQuads * RPW);
   for (int r0 = blockIdx.y * RPW; r0 < count; r0 += gridDim.y * RPW) {

@@ -5,31 +5,39 @@
 
 namespace pope {
 
-// The segment that tile `tile` belongs to, and its tile within it; seg.n = 0 where there is none.  Packed calls: the
-// lanes of a wave test 64 segments' first tiles at a time, the last one at or below `tile` has it (with bounds that
-// decrease, any segment may come out, and paged_seg bounds it).  Padded calls: the sequences' n-th tiles side by side.
-struct PagedTile { PagedSeg seg; int local; };
+// A wave's lanes as the segments that paged_index.hpp's functions go over.
+struct PagedWave {
+  PagedPlanSeg mine;
+  template <typename F>
+  __device__ __forceinline__ uint64_t operator()(F&& f) const { return __ballot(f((int)(threadIdx.x & 63))); }
+  template <typename F>
+  __device__ __forceinline__ float sum(F&& f) const {
+    float x = f(mine);
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) x += wave_shfl_xor(x, i);
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x)));
+  }
+  template <typename F>
+  __device__ __forceinline__ bool any(F&& f) const { return __any(f(mine)); }
+  template <typename F>
+  __device__ __forceinline__ int of(int i, F&& f) const { return __builtin_amdgcn_readlane(f(mine), i); }
+  template <typename F>
+  __device__ __forceinline__ int first_above(F&& f, int at, int* before) const {
+    const int lane = threadIdx.x & 63, own = f(mine);
+    int upto = own;
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) {
+      const int x = __shfl_up(upto, i, 64);
+      upto += lane >= i ? x : 0;
+    }
+    const uint64_t above = __ballot(upto > at);
+    const int i = above ? __builtin_ctzll(above) : 64;
+    *before = above ? __builtin_amdgcn_readlane(upto - own, i) : 0;
+    return i;
+  }
+};
 __device__ __forceinline__ PagedTile paged_tile(const PagedSeqs& q, int tile, int unit, int per, int extra) {
-  PagedTile t;
-  if (!q.cu) {
-    t.local = (int)((unsigned)tile / (unsigned)q.B);
-    t.seg = paged_seg(q, tile - t.local * q.B);
-    return t;
-  }
-  const int lane = threadIdx.x & 63, S = q.B + 2;
-  int found = 0;
-  for (int s0 = 0; s0 < S; s0 += 64) {
-    const int s = s0 + lane;
-    const bool at = s < S && paged_first_tile(q, s < S ? s : 0, unit, per, extra) <= tile;
-    const uint64_t w = __ballot(at);
-    if (!w) break;
-    found = s0 + 63 - __builtin_clzll(w);
-    if (found != s0 + 63) break;
-  }
-  found = __builtin_amdgcn_readfirstlane(found);
-  t.seg = paged_seg(q, found);
-  t.local = tile - paged_first_tile(q, found, unit, per, extra);
-  return t;
+  return paged_tile_of(q, tile, unit, per, extra, PagedWave{});
 }
 
 // Page of block `blk` of sequence b; -1 for a number outside the cache.
@@ -73,83 +81,12 @@ __device__ __forceinline__ PagedJob paged_job(const PagedAttnParams& p) {
   return PagedJob{(int)(n - 1 - x), (int)(id - rest * p.c.Hk), (int)split};
 }
 
-// A workgroup's tile, part of the key axis, and the least blocks of a part.
-//
-// Many rows, at most 64 segments (`slots`, the workgroups that the chip holds, is not 0): parts are cut by what the sequences
-// have, as few blocks as these workgroups get of all tiles' blocks, or more where the tiles' parts would then be more
-// than the workgroups.  A quarter of what causality takes from a prompt's first rows is left out: its heaviest tile has
-// twice the mean's blocks and would end alone (prompts of 4,096 tokens x 8 heads, D 64: 62 us so, 71 without; 8,192 x 8,
-// D 128: 270 / 309; 2 x 2,048 x 8, D 256: 139 / 161).
-// Parts that all fit then go to the first workgroups: with empty ones in between, the shader engines, which are dealt
-// workgroups in turn, get unequal work (20 rows of 16 sequences x 8 heads, D 128, every other one 64 tokens long, the
-// others 4,096: 38 us, 58 with empty ones in between).  Tiles of prompts keep paged_job's order instead, heaviest first
-// over all sequences (2 x 4,096 tokens: 89 us, 101 sequence by sequence).
-// Every workgroup computes the same sums in the same order.
-struct PagedPlan { PagedTile t; int tile, hk, split, least; };
 __device__ __forceinline__ PagedPlan paged_plan(const PagedAttnParams& p, int rows) {
-  const PagedSeqs& q = p.c.seqs;
-  const PagedJob job = paged_job(p);
-  PagedPlan r;
-  r.tile = job.tile;
-  r.hk = job.hk;
-  r.split = job.split;
-  r.least = p.least;
-  if (p.slots) {
-    const int s = threadIdx.x & 63;
-    PagedSeg g = {};
-    int tiles = 0, blocks = 0, unseen = 0;
-    if (s < (q.cu ? q.B + 2 : q.B)) {
-      g = paged_seg(q, s);
-      tiles = (int)(((int64_t)g.n * p.G.d + rows - 1) / rows);
-      blocks = (g.len + kBlockKeys - 1) / kBlockKeys;
-      unseen = p.causal ? min(g.n / kBlockKeys, blocks) / 4 : 0;
-    }
-    auto sum = [](float x) {
-#pragma unroll
-      for (int i = 1; i < 64; i *= 2) x += wave_shfl_xor(x, i);
-      return x;
-    };
-    const float slots = (float)p.slots / (float)p.c.Hk, n = (float)tiles, each = (float)(blocks - unseen);
-    int least = max(p.least, (int)fminf(__builtin_ceilf(sum(n * each) / slots), 67108864.f));   // 2^26 blocks: all positions
-    bool fits = false;
-    for (int i = 0; i < 16 && !fits; ++i) {
-      fits = sum(n * fmaxf(1.f, __builtin_ceilf(each / (float)least))) <= slots;
-      if (!fits) least += max(1, least / 16);
-    }
-    r.least = __builtin_amdgcn_readfirstlane(least);
-    if (__builtin_amdgcn_readfirstlane(fits) && !__any(tiles > 1 && 8 * unseen >= blocks)) {
-      const int parts = max(1, min(p.splits, (blocks + r.least - 1) / r.least)), mine = tiles * parts;
-      int upto = mine;
-#pragma unroll
-      for (int i = 1; i < 64; i *= 2) {
-        const int x = __shfl_up(upto, i, 64);
-        upto += s >= i ? x : 0;
-      }
-      const int at = (int)(blockIdx.x / (unsigned)p.c.Hk);
-      const uint64_t behind = __ballot(upto > at);
-      const int f = behind ? __builtin_ctzll(behind) : 0;
-      auto of = [&](int x) { return __builtin_amdgcn_readlane(x, f); };
-      r.t.seg = PagedSeg{of(g.b), of(g.batch), of(g.row0), behind ? of(g.n) : 0, of(g.len), of(g.first)};
-      const int count = max(of(tiles), 1), k = at - (of(upto) - of(mine));
-      r.split = behind ? k / count : 0;
-      r.t.local = behind ? count - 1 - (k - r.split * count) : 0;
-      r.least = max(1, of((blocks + parts - 1) / parts));   // a sequence's parts alike
-      r.tile = q.cu ? (int)paged_first_tile(q, f, p.G.d, rows, 1) + r.t.local : r.t.local * q.B + f;
-      return r;
-    }
-  }
-  r.t = paged_tile(q, job.tile, p.G.d, rows, 1);
-  return r;
+  const PagedPlanCall call{p.G, rows, p.c.Hk, p.splits, p.least, p.slots, p.tiles, p.causal != 0};
+  PagedWave w{};
+  if (p.slots) w.mine = paged_plan_seg(p.c.seqs, call, threadIdx.x & 63);
+  return paged_plan_of(p.c.seqs, call, (int)(blockIdx.x / (unsigned)p.c.Hk), w);
 }
-
-// Rows of a tile that starts at row r0 of its segment: row r0 + x is query head g Hk + hk of new token i, r = i G + g.
-struct PagedRowMap {
-  unsigned i0, rem, G;
-  PagedDiv div;
-  __device__ __forceinline__ PagedRowMap(int r0, const PagedDiv& g) : i0(g.of(r0)), rem(r0 - i0 * g.d), G(g.d), div(g) {}
-  __device__ __forceinline__ int token(int x) const { return (int)(i0 + div.of(rem + x)); }
-  __device__ __forceinline__ int group(int x) const { return (int)(rem + x - div.of(rem + x) * G); }
-};
 
 // Q_hat of a tile's rows, eight columns of a row at a time: their inputs, loaded ahead; made and stored as the sum of two
 // 16-bit parts each; and the zeros behind a row.
@@ -244,13 +181,6 @@ template <int ROWS>
 __device__ __forceinline__ void paged_query_tail(const PagedAttnParams& p, int at, int n, int cols, int stride, uint16_t* hi, uint16_t* lo) {
   const int D = p.c.D, R = p.c.R, E = R % 8 == 0 ? R + (D + 7) / 8 * 8 : D + R;
   for (int it = at; it < ROWS * (cols - E); it += n) hi[it % ROWS * stride + E + it / ROWS] = lo[it % ROWS * stride + E + it / ROWS] = 0;
-}
-
-// Blocks of keys a tile's rows see, over all of them.
-__device__ __forceinline__ int paged_tile_blocks(const PagedSeg& g, int local, int rows, const PagedDiv& G, bool causal) {
-  const int last = min((local + 1) * rows, g.n * (int)G.d) - 1;
-  const int limit = last < local * rows ? 0 : paged_limit(g.first + (int)G.of(last), g.len, causal);
-  return (limit + kBlockKeys - 1) / kBlockKeys;
 }
 
 template <typename T>

@@ -86,6 +86,32 @@ POPE_HD PagedSeg paged_seg(const PagedSeqs& q, int s) {   // packed segment s < 
   return g;
 }
 
+// The segment that tile `tile` belongs to, and its tile within it; seg.n = 0 where there is none.  Packed calls: 64 segments'
+// first tiles are tested at a time (`hits(f)`: bit i set where f(i) holds, a wave's ballot), and the last one at or below
+// `tile` has it (with bounds that decrease, any segment may come out, and paged_seg bounds it).  Padded calls: the
+// sequences' n-th tiles side by side.
+struct PagedTile { PagedSeg seg; int local; };
+template <typename Hits>
+POPE_HD PagedTile paged_tile_of(const PagedSeqs& q, int tile, int unit, int per, int extra, Hits&& hits) {
+  PagedTile t;
+  if (!q.cu) {
+    t.local = (int)((unsigned)tile / (unsigned)q.B);
+    t.seg = paged_seg(q, tile - t.local * q.B);
+    return t;
+  }
+  const int S = q.B + 2;
+  int found = 0;
+  for (int s0 = 0; s0 < S; s0 += 64) {
+    const uint64_t w = hits([&](int i) { return s0 + i < S && paged_first_tile(q, s0 + i < S ? s0 + i : 0, unit, per, extra) <= tile; });
+    if (!w) break;
+    found = s0 + 63 - __builtin_clzll(w);
+    if (found != s0 + 63) break;
+  }
+  t.seg = paged_seg(q, found);
+  t.local = (int)(tile - paged_first_tile(q, found, unit, per, extra));
+  return t;
+}
+
 // Keys a row at position pos sees: [0, limit).
 POPE_HD int paged_limit(int pos, int len, bool causal) { return !causal ? len : pos < 0 ? 0 : pos + 1 < len ? pos + 1 : len; }
 
@@ -104,6 +130,116 @@ POPE_HD PagedRange paged_range(int blocks, int splits, int least, int step, int 
   const int per = paged_split_blocks(blocks, splits, least, step);
   const int64_t lo = (int64_t)s * per, hi = lo + per;
   return PagedRange{lo < blocks ? (int)lo : blocks, hi < blocks ? (int)hi : blocks};
+}
+
+// A workgroup's tile and part of the key axis, where a tile has many rows.
+//
+// At most 64 segments (`slots`, the workgroups that the chip holds, is not 0): parts are cut by what the sequences
+// have, as few blocks as these workgroups get of all tiles' blocks, or more where the tiles' parts would then be more
+// than the workgroups.  A quarter of what causality takes from a prompt's first rows is left out: its heaviest tile has
+// twice the mean's blocks and would end alone (prompts of 4,096 tokens x 8 heads, D 64: 62 us so, 71 without; 8,192 x 8,
+// D 128: 270 / 309; 2 x 2,048 x 8, D 256: 139 / 161).
+// Parts that all fit then go to the first workgroups: with empty ones in between, the shader engines, which are dealt
+// workgroups in turn, get unequal work (20 rows of 16 sequences x 8 heads, D 128, every other one 64 tokens long, the
+// others 4,096: 38 us, 58 with empty ones in between).  Tiles of prompts keep their place instead, heaviest first over all
+// sequences (2 x 4,096 tokens: 89 us, 101 sequence by sequence).  So do those of bounds that descend: segments that share
+// rows can have more tiles than the grid, and the join would read parts that no workgroup has written.
+// Every workgroup computes the same sums in the same order.
+struct PagedPlanCall {   // the same in all of a call's workgroups
+  PagedDiv G;            // query heads of a key head
+  int rows, Hk;          // rows of a tile; key heads
+  int splits, least, slots;
+  int64_t tiles;
+  bool causal;
+};
+struct PagedPlanSeg {    // what a segment brings (a lane has one)
+  PagedSeg seg;
+  int tiles, blocks, unseen;
+  bool descends;         // its bounds do
+};
+POPE_HD PagedPlanSeg paged_plan_seg(const PagedSeqs& q, const PagedPlanCall& c, int s) {
+  PagedPlanSeg p = {};
+  if (s < (q.cu ? q.B + 2 : q.B)) {
+    p.seg = paged_seg(q, s);
+    p.descends = q.cu && paged_bound(q, s) > paged_bound(q, s + 1);
+    p.tiles = (int)(((int64_t)p.seg.n * c.G.d + c.rows - 1) / c.rows);
+    p.blocks = (p.seg.len + kBlockKeys - 1) / kBlockKeys;
+    const int rows = p.seg.n / kBlockKeys;
+    p.unseen = c.causal ? (rows < p.blocks ? rows : p.blocks) / 4 : 0;
+  }
+  return p;
+}
+// Workgroup `at` of a key head (split * tiles + tile, tiles in reverse: later ones see the most keys when causal).
+struct PagedPlan { PagedTile t; int tile, split, least; bool dealt; };
+// The wave: sum(f), any(f) and all(f) over its 64 segments; first_above(f, at): the first one whose sum of f up to and with it
+// exceeds `at`, and that sum without it (64: none does); of(i, f): f of the i-th; hits: as above.
+template <typename Wave>
+POPE_HD PagedPlan paged_plan_of(const PagedSeqs& q, const PagedPlanCall& c, int at, const Wave& w) {
+  PagedPlan r;
+  const unsigned n = (unsigned)c.tiles;
+  r.split = (int)((unsigned)at / n);
+  r.tile = (int)(n - 1 - ((unsigned)at - (unsigned)r.split * n));
+  r.least = c.least;
+  r.dealt = false;
+  if (c.slots) {
+    const float slots = (float)c.slots / (float)c.Hk;
+    const auto each = [](const PagedPlanSeg& s) { return (float)(s.blocks - s.unseen); };
+    // 2^26 blocks: all positions
+    const float even = __builtin_ceilf(w.sum([&](const PagedPlanSeg& s) { return (float)s.tiles * each(s); }) / slots);
+    const int cut = (int)(even < 67108864.f ? even : 67108864.f);
+    int least = c.least > cut ? c.least : cut;
+    bool fits = false;
+    for (int i = 0; i < 16 && !fits; ++i) {
+      fits = w.sum([&](const PagedPlanSeg& s) {
+        const float parts = __builtin_ceilf(each(s) / (float)least);
+        return (float)s.tiles * (parts > 1.f ? parts : 1.f);
+      }) <= slots;
+      if (!fits) least += least / 16 > 1 ? least / 16 : 1;
+    }
+    r.least = least;
+    if (fits && !w.any([](const PagedPlanSeg& s) { return s.descends || (s.tiles > 1 && 8 * s.unseen >= s.blocks); })) {
+      const auto parts = [&](const PagedPlanSeg& s) {
+        const int p = (s.blocks + least - 1) / least, m = p < c.splits ? p : c.splits;
+        return m > 1 ? m : 1;
+      };
+      int before;
+      const int f = w.first_above([&](const PagedPlanSeg& s) { return s.tiles * parts(s); }, at, &before);
+      r.dealt = true;
+      r.t.seg = PagedSeg{-1, 0, 0, 0, 0, 0};
+      r.t.local = r.split = r.tile = 0;
+      r.least = 1;
+      if (f == 64) return r;
+      const int count = w.of(f, [](const PagedPlanSeg& s) { return s.tiles; }), k = at - before;
+      r.split = k / count;
+      r.t.seg = PagedSeg{w.of(f, [](const PagedPlanSeg& s) { return s.seg.b; }),    w.of(f, [](const PagedPlanSeg& s) { return s.seg.batch; }),
+                         w.of(f, [](const PagedPlanSeg& s) { return s.seg.row0; }), w.of(f, [](const PagedPlanSeg& s) { return s.seg.n; }),
+                         w.of(f, [](const PagedPlanSeg& s) { return s.seg.len; }),  w.of(f, [](const PagedPlanSeg& s) { return s.seg.first; })};
+      r.t.local = count - 1 - (k - r.split * count);
+      r.tile = q.cu ? (int)paged_first_tile(q, f, c.G.d, c.rows, 1) + r.t.local : r.t.local * q.B + f;
+      const int same = w.of(f, [&](const PagedPlanSeg& s) { const int p = parts(s); return (s.blocks + p - 1) / p; });   // a sequence's parts alike
+      r.least = same > 1 ? same : 1;
+      return r;
+    }
+  }
+  r.t = paged_tile_of(q, r.tile, c.G.d, c.rows, 1, w);
+  return r;
+}
+
+// Rows of a tile that starts at row r0 of its segment: row r0 + x is query head g Hk + hk of new token i, r = i G + g.
+struct PagedRowMap {
+  unsigned i0, rem, G;
+  PagedDiv div;
+  POPE_HD PagedRowMap(int r0, const PagedDiv& g) : i0(g.of(r0)), rem(r0 - i0 * g.d), G(g.d), div(g) {}
+  POPE_HD int token(int x) const { return (int)(i0 + div.of(rem + x)); }
+  POPE_HD int group(int x) const { return (int)(rem + x - div.of(rem + x) * G); }
+};
+
+// Blocks of keys a tile's rows see, over all of them.
+POPE_HD int paged_tile_blocks(const PagedSeg& g, int local, int rows, const PagedDiv& G, bool causal) {
+  const int64_t all = (int64_t)g.n * G.d, end = (int64_t)(local + 1) * rows;
+  const int last = (int)(end < all ? end : all) - 1;
+  const int limit = last < local * rows ? 0 : paged_limit(g.first + (int)G.of(last), g.len, causal);
+  return (limit + kBlockKeys - 1) / kBlockKeys;
 }
 
 // Layout of a (page, head): blocks of 32 slots, each in the operand order of the 16x16x32 MFMAs that read it,

@@ -66,7 +66,7 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_rows_kernel(PagedA
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), lr = lane & 31, hf = lane >> 5;
 
   const PagedPlan job = paged_plan(p, kRows);
-  const int hk = job.hk;
+  const int hk = (int)(blockIdx.x % (unsigned)c.Hk);
   const PagedTile& t = job.t;
   const PagedSeg& g = t.seg;
   const int rows_all = g.n * (int)p.G.d, r0 = t.local * kRows;

@@ -29,6 +29,15 @@ def test_index_arithmetic(tmp_path):
     assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout
 
 
+def test_plan_of_many_rows(tmp_path):
+    """The plan's workgroups on the host: also with descending bounds every part that the join reads has been written."""
+    exe = str(tmp_path / "plan")
+    subprocess.run(["g++", "-O2", "-std=c++17", "-I", os.path.join(ROOT, "pope-pytorch_amd", "csrc"), os.path.join(ROOT, "tests", "paged_plan_check.cpp"),
+                    "-o", exe], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout
+
+
 # ---------------------------------------------------------------- C ABI
 
 def _desc(**kw):

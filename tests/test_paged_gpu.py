@@ -652,3 +652,18 @@ def test_refusals_on_the_gpu(cuda):
     c.v_pages = c.v_pages[:1]
     with pytest.raises(ValueError, match="do not fit"):
         paged_flash_attn_with_pope(q, c, emb, B.table, B.lengths)
+
+
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "all"])
+def test_segments_that_overlap(cuda, causal):
+    """Bounds that descend: nothing is said of these rows' values, but the call stays within its buffers (host test of the
+    plan), and the rows of the calls behind it are right."""
+    total = [4096 if causal else 1024] * 5
+    B = Batch(total, heads=1, D=32, R=16)
+    cu = torch.tensor([0, 1280, 0, 1280, 0, 1280], dtype=I32, device="cuda")
+    q = B.rand(1, 1, 1280, 32)
+    f = B.emb(torch.zeros(1280, dtype=torch.long, device="cuda"))
+    o = paged_flash_attn_with_pope(q, B.cache, f, B.table, B.lengths, cu_seqlens=cu, causal=causal)
+    torch.cuda.synchronize()
+    assert o.shape == q.shape
+    attend_and_check(B, [1280, 0, 3, 200, 1], packed=True, causal=causal)
