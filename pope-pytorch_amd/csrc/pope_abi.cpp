@@ -1065,6 +1065,15 @@ int check_pages(const pope_paged* d, const void* k, const void* v, const void* s
   return POPE_OK;
 }
 
+// A launch of workgroups of 256 threads has fewer than 2^32 threads in a dimension.  Fewer than 2^24 tiles also keep a tile's
+// first row (tile x 128) a 32-bit number, whatever bounds packed rows have.
+int check_paged_grid(int64_t tiles, int heads, int splits) {
+  const int64_t most = ((int64_t)1 << 24) - 1;
+  if (tiles > most || heads > most || tiles * heads > most || tiles * heads * splits > most)
+    return fail(POPE_ERR_UNSUPPORTED, "%lld tiles of rows x %d heads: too many workgroups", (long long)tiles, heads);
+  return POPE_OK;
+}
+
 pope::PagedCache paged_cache(const pope_paged& d, const void* k, const void* v, const void* scales, const int32_t* table,
                              const int32_t* lengths, const int32_t* cu) {
   pope::PagedCache c;
@@ -1140,9 +1149,13 @@ PagedShape paged_shape(const pope_paged& d, bool packed) {
   return s;
 }
 
-int check_paged_heads(const pope_paged* d) {
+// The shape of an attention call, or why there is none.
+int check_paged_attn(const pope_paged* d, bool packed, PagedShape* s) {
   if (d->Hq < 1 || d->Hq % d->Hk != 0) return fail(POPE_ERR_INVALID, "query heads %d must be a multiple of kv heads %d", d->Hq, d->Hk);
-  return POPE_OK;
+  if ((int64_t)d->N * (d->Hq / d->Hk) > ((int64_t)1 << 30))
+    return fail(POPE_ERR_UNSUPPORTED, "%d rows x %d query heads of a kv head: too many workgroups", d->N, d->Hq / d->Hk);
+  *s = paged_shape(*d, packed);
+  return check_paged_grid(s->tiles, d->Hk, s->splits);
 }
 
 int paged_rows(const pope_paged* d, void* k, void* v, const float* freqs, const float* bias, const void* k_pages, const void* v_pages,
@@ -1168,7 +1181,8 @@ int paged_rows(const pope_paged* d, void* k, void* v, const float* freqs, const 
   p.v_vec = whole(v, d->v_s, d->D);
   p.f_vec = d->R % 8 == 0 && aligned16(freqs) && aligned16(bias) && d->f_s[0] % 4 == 0 && d->f_s[1] % 4 == 0 && d->bias_sh % 4 == 0;
   p.blocks = pope::paged_tiles(d->B, d->N, cu != nullptr, 1, pope::kBlockKeys, 2);
-  if (p.blocks >= ((int64_t)1 << 31) || d->Hk > 65535) return fail(POPE_ERR_UNSUPPORTED, "%lld blocks of rows x %d heads: too many workgroups", (long long)p.blocks, d->Hk);
+  if (d->Hk > 65535) return fail(POPE_ERR_UNSUPPORTED, "%d kv heads: too many workgroups", d->Hk);
+  if ((rc = check_paged_grid(p.blocks, 1, 1))) return rc;   // heads: the grid's other dimension
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const hipError_t e = write ? pope::launch_paged_write(p, d->dtype, d->quantized != 0, s) : pope::launch_paged_read(p, d->dtype, d->quantized != 0, s);
   if (e != hipSuccess) return hip_fail(e, write ? "paged write launch" : "paged read launch");
@@ -1201,24 +1215,25 @@ int pope_paged_read(const pope_paged* d, const void* k_pages, const void* v_page
 }
 
 int pope_paged_workspace_bytes(const pope_paged* d, int packed, size_t* bytes) {
+  PagedShape sh;
   int rc = check_paged_call(d);
-  if (rc || (rc = check_paged_heads(d))) return rc;
+  if (rc || (rc = check_paged_attn(d, packed != 0, &sh))) return rc;
   if (!bytes) return fail(POPE_ERR_INVALID, "bytes is NULL");
-  *bytes = paged_shape(*d, packed != 0).bytes;
+  *bytes = sh.bytes;
   return POPE_OK;
 }
 
 int pope_paged_attn(const pope_paged* d, const void* q, const float* freqs, const void* k_pages, const void* v_pages, const uint8_t* scales,
                     const int32_t* table, const int32_t* lengths, const int32_t* cu, void* o, float* lse, void* workspace,
                     size_t workspace_bytes, void* stream) {
+  PagedShape sh;
   int rc = check_paged_call(d);
-  if (rc || (rc = check_paged_heads(d))) return rc;
+  if (rc || (rc = check_paged_attn(d, cu != nullptr, &sh))) return rc;
   if ((rc = check_strides("q", d->q_s, 3)) || (rc = check_strides("o", d->o_s, 3))) return rc;
   if (d->N == 0) return POPE_OK;
   if ((rc = check_pages(d, k_pages, v_pages, scales, table, lengths))) return rc;
   if (!q || !o) return fail(POPE_ERR_INVALID, "q, o must be non-NULL");
   if (d->R > 0 && !freqs) return fail(POPE_ERR_INVALID, "rotate dim %d > 0 needs freqs", d->R);
-  const PagedShape sh = paged_shape(*d, cu != nullptr);
   if ((rc = check_ws(sh.bytes, workspace, workspace_bytes))) return rc;
   pope::PagedAttnParams p;
   std::memset(&p, 0, sizeof p);
@@ -1245,7 +1260,6 @@ int pope_paged_attn(const pope_paged* d, const void* q, const float* freqs, cons
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + sh.part_o);
   p.parts = reinterpret_cast<int*>(static_cast<char*>(workspace) + sh.part_o + sh.part_ml);
-  if ((int64_t)d->N * (d->Hq / d->Hk) > ((int64_t)1 << 30) || sh.tiles * d->Hk * sh.splits >= ((int64_t)1 << 31)) return fail(POPE_ERR_UNSUPPORTED, "%lld row tiles x %d heads: too many workgroups", (long long)sh.tiles, d->Hk);
   const hipError_t e = pope::launch_paged_attn(p, sh.few, d->dtype, d->quantized != 0, reinterpret_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "paged attention launch");
   return POPE_OK;

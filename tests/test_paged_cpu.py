@@ -100,6 +100,20 @@ def test_abi_refuses_pointers_strides_and_workspace():
     assert write(d, k=None, v=None) == 0 and attn(d, None, 0) == 0
 
 
+@pytest.mark.parametrize("change", [dict(B=1 << 24, N=1), dict(B=1 << 23, N=2, Hk=2, Hq=40), dict(B=1, N=1 << 30, Hq=1, Hk=1)])
+def test_abi_refuses_grids_beyond_a_launch(change):
+    """A launch has fewer than 2^32 threads, and a tile's first row is a 32-bit number."""
+    L, d = _lib.lib(), _desc(**change)
+    n = ctypes.c_size_t()
+    calls = [lambda: L.pope_paged_write(ctypes.byref(d), _A, _A, _A, _A, _A, _A, None, _A, _A, None, None),
+             lambda: L.pope_paged_read(ctypes.byref(d), _A, _A, None, _A, _A, None, _A, _A, None)]
+    if d.N < 1 << 30:
+        calls += [lambda: L.pope_paged_workspace_bytes(ctypes.byref(d), 0, ctypes.byref(n)), lambda: L.pope_paged_workspace_bytes(ctypes.byref(d), 1, ctypes.byref(n)),
+                  lambda: L.pope_paged_attn(ctypes.byref(d), _A, _A, _A, _A, None, _A, _A, None, _A, None, _A, 1 << 14, None)]
+    for call in calls:
+        assert call() == 2 and "too many workgroups" in _lib.last_error(), _lib.last_error()
+
+
 # ---------------------------------------------------------------- Python checks
 
 def _call(**kw):
