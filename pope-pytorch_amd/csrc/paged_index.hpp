@@ -197,7 +197,7 @@ POPE_HD PagedPlan paged_plan_of(const PagedSeqs& q, const PagedPlanCall& c, int 
       if (!fits) least += least / 16 > 1 ? least / 16 : 1;
     }
     r.least = least;
-    if (fits && !w.any([](const PagedPlanSeg& s) { return s.descends || (s.tiles > 1 && 8 * s.unseen >= s.blocks); })) {
+    if (fits && !w.any([](const PagedPlanSeg& s) { return s.descends || (s.tiles > 1 && s.blocks > 0 && 8 * s.unseen >= s.blocks); })) {
       const auto parts = [&](const PagedPlanSeg& s) {
         const int p = (s.blocks + least - 1) / least, m = p < c.splits ? p : c.splits;
         return m > 1 ? m : 1;

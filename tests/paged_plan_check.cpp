@@ -130,6 +130,30 @@ int main(int argc, char**) {
     std::snprintf(g_what, sizeof g_what, "overlapping segments, causal %d", causal);
     CHECK(!walk(q, c, false));
   }
+  // Rows behind the last sequence, and sequences of length zero, have tiles and no keys: they leave the others' parts alike.
+  // (20 sequences x 2 heads of 4, 60 pages of 32; the grid as the host sizes it: at most two parts for each of 512 places)
+  for (const int gap : {0, 3, 150})
+    for (const int none : {0, 100})
+      for (const bool causal : {false, true}) {
+        int cu[21] = {0}, lens[20];
+        const int rows[] = {70, 33, none, 5, 300, 0, none, 100, 1, 40, 0, 0, 9, 8, 0, 64, 9, 8, 0, 64}, all[] = {1900, 40, 0, 1200};
+        for (int b = 0; b < 20; ++b) {
+          cu[b + 1] = cu[b] + rows[b];
+          lens[b] = all[b % 4];
+        }
+        const PagedSeqs q{lens, cu, 20, cu[20] + gap, 1920};
+        PagedPlanCall c;
+        c.G = paged_div(4);
+        c.rows = 128;
+        c.Hk = 2;
+        c.tiles = paged_tiles(20, q.N, true, 4, 128, 1);
+        c.splits = std::min<int>(4, 1024 / (2 * c.tiles));
+        c.least = 16;
+        c.slots = 512;
+        c.causal = causal;
+        std::snprintf(g_what, sizeof g_what, "%d rows behind, %d without keys, causal %d", gap, none, causal);
+        CHECK(walk(q, c, true));
+      }
   // rows: new token and query head of every row of a tile
   for (int G : {1, 2, 3, 5, 8, 20, 31}) {
     const PagedDiv div = paged_div(G);

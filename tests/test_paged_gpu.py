@@ -667,3 +667,12 @@ def test_segments_that_overlap(cuda, causal):
     torch.cuda.synchronize()
     assert o.shape == q.shape
     attend_and_check(B, [1280, 0, 3, 200, 1], packed=True, causal=causal)
+
+
+@pytest.mark.parametrize("gap", [0, 3, 150])
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "all"])
+def test_rows_without_keys_next_to_parts(cuda, causal, gap):
+    """Rows behind the last sequence and rows of sequences of length zero, several tiles of each, next to sequences whose keys
+    are cut into parts that the first workgroups get."""
+    B = Batch([1900, 40, 0, 1200] * 5, heads=2, G=4, D=96, R=48, page=32)
+    attend_and_check(B, [70, 33, 100, 5, 300, 0, 100, 100, 1, 40, 0, 0] + [9, 8, 0, 64] * 2, packed=True, causal=causal, gap=gap)
