@@ -134,6 +134,103 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_few_kernel(PagedAt
   for (int v = 0; v < VT; ++v) acc[v] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
   auto exponent = [](uint32_t w, int i) { return (int)((w >> (8 * i)) & 0xffu) - 127; };
+  // a block's running maximum and sum; P in operand order, in two parts; O^T += V^T P^T
+  float pr[8];
+  auto attend = [&](const f32x4* s, const uint32_t* sv) __attribute__((always_inline)) {
+    float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    mx = fmaxf(mx, wave_shfl_xor(mx, 16));
+    mx = half_swap_max(mx);
+    const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m - mu);
+    m = mn;
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      pr[j] = __builtin_amdgcn_exp2f(s[j >> 2][j & 3] - mu);
+      sum += pr[j];
+      if (Q8) pr[j] = __builtin_amdgcn_ldexpf(pr[j], exponent(sv[j >> 2], j & 3));
+    }
+    l = fmaf(l, alpha, sum);
+    u32x4 ph, pl;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ph[i] = V::pack2(pr[2 * i], pr[2 * i + 1]);
+      pl[i] = V::pack2(pr[2 * i] - V::to_float((uint16_t)ph[i]), pr[2 * i + 1] - V::to_float((uint16_t)(ph[i] >> 16)));
+    }
+#pragma unroll
+    for (int v = 0; v < VT; ++v) {
+      typename V::vec8 a;
+      if constexpr (Q8) a = as_vec8<typename V::vec8>(unpack_e4m3<V>(u32x2{vf[v >> 1][2 * (v & 1)], vf[v >> 1][2 * (v & 1) + 1]}, 1.f));
+      else a = as_vec8<typename V::vec8>(vf[v]);
+      acc[v] *= alpha;
+      acc[v] = V::mfma16(a, as_vec8<typename V::vec8>(ph), acc[v]);
+      acc[v] = V::mfma16(a, as_vec8<typename V::vec8>(pl), acc[v]);
+    }
+  };
+  // the values that are not finite of the keys in `odd`, where they are seen
+  auto add_seen = [&](int page, int blk, uint32_t odd) __attribute__((always_inline)) {
+    const int64_t at = paged_block_off(c, max(page, 0), hk, blk, c.v_head, VT * 512);
+#pragma unroll 1
+    for (int key = 0; key < kBlockKeys; ++key) {
+      if (!__any((odd >> key) & 1)) continue;
+      const int j = 4 * (key >> 4) + (key & 3);
+      float pk = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) pk = k == j ? pr[k] : pk;
+      pk = __shfl(pk, col + 16 * ((key & 15) >> 2), 64);
+      const bool seen = blk * kBlockKeys + key < lim;
+#pragma unroll
+      for (int v = 0; v < VT; ++v) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int64_t off = at + paged_v_off(Q8, key, v * 16 + quad * 4 + i);
+          const uint32_t w = Q8 ? ((static_cast<const uint8_t*>(c.v)[off] & 0x7f) == 0x7f ? 0x7fffu : 0u) : static_cast<const uint16_t*>(c.v)[off];
+          if (nonfinite16<T>(w) && seen) acc[v][i] = fmaf(pk, T::to_float((uint16_t)w), acc[v][i]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+  // The wave's blocks once more, for rows that infinite keys or values made NaN (paged_dev.hpp).
+  auto second_pass = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int v = 0; v < VT; ++v) acc[v] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll 1
+    for (int blk = range.begin + wave; blk < range.end; blk += WK) {
+      const int page = paged_page(c, g.b, blk);
+      if (page < 0) continue;
+      const char* keys = static_cast<const char*>(c.k) + paged_block_off(c, page, hk, blk, c.k_head, KS * 1024) * kE + lane * 16;
+      f32x4 s[2], lo[2];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) s[half] = lo[half] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          u32x4 fin, rest;
+          split_finite<T>(*reinterpret_cast<const u32x4*>(keys + (2 * ks + half) * 1024), &fin, &rest);
+          s[half] = T::mfma16(as_vec8<vec8>(fin), qh[ks], s[half]);
+          lo[half] = T::mfma16(as_vec8<vec8>(fin), ql[ks], lo[half]);
+          if (__any((rest[0] | rest[1] | rest[2] | rest[3]) != 0)) lo[half] = T::mfma16(as_vec8<vec8>(rest), sign_operand<T>(qh[ks]), lo[half]);
+        }
+      const int key0 = blk * kBlockKeys + quad * 4;
+      const uint32_t sv[2] = {0, 0};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        s[half] += lo[half];
+        if (T::kCode == 1) s[half] *= p.late;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[half][i] = key0 + 16 * half + i < lim ? s[half][i] : -INFINITY;
+      }
+      uint32_t odd = 0;
+      load_v(page, blk);
+#pragma unroll
+      for (int v = 0; v < kVL; ++v) clean_values<T, Q8>(vf[v], g.len - key0, 4 * quad, odd);
+      attend(s, sv);
+      add_seen(page, blk, odd);
+    }
+  };
   for (; blk < range.end; blk += WK) {
     const int next = blk + WK < range.end ? blk + WK : blk;   // the last one is loaded again, unused
     const int next_page = page_of(next);
@@ -178,77 +275,29 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_few_kernel(PagedAt
       // Slots from len on, and pages outside the cache, hold whatever was there: 0 x NaN must not count.  They become
       // zeros; so do values that are not finite, whose keys are noted and which are added below where they are seen.
 #pragma unroll
-      for (int v = 0; v < kVL; ++v)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t keep = 0;
-#pragma unroll
-          for (int e = 0; e < (Q8 ? 4 : 2); ++e) {
-            const int j = Q8 ? (4 * i + e) & 7 : 2 * i + e, key = 16 * (j >> 2) + (j & 3), sh = (Q8 ? 8 : 16) * e;
-            const uint32_t x = vf[v][i] >> sh;
-            const bool there = key < have, fin = Q8 ? (x & 0x7f) != 0x7f : !nonfinite16<T>(x);
-            keep |= there && fin ? (Q8 ? 0xffu : 0xffffu) << sh : 0u;
-            odd |= there && !fin ? 1u << (key + 4 * quad) : 0u;
-          }
-          vf[v][i] &= keep;
-        }
+      for (int v = 0; v < kVL; ++v) clean_values<T, Q8>(vf[v], have, 4 * quad, odd);
     }
-
-    // running maximum and sum; P in operand order, in two parts
-    float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-    mx = fmaxf(mx, wave_shfl_xor(mx, 16));
-    mx = half_swap_max(mx);
-    const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m - mu);
-    m = mn;
-    float pr[8], sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      pr[j] = __builtin_amdgcn_exp2f(s[j >> 2][j & 3] - mu);
-      sum += pr[j];
-      if (Q8) pr[j] = __builtin_amdgcn_ldexpf(pr[j], exponent(sv[j >> 2], j & 3));
-    }
-    l = fmaf(l, alpha, sum);
-    u32x4 ph, pl;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      ph[i] = V::pack2(pr[2 * i], pr[2 * i + 1]);
-      pl[i] = V::pack2(pr[2 * i] - V::to_float((uint16_t)ph[i]), pr[2 * i + 1] - V::to_float((uint16_t)(ph[i] >> 16)));
-    }
-
-    // O^T += V^T P^T
-#pragma unroll
-    for (int v = 0; v < VT; ++v) {
-      typename V::vec8 a;
-      if constexpr (Q8) a = as_vec8<typename V::vec8>(unpack_e4m3<V>(u32x2{vf[v >> 1][2 * (v & 1)], vf[v >> 1][2 * (v & 1) + 1]}, 1.f));
-      else a = as_vec8<typename V::vec8>(vf[v]);
-      acc[v] *= alpha;
-      acc[v] = V::mfma16(a, as_vec8<typename V::vec8>(ph), acc[v]);
-      acc[v] = V::mfma16(a, as_vec8<typename V::vec8>(pl), acc[v]);
-    }
+    attend(s, sv);
     load_v(next_page, next);
     if (edge && __any(odd != 0)) {
       POPE_COLD_PATH();
-      const int64_t at = paged_block_off(c, max(page, 0), hk, blk, c.v_head, VT * 512);
-#pragma unroll 1
-      for (int key = 0; key < kBlockKeys; ++key) {
-        if (!__any((odd >> key) & 1)) continue;
-        const int j = 4 * (key >> 4) + (key & 3);
-        float pk = 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) pk = k == j ? pr[k] : pk;
-        pk = __shfl(pk, col + 16 * ((key & 15) >> 2), 64);
-        const bool seen = blk * kBlockKeys + key < lim;
-#pragma unroll
-        for (int v = 0; v < VT; ++v)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int64_t off = at + paged_v_off(Q8, key, v * 16 + quad * 4 + i);
-            const uint32_t w = Q8 ? ((static_cast<const uint8_t*>(c.v)[off] & 0x7f) == 0x7f ? 0x7fffu : 0u) : static_cast<const uint16_t*>(c.v)[off];
-            if (nonfinite16<T>(w) && seen) acc[v][i] = fmaf(pk, T::to_float((uint16_t)w), acc[v][i]);
-          }
-      }
+      add_seen(page, blk, odd);
     }
     page = next_page;
+  }
+  if constexpr (!Q8) {
+    float x = l;
+#pragma unroll
+    for (int v = 0; v < VT; ++v) x += (acc[v][0] + acc[v][1]) + (acc[v][2] + acc[v][3]);
+    if (__builtin_expect(__any(x != x), 0)) {
+      POPE_COLD_PATH();
+      bool fin = true;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) fin = fin && all_finite<T>(qh[ks]);
+      const uint64_t nan = __ballot(x != x), off = __ballot(!fin);   // of a row: in any of its four lanes
+      const auto of_row = [&](uint64_t w) { return (w | w >> 16 | w >> 32 | w >> 48) & 0xffffu; };
+      if (of_row(nan) & ~of_row(off)) second_pass();
+    }
   }
   l += wave_shfl_xor(l, 16);
   l += wave_shfl_xor(l, 32);

@@ -189,4 +189,60 @@ __device__ __forceinline__ bool nonfinite16(uint32_t bits) {
   return (bits & e) == e;
 }
 
+// Rows that are NaN although their queries are not: infinite keys and values.  Products of a sum of two 16-bit parts, or of
+// a P that is 0 in 16 bits, turn an infinity into NaN (hi x inf + lo x inf; 0 x inf) where the formula has +-inf, or a score
+// of -inf and so a weight of 0.  The loops do not look for that: a wave (many rows: a workgroup) that ends with such rows goes
+// over its blocks a second time, with the finite elements of K times both parts, the others times the signs of Q_hat, and V's
+// others outside the product, as in blocks with keys that some row does not see.  What is finite goes through the same
+// operations in the same order, so the other rows keep their bits.  (A query column that 16 bits round to 0 counts as 0;
+// a row whose values or keys hold a NaN that it sees is computed twice and stays NaN.)  8-bit pages hold no infinity.
+//
+// A 16-bit operand's finite elements, and the others; zeros in the places of either's rest.
+template <typename T>
+__device__ __forceinline__ void split_finite(u32x4 w, u32x4* fin, u32x4* rest) {
+  constexpr uint32_t kOne = T::kCode == 2 ? 0x00800080u : 0x04000400u;   // carries into the sign where all exponent bits are set
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t m = ((((w[i] & 0x7fff7fffu) + kOne) & 0x80008000u) >> 15) * 0xffffu;
+    (*fin)[i] = w[i] & ~m;
+    (*rest)[i] = w[i] & m;
+  }
+}
+// The signs of an operand's elements: -1, 0 or 1.
+template <typename T>
+__device__ __forceinline__ typename T::vec8 sign_operand(typename T::vec8 q) {
+  constexpr uint32_t kUnit = T::kCode == 2 ? 0x3f803f80u : 0x3c003c00u;
+  u32x4 w = __builtin_bit_cast(u32x4, q);
+  asm volatile("" : "+v"(w));   // made where it is used, not in front of the loop
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = ((w[i] & 0x80008000u) | kUnit) & (((((w[i] & 0x7fff7fffu) + 0x7fff7fffu) & 0x80008000u) >> 15) * 0xffffu);
+  return as_vec8<typename T::vec8>(w);
+}
+template <typename T>
+__device__ __forceinline__ bool all_finite(typename T::vec8 q) {
+  u32x4 fin, rest;
+  split_finite<T>(__builtin_bit_cast(u32x4, q), &fin, &rest);
+  return (rest[0] | rest[1] | rest[2] | rest[3]) == 0;
+}
+
+// A 16-byte unit of values, of which the first keys below `have` are there (key 16 (j / 4) + j % 4 for element j of a 16-bit
+// unit; 8-bit: two units of 8): the others and what is not finite become zeros, and the latter's keys are noted in `odd`
+// (at `key0` in the block).
+template <typename T, bool Q8>
+__device__ __forceinline__ void clean_values(u32x4& w, int have, int key0, uint32_t& odd) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t keep = 0;
+#pragma unroll
+    for (int e = 0; e < (Q8 ? 4 : 2); ++e) {
+      const int j = Q8 ? (4 * i + e) & 7 : 2 * i + e, key = 16 * (j >> 2) + (j & 3), sh = (Q8 ? 8 : 16) * e;
+      const uint32_t x = w[i] >> sh;
+      const bool there = key < have, fin = Q8 ? (x & 0x7f) != 0x7f : !nonfinite16<T>(x);
+      keep |= there && fin ? (Q8 ? 0xffu : 0xffffu) << sh : 0u;
+      odd |= there && !fin ? 1u << (key + key0) : 0u;
+    }
+    w[i] &= keep;
+  }
+}
+
 }  // namespace pope

@@ -181,6 +181,26 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_rows_kernel(PagedA
   // to the compiler, each read stood right before its product and the vector work in front of or behind them all, and a
   // step of two workgroups took the sum of both, 3,700 cycles at D 64, R 32; it takes 2,860 so (the products alone: 2,048).
   constexpr int kAhead = Q8 || VT < 8 ? 6 : 4;
+  // what the products do not carry: fp16 takes a row's scale, and a softmax scale above 1, behind them
+  auto finish = [&](int slot, f32x16* s) {
+    if constexpr (kLate) {
+      if (Q8 || p.late != 1.f) {
+#pragma unroll
+        for (int b = 0; b < BG; ++b)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t w = Q8 ? *reinterpret_cast<const uint32_t*>(scales_of(slot, b) + paged_scale_off(key_of(4 * q) + 4 * hf, 0)) : 0u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[b][4 * q + i] = s[b][4 * q + i] * ((Q8 ? power(w, i) : 1.f) * p.late) - m;
+          }
+      } else {
+#pragma unroll
+        for (int b = 0; b < BG; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[b][i] -= m;
+      }
+    }
+  };
   auto scores = [&](int slot, f32x16* s, auto&& between) {
     const char* stage = stage_of(slot);
     float unit[BG];
@@ -207,24 +227,26 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_rows_kernel(PagedA
       between(2 * i + 1, 2 * n);
       __builtin_amdgcn_sched_barrier(0);
     }
-    // what the products do not carry: fp16 takes a row's scale, and a softmax scale above 1, behind them
-    if constexpr (kLate) {
-      if (Q8 || p.late != 1.f) {
+    finish(slot, s);
+  };
+  // the same in the second pass: finite elements of K times both parts of Q_hat, the others times its signs
+  auto careful_scores = [&](int slot, f32x16* s) {
+    const char* stage = stage_of(slot);
 #pragma unroll
-        for (int b = 0; b < BG; ++b)
+    for (int b = 0; b < BG; ++b)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint32_t w = Q8 ? *reinterpret_cast<const uint32_t*>(scales_of(slot, b) + paged_scale_off(key_of(4 * q) + 4 * hf, 0)) : 0u;
+      for (int i = 0; i < 16; ++i) s[b][i] = kLate ? 0.f : -m;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[b][4 * q + i] = s[b][4 * q + i] * ((Q8 ? power(w, i) : 1.f) * p.late) - m;
-          }
-      } else {
-#pragma unroll
-        for (int b = 0; b < BG; ++b)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[b][i] -= m;
-      }
+    for (int i = 0; i < K16 * BG; ++i) {
+      const int b = i % BG, k = i / BG;
+      u32x4 w, fin, rest;
+      if constexpr (!Q8) w = k_read(stage, b, k);
+      split_finite<T>(w, &fin, &rest);
+      s[b] = T::mfma32(as_vec8<vec8>(fin), qh[k], s[b]);
+      s[b] = T::mfma32(as_vec8<vec8>(fin), ql[k], s[b]);
+      if (__any((rest[0] | rest[1] | rest[2] | rest[3]) != 0)) s[b] = T::mfma32(as_vec8<vec8>(rest), sign_operand<T>(qh[k]), s[b]);
     }
+    finish(slot, s);
   };
   auto mask = [&](int st, f32x16* s) {
 #pragma unroll
@@ -314,6 +336,7 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_rows_kernel(PagedA
   // Blocks with keys that some row of the tile does not see: 0 x NaN must not count.  Slots from len on, and pages outside
   // the cache, hold whatever was there and become zeros in the stage; values that are not finite do too, and their keys are
   // noted, for `add_seen` to add them outside the product where they are seen.
+  // The second pass (rows that infinite keys or values made NaN, paged_dev.hpp) does so in all blocks.
   auto tile_edge = [&](int st) { return range.begin + (st + 1) * BG > tile_blocks || lost; };
   auto sanitize = [&](int st, int slot) {
     char* stage = smem + slot;
@@ -430,7 +453,11 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_rows_kernel(PagedA
     if (st + C::kSlots - 1 < steps) issue(st + C::kSlots - 1, put);
     put = next_slot(put);
   };
-  if (wave * 32 >= count) {   // a wave without rows: the others' loads and barriers
+  const bool idle = wave * 32 >= count;
+  f32x16 sa[BG], sb[C::kPipe ? BG : 1];
+  u32x4 pw[BG][2 * kParts];
+  int slot = 0;   // stage of the current step
+  if (idle) {   // a wave without rows: the others' loads and barriers
     int at = 0;
     if constexpr (C::kPipe) {
       if (steps > 0) {
@@ -458,111 +485,160 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_rows_kernel(PagedA
         at = next_slot(at);
       }
     }
-    return;
-  }
-  f32x16 sa[BG], sb[C::kPipe ? BG : 1];
-  u32x4 pw[BG][2 * kParts];
-  int slot = 0;   // stage of the current step
-  if constexpr (C::kPipe) {
-    float mx = -INFINITY;
-    if (steps > 0) {
-      if (steps >= C::kSlots - 1) wait_vmcnt<(C::kSlots - 2) * kLeast>();
-      else wait_vmcnt<0>();
-      __syncthreads();
-      if (tile_edge(0)) {
-        POPE_COLD_PATH();
-        sanitize(0, 0);
-      }
-      scores(0, sa, nothing);
-      if (edge_of(0)) {
-        POPE_COLD_PATH();
-        mask(0, sa);
-      }
-      mx = row_max(sa);
-    }
-    auto step = [&](int st, f32x16* cur, f32x16* nxt) {
-      const int ahead = next_slot(slot);
-      rescale(mx, cur);
-      landed(st + 1);
-      __syncthreads();   // stage st + 1 is whole, and the values of stage st are clean; stage st - 1 is free
-      refill(st);
-      if (tile_edge(st + 1)) {
-        POPE_COLD_PATH();
-        sanitize(st + 1, ahead);   // its V is read behind the next barrier
-      }
-#pragma unroll
-      for (int b = 0; b < BG; ++b) asm volatile("" : "+v"(cur[b]));   // nothing of it above the branches before
-      scores(ahead, nxt, [&](int i, int n) {
-#pragma unroll
-        for (int u = i * 8 * BG / n; u < (i + 1) * 8 * BG / n; ++u) prob(slot, cur, pw, u);
-      });
-      if (edge_of(st + 1)) {
-        POPE_COLD_PATH();
-        mask(st + 1, nxt);
-      }
-      mx = -INFINITY;
-      products(slot, pw, [&](int i, int n) {
-#pragma unroll
-        for (int x = i * 16 * BG / n; x < (i + 1) * 16 * BG / n; ++x) mx = fmaxf(mx, nxt[x / 16][x % 16]);
-        asm volatile("" : "+v"(mx));
-      });
-      mx = half_swap_max(mx);
-      if (tile_edge(st)) {
-        POPE_COLD_PATH();
-        add_seen(st, cur);
-      }
-      slot = ahead;
-    };
-    auto last = [&](int st, f32x16* cur) {
-      __syncthreads();   // the values of stage st are clean
-      rescale(mx, cur);
-      probs(slot, cur, pw);
-      products(slot, pw, nothing);
-      if (tile_edge(st)) {
-        POPE_COLD_PATH();
-        add_seen(st, cur);
-      }
-    };
-    int st = 0;
-    for (; st + 2 < steps; st += 2) {
-      step(st, sa, sb);
-      step(st + 1, sb, sa);
-    }
-    if (st + 2 == steps) {
-      step(st, sa, sb);
-      last(st + 1, sb);
-    } else if (st + 1 == steps) {
-      last(st, sa);
-    }
   } else {
-    for (int st = 0; st < steps; ++st) {
-      landed(st);
-      __syncthreads();   // stage st is whole; stage st - 1 is free
-      refill(st);
-      const bool edge = tile_edge(st);
-      if (edge) {
-        POPE_COLD_PATH();
+    if constexpr (C::kPipe) {
+      float mx = -INFINITY;
+      if (steps > 0) {
+        if (steps >= C::kSlots - 1) wait_vmcnt<(C::kSlots - 2) * kLeast>();
+        else wait_vmcnt<0>();
+        __syncthreads();
+        if (tile_edge(0)) {
+          POPE_COLD_PATH();
+          sanitize(0, 0);
+        }
+        scores(0, sa, nothing);
+        if (edge_of(0)) {
+          POPE_COLD_PATH();
+          mask(0, sa);
+        }
+        mx = row_max(sa);
+      }
+      auto step = [&](int st, f32x16* cur, f32x16* nxt) {
+        const int ahead = next_slot(slot);
+        rescale(mx, cur);
+        landed(st + 1);
+        __syncthreads();   // stage st + 1 is whole, and the values of stage st are clean; stage st - 1 is free
+        refill(st);
+        if (tile_edge(st + 1)) {
+          POPE_COLD_PATH();
+          sanitize(st + 1, ahead);   // its V is read behind the next barrier
+        }
+#pragma unroll
+        for (int b = 0; b < BG; ++b) asm volatile("" : "+v"(cur[b]));   // nothing of it above the branches before
+        scores(ahead, nxt, [&](int i, int n) {
+#pragma unroll
+          for (int u = i * 8 * BG / n; u < (i + 1) * 8 * BG / n; ++u) prob(slot, cur, pw, u);
+        });
+        if (edge_of(st + 1)) {
+          POPE_COLD_PATH();
+          mask(st + 1, nxt);
+        }
+        mx = -INFINITY;
+        products(slot, pw, [&](int i, int n) {
+#pragma unroll
+          for (int x = i * 16 * BG / n; x < (i + 1) * 16 * BG / n; ++x) mx = fmaxf(mx, nxt[x / 16][x % 16]);
+          asm volatile("" : "+v"(mx));
+        });
+        mx = half_swap_max(mx);
+        if (tile_edge(st)) {
+          POPE_COLD_PATH();
+          add_seen(st, cur);
+        }
+        slot = ahead;
+      };
+      auto last = [&](int st, f32x16* cur) {
+        __syncthreads();   // the values of stage st are clean
+        rescale(mx, cur);
+        probs(slot, cur, pw);
+        products(slot, pw, nothing);
+        if (tile_edge(st)) {
+          POPE_COLD_PATH();
+          add_seen(st, cur);
+        }
+      };
+      int st = 0;
+      for (; st + 2 < steps; st += 2) {
+        step(st, sa, sb);
+        step(st + 1, sb, sa);
+      }
+      if (st + 2 == steps) {
+        step(st, sa, sb);
+        last(st + 1, sb);
+      } else if (st + 1 == steps) {
+        last(st, sa);
+      }
+    } else {
+      for (int st = 0; st < steps; ++st) {
+        landed(st);
+        __syncthreads();   // stage st is whole; stage st - 1 is free
+        refill(st);
+        const bool edge = tile_edge(st);
+        if (edge) {
+          POPE_COLD_PATH();
+          sanitize(st, slot);
+          __syncthreads();
+        }
+        scores(slot, sa, nothing);
+        if (edge_of(st)) {
+          POPE_COLD_PATH();
+          mask(st, sa);
+        }
+        rescale(row_max(sa), sa);
+        // the first half of the keys' probabilities, the second half's under the first half's products
+#pragma unroll
+        for (int u = 0; u < 4; ++u) prob(slot, sa, pw, u);
+        products(slot, pw, [&](int i, int) {
+#pragma unroll
+          for (int u = 4 + 4 * i / NDB; u < 8 && u < 4 + 4 * (i + 1) / NDB; ++u) prob(slot, sa, pw, u);
+        });
+        if (edge) {
+          POPE_COLD_PATH();
+          add_seen(st, sa);
+        }
+        slot = next_slot(slot);
+      }
+    }
+  }
+  // ---- a second pass, for rows that infinite keys or values made NaN (paged_dev.hpp) ----------------------------
+  if constexpr (!Q8) {
+    float x = l;
+#pragma unroll
+    for (int d = 0; d < NDB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x += acc[d][i];
+    if (__builtin_expect(__any(x != x), false)) {
+      POPE_COLD_PATH();
+      bool fin = true;
+#pragma unroll
+      for (int k = 0; k < K16; ++k) fin = fin && all_finite<T>(qh[k]);
+      const uint64_t nan = __ballot(x != x && live), off = __ballot(!fin);   // of a row: in either of its lanes
+      if ((uint32_t)(nan | nan >> 32) & ~(uint32_t)(off | off >> 32)) odd[3] = 1;   // no step has a fourth block
+    }
+    __syncthreads();
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(odd[3]), 0)) {
+      POPE_COLD_PATH();
+      m = l = 0.f;
+      set = false;
+#pragma unroll
+      for (int d = 0; d < NDB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+      page_base = range.begin >> c.blk_shift;
+      window();
+      put = 0;
+#pragma unroll 1
+      for (int st = 0; st < C::kSlots - 1; ++st) {
+        if (st < steps) issue(st, put);
+        put += C::kStage;
+      }
+      slot = 0;
+#pragma unroll 1
+      for (int st = 0; st < steps; ++st) {
+        landed(st);
+        __syncthreads();
+        refill(st);
         sanitize(st, slot);
         __syncthreads();
+        if (!idle) {
+          careful_scores(slot, sa);
+          mask(st, sa);
+          rescale(row_max(sa), sa);
+          probs(slot, sa, pw);
+          products(slot, pw, nothing);
+          add_seen(st, sa);
+        }
+        slot = next_slot(slot);
       }
-      scores(slot, sa, nothing);
-      if (edge_of(st)) {
-        POPE_COLD_PATH();
-        mask(st, sa);
-      }
-      rescale(row_max(sa), sa);
-      // the first half of the keys' probabilities, the second half's under the first half's products
-#pragma unroll
-      for (int u = 0; u < 4; ++u) prob(slot, sa, pw, u);
-      products(slot, pw, [&](int i, int) {
-#pragma unroll
-        for (int u = 4 + 4 * i / NDB; u < 8 && u < 4 + 4 * (i + 1) / NDB; ++u) prob(slot, sa, pw, u);
-      });
-      if (edge) {
-        POPE_COLD_PATH();
-        add_seen(st, sa);
-      }
-      slot = next_slot(slot);
     }
   }
   l += wave_shfl_xor(l, 32);

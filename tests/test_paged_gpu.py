@@ -676,3 +676,92 @@ def test_rows_without_keys_next_to_parts(cuda, causal, gap):
     are cut into parts that the first workgroups get."""
     B = Batch([1900, 40, 0, 1200] * 5, heads=2, G=4, D=96, R=48, page=32)
     attend_and_check(B, [70, 33, 100, 5, 300, 0, 100, 100, 1, 40, 0, 0] + [9, 8, 0, 64] * 2, packed=True, causal=causal, gap=gap)
+
+
+def with_infinities(q, freqs, k, v, R, scale, causal, dtype):
+    """`reference` where held rows have infinities and NaN: the formula in 64 bits, an infinite value counting where its key
+    is seen.  The bounds are `reference`'s, with the formula's own weights (a key of score -inf has none, so it must not
+    share in sum_j p_j |v_j|, as it does where its infinity is taken for 0) and the finite elements of keys and values: an
+    infinity that counts leaves nothing to round."""
+    n, L, G = q.shape[1], k.shape[1], q.shape[0] // k.shape[0]
+    fin = lambda t: torch.where(t.isfinite(), t, 0.0)
+    qh = rows64(q, freqs, torch.zeros(1, R, device="cuda"), R).cpu()
+    k, v = k.repeat(G, 1, 1).cpu(), v.repeat(G, 1, 1).cpu()
+    see = torch.arange(L) <= (L - n + torch.arange(n))[:, None] if causal else torch.ones(n, L, dtype=torch.bool)
+    sc = (torch.bmm(qh, k.transpose(1, 2).contiguous()) * scale).masked_fill(~see, -INF)
+    p = torch.softmax(sc.masked_fill(~see.any(-1)[:, None], 0.0), -1).masked_fill(~see, 0.0)
+    o, pv = torch.bmm(p, fin(v)), torch.bmm(p, fin(v).abs())
+    A = (torch.bmm(qh.abs(), fin(k).abs().transpose(1, 2).contiguous()) * abs(scale)).masked_fill(sc == -INF, 0.0)
+    u, f16 = torch.finfo(dtype).eps / 2, dtype == torch.float16
+    x = (u * u + k.shape[-1] * 2.0 ** -24 + 1e-6) * A.amax(-1, keepdim=True)
+    if f16:
+        x = x + 2.0 ** -25 * fin(k).abs().sum(-1).amax(-1)[:, None, None] * abs(scale)
+    tol = u * o.abs() + (u + 2 * x + 2e-5) * pv + 2.0 ** -25
+    if f16:
+        tol = tol + 2.0 ** -25 * fin(v).abs().sum(1, keepdim=True)
+    for j in (~v.isfinite()).any(-1).any(0).nonzero().flatten().tolist():
+        o += torch.where(see[:, j, None] & ~v[:, j].isfinite()[:, None, :], p[..., j, None] * torch.where(v[:, j].isfinite(), 0.0, v[:, j])[:, None, :], 0.0)
+    return o.cuda(), torch.logsumexp(sc, -1).cuda(), tol.cuda(), x[..., 0].cuda() + 1e-5
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("D", [64, 128, 200])
+@pytest.mark.parametrize("n,G", [(1, 1), (3, 4), (40, 1), (150, 2)])
+@pytest.mark.parametrize("where", ["values", "keys", "both"])
+def test_infinities_seen(cuda, dtype, D, n, G, where):
+    """Infinite keys and values that rows see, in every block: a key's infinity against a column of the other sign has weight 0,
+    an infinite value makes its column of the output infinite."""
+    total = [2500, 700, 151, 33]
+    B = Batch(total, heads=2, G=G, D=D, R=32, dtype=dtype)
+    for b, t in enumerate(total):
+        at = int(B.cu[b])
+        if where != "keys":
+            for pos, col, x in ((3, 5, INF), (31, 6, -INF), (t // 2, 7, INF), (t // 2 + 1, 7, -INF), (t - 1, 8, INF), (t // 3, D - 1, -INF)):
+                B.v[0, :, at + pos, col] = x
+        if where != "values":
+            for pos, col, x in ((2, 40, INF), (t // 2, 41, -INF), (t - 1, 40, INF)):
+                B.k[0, :, at + pos, col] = x
+    paged_cache_write(B.cache, B.k, B.v, B.emb(B.pos), B.table, B.lengths, cu_seqlens=B.cu)
+    pos = B.lengths[:, None].long() - n + torch.arange(n, device="cuda")
+    q = B.rand(4, 2 * G, n, D)
+    q[:, ::2, :, 40].abs_().neg_()   # half of the heads give the infinite keys no weight, where their rows' signs are such
+    q[:, ::2, :, 41].abs_()
+    for causal in (True, False):
+        o, lse = paged_flash_attn_with_pope(q, B.cache, B.emb(pos), B.table, B.lengths, causal=causal, return_lse=True)
+        for b in range(4):
+            k, v = B.rows(b)
+            want, wl, tol, ltol = with_infinities(q[b], angles(pos[b], 32), k, v, 32, D ** -0.5, causal, dtype)
+            got = o[b].double()
+            assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf()) and torch.equal(got[got.isinf()], want[want.isinf()])
+            fin = want.isfinite()
+            assert ((got - want).abs()[fin] <= tol[fin]).all(), ((got - want).abs() / tol)[fin].max().item()
+            assert fin.any()
+            gl = lse[b].double()
+            assert torch.equal(gl.isnan(), wl.isnan() | (wl == INF))   # a score of +inf: no weights, and no sum of them
+            fin = wl.isfinite()
+            assert torch.equal(gl.isfinite(), fin) and ((gl - wl).abs()[fin] <= (ltol + 1e-6 * wl.abs())[fin]).all()
+
+
+@pytest.mark.parametrize("n,G", [(1, 1), (40, 1)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_infinities_next_to_bad_pages(cuda, n, G, D):
+    """Infinities seen where pages of the same sequence lie outside the cache: as the CPU cache has it."""
+    B = Batch([1500, 90], heads=2, G=G, D=D, R=32, page=32)
+    B.v[0, :, 10, 4], B.v[0, :, 700, 5], B.k[0, :, 300, 40] = INF, -INF, INF
+    B.v[0, :, 1500 + 33, 6] = -INF
+    paged_cache_write(B.cache, B.k, B.v, B.emb(B.pos), B.table, B.lengths, cu_seqlens=B.cu)
+    B.table[0, 3], B.table[0, 20], B.table[1, 0] = -1, 2 ** 31 - 1, B.cache.num_pages
+    C = PagedPoPECache(B.cache.num_pages, heads=2, dim=D, rotate_dim=32, page_size=32)
+    C.k_pages.copy_(B.cache.k_pages), C.v_pages.copy_(B.cache.v_pages)
+    pos = B.lengths[:, None].long() - n + torch.arange(n, device="cuda")
+    q = B.rand(2, 2 * G, n, D)
+    q[:, ::2, :, 40].abs_().neg_()
+    emb = B.emb(pos)
+    for causal in (True, False):
+        got = paged_flash_attn_with_pope(q, B.cache, emb, B.table, B.lengths, causal=causal).float().cpu()
+        want = paged_flash_attn_with_pope(q.cpu(), C, tuple(t.cpu() for t in emb), B.table.cpu(), B.lengths.cpu(), causal=causal).float()
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf()) and torch.equal(got[got.isinf()], want[got.isinf()])
+        fin = want.isfinite()
+        assert fin.any() and want.isinf().any()
+        # both fp32 arithmetic over the same rows: a rounding each, and P's in the many-row kernel, of outputs below 4
+        assert ((got - want).abs()[fin] <= 4 * 2.0 ** -8 * 3).all()
