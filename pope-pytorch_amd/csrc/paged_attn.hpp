@@ -330,12 +330,12 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_few_kernel(PagedAt
 
   // ---- output, or this split's part ----------------------------------------------------------------------------
   const int64_t row = (((int64_t)job.tile * c.Hk + hk) * kRows + col) * p.splits + job.split;
-  const float inv = part ? 1.f : l == 0.f ? 0.f : 1.f / l;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   uint16_t* dst = p.o + (int64_t)g.batch * p.o_s[0] + (int64_t)row_h * p.o_s[1] + (int64_t)(g.row0 + row_i) * p.o_s[2];
 #pragma unroll
   for (int v = 0; v < VT; ++v) {
     const int d = v * 16 + quad * 4;
-    const f32x4 x = acc[v] * inv;
+    const f32x4 x = part ? acc[v] : averages<T>(acc[v] * inv);
     if (part) {
       *reinterpret_cast<f32x4*>(p.part_o + row * (VT * 16) + d) = x;
     } else if (p.o_vec) {
@@ -403,12 +403,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p, int 
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int r = t.local * rows + rr, i = (int)p.G.of(r), h = (r - i * (int)p.G.d) * c.Hk + hk;
     uint16_t* dst = p.o + (int64_t)g.batch * p.o_s[0] + (int64_t)h * p.o_s[1] + (int64_t)(g.row0 + i) * p.o_s[2] + d;
+    const f32x4 x = averages<T>(o * inv);
     if (p.o_vec) {
-      *reinterpret_cast<u32x2*>(dst) = u32x2{T::pack2(o[0] * inv, o[1] * inv), T::pack2(o[2] * inv, o[3] * inv)};
+      *reinterpret_cast<u32x2*>(dst) = u32x2{T::pack2(x[0], x[1]), T::pack2(x[2], x[3])};
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (d + k < c.D) dst[k] = T::bits(o[k] * inv);
+        if (d + k < c.D) dst[k] = T::bits(x[k]);
     }
     if (p.lse && d == 0)
       p.lse[((int64_t)g.batch * p.Hq + h) * p.N + g.row0 + i] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;

@@ -74,9 +74,6 @@ __device__ __forceinline__ int row_exponent(float amax) {
   return min(max(e, -126), 126) + 127;
 }
 
-// What counts for a row's maximum, and what is stored of x: e4m3 has no infinity.
-__device__ __forceinline__ bool finite_f(float x) { return fabsf(x) <= 3.402823466e38f; }
-
 // The block's tokens of the call.
 struct Block {
   PagedSeg seg;
@@ -299,11 +296,16 @@ __global__ __launch_bounds__(kThreads) void paged_write_kernel(PagedRowsParams p
   }
 }
 
-// A dequantised value in the 16-bit type; fp16 has no value above 65504 (a code may round up to one).
+// 8-bit rows: the code of a row's largest may stand for more than the 16-bit type holds (fp16: 65536, bf16: 2^128), where the
+// row's exponent is above kMostExp (448 2^kMostExp is in range).  e4m3 has no infinity, so that an infinity of a dequantised
+// pair of values is such a code, and becomes the type's largest.
 template <typename T>
-__device__ __forceinline__ uint16_t value_bits(float x) {
-  if (T::kCode == 1 && finite_f(x)) x = fminf(fmaxf(x, -65504.f), 65504.f);
-  return T::bits(x);
+constexpr int kMostExp = T::kCode == 1 ? 7 : 119;
+template <typename T>
+__device__ __forceinline__ uint32_t in_range(uint32_t pair) {
+  constexpr uint32_t kInf = T::kCode == 1 ? 0x7c007c00u : 0x7f807f80u;
+  const uint32_t other = (((pair ^ kInf) & 0x7fff7fffu) + 0x7fff7fffu) & 0x80008000u;
+  return pair - ((other ^ 0x80008000u) >> 15);
 }
 
 template <typename T, bool Q8, int VT>
@@ -318,6 +320,7 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(PagedRowsParams p)
   const uint8_t* scales = Q8 && b.page >= 0 ? c.scales + paged_scale_base(c, b.page, hk, b.blk) : nullptr;
   const int D = c.D, R = c.R, E = D + R, KE = c.steps * 32;
   auto scale = [&](int t, int which) { return (int)scales[paged_scale_off(t, which)] - 127; };
+  const bool wide = Q8 && scales && __any((int)scales[lane] - 127 > kMostExp<T>);   // of the block's rows, some may leave the type
   auto code_at = [&](u32x2 w, int j) {
     const uint32_t x = w[j >> 2] >> (8 * (j & 3));
     return __builtin_amdgcn_cvt_f32_fp8((int)x, 0);
@@ -335,8 +338,7 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(PagedRowsParams p)
             const int e = scale(t, 0);
 #pragma unroll
             for (int j = 0; j < 8; j += 2)
-              *reinterpret_cast<uint32_t*>(rows + t * ST + e0 + j) = value_bits<T>(__builtin_amdgcn_ldexpf(code_at(w, j), e)) |
-                                                                    (uint32_t)value_bits<T>(__builtin_amdgcn_ldexpf(code_at(w, j + 1), e)) << 16;
+              *reinterpret_cast<uint32_t*>(rows + t * ST + e0 + j) = T::pack2(__builtin_amdgcn_ldexpf(code_at(w, j), e), __builtin_amdgcn_ldexpf(code_at(w, j + 1), e));
           } else {
             const int ln = u & 63, half = (u >> 6) & 1, st = u >> 7, t = half * 16 + (ln & 15), e0 = st * 32 + 8 * (ln >> 4);
             *reinterpret_cast<u32x4*>(rows + t * ST + e0) = *reinterpret_cast<const u32x4*>(src + u * 16);
@@ -351,7 +353,7 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(PagedRowsParams p)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const int t = t0 + 16 * (j >> 2) + (j & 3);
-              rows[t * ST + d] = value_bits<T>(__builtin_amdgcn_ldexpf(code_at(w, j), scale(t, 1)));
+              rows[t * ST + d] = T::bits(__builtin_amdgcn_ldexpf(code_at(w, j), scale(t, 1)));
             }
           } else {
             const int ln = u & 63, d = (u >> 6) * 16 + (ln & 15), t0 = 4 * (ln >> 4);
@@ -380,6 +382,11 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(PagedRowsParams p)
             for (int k = 0; k < 4; ++k) w[k] = ((cs[k >> 1] >> (16 * (k & 1))) & 0xffffu) | (sn[k >> 1] >> (16 * (k & 1))) << 16;
           }
         }
+        if (Q8 && wide) {
+          POPE_COLD_PATH();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = in_range<T>(w[k]);
+        }
         uint16_t* dst = which ? static_cast<uint16_t*>(p.v) + b.seg.batch * p.v_s[0] + hk * p.v_s[1] + n * p.v_s[2]
                               : static_cast<uint16_t*>(p.k) + b.seg.batch * p.k_s[0] + hk * p.k_s[1] + n * p.k_s[2];
         *reinterpret_cast<u32x4*>(dst + x) = w;
@@ -392,7 +399,8 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(PagedRowsParams p)
                               : static_cast<uint16_t*>(p.k) + b.seg.batch * p.k_s[0] + hk * p.k_s[1] + n * p.k_s[2];
         for (int x = lane; x < cols; x += 64) {
           const int e = which || x >= 2 * R ? x : (x & 1) * R + (x >> 1);
-          dst[x] = b.page >= 0 ? rows[t * ST + e] : (uint16_t)0;
+          const uint16_t w = b.page >= 0 ? rows[t * ST + e] : (uint16_t)0;
+          dst[x] = Q8 && wide ? (uint16_t)in_range<T>(w) : w;
         }
       }
     }

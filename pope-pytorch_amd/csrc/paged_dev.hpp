@@ -189,6 +189,19 @@ __device__ __forceinline__ bool nonfinite16(uint32_t bits) {
   return (bits & e) == e;
 }
 
+__device__ __forceinline__ bool finite_f(float x) { return fabsf(x) <= 3.402823466e38f; }
+
+// An average of values, as it goes out: fp16's stay finite where the values were.  A value of an 8-bit page may stand for 65536
+// (it is read as 65504 too), and P is rounded where its sum is not, which may carry an average up to 2^-11 past the values.
+template <typename T>
+__device__ __forceinline__ f32x4 averages(f32x4 x) {
+  if constexpr (T::kCode == 1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = finite_f(x[i]) ? fminf(fmaxf(x[i], -65504.f), 65504.f) : x[i];
+  }
+  return x;
+}
+
 // Rows that are NaN although their queries are not: infinite keys and values.  Products of a sum of two 16-bit parts, or of
 // a P that is 0 in 16 bits, turn an infinity into NaN (hi x inf + lo x inf; 0 x inf) where the formula has +-inf, or a score
 // of -inf and so a weight of 0.  The loops do not look for that: a wave (many rows: a workgroup) that ends with such rows goes

@@ -658,6 +658,7 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_rows_kernel(PagedA
       f32x4 x;
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[i] = acc[d][4 * q + i] * f;
+      if (!part) x = averages<T>(x);
       if (part) {
         *reinterpret_cast<f32x4*>(p.part_o + row * (VT * 16) + col) = x;
       } else if (p.o_vec) {

@@ -414,8 +414,8 @@ def _read_torch(cache, page_table, lengths, cu_seqlens, n):
     for b, at, row0, m, length in _segments(len(page_table), lengths, cu_seqlens, n, page_table.shape[1] * cache.page_size):
         kr, vr, _ = _load_torch(cache, page_table[b], length - m + torch.arange(m))
         for out, rows in ((k, _interleave(kr, cache.rotate_dim)), (v, vr)):
-            # fp16 has no value above 65504; an 8-bit code may round up to one
-            rows = torch.where(rows.isfinite(), rows.clamp(-most, most), rows)
+            # a 16-bit page has nothing beyond its type, and an 8-bit one no infinity: its codes may round up past the largest
+            rows = rows.clamp(-most, most) if cache.quantized else rows
             out[at, :, row0:row0 + m] = rows.to(cache.dtype)
     return k, v
 
@@ -446,6 +446,8 @@ def _attend_torch(cache, q, freqs, page_table, lengths, cu_seqlens, causal, scal
         for j in bad.any(-1).any(0).nonzero().flatten().tolist():   # values that are not finite count where they are seen
             extra = torch.where(bad[:, j], vr[:, j], 0.0)
             out += torch.where(keep[:, j, None] & bad[:, j][None, :, None, :], p[..., j, None] * extra[:, None, :], 0.0)
+        if o.dtype == torch.float16:   # averages of values that were finite; 8-bit ones may stand for 65536
+            out = torch.where(out.isfinite(), out.clamp(-65504.0, 65504.0), out)
         o[at, :, row0:row0 + n] = out.reshape(G * Hk, n, -1).to(o.dtype)
         lse[at, :, row0:row0 + n] = torch.logsumexp(sc, -1).reshape(G * Hk, n)
     return o, lse

@@ -328,3 +328,18 @@ def test_module_positions_feed_the_cache():
         ref = pope_amd.flash_attn_with_pope(q.float(), k.float(), v.float(), pos_emb=pope(40), causal=True)
     # a cached key is off by half a bf16 step (2^-9), so scores by about 2^-9 of sum |q k| / 4, the output by twice that
     assert (o.float() - ref).abs().max() <= 6e-2
+
+
+def test_8_bit_rows_at_the_end_of_their_type_on_the_cpu():
+    """e4m3 may round a row's largest values past the type's range; they are read, and averaged, as its largest."""
+    for dtype, x in ((torch.float16, 65000.0), (torch.bfloat16, torch.finfo(torch.bfloat16).max)):
+        most = torch.finfo(dtype).max
+        cache = PagedPoPECache(1, heads=1, dim=8, page_size=32, dtype=dtype, quantized=True)
+        v = torch.full((1, 1, 3, 8), x, dtype=dtype)
+        v[..., 1::2] *= -1
+        table, lens = torch.tensor([[0]], dtype=I32), torch.tensor([3], dtype=I32)
+        paged_cache_write(cache, torch.zeros_like(v), v, None, table, lens)
+        assert (paged_cache_read(cache, table, lens, 3)[1].abs() == most).all()
+        if dtype == torch.float16:
+            o = paged_flash_attn_with_pope(torch.zeros_like(v), cache, None, table, lens)
+            assert (o.abs() == most).all()

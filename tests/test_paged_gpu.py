@@ -765,3 +765,45 @@ def test_infinities_next_to_bad_pages(cuda, n, G, D):
         assert fin.any() and want.isinf().any()
         # both fp32 arithmetic over the same rows: a rounding each, and P's in the many-row kernel, of outputs below 4
         assert ((got - want).abs()[fin] <= 4 * 2.0 ** -8 * 3).all()
+
+
+@pytest.mark.parametrize("q8", [False, True], ids=["16bit", "8bit"])
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("D", [64, 200])
+def test_values_at_the_end_of_fp16(cuda, q8, n, D):
+    """Averages of values next to fp16's largest stay finite: an 8-bit code may stand for 65536 (65000 does), and P's rounding
+    may carry an average past the values'.  The true average is 65504 (what reads give), P is off by 2^-11, a sum by less."""
+    B = Batch([1, 70, 3000], heads=2, D=D, dtype=torch.float16, q8=q8)
+    B.v = torch.full_like(B.v, 65000.0 if q8 else 65504.0)
+    B.v[..., 1::2] *= -1
+    paged_cache_write(B.cache, B.k, B.v, B.emb(B.pos), B.table, B.lengths, cu_seqlens=B.cu)
+    assert (B.rows(2)[1].abs() == 65504).all()
+    pos = (B.lengths[:, None].long() - n + torch.arange(n, device="cuda")).clamp_min(0)
+    o = paged_flash_attn_with_pope(B.rand(3, 2, n, D), B.cache, B.emb(pos), B.table, B.lengths, causal=False).double()
+    assert o.isfinite().all() and (o.abs() >= 65504 * (1 - 3 * 2.0 ** -11)).all() and (o[..., 0] > 0).all() and (o[..., 1] < 0).all()
+
+
+def test_rounded_weights_at_the_end_of_fp16(cuda):
+    """Many rows: a weight of 2^7.00073 = 128.0648 (against 1 three blocks before) is 128.125 in fp16 and itself in their sum: the
+    average would be 65504 (1 + 0.0602 / 129.06) = 65534, which rounds to infinity."""
+    c = PagedPoPECache(4, heads=1, dim=32, page_size=32, dtype=torch.float16, device="cuda")
+    k = torch.zeros(1, 1, 128, 32, device="cuda").half()
+    k[..., 0] = -60
+    k[0, 0, 3, 0], k[0, 0, 100, 0] = 0, 7
+    v, q = torch.full_like(k, 65504.0), torch.zeros_like(k[:, :, :40])
+    q[..., 0] = 1
+    table, lens = torch.tensor([[1, 0, 3, 2]], dtype=I32, device="cuda"), torch.tensor([128], dtype=I32, device="cuda")
+    paged_cache_write(c, k, v, None, table, lens)
+    o = paged_flash_attn_with_pope(q, c, None, table, lens, causal=False, softmax_scale=7.00073 / 7 * math.log(2))
+    assert (o == 65504).all()
+
+
+def test_8_bit_rows_at_the_end_of_bf16(cuda):
+    """3.39e38 has a code that stands for 2^128: it is read as bf16's largest, as fp16's are."""
+    c = PagedPoPECache(1, heads=1, dim=8, page_size=32, quantized=True, device="cuda")
+    k = torch.full((1, 1, 2, 8), torch.finfo(torch.bfloat16).max, device="cuda").bfloat16()
+    k[..., 1::2] *= -1
+    table, lens = torch.zeros(1, 1, dtype=I32, device="cuda"), torch.tensor([2], dtype=I32, device="cuda")
+    paged_cache_write(c, k, k, None, table, lens)
+    for got in paged_cache_read(c, table, lens, 2):
+        assert torch.equal(got, k)
