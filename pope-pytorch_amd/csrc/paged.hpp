@@ -35,7 +35,7 @@ struct PagedAttnParams {
   uint16_t* o; float* lse;             // lse may be null: (batch, Hq, rows) natural log
   PagedDiv G;                          // Hq / Hk
   int Hq, causal, N;                   // N: rows per batch entry (all of them when packed)
-  int splits, least;                   // splits of the key axis, the least blocks of one
+  int splits, least;                   // splits of the key axis, the least blocks of one (few rows: paged_few_least)
   int slots;                           // workgroups that the chip holds: paged_plan raises `least` (many rows); 0: `least` stands
   int64_t tiles;                       // row tiles
   // Scores come out of the products in log2 units: Q_hat carries q_factor = softmax scale x log2 e.  fp16 does not hold

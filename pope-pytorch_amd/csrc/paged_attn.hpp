@@ -53,8 +53,9 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_few_kernel(PagedAt
   if (r0 >= rows_all) return;
   const bool causal = p.causal != 0;
   const int blocks = paged_tile_blocks(g, t.local, kRows, p.G, causal);
-  const PagedRange range = paged_range(blocks, p.splits, p.least, WK, job.split);
-  const int parts = paged_parts(blocks, p.splits, p.least, WK);
+  const int least = paged_few_least(blocks, p.tiles * c.Hk);
+  const PagedRange range = paged_range(blocks, p.splits, least, WK, job.split);
+  const int parts = paged_parts(blocks, p.splits, least, WK);
   if (job.split > 0 && range.begin >= range.end) return;
   if (p.splits > 1 && job.split == 0 && threadIdx.x == 0) p.parts[(int64_t)job.tile * c.Hk + hk] = parts;
   const bool part = parts > 1;

@@ -132,6 +132,15 @@ POPE_HD PagedRange paged_range(int blocks, int splits, int least, int step, int 
   return PagedRange{lo < blocks ? (int)lo : blocks, hi < blocks ? (int)hi : blocks};
 }
 
+// Least blocks of a part, few rows, of a tile of `blocks` blocks in a launch of `tiles` tiles over all heads: 16, or as few as 8
+// where 16 leave some of the 256 CUs without a part (the rule's figures are beside the host's, pope_abi.cpp).  By what the
+// tile sees, not by the page table's width, which a serving program sizes for its longest context.
+POPE_HD int paged_few_least(int blocks, int64_t tiles) {
+  if (blocks <= 16) return 16;
+  const int64_t even = tiles * blocks / 256;
+  return even < 8 ? 8 : even > 16 ? 16 : (int)even;
+}
+
 // A workgroup's tile and part of the key axis, where a tile has many rows.
 //
 // At most 64 segments (`slots`, the workgroups that the chip holds, is not 0): parts are cut by what the sequences

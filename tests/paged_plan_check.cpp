@@ -154,6 +154,19 @@ int main(int argc, char**) {
         std::snprintf(g_what, sizeof g_what, "%d rows behind, %d without keys, causal %d", gap, none, causal);
         CHECK(walk(q, c, true));
       }
+  // Few rows: a tile's parts by what it sees, whatever the page table's width lets the grid have.
+  for (const int splits : {7, 64, 128}) {
+    CHECK(paged_parts(63, splits, paged_few_least(63, 8), 4) == (splits == 7 ? 6 : 8));   // 2,000 keys, 8 heads: parts of 8 or 12
+    CHECK(paged_parts(16, splits, paged_few_least(16, 8), 4) == 1);                       // 512 keys: one part
+    CHECK(paged_parts(500, splits, paged_few_least(500, 8), 4) == (splits == 7 ? 7 : 32));
+    CHECK(paged_parts(63, splits, paged_few_least(63, 128), 4) == 4);                     // the chip is full: parts of 16
+  }
+  for (int blocks = 0; blocks < 2000; ++blocks)
+    for (const int64_t tiles : {1, 8, 40, 100, 256, 5000}) {
+      const int least = paged_few_least(blocks, tiles);
+      CHECK(least >= 8 && least <= 16 && (blocks > 16 || least == 16));
+    }
+  CHECK(paged_few_least(1 << 26, (1 << 24) - 1) == 16);
   // rows: new token and query head of every row of a tile
   for (int G : {1, 2, 3, 5, 8, 20, 31}) {
     const PagedDiv div = paged_div(G);
