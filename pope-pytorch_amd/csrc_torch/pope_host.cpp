@@ -844,7 +844,7 @@ struct PagedCall {
 
   int64_t batch() const { return cu.defined() ? 1 : table.size(0); }
   bool here(const Tensor& t) const { return t.device() == k_pages.device(); }
-  bool tracked(const Tensor& t) const { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
+  bool tracked(const Tensor& t) const { return t.defined() && ((t.requires_grad() && at::GradMode::is_enabled()) || t._fw_grad(0).defined()); }
   bool seqs() const {
     const auto ints = [&](const Tensor& t, int64_t dim) { return t.scalar_type() == at::kInt && here(t) && t.dim() == dim && t.stride(-1) == 1; };
     return k_pages.is_cuda() && ints(table, 2) && table.size(0) > 0 && table.size(1) > 0 && ints(lengths, 1) && lengths.size(0) == table.size(0) &&

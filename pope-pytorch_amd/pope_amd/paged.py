@@ -32,6 +32,7 @@ from typing import Optional
 import torch
 import torch.nn.functional as F
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -169,7 +170,9 @@ def _check_pos_emb(cache: PagedPoPECache, pos_emb, batch: int, n: int):
 
 
 def _no_grad(*ts):
-    if torch.is_grad_enabled() and any(exists(t) and t.requires_grad for t in ts):
+    ts = [t for t in ts if exists(t)]
+    if (torch.is_grad_enabled() and any(t.requires_grad for t in ts)) or (
+            not torch.compiler.is_compiling() and any(exists(forward_ad.unpack_dual(t).tangent) for t in ts)):
         raise RuntimeError("pope_amd paged cache: no gradient is defined; call it under torch.no_grad() or on detached tensors")
 
 

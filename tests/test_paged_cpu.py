@@ -343,3 +343,23 @@ def test_8_bit_rows_at_the_end_of_their_type_on_the_cpu():
         if dtype == torch.float16:
             o = paged_flash_attn_with_pope(torch.zeros_like(v), cache, None, table, lens)
             assert (o.abs() == most).all()
+
+
+def test_forward_mode_tangents_are_refused():
+    import torch.autograd.forward_ad as fwd
+    c, a = _call()
+    for name in ("q", "k", "v"):
+        with fwd.dual_level():
+            b = dict(a, **{name: fwd.make_dual(a[name], torch.ones_like(a[name]))})
+            for grad in (torch.enable_grad, torch.no_grad):   # no_grad is no word on tangents
+                with grad(), pytest.raises(RuntimeError, match="gradient"):
+                    (_attend if name == "q" else _write)(c, b)
+    with fwd.dual_level():
+        f = fwd.make_dual(a["pos_emb"][0], torch.ones(3, 8))
+        for call in (_attend, _write):
+            with pytest.raises(RuntimeError, match="gradient"):
+                call(c, dict(a, pos_emb=(f, a["pos_emb"][1])))
+    with pytest.raises(RuntimeError, match="gradient"):
+        torch.func.jvp(lambda q: _attend(c, dict(a, q=q)), (a["q"],), (torch.ones_like(a["q"]),))
+    with pytest.raises(RuntimeError, match="gradient"):
+        torch.func.grad(lambda q: _attend(c, dict(a, q=q)).float().sum())(a["q"])

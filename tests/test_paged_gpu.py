@@ -807,3 +807,17 @@ def test_8_bit_rows_at_the_end_of_bf16(cuda):
     paged_cache_write(c, k, k, None, table, lens)
     for got in paged_cache_read(c, table, lens, 2):
         assert torch.equal(got, k)
+
+
+def test_forward_mode_tangents_are_refused(cuda):
+    import torch.autograd.forward_ad as fwd
+    B = Batch([70], heads=2)
+    q, emb = B.rand(1, 2, 1, 64), B.emb(torch.tensor([69], device="cuda"))
+    one = lambda t: fwd.make_dual(t, torch.ones_like(t))
+    with fwd.dual_level(), torch.no_grad():
+        for call in (lambda: paged_flash_attn_with_pope(one(q), B.cache, emb, B.table, B.lengths),
+                     lambda: paged_flash_attn_with_pope(q, B.cache, (one(emb[0]), emb[1]), B.table, B.lengths),
+                     lambda: paged_cache_write(B.cache, one(q), q, emb, B.table, B.lengths), lambda: paged_cache_write(B.cache, q, one(q), emb, B.table, B.lengths),
+                     lambda: paged_cache_write(B.cache, q, q, (emb[0], one(emb[1])), B.table, B.lengths)):
+            with pytest.raises(RuntimeError, match="gradient"):
+                call()
