@@ -768,6 +768,14 @@ const float* floats(const Tensor& t) { return static_cast<const float*>(data(t))
 
 using OptTensor = const std::optional<Tensor>&;
 
+// Rows like q's, of unit feature stride: empty_like() may put another dim last where q's rows overlap (a window that
+// slides by one element has two dims of stride 1).
+Tensor rows_like(const Tensor& q) {
+  const auto opt = q.options().requires_grad(false);
+  const Tensor o = at::empty_like(q, opt);
+  return o.stride(-1) == 1 ? o : at::empty(q.sizes(), opt);
+}
+
 void paged_write(const Tensor& k, const Tensor& v, OptTensor freqs_, OptTensor bias_, const Tensor& k_pages, const Tensor& v_pages,
                  const Tensor& scales, const Tensor& table, const Tensor& lengths, OptTensor cu_, int64_t page_size) {
   const Tensor freqs = opt(freqs_), bias = opt(bias_), cu = opt(cu_);
@@ -815,7 +823,7 @@ std::pair<Tensor, Tensor> paged_attn(const Tensor& q, OptTensor freqs_, const Te
   p.d.Hq = (int32_t)q.size(1);
   p.d.causal = causal;
   p.d.softmax_scale = (float)softmax_scale;
-  const Tensor o = at::empty_like(q, q.options().requires_grad(false));
+  const Tensor o = rows_like(q);
   const Tensor lse = fp32_like(q, with_lse ? q.sizes().slice(0, 3) : at::IntArrayRef({0}));
   strides3(p.d.q_s, q);
   strides3(p.d.o_s, o);
@@ -916,7 +924,7 @@ std::optional<std::pair<Tensor, Tensor>> paged_attn_eager(const Tensor& q, OptTe
   p.d.Hq = (int32_t)q.size(c.h);
   p.d.causal = causal;
   p.d.softmax_scale = (float)softmax_scale;
-  const Tensor o = at::empty_like(q, q.options().requires_grad(false));
+  const Tensor o = rows_like(q);
   Tensor lse;
   if (with_lse) lse = fp32_like(q, {q.size(0), q.size(c.h), q.size(c.n)});
   c.strides(p.d.q_s, q);

@@ -213,7 +213,9 @@ def paged_attn_op(q: Tensor, freqs: Optional[Tensor], k_pages: Tensor, v_pages: 
 
 @paged_attn_op.register_fake
 def _(q, freqs, k_pages, v_pages, scales, page_table, lengths, cu_seqlens, page_size, causal, softmax_scale, with_lse):
-    return torch.empty_like(q), q.new_empty(q.shape[:3] if with_lse else (0,), dtype=torch.float32)
+    o = torch.empty_like(q)
+    o = o if o.stride(-1) == 1 else q.new_empty(q.shape)   # rows_like of csrc_torch/pope_host.cpp
+    return o, q.new_empty(q.shape[:3] if with_lse else (0,), dtype=torch.float32)
 
 
 # ---------------------------------------------------------------- public calls

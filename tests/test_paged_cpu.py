@@ -363,3 +363,16 @@ def test_forward_mode_tangents_are_refused():
         torch.func.jvp(lambda q: _attend(c, dict(a, q=q)), (a["q"],), (torch.ones_like(a["q"]),))
     with pytest.raises(RuntimeError, match="gradient"):
         torch.func.grad(lambda q: _attend(c, dict(a, q=q)).float().sum())(a["q"])
+
+
+def test_the_output_of_rows_that_overlap_has_unit_feature_stride():
+    """Shapes and strides alone (the kernels write rows of unit feature stride): windows that slide by one element."""
+    from torch._subclasses import FakeTensorMode
+    c, a = _call()
+    q = torch.zeros(2, 4, 3 + 15, dtype=torch.bfloat16).unfold(2, 16, 1)
+    assert q.shape == (2, 4, 3, 16) and torch.empty_like(q).stride(-1) != 1
+    freqs = a["pos_emb"][0][None]
+    with FakeTensorMode() as mode:
+        f = lambda t: mode.from_tensor(t).to("cuda") if t is not None else None
+        o, _ = paged.paged_attn_op(f(q), f(freqs), f(c.k_pages), f(c.v_pages), f(c.scales), f(a["page_table"]), f(a["lengths"]), None, 32, True, 0.25, False)
+    assert o.shape == q.shape and o.stride() == (4 * 3 * 16, 3 * 16, 16, 1)

@@ -821,3 +821,25 @@ def test_forward_mode_tangents_are_refused(cuda):
                      lambda: paged_cache_write(B.cache, q, q, (emb[0], one(emb[1])), B.table, B.lengths)):
             with pytest.raises(RuntimeError, match="gradient"):
                 call()
+
+
+@pytest.mark.parametrize("n", [1, 3, 70])
+def test_rows_that_overlap(cuda, n):
+    """Windows that slide by one element: two dims of stride 1, of which the features stay the output's last."""
+    from pope_amd import paged as m
+    B = Batch([90, 75], heads=2, D=32, R=16)
+    flat = B.rand(2, 2, n + 31)
+    q = flat.unfold(2, 32, 1)
+    assert q.shape == (2, 2, n, 32) and q.stride(2) == q.stride(3) == 1
+    emb = B.emb(B.lengths[:, None].long() - n + torch.arange(n, device="cuda"))
+    want = paged_flash_attn_with_pope(q.contiguous(), B.cache, emb, B.table, B.lengths)
+    got = paged_flash_attn_with_pope(q, B.cache, emb, B.table, B.lengths)
+    assert got.stride(-1) == 1 and torch.equal(got, want)
+    c = B.cache
+    args = (q, emb[0], c.k_pages, c.v_pages, c.scales, B.table, B.lengths, None, 64, True, 32 ** -0.5, False)
+    assert torch.equal(m.paged_attn_op(*args)[0], want)
+    torch.library.opcheck(m.paged_attn_op, args, test_utils=("test_faketensor",))
+    paged_cache_write(c, q, q, emb, B.table, B.lengths)   # read rows may overlap too
+    a = [t.clone() for t in (c.k_pages, c.v_pages)]
+    paged_cache_write(c, q.contiguous(), q.contiguous(), emb, B.table, B.lengths)
+    assert torch.equal(a[0], c.k_pages) and torch.equal(a[1], c.v_pages)
