@@ -336,7 +336,8 @@ int pope_paged_read(const pope_paged* desc, const void* k_pages, const void* v_p
                     void* v, void* stream);
 
 /* Attention of the new rows' queries over their sequences' slots.  o (dtype, o_s); lse NULL or fp32 (batch, Hq, N)
- * contiguous, natural log; rows that see no key give 0 and -inf.  Every row is written.  Workspace:
+ * contiguous, natural log; rows that see no key, or none with a score above -inf, give 0 and -inf; a score of +inf
+ * makes both NaN.  Every row is written.  Workspace:
  * pope_paged_workspace_bytes, 256-byte aligned (0: none), free again once the call's work is done. */
 int pope_paged_workspace_bytes(const pope_paged* desc, int packed, size_t* bytes);
 int pope_paged_attn(const pope_paged* desc, const void* q, const float* freqs, const void* k_pages,

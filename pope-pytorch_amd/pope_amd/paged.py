@@ -18,8 +18,9 @@ stands at position lengths - n + i, and ``pos_emb`` has one row of angles per ne
 step is a write and an attention call with the same page table, lengths and cu_seqlens.
 
 Rows without a slot (negative positions, packed rows outside every sequence, page numbers outside the cache) are not
-written, read as zeros and never seen; rows that see no key give 0.  Nothing synchronises or reads lengths on the host,
-so a captured graph replays with new page tables and lengths in the same tensors.  There is no gradient.
+written, read as zeros and never seen; rows that see no key, or none with a score above -inf, give 0.  Nothing
+synchronises or reads lengths on the host, so a captured graph replays with new page tables and lengths in the same
+tensors.  There is no gradient.
 
 No counterpart in the reference, whose decoding caches plain k and transforms all of it for every token
 (PoPE_pytorch/attention.py:75-145).  GPU caches run the HIP kernels (csrc/paged_*.hip), CPU caches the torch
@@ -444,8 +445,8 @@ def _attend_torch(cache, q, freqs, page_table, lengths, cu_seqlens, causal, scal
         if causal:
             keep = keep & (torch.arange(length) <= (length - n + torch.arange(n))[:, None])
         sc = sc.masked_fill(~keep, float("-inf"))
-        row_any = keep.any(-1)[:, None]
-        p = torch.softmax(sc.masked_fill(~row_any, 0.0), -1).masked_fill(~keep, 0.0)
+        row_any = (sc != float("-inf")).any(-1, keepdim=True)
+        p = torch.softmax(sc.masked_fill(~row_any, 0.0), -1).masked_fill(~keep | ~row_any, 0.0)
         bad = ~vr.isfinite()
         out = torch.matmul(p, vr.masked_fill(bad, 0.0))
         for j in bad.any(-1).any(0).nonzero().flatten().tolist():   # values that are not finite count where they are seen

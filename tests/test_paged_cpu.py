@@ -376,3 +376,17 @@ def test_the_output_of_rows_that_overlap_has_unit_feature_stride():
         f = lambda t: mode.from_tensor(t).to("cuda") if t is not None else None
         o, _ = paged.paged_attn_op(f(q), f(freqs), f(c.k_pages), f(c.v_pages), f(c.scales), f(a["page_table"]), f(a["lengths"]), None, 32, True, 0.25, False)
     assert o.shape == q.shape and o.stride() == (4 * 3 * 16, 3 * 16, 16, 1)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_rows_whose_keys_all_have_weight_zero_on_the_cpu(causal):
+    """Every visible score -inf: as with no key to see, 0 and a log-sum-exp of -inf; a NaN score stays NaN."""
+    cache = PagedPoPECache(2, heads=1, dim=16, page_size=32)
+    k, v, q = (torch.randn(1, 1, 5, 16).bfloat16() for _ in range(3))
+    k[..., 2], q[..., 2] = -math.inf, 1.0
+    q[0, 0, 3, 5] = math.nan
+    table, lens = torch.tensor([[1]], dtype=I32), torch.tensor([5], dtype=I32)
+    paged_cache_write(cache, k, v, None, table, lens)
+    o, lse = paged_flash_attn_with_pope(q, cache, None, table, lens, causal=causal, return_lse=True)
+    good = torch.tensor([0, 1, 2, 4])
+    assert not o[0, 0, good].any() and (lse[0, 0, good] == -math.inf).all() and o[0, 0, 3].isnan().all() and lse[0, 0, 3].isnan()

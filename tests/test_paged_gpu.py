@@ -843,3 +843,18 @@ def test_rows_that_overlap(cuda, n):
     a = [t.clone() for t in (c.k_pages, c.v_pages)]
     paged_cache_write(c, q.contiguous(), q.contiguous(), emb, B.table, B.lengths)
     assert torch.equal(a[0], c.k_pages) and torch.equal(a[1], c.v_pages)
+
+
+@pytest.mark.parametrize("n,total", [(1, 5), (3, 2500), (40, 70), (40, 2500)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_rows_whose_keys_all_have_weight_zero(cuda, n, total, dtype):
+    """Every visible score -inf: as with no key to see, 0 and a log-sum-exp of -inf, as CPU caches have it."""
+    c = PagedPoPECache(-(-total // 32), heads=2, dim=48, page_size=32, dtype=dtype, device="cuda")
+    k, v, q = (torch.randn(1, 2, m, 48, device="cuda").to(dtype) for m in (total, total, n))
+    k[..., 2], q[:, 0, :, 2], q[:, 1, :, 2] = -INF, 1.0, -1.0
+    table, lens = torch.arange(c.num_pages, device="cuda").to(I32)[None], torch.tensor([total], dtype=I32, device="cuda")
+    paged_cache_write(c, k, v, None, table, lens)
+    for causal in (True, False):
+        o, lse = paged_flash_attn_with_pope(q, c, None, table, lens, causal=causal, return_lse=True)
+        assert not o[0, 0].any() and (lse[0, 0] == -INF).all()
+        assert o[0, 1].isnan().all()   # scores of +inf
