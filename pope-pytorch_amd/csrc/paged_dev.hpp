@@ -131,7 +131,6 @@ __device__ __forceinline__ void paged_query_make(const PagedAttnParams& p, const
   if (d0 >= D) return;
   float x[8], a[8], b[8];   // a: cosine part, or the raw value; b: sine part
   unpack8<T>(in.x, x);
-  const bool off = p.q_factor == 0.f;   // scores are 0, also of values that are not finite
   if (!live) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) a[k] = b[k] = 0.f;
@@ -142,12 +141,12 @@ __device__ __forceinline__ void paged_query_make(const PagedAttnParams& p, const
       sincos_rev(in.f[k >> 2][k & 3], &sn, &cs);
       const float m = softplus_f(x[k]) * p.q_factor;
       const bool rot = d0 + k < R;
-      a[k] = off ? 0.f : rot ? m * cs : x[k] * p.q_factor;
-      b[k] = off ? 0.f : m * sn;
+      a[k] = rot ? m * cs : x[k] * p.q_factor;
+      b[k] = m * sn;
     }
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) a[k] = off ? 0.f : x[k] * p.q_factor;
+    for (int k = 0; k < 8; ++k) a[k] = x[k] * p.q_factor;
   }
   auto store = [&](int e, const float* v) {   // eight columns from e on
     u32x4 wh, wl;

@@ -858,3 +858,24 @@ def test_rows_whose_keys_all_have_weight_zero(cuda, n, total, dtype):
         o, lse = paged_flash_attn_with_pope(q, c, None, table, lens, causal=causal, return_lse=True)
         assert not o[0, 0].any() and (lse[0, 0] == -INF).all()
         assert o[0, 1].isnan().all()   # scores of +inf
+
+
+@pytest.mark.parametrize("n", [2, 40])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_softmax_scale_zero_keeps_nan(cuda, n, dtype):
+    """0 x inf is NaN, in queries and keys, as the formula and CPU caches have it; finite rows average the values."""
+    B = Batch([100], heads=2, dtype=dtype)
+    pos = torch.arange(100 - n, 100, device="cuda")
+    q = B.rand(1, 2, n, 64)
+    q[0, 0, 0, 3], q[0, 0, 1, 40], q[0, 1, 0, 50] = NAN, INF, -INF
+    bad = ~q.isfinite().all(-1)
+    run = lambda: paged_flash_attn_with_pope(q, B.cache, B.emb(pos), B.table, B.lengths, softmax_scale=0.0, causal=False)
+    o = run()
+    assert o[bad].isnan().all() and o[~bad].isfinite().all()
+    mean = B.v[0].double().mean(1, keepdim=True)
+    err = (o[0].double() - mean).abs()[~bad[0]]
+    assert (err <= 2e-2).all()   # an average of 100 values: P is exact, 2^-9 of a mean below 1 and fp32 sums
+    B.k[0, 0, 9, 45] = INF
+    paged_cache_write(B.cache, B.k, B.v, B.emb(B.pos), B.table, B.lengths, cu_seqlens=B.cu)
+    o = run()
+    assert o[0, 0].isnan().all() and torch.equal(o[0, 1].isnan().all(-1), bad[0, 1])
