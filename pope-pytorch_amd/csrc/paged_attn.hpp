@@ -107,7 +107,7 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_few_kernel(PagedAt
 #pragma unroll
   for (int k = 0; k < (VT + 7) / 8; ++k) in[k] = paged_query_load<T>(p, g, map, (threadIdx.x + 256 * k) % kRows, count, hk, (threadIdx.x + 256 * k) / kRows * 8);
   if (blk < range.end) {
-    page_base = -1 << 20;
+    page_base = -(1 << 20);
     page = page_of(blk);
     load_k(page, blk);
     load_v(page, blk);

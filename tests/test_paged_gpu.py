@@ -879,3 +879,27 @@ def test_softmax_scale_zero_keeps_nan(cuda, n, dtype):
     paged_cache_write(B.cache, B.k, B.v, B.emb(B.pos), B.table, B.lengths, cu_seqlens=B.cu)
     o = run()
     assert o[0, 0].isnan().all() and torch.equal(o[0, 1].isnan().all(-1), bad[0, 1])
+
+
+@pytest.mark.parametrize("n,G", [(2, 8), (90, 1)])
+@pytest.mark.parametrize("q8", [False, True], ids=["16bit", "8bit"])
+def test_infinities_beyond_64_pages(cuda, n, G, q8):
+    """Page numbers are held 64 at a time: more pages than that, infinities in the first and the last ones."""
+    B = Batch([2500, 5000], heads=2, G=G, D=64, R=32, page=32, q8=q8)
+    clean = B.rows(1)[1]
+    for b, t in enumerate(B.total):
+        B.v[0, :, int(B.cu[b]) + 40, 5], B.v[0, :, int(B.cu[b]) + t - 300, 6] = INF, -INF
+    paged_cache_write(B.cache, B.k, B.v, B.emb(B.pos), B.table, B.lengths, cu_seqlens=B.cu)
+    pos = B.lengths[:, None].long() - n + torch.arange(n, device="cuda")
+    q = B.rand(2, 2 * G, n, 64)
+    o = paged_flash_attn_with_pope(q, B.cache, B.emb(pos), B.table, B.lengths)
+    for b in range(2):
+        k, v = B.rows(b)
+        want, _, tol, _ = with_infinities(q[b], angles(pos[b], 32), k, v, 32, 0.125, True, B.dtype)
+        got = o[b].double()
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf()) and torch.equal(got[got.isinf()], want[want.isinf()])
+        fin = want.isfinite()
+        assert ((got - want).abs()[fin] <= tol[fin]).all() and fin.any()
+        # 8 bits have no infinity: the values are stored as NaN
+        assert o[b, ..., 5].isnan().all() if q8 else (o[b, ..., 5] == INF).all() and (o[b, ..., 6] == -INF).all()
+    assert clean.isfinite().all()
