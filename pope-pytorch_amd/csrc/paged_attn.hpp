@@ -295,7 +295,7 @@ __global__ __launch_bounds__(256, VT <= 8 ? 2 : 1) void paged_few_kernel(PagedAt
       bool fin = true;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) fin = fin && all_finite<T>(qh[ks]);
-      const uint64_t nan = __ballot(x != x), off = __ballot(!fin);   // of a row: in any of its four lanes
+      const uint64_t nan = __ballot(x != x && live), off = __ballot(!fin);   // of a row: in any of its four lanes
       const auto of_row = [&](uint64_t w) { return (w | w >> 16 | w >> 32 | w >> 48) & 0xffffu; };
       if (of_row(nan) & ~of_row(off)) second_pass();
     }
