@@ -10,10 +10,12 @@
 // columns of a row (16-byte loads, all of a workgroup's in flight at once).  Slots of other tokens in the block are not
 // touched: units of 16 bytes are stored whole only where all their tokens are written.
 //
-// Bound by HBM, and by the launch where there is little to move.  Measured: write 4 x 2,048 tokens x 8 heads, D 128, R 64, to
-// 8 bits, 120 MB in 25 us; 2,047 x 8, D 256, R 256, fp16, 94 MB in 24 us (4.7 and 4.0 TB/s: a copy reaches 4.7, part of
-// these stays in the caches); one token of 16 sequences 4 us.  Read 8 x 8,192 tokens x 16 heads, D 64, R 64, 805 MB in
-// 149 us (5.4 TB/s); 8 x 500 x 8, D 72, R 40, 8 bits, 18 MB in 8 us.
+// Reads are bound by HBM, and by the launch where there is little to move: 8 x 8,192 tokens x 16 heads, D 64, R 64, 805 MB in
+// 149 us (5.4 TB/s; a copy reaches 4.7, half of it writes); 8 x 500 x 8, D 72, R 40, 8 bits, 18 MB in 8 us.  Writes of many
+// tokens are not, by half: 4 x 2,048 tokens x 8 heads, D 128, R 64, to 8 bits, 57 MB in 25 us (2.3 TB/s); 2,047 x 8, D 256,
+// R 256, fp16, 44 MB in 23.5 us (1.9 TB/s).  Every head computes the sines and cosines of its F + bias (with softplus about 100
+// vector instructions per rotated column), and load, transform and store stand in turn between barriers, in about one
+// round of workgroups.  One token of 16 sequences: 4 us.
 //
 // The angle F + bias is kept as a sum of two floats (in one, at position 32,768, it would be off by up to 2e-3 rad) and the
 // functions are accurate to about an ulp, so that a stored value is the rounding of the exact one except next to a rounding

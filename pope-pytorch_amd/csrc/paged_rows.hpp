@@ -23,6 +23,11 @@
 // A step's score products run between the exponentials of the step before (a wave alone keeps both units busy), its
 // P V products between the maxima of the scores just made.  The running maximum m moves only when a row's maximum
 // exceeds it by more than 2^8 in p (or is the row's first): p <= 2^8 loses nothing, and O is rescaled rarely.
+//
+// Precision: as in paged_attn.hpp, but P is rounded once to 16 bits (8-bit pages: times the value's scale, to bf16; two parts where
+// outputs are fp16): its second part would double the second product, a quarter of all products at R = D / 2.  Against
+// 64 bits, relative to the output's norm, bf16 0.0021-0.0024 (an fp32 computation rounded once: 0.0016), fp16 0.00029
+// (0.00021).  l sums what P was before.
 #pragma once
 #include <type_traits>
 

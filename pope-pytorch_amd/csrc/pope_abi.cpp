@@ -1096,11 +1096,12 @@ pope::PagedCache paged_cache(const pope_paged& d, const void* k, const void* v, 
 
 // Parts of the key axis.  A tile's blocks of keys go to as many workgroups as they have parts (at most `splits`, the
 // grid's) of at least `least` blocks; tiles of one part write their output themselves, the others a second launch joins.
-//   few rows   as many parts as bring the grid to kPagedGrid workgroups, of 16 blocks (512 keys) or more (8 where
-//              16 leave half of the 256 CUs without one: 1 sequence of 2,000 keys, 8 heads, D 128, R 64 12.3 us, 13.5 with
-//              16; of 16,000 20.9 with 16, 22.3 with 8; up to 512 keys one part: 10.5 us, 12.2 in wider tables,
-//              whose calls launch the join: paged_few_least, of what a tile sees), and of at most kPagedPart blocks (sequences differ in length, and what the longest
-//              parts leave to do alone is lost) within kPagedMost workgroups, which bounds the workspace of wide page tables
+//   few rows   as many parts as bring the grid to kPagedGrid workgroups, of 16 blocks (512 keys) or more, 8 where 16 leave
+//              half of the 256 CUs without one (paged_few_least, of what a tile sees: 1 sequence of 2,000 keys, 8 heads,
+//              D 128, R 64 12.1 us, 13.5 with 16; of 16,000 20.9 with 16, 22.3 with 8; up to 512 keys one part: 10.5 us, 12.2
+//              in tables of more slots, whose calls launch the join), and of at most kPagedPart blocks (sequences differ
+//              in length, and what the longest parts leave to do alone is lost) within kPagedMost workgroups, which
+//              bounds the workspace of wide page tables
 //   many rows  the chip holds kPagedSlots workgroups (half where values are wider than 128 columns).  The kernel cuts parts
 //              by the sequences' lengths so that these places get equal work (paged_plan), up to two parts per place; with
 //              more than 64 segments, which it does not look at, by the page table's width.  By the width, tokens of 16

@@ -13,9 +13,11 @@ angles only.  ``quantized`` caches hold e4m3 codes times a power of two per (tok
 
 New rows are (batch, heads, n, dim), or (batch, n, heads, dim) with ``head_dimension_at_first=False``: sequence b's
 are batch entry b.  Packed calls have batch 1 and ``cu_seqlens`` (batch + 1 ascending numbers; of rows that numbers
-which descend leave out or count twice nothing is said): rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 belong to sequence b.  ``lengths`` counts a sequence's tokens with the new ones; row i of n
-stands at position lengths - n + i, and ``pos_emb`` has one row of angles per new row, ``pope(positions)``.  A serving
-step is a write and an attention call with the same page table, lengths and cu_seqlens.
+which descend leave out or count twice nothing is said): rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 belong to sequence b.
+``lengths`` counts a sequence's tokens with the new ones; row i of n stands at position lengths - n + i, and
+``pos_emb`` has one row of angles per new row, ``pope(positions)``.  Lengths beyond the slots of a page table's row
+count as those slots: the new rows then take the last ones.  A serving step is a write and an attention call with the
+same page table, lengths and cu_seqlens.
 
 Rows without a slot (negative positions, packed rows outside every sequence, page numbers outside the cache) are not
 written, read as zeros and never seen; rows that see no key, or none with a score above -inf, give 0.  Nothing
@@ -67,7 +69,7 @@ class PagedPoPECache:
 
     ``dim`` 1 to 256, ``rotate_dim`` 0 (plain attention) to ``dim``, ``page_size`` a power of two from 32 to 1024,
     ``dtype`` bf16 or fp16 (of k, v, q and the outputs).  ``quantized``: e4m3 codes times a power of two per row, half
-    the memory.  ``k_pages``, ``v_pages`` and ``scales`` are the pages, in the kernels' operand order."""
+    the memory; values that are not finite are held as NaN.  ``k_pages``, ``v_pages`` and ``scales`` are the pages, in the kernels' operand order."""
 
     def __init__(self, num_pages: int, *, heads: int, dim: int, rotate_dim: int = 0, page_size: int = 64,
                  dtype: torch.dtype = torch.bfloat16, quantized: bool = False, device=None):
@@ -287,7 +289,8 @@ def paged_flash_attn_with_pope(q: Tensor, cache: PagedPoPECache, pos_emb, page_t
     """Attention of the new rows q (batch, query heads, n, dim) over their sequences' cached rows, the new ones included
     (they are written before).  Query head h reads kv head h % heads.  ``causal``: a row sees positions up to its own
     (bottom-right aligned: the last row sees everything), otherwise all of its sequence.  ``pos_emb``: the new rows'
-    (freqs, bias); bias is not read.  ``return_lse``: also the scores' log-sum-exp, fp32 (batch, query heads, n)."""
+    (freqs, bias); bias is not read.  ``return_lse``: also the scores' log-sum-exp, fp32 (batch, query heads, n).  Sums are
+    fp32: a row's values times their keys' number stay below 2^119."""
     on_gpu = cache.k_pages.is_cuda
     scale = cache.dim ** -0.5 if softmax_scale is None else float(softmax_scale)
     freqs = pos_emb[0] if exists(pos_emb) else None
