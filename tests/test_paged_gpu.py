@@ -903,3 +903,33 @@ def test_infinities_beyond_64_pages(cuda, n, G, q8):
         # 8 bits have no infinity: the values are stored as NaN
         assert o[b, ..., 5].isnan().all() if q8 else (o[b, ..., 5] == INF).all() and (o[b, ..., 6] == -INF).all()
     assert clean.isfinite().all()
+
+
+@pytest.mark.parametrize("D,R", [(256, 256), (200, 190)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("q8", [False, True], ids=["16bit", "8bit"])
+def test_widest_rows(cuda, D, R, dtype, q8):
+    """More than 384 columns of K_hat: written, read, and attended by single tokens, a few rows, many rows, in parts too."""
+    B = Batch([300, 33, 65, 1, 1700], heads=2, G=2, D=D, R=R, dtype=dtype, q8=q8)
+    k, v = B.rows(0)
+    s = slice(0, 300)
+    want = rows64(B.k[0, :, s], angles(B.pos[s], R), B.bias, R)
+    assert ((k - want).abs() <= held(want, dtype, q8)).all() and ((v - B.v[0, :, s].double()).abs() <= held(B.v[0, :, s].double(), dtype, q8)).all()
+    for causal in (True, False):
+        attend_and_check(B, [1] * 5, packed=False, causal=causal)
+        attend_and_check(B, [7] * 5, packed=False, causal=causal, head_first=False)
+        attend_and_check(B, [17, 1, 5, 0, 3], packed=True, gap=1, causal=causal)
+        attend_and_check(B, [299, 33, 64, 1, 200], packed=True, causal=causal)
+    if q8:
+        return
+    B.v[0, :, 60, 3], B.v[0, :, 61, D - 1], B.k[0, :, 100, R - 1] = INF, -INF, -INF   # softplus(-inf) is 0
+    paged_cache_write(B.cache, B.k, B.v, B.emb(B.pos), B.table, B.lengths, cu_seqlens=B.cu)
+    for n in (1, 40):
+        pos = B.lengths[:1, None].long() - n + torch.arange(n, device="cuda")
+        q = B.rand(1, 4, n, D)
+        o = paged_flash_attn_with_pope(q, B.cache, B.emb(pos), B.table[:1], B.lengths[:1])[0].double()
+        k, v = B.rows(0)
+        want, _, tol, _ = with_infinities(q[0], angles(pos[0], R), k, v, R, D ** -0.5, True, dtype)
+        assert torch.equal(o.isnan(), want.isnan()) and torch.equal(o.isinf(), want.isinf()) and (o[..., 3] == INF).all() and (o[..., D - 1] == -INF).all()
+        fin = want.isfinite()
+        assert ((o - want).abs()[fin] <= tol[fin]).all() and fin.any()
