@@ -56,7 +56,7 @@ __device__ __forceinline__ void sincos_sum(float a, float b, float* s, float* c)
 }
 
 // softplus to about an ulp: max(x, 0) + log(1 + e), e = e^-|x|: the exponent's product in two parts, and the logarithm as
-// 2 artanh(y), y = e / (2 + e) <= 1/3 (the series' first term left out is below 1e-9).
+// 2 artanh(y), y = e / (2 + e) <= 1/3 (the series' first term left out is below 1e-9).  An e below 2^-126 (x < -87.3) is 0.
 __device__ __forceinline__ float softplus_accurate(float x) {
   constexpr double kL2e = 1.44269504088896340736;
   constexpr float l1 = (float)kL2e, l2 = (float)(kL2e - (double)l1);

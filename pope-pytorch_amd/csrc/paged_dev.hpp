@@ -206,8 +206,9 @@ __device__ __forceinline__ f32x4 averages(f32x4 x) {
 // of -inf and so a weight of 0.  The loops do not look for that: a wave (many rows: a workgroup) that ends with such rows goes
 // over its blocks a second time, with the finite elements of K times both parts, the others times the signs of Q_hat, and V's
 // others outside the product, as in blocks with keys that some row does not see.  What is finite goes through the same
-// operations in the same order, so the other rows keep their bits.  (A query column that 16 bits round to 0 counts as 0;
-// a row whose values or keys hold a NaN that it sees is computed twice and stays NaN.)  8-bit pages hold no infinity.
+// operations in the same order, so the other rows keep their bits.  (A query column that 16 bits round to 0 counts as 0, as
+// does a weight that fp32 does; a row whose values or keys hold a NaN that it sees is computed twice and stays NaN.)  8-bit
+// pages hold no infinity.
 //
 // A 16-bit operand's finite elements, and the others; zeros in the places of either's rest.
 template <typename T>
