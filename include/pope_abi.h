@@ -306,6 +306,8 @@ int pope_pad_rows(const pope_pad* tensors, int n, void* stream);
  * read gives zeros, and keys on such pages are not seen.  lengths beyond the page table's row are cut to it.
  * cu_seqlens that decrease, and two rows of one call in the same slot, leave unspecified values (never an access
  * out of bounds).
+ * Calls that need 2^24 workgroups or more (tiles of rows, for attention times heads and parts of the keys) return
+ * POPE_ERR_UNSUPPORTED.
  */
 typedef struct pope_paged {
   int32_t pages, page_size;  /* page_size: a power of two, 32 .. 1024 */
