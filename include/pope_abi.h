@@ -348,6 +348,80 @@ int pope_paged_attn(const pope_paged* desc, const void* q, const float* freqs, c
                     size_t workspace_bytes, void* stream);
 
 /*
+ * Linear attention of PoPE rows with a decay for each head.  No counterpart in the reference.
+ *
+ * With q_hat, k_hat the rows of pope_polar_fwd (D + R columns, (cos, sin) pairs interleaved, unrounded), g = exp(log_decay) of
+ * the kv head (NULL: 1) and S its state of (D + R, Dv):
+ *   S_i = g S_(i-1) + k_hat_i v_i^T,   o_i = scale S_i^T q_hat_i
+ * over the rows i of a sequence; query head h reads kv head h % Hk.  Rows whose mask byte (B, N) is 0 have no key and no value
+ * (their query still has an output).  Padded batches: B sequences of N rows; packed (cu_seqlens given): N rows in one batch entry,
+ * sequence b owning rows cu_seqlens[b] <= r < cu_seqlens[b + 1]; outputs and gradients of rows outside every sequence are 0.
+ * cu_seqlens that decrease leave unspecified values (never an access out of bounds).  States are fp32 (B, Hk, D + R, Dv),
+ * contiguous; `initial` NULL: zeros.  Calls that need 2^22 workgroups or more return POPE_ERR_UNSUPPORTED.
+ */
+typedef struct pope_linear {
+  int32_t B, N, Hq, Hk;      /* sequences; rows per sequence (packed: in all); heads */
+  int32_t D, R, Dv;          /* 1 <= D <= 256, 0 <= R <= D, 1 <= Dv <= 256, any values */
+  int32_t dtype;             /* enum pope_dtype of rows: POPE_F16 or POPE_BF16 */
+  float scale;
+  int64_t q_s[3], k_s[3], v_s[3], o_s[3];      /* (b, h, n) element strides, unit feature stride, any alignment */
+  int64_t do_s[3], dq_s[3], dk_s[3], dv_s[3];
+  int64_t f_s[2], bias_sh;   /* freqs (b, n): a row of angles per row; bias (1 or Hk, R) */
+  int64_t df_s[2];           /* of dfreqs: f_s, or a batch stride of 0 where the table is one for all */
+  int64_t mask_sb;
+} pope_linear;
+
+/* bytes[0]: the states that segments of rows start from (0: a call that needs none), written by pope_linear_fwd and read by
+ * pope_linear_bwd of the same descriptor; bytes[1]: the backward's workspace.  `final`: whether the call returns the final states.
+ * `want_dfreqs`: whether the backward is given dfreqs.  Both 256-byte aligned. */
+int pope_linear_bytes(const pope_linear* desc, int packed, int final, int want_dfreqs, size_t bytes[2]);
+
+/* o (dtype, o_s), every row; `last` NULL or the states behind the sequences. */
+int pope_linear_fwd(const pope_linear* desc, const void* q, const void* k, const void* v, const float* freqs,
+                    const float* bias, const float* log_decay, const uint8_t* mask, const int32_t* cu_seqlens,
+                    const float* initial, void* o, float* last, void* states, size_t states_bytes, void* stream);
+
+/* Gradients of o's `dout` and the final states' `dlast` (NULL: zeros): dq, dk, dv (dtype); dfreqs (fp32, df_s), dbias (fp32, rows of
+ * R) and dinitial (fp32) or NULL.  All are written, not accumulated into, in a fixed order. */
+int pope_linear_bwd(const pope_linear* desc, const void* dout, const float* dlast, const void* q, const void* k,
+                    const void* v, const float* freqs, const float* bias, const float* log_decay,
+                    const uint8_t* mask, const int32_t* cu_seqlens, const float* initial, const void* states,
+                    size_t states_bytes, void* dq, void* dk, void* dv, float* dfreqs, float* dbias, float* dinitial,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Rows of a head normalised and gated: y = x / sqrt(mean x^2 + eps) * weight * silu(gate).  No counterpart in the reference.
+ * x, gate, y (b, h, n) rows of 1 <= cols <= 512 values of `dtype`, any alignment; weight NULL (ones) or (1 or H, cols), of
+ * `dtype` or fp32 (weight_f32).
+ */
+typedef struct pope_gated_norm {
+  int32_t B, H, N, cols, dtype;
+  int32_t weight_rows, weight_f32;  /* weight_rows: 1 or H */
+  float eps;
+  int64_t x_s[3], gate_s[3], y_s[3], dy_s[3], dx_s[3], dgate_s[3], weight_sh;
+} pope_gated_norm;
+
+int pope_gated_norm_fwd(const pope_gated_norm* desc, const void* x, const void* gate, const void* weight, void* y, void* stream);
+
+/* dx, dgate (dtype); dweight NULL or (weight_rows, cols) contiguous in the weight's type, summed in a fixed order through the
+ * workspace (pope_gated_norm_bytes; not needed without dweight). */
+int pope_gated_norm_bytes(const pope_gated_norm* desc, size_t* bytes);
+int pope_gated_norm_bwd(const pope_gated_norm* desc, const void* dy, const void* x, const void* gate, const void* weight, void* dx,
+                        void* dgate, void* dweight, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * One row for each of B sequences (N = 1) against its state: read from slot `from[b]` of `states` (slots of (Hk, D + R, Dv) fp32,
+ * slot_s elements apart), written to slot `to[b]` after the row; from NULL: slot b, to NULL: where it was read.  A sequence whose
+ * `from` is no slot has no state: its output is 0 and nothing is written; a `to` that is none is not written.  No slot may be
+ * written by two sequences, or written by one and read by another (their values are then unspecified).  With `norm` (H = Hq, N = 1,
+ * cols = Dv; NULL: none) and `gate`, o is the gated norm of the output.
+ */
+int pope_linear_step(const pope_linear* desc, const void* q, const void* k, const void* v, const float* freqs,
+                     const float* bias, const float* log_decay, float* states, int32_t slots, int64_t slot_s,
+                     const int32_t* from, const int32_t* to, const pope_gated_norm* norm, const void* gate,
+                     const void* weight, void* o, void* stream);
+
+/*
  * Per-kernel timing.  No counterpart in the reference (its tests print only
  * parity diffs, tests/test_flash_attn.py:61,109).  While enabled, every kernel
  * launch of the library carries a pair of hipEvents that its dispatch stamps with

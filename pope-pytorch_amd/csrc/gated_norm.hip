@@ -1,0 +1,165 @@
+// Norm of head rows with a gate (gfx950): y = x r w silu(gate), r = 1 / sqrt(mean x^2 + eps), and its gradients
+//   t = dy w silu(gate),  dx = r (t - x r^2 mean(t x)),  dgate = dy x r w silu'(gate),  dw = sum over rows of dy x r silu(gate)
+//
+// Bound by HBM (three rows of 16-bit values forward, five backward) or the launch.  A row is 8 columns for each of 8 to 64 lanes;
+// all arithmetic is fp32, rounded once.
+#include <algorithm>
+
+#include "linear_dev.hpp"
+
+namespace pope {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kNormGrid = 2048, kNormRows = 4;   // workgroups that fill the chip; the least turns of one
+
+__device__ __forceinline__ float weight_at(const GatedNormParams& p, int h, int d, float (*f16)(uint16_t)) {
+  if (d >= p.x.cols) return 0.f;
+  return p.w_f32 ? static_cast<const float*>(p.weight)[h * p.w_sh + d] : f16(static_cast<const uint16_t*>(p.weight)[h * p.w_sh + d]);
+}
+template <typename T>
+__device__ __forceinline__ void load8(const LinRows& r, int64_t off, int d0, float* f) {
+  unpack8<T>(lin_load8(r.p + off, d0, r.cols, r.vec), f);
+}
+template <typename T>
+__device__ __forceinline__ void store8(const LinRows& r, int64_t off, int d0, const float* f) {
+  uint16_t* at = r.p + off + d0;
+  if (r.vec) {
+    *reinterpret_cast<u32x4*>(at) = u32x4{T::pack2(f[0], f[1]), T::pack2(f[2], f[3]), T::pack2(f[4], f[5]), T::pack2(f[6], f[7])};
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (d0 + k < r.cols) at[k] = T::bits(f[k]);
+  }
+}
+
+// LPR lanes for a row.  A workgroup has p.per rows of a head (rows: batch x n).
+template <typename T, int LPR, bool BWD>
+__global__ __launch_bounds__(kThreads) void gated_norm_kernel(GatedNormParams p) {
+  constexpr int kRows = kThreads / LPR;
+  __shared__ float red[BWD ? kThreads * 8 : 1];
+  const int tid = threadIdx.x, d0 = tid % LPR * 8, r0 = tid / LPR, h = blockIdx.y;
+  const int cols = p.x.cols;
+  const bool on = d0 < cols;
+  const int64_t rows = (int64_t)p.B * p.N, first = (int64_t)blockIdx.x * p.per;
+  float w[8], dw[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) w[k] = p.weight ? weight_at(p, h, d0 + k, T::to_float) : 1.f, dw[k] = 0.f;
+  const float inv = 1.f / cols;
+  for (int i = r0; i < p.per; i += kRows) {
+    const int64_t row = first + i;
+    if (row >= rows) break;   // a row's lanes leave together
+    const int64_t b = row / p.N, n = row - b * p.N;
+    const auto off = [&](const LinRows& r) { return b * r.s[0] + h * r.s[1] + n * r.s[2]; };
+    float x[8], g[8], y[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = g[k] = y[k] = 0.f;
+    if (on) {
+      load8<T>(p.x, off(p.x), d0, x);
+      load8<T>(p.gate, off(p.gate), d0, g);
+      if (BWD) load8<T>(p.y, off(p.y), d0, y);
+    }
+    float sg[8], ss = 0.f, tx = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      sg[k] = sigmoid_f(g[k]);
+      ss = fmaf(x[k], x[k], ss);
+    }
+    float t[8];
+    if (BWD)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) t[k] = y[k] * w[k] * g[k] * sg[k], tx = fmaf(t[k], x[k], tx);
+#pragma unroll
+    for (int m = 1; m < LPR; m *= 2) {
+      ss += wave_shfl_xor(ss, m);
+      if (BWD) tx += wave_shfl_xor(tx, m);
+    }
+    const float r = 1.f / __builtin_sqrtf(fmaf(ss, inv, p.eps));
+    if (!on) continue;
+    if (!BWD) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) y[k] = x[k] * r * w[k] * g[k] * sg[k];
+      store8<T>(p.y, off(p.y), d0, y);
+    } else {
+      const float back = r * r * tx * inv;
+      float dx[8], dg[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float xr = x[k] * r;
+        dx[k] = r * (t[k] - x[k] * back);
+        dg[k] = y[k] * xr * w[k] * sg[k] * fmaf(g[k], 1.f - sg[k], 1.f);
+        dw[k] = fmaf(y[k] * xr, g[k] * sg[k], dw[k]);
+      }
+      store8<T>(p.dx, off(p.dx), d0, dx);
+      store8<T>(p.dgate, off(p.dgate), d0, dg);
+    }
+  }
+  if (BWD && p.part) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) red[k * kThreads + tid] = dw[k];
+    __syncthreads();
+    for (int d = tid; d < cols; d += kThreads) {
+      float s = 0.f;
+      for (int r = 0; r < kRows; ++r) s += red[d % 8 * kThreads + r * LPR + d / 8];
+      p.part[((int64_t)h * gridDim.x + blockIdx.x) * cols + d] = s;
+    }
+  }
+}
+
+// dweight: the workgroups' sums, of a head or of all.
+constexpr int kSumThreads = 1024;
+template <typename T>
+__global__ __launch_bounds__(kSumThreads) void gated_norm_weight_kernel(GatedNormParams p, int per_head) {
+  __shared__ float red[kSumThreads];
+  const int tid = threadIdx.x, lane = tid & 63, q = tid >> 6, d = blockIdx.x * 64 + lane, hw = blockIdx.y;
+  const int n = p.heads_w == 1 ? p.H * per_head : per_head;
+  const float* src = p.part + (p.heads_w == 1 ? 0 : (int64_t)hw * per_head * p.x.cols);
+  float s = 0.f;
+  if (d < p.x.cols)
+#pragma unroll 8
+    for (int i = q; i < n; i += kSumThreads / 64) s += src[(int64_t)i * p.x.cols + d];
+  red[tid] = s;
+  __syncthreads();
+  if (q || d >= p.x.cols) return;
+  for (int i = 1; i < kSumThreads / 64; ++i) s += red[64 * i + lane];
+  const int64_t at = (int64_t)hw * p.x.cols + d;
+  if (p.w_f32) static_cast<float*>(p.dweight)[at] = s;
+  else static_cast<uint16_t*>(p.dweight)[at] = T::bits(s);
+}
+
+// Rows of a head per workgroup: as many workgroups as fill the chip, of at least kNormRows turns.
+int rows_per(int64_t rows, int H, int at_once) {
+  const int64_t grid = std::max<int64_t>(1, kNormGrid / H), least = (int64_t)at_once * kNormRows;
+  return (int)std::min<int64_t>(std::max<int64_t>(least, (rows + grid - 1) / grid), (int64_t)1 << 30);
+}
+int lanes_per(int cols) { return cols <= 64 ? 8 : cols <= 128 ? 16 : cols <= 256 ? 32 : 64; }
+
+template <typename T, bool BWD>
+hipError_t norm_t(GatedNormParams p, hipStream_t s) {
+  const int lpr = lanes_per(p.x.cols);
+  const int64_t rows = (int64_t)p.B * p.N;
+  p.per = rows_per(rows, p.H, kThreads / lpr);
+  const dim3 grid((unsigned)((rows + p.per - 1) / p.per), p.H), block(kThreads);
+  const char* name = BWD ? "gated_norm_bwd" : "gated_norm";
+  hipError_t e = lpr == 8 ? launch_named(name, gated_norm_kernel<T, 8, BWD>, grid, block, s, p)
+                 : lpr == 16 ? launch_named(name, gated_norm_kernel<T, 16, BWD>, grid, block, s, p)
+                 : lpr == 32 ? launch_named(name, gated_norm_kernel<T, 32, BWD>, grid, block, s, p)
+                             : launch_named(name, gated_norm_kernel<T, 64, BWD>, grid, block, s, p);
+  if (e != hipSuccess || !BWD || !p.part) return e;
+  return launch_named("gated_norm_weight", gated_norm_weight_kernel<T>, dim3((p.x.cols + 63) / 64, p.heads_w), dim3(kSumThreads), s, p, (int)grid.x);
+}
+
+}  // namespace
+
+int gated_norm_parts(int B, int H, int N, int cols) {
+  const int64_t rows = (int64_t)B * N, per = rows_per(rows, H, kThreads / lanes_per(cols));
+  return (int)((rows + per - 1) / per) * H;
+}
+
+hipError_t launch_gated_norm(const GatedNormParams& p, int dtype, bool bwd, hipStream_t s) {
+  if (dtype == BF16::kCode) return bwd ? norm_t<BF16, true>(p, s) : norm_t<BF16, false>(p, s);
+  return bwd ? norm_t<F16, true>(p, s) : norm_t<F16, false>(p, s);
+}
+
+}  // namespace pope

@@ -1,0 +1,111 @@
+// Parameter blocks and launchers of the linear attention's kernels and of the gated norm, shared with the C ABI.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "pope_kernels.hpp"
+
+namespace pope {
+
+// Rows (b, h, n) of `cols` 16-bit elements.
+struct LinRows {
+  uint16_t* p;
+  int64_t s[3];
+  int cols;
+  int vec;   // inputs: rows of whole, aligned 16-byte units; outputs: of 8-byte units
+};
+
+// The rows of a call as segments of at most L rows of one sequence.  Padded batches: M segments for each of B sequences.
+// Packed rows: a sequence's segments follow those of the sequences before it; T is the most that N rows can have.
+struct LinSeqs {
+  const int* cu;   // packed: B + 1 bounds
+  int B, N, L, M, T;
+};
+
+struct LinCall {
+  LinSeqs seqs;
+  LinRows q, k, v, g;            // g: dO
+  const float* freqs; int64_t f_s[2]; int f_vec;
+  const float* bias; int64_t bias_sh;
+  const float* log_decay;        // one for each kv head, or null: no decay
+  const uint8_t* mask; int64_t mask_sb;
+  int Hq, Hk, G, D, R, E, Dv;    // E = D + R
+  float scale;
+};
+
+// What each segment adds to the state behind it (forward), or to the gradient of the state before it (reverse):
+// (T, Hk, E, Dv) fp32, rows in the column order of apply_pope_to_qk.
+struct LinStateParams {
+  LinCall c;
+  float* states;
+  int reverse, tiles;            // tiles: column tiles of the value dim (set by the launcher)
+};
+hipError_t launch_linear_states(const LinStateParams& p, int dtype, hipStream_t s);
+
+// Those sums to the states that segments start from, in place; `first` (B, Hk, E, Dv) or null: the state before everything
+// (reverse: the gradient of the state behind it), `last` or null takes what is left at the other end.
+struct LinScanParams {
+  LinCall c;
+  float* states; const float* first; float* last;
+  int reverse;
+};
+hipError_t launch_linear_scan(const LinScanParams& p, hipStream_t s);
+
+// What a job computes: rows x_i, y_j of P columns and z_j, out_i = sum_{j <= i} g^(i - j) (x_i . y_j) z_j + what the state
+// carries in.  Gradients of keys and values go over the rows in reverse.
+enum LinKind { kLinOut = 0, kLinDq = 1, kLinDk = 2, kLinDv = 3 };
+struct LinOutParams {
+  LinCall c;
+  LinRows out[2];                // of the launch's kinds: one, or dq and dk
+  const float* states[2];        // (T, Hk, E, Dv) that segments start from, forward and reverse; null: `first`
+  const float* first[2];         // (B, Hk, E, Dv) or null: zeros
+  float* dbias;                  // kLinDk: (T, Hk, R), or null
+  float* dphase[2];              // (b, h, n, R) of the kind's rows, or null
+  int heads_per;                 // query heads of a key head per workgroup (kLinOut, kLinDq)
+  int tiles, wgs;                // set by the launchers
+};
+// One translation unit each.
+hipError_t launch_linear_out_bf16(const LinOutParams& p, hipStream_t s);
+hipError_t launch_linear_out_f16(const LinOutParams& p, hipStream_t s);
+hipError_t launch_linear_dqk_bf16(const LinOutParams& p, hipStream_t s);
+hipError_t launch_linear_dqk_f16(const LinOutParams& p, hipStream_t s);
+hipError_t launch_linear_dv_bf16(const LinOutParams& p, hipStream_t s);
+hipError_t launch_linear_dv_f16(const LinOutParams& p, hipStream_t s);
+
+// dbias (Hb, R) from the segments' parts; dfreqs (Fb, N, R) from the rows' dphase of queries and keys.
+struct LinPhaseParams {
+  LinCall c;
+  const float* part; float* dbias; int Hb;
+  const float* dphase_q; const float* dphase_k; float* dfreqs; int64_t df_s[2]; int Fb;
+};
+hipError_t launch_linear_phase(const LinPhaseParams& p, hipStream_t s);
+
+// One token for each of B sequences against its state.
+struct LinStepParams {
+  LinCall c;
+  LinRows o;
+  const float* from; float* to;  // (slots, Hk, E, Dv), slots `slot_s` elements apart
+  const int* read; const int* write;   // slots of the sequences, or null: their numbers
+  int64_t slot_s;
+  int slots;
+  const uint16_t* gate; int64_t g_s[3]; const void* weight; int64_t w_sh; int w_f32; float eps;
+  int split;                     // workgroups for a (sequence, kv head): each has some of the value's columns
+};
+constexpr int kLinStepHeads = 4;   // query heads of a key head that a thread sums at once
+hipError_t launch_linear_step(const LinStepParams& p, int dtype, hipStream_t s);
+
+// y = x rsqrt(mean x^2 + eps) w silu(gate) over rows (b, h, n), and its gradients.
+struct GatedNormParams {
+  LinRows x, gate, y;            // backward: y is dy
+  LinRows dx, dgate;
+  const void* weight; int64_t w_sh; int w_f32;   // (1 or H, cols), null: ones
+  float* part;                   // backward: (workgroups, cols) sums of dweight, or null
+  void* dweight;                 // (1 or H, cols) in the weight's type
+  int B, H, N, heads_w;          // heads_w: rows of the weight
+  float eps;
+  int per;                       // set by the launcher: rows of a head per workgroup
+};
+int gated_norm_parts(int B, int H, int N, int cols);   // workgroups of the backward
+hipError_t launch_gated_norm(const GatedNormParams& p, int dtype, bool bwd, hipStream_t s);
+
+}  // namespace pope

@@ -1,0 +1,325 @@
+// Device helpers of the linear attention's kernels: segments of sequences, and rows on their way into LDS.
+#pragma once
+#include "linear.hpp"
+#include "pope_common.hpp"
+
+namespace pope {
+
+// ---------------------------------------------------------------- segments
+
+struct LinSeg {
+  int seq, batch;   // seq < 0: none
+  int row0, len;    // rows row0 .. row0 + len - 1 of the batch entry
+  int m;            // which of the sequence's
+};
+
+__device__ __forceinline__ int lin_bound(const LinSeqs& q, int i) { return min(max(q.cu[i], 0), q.N); }
+
+// Segments of the packed sequences before `seq` (all lanes of a wave call it), and of itself.
+__device__ __forceinline__ int lin_first(const LinSeqs& q, int seq, int* row0, int* rows) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int s0 = 0; s0 < seq; s0 += 64) {
+    const int s = s0 + lane;
+    int c = s < seq ? (max(lin_bound(q, s + 1) - lin_bound(q, s), 0) + q.L - 1) / q.L : 0;
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) c += __shfl_xor(c, i, 64);
+    before += c;
+  }
+  *row0 = lin_bound(q, seq);
+  *rows = max(lin_bound(q, seq + 1) - *row0, 0);
+  return __builtin_amdgcn_readfirstlane(before);
+}
+
+// Segment `at` of the call (uniform; all lanes of a wave call it).
+__device__ __forceinline__ LinSeg lin_segment(const LinSeqs& q, int at) {
+  LinSeg g;
+  if (!q.cu) {
+    g.seq = g.batch = at / q.M;
+    g.m = at - g.seq * q.M;
+    g.row0 = g.m * q.L;
+    g.len = min(q.L, q.N - g.row0);
+    return g;
+  }
+  const int lane = threadIdx.x & 63;
+  g.seq = -1;
+  g.batch = 0;
+  g.row0 = g.len = g.m = 0;
+  int before = 0;
+  for (int s0 = 0; s0 < q.B; s0 += 64) {
+    const int s = s0 + lane;
+    int a = 0, n = 0;
+    if (s < q.B) a = lin_bound(q, s), n = max(lin_bound(q, s + 1) - a, 0);
+    const int own = (n + q.L - 1) / q.L;
+    int upto = own;
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) {
+      const int x = __shfl_up(upto, i, 64);
+      upto += lane >= i ? x : 0;
+    }
+    const uint64_t above = __ballot(before + upto > at);
+    if (above) {
+      const int i = __builtin_ctzll(above);
+      const int first = before + __builtin_amdgcn_readlane(upto - own, i);
+      g.seq = s0 + i;
+      g.m = at - first;
+      g.row0 = __builtin_amdgcn_readlane(a, i) + g.m * q.L;
+      g.len = min(q.L, __builtin_amdgcn_readlane(n, i) - g.m * q.L);
+      return g;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return g;
+}
+
+// ---------------------------------------------------------------- decay
+
+// g^n from log2 g.  g^0 is 1 whatever g is (a decay of 0 has log2 g = -inf).
+__device__ __forceinline__ float lin_power(float lg, int n) { return n == 0 ? 1.f : __builtin_amdgcn_exp2f(lg * (float)n); }
+__device__ __forceinline__ float lin_log2(const LinCall& c, int hk) { return c.log_decay ? c.log_decay[hk] * kLog2e : 0.f; }
+
+// ---------------------------------------------------------------- rows
+
+// sin and cos of x + 2 pi turns: as sincos_rev, with `turns` in [-1/2, 1/2] added to the fraction, so that the sum of a far
+// position's angle and a bias is not rounded.
+__device__ __forceinline__ void sincos_turns(float x, float turns, float* s, float* c) {
+#pragma clang fp contract(off)
+  constexpr float kHi = 0.15915494f;
+  constexpr float kLo = (float)(0.15915494309189533577 - (double)0.15915494f);
+  const float hi = x * kHi;
+  const float lo = fmaf(x, kHi, -hi) + x * kLo;
+  const float fr = (hi - __builtin_rintf(hi)) + (lo + turns);
+  *s = __builtin_amdgcn_sinf(fr);
+  *c = __builtin_amdgcn_cosf(fr);
+}
+// A bias as turns.
+__device__ __forceinline__ float lin_turns(float b) {
+  const float t = b * 0.15915494309189533577f;
+  return t - __builtin_rintf(t);
+}
+
+__device__ __forceinline__ u32x4 lin_load8(const uint16_t* row, int d0, int cols, bool vec) {
+  u32x4 w = {0, 0, 0, 0};
+  if (vec) {
+    w = *reinterpret_cast<const u32x4*>(row + d0);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (d0 + k < cols) w[k >> 1] |= (uint32_t)row[d0 + k] << (16 * (k & 1));
+  }
+  return w;
+}
+__device__ __forceinline__ void lin_angles8(const float* row, int d0, int R, bool vec, f32x4* f) {
+  f[0] = f[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (d0 >= R) return;
+  if (vec) {
+    f[0] = *reinterpret_cast<const f32x4*>(row + d0);
+    f[1] = *reinterpret_cast<const f32x4*>(row + d0 + 4);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (d0 + k < R) f[k >> 2][k & 3] = row[d0 + k];
+  }
+}
+
+__device__ __forceinline__ const float* lin_angle_row(const LinCall& c, int batch, int row) {
+  return c.freqs + (int64_t)batch * c.f_s[0] + (int64_t)row * c.f_s[1];
+}
+
+// A tile's place of column e in rows that the products read as operands of 32 columns, eight for each quarter of a wave:
+// column 16 h + 4 q + i of a group of 32 at 8 q + 4 h + i, which is where a 16x16 result's rows (4 q + i of tile h) come back as an
+// operand.  Only tiles read along their rows are laid out so; those read across them keep their columns.
+template <bool PERM>
+__device__ __forceinline__ int lin_place(int e) {
+  return PERM ? (e & ~31) | ((e >> 2) & 3) << 3 | ((e >> 4) & 1) << 2 | (e & 3) : e;
+}
+
+// bf16 parts of fp32 values: one, rounded, or the sum of two (16 significant bits).
+template <int PL>
+__device__ __forceinline__ void lin_pack4(f32x4 v, u32x2* w) {
+  w[0] = u32x2{BF16::pack2(v[0], v[1]), BF16::pack2(v[2], v[3])};
+  if constexpr (PL == 2)
+    w[1] = u32x2{BF16::pack2(v[0] - BF16::to_float((uint16_t)w[0][0]), v[1] - BF16::to_float((uint16_t)(w[0][0] >> 16))),
+                 BF16::pack2(v[2] - BF16::to_float((uint16_t)w[0][1]), v[3] - BF16::to_float((uint16_t)(w[0][1] >> 16)))};
+}
+
+// A tile of rows in LDS: PL planes of `stride` elements a row, `plane` elements apart.
+struct LinTile {
+  uint16_t* p;
+  int stride, plane;
+};
+
+// Eight columns from e on (e a multiple of 8), all inside the tile.
+template <int PL, bool PERM>
+__device__ __forceinline__ void lin_put8(const LinTile& t, int row, int e, const float* v) {
+  u32x2 a[PL], b[PL];
+  lin_pack4<PL>(f32x4{v[0], v[1], v[2], v[3]}, a);
+  lin_pack4<PL>(f32x4{v[4], v[5], v[6], v[7]}, b);
+#pragma unroll
+  for (int l = 0; l < PL; ++l) {
+    uint16_t* at = t.p + l * t.plane + row * t.stride;
+    if constexpr (PERM) {
+      *reinterpret_cast<u32x2*>(at + lin_place<true>(e)) = a[l];
+      *reinterpret_cast<u32x2*>(at + lin_place<true>(e + 4)) = b[l];
+    } else {
+      *reinterpret_cast<u32x4*>(at + e) = u32x4{a[l][0], a[l][1], b[l][0], b[l][1]};
+    }
+  }
+}
+template <int PL, bool PERM>
+__device__ __forceinline__ void lin_put1(const LinTile& t, int row, int e, float v) {
+  const uint16_t h = BF16::bits(v);
+  uint16_t* at = t.p + row * t.stride + lin_place<PERM>(e);
+  *at = h;
+  if constexpr (PL == 2) at[t.plane] = BF16::bits(v - BF16::to_float(h));
+}
+
+// Eight columns of a plain row, from column d0 of the tile on.  Returns whether all are finite.
+template <typename T, int PL, bool PERM>
+__device__ __forceinline__ bool lin_put_plain(const LinTile& t, int row, int d0, u32x4 x, float factor = 1.f) {
+  float v[8];
+  unpack8<T>(x, v);
+  bool fin = true;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) fin = fin && fabsf(v[k]) <= 3.402823466e38f, v[k] *= factor;
+  lin_put8<PL, PERM>(t, row, d0, v);
+  return fin;
+}
+
+// Eight columns d0 .. of a row, expanded: (softplus(x) cos, softplus(x) sin) pairs of the rotated dims, then the others, all
+// times `factor`; columns e_lo .. e_lo + e_n - 1 of the expanded row are the tile's.  Rows that are not `live` are zeros.
+// turns: the bias of the keys in LDS, or null.  Returns whether all that the tile gets is finite.
+template <typename T, int PL, bool PERM>
+__device__ __forceinline__ bool lin_put_polar(const LinTile& t, int row, int d0, u32x4 x8, const f32x4* f, bool live, float factor, const float* turns,
+                                              int D, int R, int e_lo, int e_n) {
+  float x[8], a[8], b[8];
+  unpack8<T>(x8, x);
+  bool fin = true;
+  if (!live) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) a[k] = b[k] = 0.f;
+  } else if (d0 < R) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      float sn, cs;
+      const bool rot = d0 + k < R;
+      sincos_turns(f[k >> 2][k & 3], turns && rot ? turns[d0 + k] : 0.f, &sn, &cs);
+      const float m = softplus_f(x[k]) * factor;
+      a[k] = rot ? m * cs : x[k] * factor;
+      b[k] = rot ? m * sn : 0.f;
+      fin = fin && fabsf(a[k]) <= 3.402823466e38f && fabsf(b[k]) <= 3.402823466e38f;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) a[k] = x[k] * factor, fin = fin && fabsf(a[k]) <= 3.402823466e38f;
+  }
+  if (R % 8 == 0) {   // a chunk is all rotated or all not, and its columns start on a multiple of 8
+    if (d0 < R) {
+      const int e = 2 * d0 - e_lo;
+      if ((unsigned)e < (unsigned)e_n) {
+        float w[16];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[2 * k] = a[k], w[2 * k + 1] = b[k];
+        lin_put8<PL, PERM>(t, row, e, w);
+        lin_put8<PL, PERM>(t, row, e + 8, w + 8);
+        return fin;
+      }
+    } else {
+      const int e = R + d0 - e_lo;   // columns behind the row (D no multiple of 8) are zeros
+      if ((unsigned)e < (unsigned)e_n) {
+        lin_put8<PL, PERM>(t, row, e, a);
+        return fin;
+      }
+    }
+    return true;
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int d = d0 + k, e = (d < R ? 2 * d : R + d) - e_lo;
+    if (d >= D) break;
+    if ((unsigned)e < (unsigned)e_n) lin_put1<PL, PERM>(t, row, e, a[k]);
+    if (d < R && (unsigned)(e + 1) < (unsigned)e_n) lin_put1<PL, PERM>(t, row, e + 1, b[k]);
+  }
+  return fin;
+}
+
+// A thread's u-th chunk of eight columns of a tile of C rows: four side by side in a row, the next rows, then the next
+// four: a wave's chunks are all rotated or mostly not.
+template <int C, int THREADS>
+struct LinItem {
+  int row, d0;
+  __device__ __forceinline__ explicit LinItem(int u) {
+    const int t = (int)threadIdx.x + THREADS * u;
+    row = (t >> 2) % C;
+    d0 = ((t & 3) + 4 * (t / (4 * C))) * 8;
+  }
+};
+
+// Operand of 16 rows x 32 columns, read across: lane l gets column n0 + l % 16 of rows r0 + 4 q + i, then r0 + 16 + 4 q + i
+// (q = l / 16).  Row strides are an odd multiple of two 16-byte units, so that the eight rows of half a wave fall on different banks.
+__device__ __forceinline__ u32x4 lin_across(const uint16_t* tile, int stride, int r0, int n0, int lane) {
+  const int q = lane >> 4, j = lane & 15;
+  const uint16_t* p = tile + (r0 + 4 * q + (j >> 2)) * stride + n0 + 4 * (j & 3);
+  const u32x2 lo = lds_read_tr16(p), hi = lds_read_tr16(p + 16 * stride);
+  return u32x4{lo[0], lo[1], hi[0], hi[1]};
+}
+// The same operand read along rows that keep their columns (two pieces), and that were permuted (one).
+__device__ __forceinline__ u32x4 lin_along(const uint16_t* tile, int stride, int r0, int n0, int lane) {
+  const uint16_t* p = tile + (r0 + (lane & 15)) * stride + n0 + 4 * (lane >> 4);
+  const u32x2 lo = *reinterpret_cast<const u32x2*>(p), hi = *reinterpret_cast<const u32x2*>(p + 16);
+  return u32x4{lo[0], lo[1], hi[0], hi[1]};
+}
+__device__ __forceinline__ u32x4 lin_along_placed(const uint16_t* tile, int stride, int r0, int n0, int lane) {
+  return *reinterpret_cast<const u32x4*>(tile + (r0 + (lane & 15)) * stride + n0 + 8 * (lane >> 4));
+}
+
+// c + a b over operands of PA and PB bf16 parts; the product of two second parts is below what fp32 keeps of the others.
+template <int PA, int PB>
+__device__ __forceinline__ f32x4 lin_mfma(const u32x4* a, const u32x4* b, f32x4 c) {
+#pragma unroll
+  for (int i = PA - 1; i >= 0; --i)
+#pragma unroll
+    for (int j = PB - 1; j >= 0; --j)
+      if (i + j < 2) c = BF16::mfma16(as_vec8<bf16x8>(a[i]), as_vec8<bf16x8>(b[j]), c);
+  return c;
+}
+
+// Tile shapes: P columns of the contraction, NT columns of the result per workgroup, NW waves of SL columns each.
+template <typename T, int P_, int NT_, int NW_>
+struct LinCfg {
+  static constexpr int P = P_, NT = NT_, NW = NW_, SL = NT / NW, CT = SL / 16;
+  static constexpr int kThreads = 64 * NW;
+  // bf16 rows are one part, fp16 rows two, exactly
+  static constexpr int PL = T::kCode == 2 ? 1 : 2;
+  static constexpr int C = PL == 1 ? 64 : 32, KS = C / 32, IT = C / 16;
+  static constexpr int XS = P + 8, YS = P + 16, ZS = NT + 16, AS = C + 8;
+  static constexpr int TP = (C * (P / 8) + kThreads - 1) / kThreads, TZ = (C * (NT / 8) + kThreads - 1) / kThreads;
+};
+
+// Rows of P / NT that a call takes: dispatch over (P, NT), P for the contraction's columns, NT for the result's.
+// Wide results go in tiles of 256 columns over eight waves; states of more than 256 rows leave room for 16 columns a wave.
+template <typename T, template <typename> class Launch, typename... A>
+hipError_t lin_dispatch(int pcols, int ncols, A&&... args) {
+  const int p = pcols <= 64 ? 64 : pcols <= 128 ? 128 : pcols <= 256 ? 256 : 512;
+  const int n = ncols <= 64 ? 64 : ncols <= 128 ? 128 : 256;
+#define POPE_LIN_CASE(PP, NN, WW) return Launch<LinCfg<T, PP, NN, WW>>::go(args...)
+  if (p == 64) {
+    if (n == 64) POPE_LIN_CASE(64, 64, 4);
+    if (n == 128) POPE_LIN_CASE(64, 128, 4);
+    POPE_LIN_CASE(64, 256, 8);
+  }
+  if (p == 128) {
+    if (n == 64) POPE_LIN_CASE(128, 64, 4);
+    if (n == 128) POPE_LIN_CASE(128, 128, 4);
+    POPE_LIN_CASE(128, 256, 8);
+  }
+  if (p == 256) {
+    if (n == 64) POPE_LIN_CASE(256, 64, 4);
+    if (n == 128) POPE_LIN_CASE(256, 128, 4);
+    POPE_LIN_CASE(256, 256, 8);
+  }
+  POPE_LIN_CASE(512, 128, 8);
+#undef POPE_LIN_CASE
+}
+
+}  // namespace pope

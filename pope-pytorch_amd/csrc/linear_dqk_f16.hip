@@ -1,0 +1,8 @@
+// Linear attention of fp16 rows: gradients of the queries and keys.
+#include "linear_out.hpp"
+
+namespace pope {
+
+hipError_t launch_linear_dqk_f16(const LinOutParams& p, hipStream_t s) { return launch_linear_out_t<F16, kLinDq>(p, "linear_dqk", s); }
+
+}  // namespace pope

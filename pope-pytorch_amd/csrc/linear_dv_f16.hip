@@ -1,0 +1,8 @@
+// Linear attention of fp16 rows: gradients of the values.
+#include "linear_out.hpp"
+
+namespace pope {
+
+hipError_t launch_linear_dv_f16(const LinOutParams& p, hipStream_t s) { return launch_linear_out_t<F16, kLinDv>(p, "linear_dv", s); }
+
+}  // namespace pope

@@ -10,6 +10,7 @@
 #include <cstring>
 #include <string>
 
+#include "linear.hpp"
 #include "paged.hpp"
 #include "pope_kernels.hpp"
 
@@ -1264,6 +1265,340 @@ int pope_paged_attn(const pope_paged* d, const void* q, const float* freqs, cons
   p.parts = reinterpret_cast<int*>(static_cast<char*>(workspace) + sh.part_o + sh.part_ml);
   const hipError_t e = pope::launch_paged_attn(p, sh.few, d->dtype, d->quantized != 0, reinterpret_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "paged attention launch");
+  return POPE_OK;
+}
+
+}  // extern "C"
+
+namespace {
+
+// ---------------------------------------------------------------- linear attention
+
+int check_linear(const pope_linear* d) {
+  if (!d) return fail(POPE_ERR_INVALID, "descriptor is NULL");
+  if (d->B < 1 || d->N < 0 || d->Hq < 1 || d->Hk < 1)
+    return fail(POPE_ERR_INVALID, "B, Hq, Hk must be >= 1 and N >= 0 (got %d, %d, %d, %d)", d->B, d->Hq, d->Hk, d->N);
+  if (d->Hq % d->Hk != 0) return fail(POPE_ERR_INVALID, "query heads %d must be a multiple of kv heads %d", d->Hq, d->Hk);
+  if (d->D < 1 || d->D > 256 || d->Dv < 1 || d->Dv > 256)
+    return fail(POPE_ERR_UNSUPPORTED, "linear attention covers head and value dims 1 to 256 (got %d, %d)", d->D, d->Dv);
+  if (d->R < 0 || d->R > d->D) return fail(POPE_ERR_INVALID, "rotate dim %d must be in [0, head dim %d]", d->R, d->D);
+  if (d->dtype != POPE_F16 && d->dtype != POPE_BF16) return fail(POPE_ERR_INVALID, "linear attention takes fp16 or bf16 rows (dtype %d)", d->dtype);
+  if (d->N > (1 << 28) || d->B > (1 << 20) || d->Hq > 65535)
+    return fail(POPE_ERR_UNSUPPORTED, "%d sequences, %d rows, %d heads: too many", d->B, d->N, d->Hq);
+  if (d->bias_sh < 0 || d->mask_sb < 0) return fail(POPE_ERR_INVALID, "negative bias / mask stride");
+  int rc = check_strides("freqs", d->f_s, 2);
+  if (!rc) rc = check_strides("q", d->q_s, 3);
+  if (!rc) rc = check_strides("k", d->k_s, 3);
+  if (!rc) rc = check_strides("v", d->v_s, 3);
+  if (!rc) rc = check_strides("o", d->o_s, 3);
+  return rc;
+}
+
+// Rows of a segment: a multiple of 64 (a chunk) that brings the workgroups to about kLinGrid.
+constexpr int kLinGrid = 512, kLinChunk = 64;
+
+struct LinShape {
+  int L, M, T;
+  bool parts;      // some sequence may have more than one segment
+  size_t states;   // bytes of the states of all segments
+};
+
+LinShape linear_shape(const pope_linear& d, bool packed) {
+  LinShape s;
+  const int64_t rows = (packed ? 1 : (int64_t)d.B) * d.N;
+  const int64_t want = std::max<int64_t>(1, (rows * d.Hk + kLinGrid - 1) / kLinGrid);
+  s.L = (int)std::min<int64_t>((want + kLinChunk - 1) / kLinChunk * kLinChunk, (int64_t)(d.N + kLinChunk - 1) / kLinChunk * kLinChunk);
+  s.L = std::max(s.L, kLinChunk);
+  s.M = std::max(1, (d.N + s.L - 1) / s.L);
+  s.T = packed ? (int)std::min<int64_t>(d.N, (int64_t)d.N / s.L + d.B) : d.B * s.M;
+  s.parts = d.N > s.L;
+  s.states = align_up((size_t)s.T * d.Hk * (d.D + d.R) * d.Dv * sizeof(float));
+  return s;
+}
+
+struct LinBytes { size_t reverse, dbias, dq, dk, all; };
+LinBytes linear_bwd_bytes(const pope_linear& d, const LinShape& s, bool packed, bool want_dfreqs) {
+  LinBytes b;
+  const size_t rows = (size_t)(packed ? 1 : d.B) * d.N;
+  b.reverse = s.states;   // also for calls that want the initial state's gradient only
+  b.dbias = align_up((size_t)s.T * d.Hk * d.R * sizeof(float));
+  b.dq = want_dfreqs ? align_up(rows * d.Hq * d.R * sizeof(float)) : 0;
+  b.dk = want_dfreqs ? align_up(rows * d.Hk * d.R * sizeof(float)) : 0;
+  b.all = b.reverse + b.dbias + b.dq + b.dk;
+  return b;
+}
+
+pope::LinRows lin_rows(const void* p, const int64_t* s, int cols, int unit) {
+  pope::LinRows r;
+  r.p = static_cast<uint16_t*>(const_cast<void*>(p));
+  copy3(r.s, s);
+  r.cols = cols;
+  r.vec = cols % unit == 0 && reinterpret_cast<uintptr_t>(p) % (2 * unit) == 0 && s[0] % unit == 0 && s[1] % unit == 0 && s[2] % unit == 0;
+  return r;
+}
+
+pope::LinCall linear_call(const pope_linear& d, const LinShape& s, const void* q, const void* k, const void* v, const float* freqs,
+                          const float* bias, const float* log_decay, const uint8_t* mask, const int32_t* cu) {
+  pope::LinCall c;
+  std::memset(&c, 0, sizeof c);
+  c.seqs = pope::LinSeqs{cu, d.B, d.N, s.L, s.M, s.T};
+  c.q = lin_rows(q, d.q_s, d.D, 8);
+  c.k = lin_rows(k, d.k_s, d.D, 8);
+  c.v = lin_rows(v, d.v_s, d.Dv, 8);
+  c.freqs = freqs;
+  c.f_s[0] = d.f_s[0]; c.f_s[1] = d.f_s[1];
+  c.f_vec = d.R % 8 == 0 && aligned16(freqs) && d.f_s[0] % 4 == 0 && d.f_s[1] % 4 == 0;
+  c.bias = bias; c.bias_sh = d.bias_sh;
+  c.log_decay = log_decay;
+  c.mask = mask; c.mask_sb = d.mask_sb;
+  c.Hq = d.Hq; c.Hk = d.Hk; c.G = d.Hq / d.Hk; c.D = d.D; c.R = d.R; c.E = d.D + d.R; c.Dv = d.Dv;
+  c.scale = d.scale;
+  return c;
+}
+
+int check_linear_ptrs(const pope_linear* d, const void* q, const void* k, const void* v, const float* freqs, const float* bias) {
+  if (!q || !k || !v) return fail(POPE_ERR_INVALID, "q, k, v must be non-NULL");
+  if (d->R > 0 && (!freqs || !bias)) return fail(POPE_ERR_INVALID, "rotate dim %d > 0 needs freqs and bias", d->R);
+  return POPE_OK;
+}
+
+// Query heads of a key head per workgroup: all, where that fills the chip, or as many as divide them.
+int lin_heads_per(const pope_linear& d, const LinShape& s) {
+  const int G = d.Hq / d.Hk;
+  for (int n = G; n > 1; --n)
+    if (G % n == 0 && (int64_t)s.T * d.Hk * (G / n) >= kLinGrid) return n;
+  return 1;
+}
+
+int lin_fail(hipError_t e, const char* what) {
+  if (e == hipErrorInvalidValue) return fail(POPE_ERR_UNSUPPORTED, "%s: too many workgroups", what);
+  return hip_fail(e, what);
+}
+
+int check_norm(const pope_gated_norm* d) {
+  if (!d) return fail(POPE_ERR_INVALID, "descriptor is NULL");
+  if (d->B < 0 || d->H < 1 || d->N < 0) return fail(POPE_ERR_INVALID, "H must be >= 1 and B, N >= 0 (got %d, %d, %d)", d->H, d->B, d->N);
+  if (d->cols < 1 || d->cols > 512) return fail(POPE_ERR_UNSUPPORTED, "the gated norm covers rows of 1 to 512 values (got %d)", d->cols);
+  if (d->dtype != POPE_F16 && d->dtype != POPE_BF16) return fail(POPE_ERR_INVALID, "the gated norm takes fp16 or bf16 rows (dtype %d)", d->dtype);
+  if (d->weight_rows != 1 && d->weight_rows != d->H) return fail(POPE_ERR_INVALID, "weight rows %d must be 1 or %d", d->weight_rows, d->H);
+  if (d->H > 65535 || (int64_t)d->B * d->N > ((int64_t)1 << 32)) return fail(POPE_ERR_UNSUPPORTED, "%d x %d rows, %d heads: too many", d->B, d->N, d->H);
+  if (d->weight_sh < 0) return fail(POPE_ERR_INVALID, "negative weight stride");
+  int rc = check_strides("x", d->x_s, 3);
+  if (!rc) rc = check_strides("gate", d->gate_s, 3);
+  return rc;
+}
+
+pope::GatedNormParams norm_params(const pope_gated_norm& d, const void* x, const void* gate, const void* weight) {
+  pope::GatedNormParams p;
+  std::memset(&p, 0, sizeof p);
+  p.x = lin_rows(x, d.x_s, d.cols, 8);
+  p.gate = lin_rows(gate, d.gate_s, d.cols, 8);
+  p.weight = weight;
+  p.w_sh = d.weight_rows > 1 ? d.weight_sh : 0;
+  p.w_f32 = d.weight_f32;
+  p.B = d.B; p.H = d.H; p.N = d.N; p.heads_w = d.weight_rows;
+  p.eps = d.eps;
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+int pope_linear_bytes(const pope_linear* d, int packed, int final, int want_dfreqs, size_t bytes[2]) {
+  const int rc = check_linear(d);
+  if (rc) return rc;
+  if (!bytes) return fail(POPE_ERR_INVALID, "bytes is NULL");
+  const LinShape s = linear_shape(*d, packed != 0);
+  bytes[0] = s.parts || final ? s.states : 0;
+  bytes[1] = linear_bwd_bytes(*d, s, packed != 0, want_dfreqs != 0).all;
+  return POPE_OK;
+}
+
+int pope_linear_fwd(const pope_linear* d, const void* q, const void* k, const void* v, const float* freqs, const float* bias,
+                    const float* log_decay, const uint8_t* mask, const int32_t* cu, const float* initial, void* o, float* last,
+                    void* states, size_t states_bytes, void* stream) {
+  int rc = check_linear(d);
+  if (rc) return rc;
+  if (d->N == 0) return POPE_OK;
+  if ((rc = check_linear_ptrs(d, q, k, v, freqs, bias))) return rc;
+  if (!o) return fail(POPE_ERR_INVALID, "o must be non-NULL");
+  const LinShape sh = linear_shape(*d, cu != nullptr);
+  const bool sums = sh.parts || last;
+  if ((rc = check_ws(sums ? sh.states : 0, states, states_bytes))) return rc;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const pope::LinCall c = linear_call(*d, sh, q, k, v, freqs, bias, log_decay, mask, cu);
+  if (sums) {
+    const pope::LinStateParams sp{c, static_cast<float*>(states), 0, 0};
+    hipError_t e = pope::launch_linear_states(sp, d->dtype, s);
+    if (e != hipSuccess) return lin_fail(e, "linear attention states launch");
+    const pope::LinScanParams cp{c, static_cast<float*>(states), initial, last, 0};
+    if ((e = pope::launch_linear_scan(cp, s)) != hipSuccess) return lin_fail(e, "linear attention scan launch");
+  }
+  pope::LinOutParams p;
+  std::memset(&p, 0, sizeof p);
+  p.c = c;
+  p.out[0] = lin_rows(o, d->o_s, d->Dv, 4);
+  p.states[0] = sums ? static_cast<const float*>(states) : nullptr;
+  p.first[0] = initial;
+  p.heads_per = lin_heads_per(*d, sh);
+  const hipError_t e = d->dtype == POPE_BF16 ? pope::launch_linear_out_bf16(p, s) : pope::launch_linear_out_f16(p, s);
+  if (e != hipSuccess) return lin_fail(e, "linear attention launch");
+  return POPE_OK;
+}
+
+int pope_linear_bwd(const pope_linear* d, const void* dout, const float* dlast, const void* q, const void* k, const void* v,
+                    const float* freqs, const float* bias, const float* log_decay, const uint8_t* mask, const int32_t* cu,
+                    const float* initial, const void* states, size_t states_bytes, void* dq, void* dk, void* dv, float* dfreqs,
+                    float* dbias, float* dinitial, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_linear(d);
+  if (rc) return rc;
+  for (const int64_t* st : {d->do_s, d->dq_s, d->dk_s, d->dv_s})
+    if ((rc = check_strides("gradient", st, 3))) return rc;
+  if ((rc = check_strides("dfreqs", d->df_s, 2))) return rc;
+  if (d->N == 0) return POPE_OK;
+  if ((rc = check_linear_ptrs(d, q, k, v, freqs, bias))) return rc;
+  if (!dout || !dq || !dk || !dv) return fail(POPE_ERR_INVALID, "dout, dq, dk, dv must be non-NULL");
+  const LinShape sh = linear_shape(*d, cu != nullptr);
+  if ((rc = check_ws(sh.parts ? sh.states : 0, const_cast<void*>(states), states_bytes))) return rc;
+  const LinBytes lb = linear_bwd_bytes(*d, sh, cu != nullptr, dfreqs != nullptr);
+  if ((rc = check_ws(lb.all, workspace, workspace_bytes))) return rc;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  float* reverse = reinterpret_cast<float*>(ws);
+  pope::LinCall c = linear_call(*d, sh, q, k, v, freqs, bias, log_decay, mask, cu);
+  c.g = lin_rows(dout, d->do_s, d->Dv, 8);
+  hipError_t e;
+  const bool sums = sh.parts || dinitial;
+  if (sums) {
+    const pope::LinStateParams sp{c, reverse, 1, 0};
+    if ((e = pope::launch_linear_states(sp, d->dtype, s)) != hipSuccess) return lin_fail(e, "linear attention states launch");
+    const pope::LinScanParams cp{c, reverse, dlast, dinitial, 1};
+    if ((e = pope::launch_linear_scan(cp, s)) != hipSuccess) return lin_fail(e, "linear attention scan launch");
+  }
+  pope::LinOutParams p;
+  std::memset(&p, 0, sizeof p);
+  p.c = c;
+  p.states[0] = sh.parts ? static_cast<const float*>(states) : nullptr;
+  p.first[0] = initial;
+  p.states[1] = sums ? reverse : nullptr;
+  p.first[1] = dlast;
+  p.heads_per = lin_heads_per(*d, sh);
+  p.out[0] = lin_rows(dq, d->dq_s, d->D, 4);
+  p.out[1] = lin_rows(dk, d->dk_s, d->D, 4);
+  if (d->R > 0) {
+    if (dbias) p.dbias = reinterpret_cast<float*>(ws + lb.reverse);
+    if (dfreqs) {
+      p.dphase[0] = reinterpret_cast<float*>(ws + lb.reverse + lb.dbias);
+      p.dphase[1] = reinterpret_cast<float*>(ws + lb.reverse + lb.dbias + lb.dq);
+    }
+  }
+  const bool bf16 = d->dtype == POPE_BF16;
+  if ((e = bf16 ? pope::launch_linear_dqk_bf16(p, s) : pope::launch_linear_dqk_f16(p, s)) != hipSuccess) return lin_fail(e, "linear attention launch");
+  pope::LinOutParams pv = p;
+  pv.out[0] = lin_rows(dv, d->dv_s, d->Dv, 4);
+  pv.dphase[0] = pv.dphase[1] = nullptr;
+  if ((e = bf16 ? pope::launch_linear_dv_bf16(pv, s) : pope::launch_linear_dv_f16(pv, s)) != hipSuccess) return lin_fail(e, "linear attention launch");
+  if (d->R > 0 && (dbias || dfreqs)) {
+    pope::LinPhaseParams ph;
+    std::memset(&ph, 0, sizeof ph);
+    ph.c = c;
+    ph.part = p.dbias; ph.dbias = dbias; ph.Hb = d->bias_sh ? d->Hk : 1;
+    ph.dphase_q = p.dphase[0]; ph.dphase_k = p.dphase[1]; ph.dfreqs = dfreqs;
+    ph.df_s[0] = d->df_s[0]; ph.df_s[1] = d->df_s[1];
+    ph.Fb = d->df_s[0] && !cu ? d->B : 1;
+    if ((e = pope::launch_linear_phase(ph, s)) != hipSuccess) return lin_fail(e, "linear attention phase launch");
+  }
+  return POPE_OK;
+}
+
+int pope_gated_norm_fwd(const pope_gated_norm* d, const void* x, const void* gate, const void* weight, void* y, void* stream) {
+  int rc = check_norm(d);
+  if (rc || (rc = check_strides("y", d->y_s, 3))) return rc;
+  if (d->B == 0 || d->N == 0) return POPE_OK;
+  if (!x || !gate || !y) return fail(POPE_ERR_INVALID, "x, gate, y must be non-NULL");
+  pope::GatedNormParams p = norm_params(*d, x, gate, weight);
+  p.y = lin_rows(y, d->y_s, d->cols, 8);
+  const hipError_t e = pope::launch_gated_norm(p, d->dtype, false, reinterpret_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "gated norm launch");
+  return POPE_OK;
+}
+
+int pope_gated_norm_bytes(const pope_gated_norm* d, size_t* bytes) {
+  const int rc = check_norm(d);
+  if (rc) return rc;
+  if (!bytes) return fail(POPE_ERR_INVALID, "bytes is NULL");
+  *bytes = d->B && d->N ? align_up((size_t)pope::gated_norm_parts(d->B, d->H, d->N, d->cols) * d->cols * sizeof(float)) : 0;
+  return POPE_OK;
+}
+
+int pope_gated_norm_bwd(const pope_gated_norm* d, const void* dy, const void* x, const void* gate, const void* weight, void* dx,
+                        void* dgate, void* dweight, void* workspace, size_t workspace_bytes, void* stream) {
+  size_t need = 0;
+  int rc = pope_gated_norm_bytes(d, &need);
+  if (rc) return rc;
+  for (const int64_t* st : {d->dy_s, d->dx_s, d->dgate_s})
+    if ((rc = check_strides("gradient", st, 3))) return rc;
+  if (d->B == 0 || d->N == 0) return POPE_OK;
+  if (!dy || !x || !gate || !dx || !dgate) return fail(POPE_ERR_INVALID, "dy, x, gate, dx, dgate must be non-NULL");
+  if (dweight && !weight) return fail(POPE_ERR_INVALID, "dweight wanted, but there is no weight");
+  if (dweight && (rc = check_ws(need, workspace, workspace_bytes))) return rc;
+  pope::GatedNormParams p = norm_params(*d, x, gate, weight);
+  p.y = lin_rows(dy, d->dy_s, d->cols, 8);
+  p.dx = lin_rows(dx, d->dx_s, d->cols, 8);
+  p.dgate = lin_rows(dgate, d->dgate_s, d->cols, 8);
+  p.part = dweight ? static_cast<float*>(workspace) : nullptr;
+  p.dweight = dweight;
+  const hipError_t e = pope::launch_gated_norm(p, d->dtype, true, reinterpret_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "gated norm backward launch");
+  return POPE_OK;
+}
+
+int pope_linear_step(const pope_linear* d, const void* q, const void* k, const void* v, const float* freqs, const float* bias,
+                     const float* log_decay, float* states, int32_t slots, int64_t slot_s, const int32_t* from, const int32_t* to,
+                     const pope_gated_norm* norm, const void* gate, const void* weight, void* o, void* stream) {
+  int rc = check_linear(d);
+  if (rc) return rc;
+  if (d->N != 1) return fail(POPE_ERR_INVALID, "a step takes one row for each sequence (N = %d)", d->N);
+  if ((rc = check_linear_ptrs(d, q, k, v, freqs, bias))) return rc;
+  if (!o || !states || slots < 1) return fail(POPE_ERR_INVALID, "o, states must be non-NULL and slots >= 1 (got %d)", slots);
+  if (slot_s < (int64_t)d->Hk * (d->D + d->R) * d->Dv) return fail(POPE_ERR_INVALID, "slots of %lld elements overlap", (long long)slot_s);
+  if (!from && d->B > slots) return fail(POPE_ERR_INVALID, "%d sequences, %d slots", d->B, slots);
+  if ((norm != nullptr) != (gate != nullptr)) return fail(POPE_ERR_INVALID, "norm and gate come together");
+  if (norm) {
+    if ((rc = check_norm(norm))) return rc;
+    if (norm->B != d->B || norm->H != d->Hq || norm->N != 1 || norm->cols != d->Dv || norm->dtype != d->dtype)
+      return fail(POPE_ERR_INVALID, "the norm's rows are not the step's");
+  }
+  const LinShape sh = linear_shape(*d, false);
+  pope::LinStepParams p;
+  std::memset(&p, 0, sizeof p);
+  p.c = linear_call(*d, sh, q, k, v, freqs, bias, log_decay, nullptr, nullptr);
+  p.o = lin_rows(o, d->o_s, d->Dv, 4);
+  p.from = states; p.to = states;
+  p.read = from; p.write = to;
+  p.slots = slots; p.slot_s = slot_s;
+  // More query heads of a key head than a thread sums at once go over columns held in LDS, 16 for each workgroup; the norm, which
+  // needs a row's columns together, is then a launch of its own.
+  const bool many = p.c.G > pope::kLinStepHeads, own = norm && many;
+  if (norm && !own) {
+    p.gate = static_cast<const uint16_t*>(gate);
+    copy3(p.g_s, norm->gate_s);
+    p.weight = weight; p.w_sh = norm->weight_rows > 1 ? norm->weight_sh : 0; p.w_f32 = norm->weight_f32; p.eps = norm->eps;
+    p.split = 1;
+  } else {
+    const int most = (d->Dv + 15) / 16;
+    const int64_t wgs = (int64_t)d->B * d->Hk;
+    p.split = many ? most : (int)std::min<int64_t>(most, std::max<int64_t>(1, kLinGrid / wgs));
+  }
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  hipError_t e = pope::launch_linear_step(p, d->dtype, s);
+  if (e != hipSuccess) return lin_fail(e, "linear attention step launch");
+  if (own) {
+    pope::GatedNormParams n = norm_params(*norm, o, gate, weight);
+    n.x = n.y = lin_rows(o, d->o_s, d->Dv, 8);
+    if ((e = pope::launch_gated_norm(n, d->dtype, false, s)) != hipSuccess) return hip_fail(e, "gated norm launch");
+  }
   return POPE_OK;
 }
 

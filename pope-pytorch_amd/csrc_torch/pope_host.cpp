@@ -937,6 +937,10 @@ std::optional<std::pair<Tensor, Tensor>> paged_attn_eager(const Tensor& q, OptTe
   return std::make_pair(o, lse);
 }
 
+// ---------------------------------------------------------------- linear attention
+
+#include "linear_host.hpp"
+
 }  // namespace
 
 PYBIND11_MODULE(_pope_host, m) {
@@ -953,6 +957,14 @@ PYBIND11_MODULE(_pope_host, m) {
   m.def("paged_write_eager", &paged_write_eager, nogil);
   m.def("paged_read_eager", &paged_read_eager, nogil);
   m.def("paged_attn_eager", &paged_attn_eager, nogil);
+  m.def("linear_eager", &linear_eager, nogil);
+  m.def("linear_fwd", &linear_fwd_impl, nogil);
+  m.def("linear_bwd", &linear_bwd_impl, nogil);
+  m.def("linear_step_eager", &linear_step_eager, nogil);
+  m.def("linear_step", &linear_step_impl, nogil);
+  m.def("gated_norm_eager", &gated_norm_eager, nogil);
+  m.def("gated_norm_fwd", &gated_norm_fwd_impl, nogil);
+  m.def("gated_norm_bwd", &gated_norm_bwd_impl, nogil);
   m.def("untraced", &untraced);
   m.def("last_bwd_prepared", [] { return g_last_bwd_prepared.load(); });
   m.def("abi_version", [] { return POPE_ABI_VERSION; });

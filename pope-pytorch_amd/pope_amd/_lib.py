@@ -59,11 +59,34 @@ class PopePaged(ctypes.Structure):
     ]
 
 
+class PopeLinear(ctypes.Structure):
+    """Mirror of ``struct pope_linear`` (include/pope_abi.h)."""
+
+    _fields_ = [
+        ("B", ctypes.c_int32), ("N", ctypes.c_int32), ("Hq", ctypes.c_int32), ("Hk", ctypes.c_int32), ("D", ctypes.c_int32),
+        ("R", ctypes.c_int32), ("Dv", ctypes.c_int32), ("dtype", ctypes.c_int32), ("scale", ctypes.c_float),
+        ("q_s", _I64x3), ("k_s", _I64x3), ("v_s", _I64x3), ("o_s", _I64x3), ("do_s", _I64x3), ("dq_s", _I64x3), ("dk_s", _I64x3),
+        ("dv_s", _I64x3), ("f_s", ctypes.c_int64 * 2), ("bias_sh", ctypes.c_int64), ("df_s", ctypes.c_int64 * 2), ("mask_sb", ctypes.c_int64),
+    ]
+
+
+class PopeGatedNorm(ctypes.Structure):
+    """Mirror of ``struct pope_gated_norm`` (include/pope_abi.h)."""
+
+    _fields_ = [
+        ("B", ctypes.c_int32), ("H", ctypes.c_int32), ("N", ctypes.c_int32), ("cols", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("weight_rows", ctypes.c_int32), ("weight_f32", ctypes.c_int32), ("eps", ctypes.c_float), ("x_s", _I64x3), ("gate_s", _I64x3),
+        ("y_s", _I64x3), ("dy_s", _I64x3), ("dx_s", _I64x3), ("dgate_s", _I64x3), ("weight_sh", ctypes.c_int64),
+    ]
+
+
 EXPORTS = (
     "pope_abi_version", "pope_last_error", "pope_workspace_bytes", "pope_sim_fwd", "pope_sim_bwd",
     "pope_flash_fwd", "pope_flash_fwd_split", "pope_flash_bwd", "pope_flash_bwd_split", "pope_flash_decode", "pope_flash_decode_noalloc", "pope_polar_fwd",
     "pope_polar_bwd", "pope_cast_f16", "pope_pad_rows", "pope_paged_cache_bytes",
-    "pope_paged_write", "pope_paged_read", "pope_paged_workspace_bytes", "pope_paged_attn", "pope_profile_enable", "pope_profile_read", "pope_profile_reset",
+    "pope_paged_write", "pope_paged_read", "pope_paged_workspace_bytes", "pope_paged_attn",
+    "pope_linear_bytes", "pope_linear_fwd", "pope_linear_bwd", "pope_linear_step", "pope_gated_norm_bytes", "pope_gated_norm_fwd", "pope_gated_norm_bwd",
+    "pope_profile_enable", "pope_profile_read", "pope_profile_reset",
 )
 
 _lib = None
@@ -112,6 +135,21 @@ def _declare(lib):
     lib.pope_paged_workspace_bytes.argtypes = [gp, i32, ctypes.POINTER(sz)]
     lib.pope_paged_attn.restype = i32
     lib.pope_paged_attn.argtypes = [gp] + [vp] * 11 + [sz, vp]
+    lp, np_ = ctypes.POINTER(PopeLinear), ctypes.POINTER(PopeGatedNorm)
+    lib.pope_linear_bytes.restype = i32
+    lib.pope_linear_bytes.argtypes = [lp, i32, i32, i32, ctypes.POINTER(sz)]
+    lib.pope_linear_fwd.restype = i32
+    lib.pope_linear_fwd.argtypes = [lp] + [vp] * 12 + [sz, vp]
+    lib.pope_linear_bwd.restype = i32
+    lib.pope_linear_bwd.argtypes = [lp] + [vp] * 12 + [sz] + [vp] * 7 + [sz, vp]
+    lib.pope_linear_step.restype = i32
+    lib.pope_linear_step.argtypes = [lp] + [vp] * 7 + [ctypes.c_int32, ctypes.c_int64, vp, vp, np_, vp, vp, vp, vp]
+    lib.pope_gated_norm_bytes.restype = i32
+    lib.pope_gated_norm_bytes.argtypes = [np_, ctypes.POINTER(sz)]
+    lib.pope_gated_norm_fwd.restype = i32
+    lib.pope_gated_norm_fwd.argtypes = [np_] + [vp] * 5
+    lib.pope_gated_norm_bwd.restype = i32
+    lib.pope_gated_norm_bwd.argtypes = [np_] + [vp] * 8 + [sz, vp]
     lib.pope_profile_enable.restype = i32
     lib.pope_profile_enable.argtypes = [i32]
     lib.pope_profile_read.restype = i32
