@@ -357,12 +357,14 @@ int pope_paged_attn(const pope_paged* desc, const void* q, const float* freqs, c
  * (their query still has an output).  Padded batches: B sequences of N rows; packed (cu_seqlens given): N rows in one batch entry,
  * sequence b owning rows cu_seqlens[b] <= r < cu_seqlens[b + 1]; outputs and gradients of rows outside every sequence are 0.
  * cu_seqlens that decrease leave unspecified values (never an access out of bounds).  States are fp32 (B, Hk, D + R, Dv),
- * contiguous; `initial` NULL: zeros.  Calls that need 2^22 workgroups or more return POPE_ERR_UNSUPPORTED.
+ * contiguous; `initial` NULL: zeros.  Products take bf16 rows as they are; fp16 and fp32 rows, and bf16 rows with o_f32, as the sum of two
+ * bf16 parts (2^-17 of each factor).  Calls that need 2^22 workgroups or more return POPE_ERR_UNSUPPORTED.
  */
 typedef struct pope_linear {
   int32_t B, N, Hq, Hk;      /* sequences; rows per sequence (packed: in all); heads */
   int32_t D, R, Dv;          /* 1 <= D <= 256, 0 <= R <= D, 1 <= Dv <= 256, any values */
-  int32_t dtype;             /* enum pope_dtype of rows: POPE_F16 or POPE_BF16 */
+  int32_t dtype;             /* enum pope_dtype of rows */
+  int32_t o_f32;             /* o and its gradient in fp32, whatever dtype is */
   float scale;
   int64_t q_s[3], k_s[3], v_s[3], o_s[3];      /* (b, h, n) element strides, unit feature stride, any alignment */
   int64_t do_s[3], dq_s[3], dk_s[3], dv_s[3];
@@ -371,32 +373,32 @@ typedef struct pope_linear {
   int64_t mask_sb;
 } pope_linear;
 
-/* bytes[0]: the states that segments of rows start from (0: a call that needs none), written by pope_linear_fwd and read by
- * pope_linear_bwd of the same descriptor; bytes[1]: the backward's workspace.  `final`: whether the call returns the final states.
- * `want_dfreqs`: whether the backward is given dfreqs.  Both 256-byte aligned. */
+/* bytes[0]: `kept`, the expanded rows and the states that segments of rows start from: the forward's workspace, and what
+ * pope_linear_bwd of the same descriptor reads; bytes[1]: the backward's workspace.  `final`: whether the call returns the final states;
+ * `want_dfreqs`: whether its backward is given dfreqs.  Both 256-byte aligned. */
 int pope_linear_bytes(const pope_linear* desc, int packed, int final, int want_dfreqs, size_t bytes[2]);
 
 /* o (dtype, o_s), every row; `last` NULL or the states behind the sequences. */
 int pope_linear_fwd(const pope_linear* desc, const void* q, const void* k, const void* v, const float* freqs,
                     const float* bias, const float* log_decay, const uint8_t* mask, const int32_t* cu_seqlens,
-                    const float* initial, void* o, float* last, void* states, size_t states_bytes, void* stream);
+                    const float* initial, void* o, float* last, void* kept, size_t kept_bytes, void* stream);
 
 /* Gradients of o's `dout` and the final states' `dlast` (NULL: zeros): dq, dk, dv (dtype); dfreqs (fp32, df_s), dbias (fp32, rows of
  * R) and dinitial (fp32) or NULL.  All are written, not accumulated into, in a fixed order. */
 int pope_linear_bwd(const pope_linear* desc, const void* dout, const float* dlast, const void* q, const void* k,
                     const void* v, const float* freqs, const float* bias, const float* log_decay,
-                    const uint8_t* mask, const int32_t* cu_seqlens, const float* initial, const void* states,
-                    size_t states_bytes, void* dq, void* dk, void* dv, float* dfreqs, float* dbias, float* dinitial,
+                    const uint8_t* mask, const int32_t* cu_seqlens, const float* initial, const void* kept,
+                    size_t kept_bytes, void* dq, void* dk, void* dv, float* dfreqs, float* dbias, float* dinitial,
                     void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Rows of a head normalised and gated: y = x / sqrt(mean x^2 + eps) * weight * silu(gate).  No counterpart in the reference.
- * x, gate, y (b, h, n) rows of 1 <= cols <= 512 values of `dtype`, any alignment; weight NULL (ones) or (1 or H, cols), of
- * `dtype` or fp32 (weight_f32).
+ * gate, y (b, h, n) rows of 1 <= cols <= 512 values of `dtype`, any alignment; x and its gradient of `dtype` or fp32 (x_f32); weight
+ * NULL (ones) or (1 or H, cols), of `dtype` or fp32 (weight_f32).
  */
 typedef struct pope_gated_norm {
   int32_t B, H, N, cols, dtype;
-  int32_t weight_rows, weight_f32;  /* weight_rows: 1 or H */
+  int32_t x_f32, weight_rows, weight_f32;  /* weight_rows: 1 or H */
   float eps;
   int64_t x_s[3], gate_s[3], y_s[3], dy_s[3], dx_s[3], dgate_s[3], weight_sh;
 } pope_gated_norm;

@@ -14,28 +14,26 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kNormGrid = 2048, kNormRows = 4;   // workgroups that fill the chip; the least turns of one
 
-__device__ __forceinline__ float weight_at(const GatedNormParams& p, int h, int d, float (*f16)(uint16_t)) {
-  if (d >= p.x.cols) return 0.f;
-  return p.w_f32 ? static_cast<const float*>(p.weight)[h * p.w_sh + d] : f16(static_cast<const uint16_t*>(p.weight)[h * p.w_sh + d]);
-}
-template <typename T>
-__device__ __forceinline__ void load8(const LinRows& r, int64_t off, int d0, float* f) {
-  unpack8<T>(lin_load8(r.p + off, d0, r.cols, r.vec), f);
-}
-template <typename T>
-__device__ __forceinline__ void store8(const LinRows& r, int64_t off, int d0, const float* f) {
-  uint16_t* at = r.p + off + d0;
-  if (r.vec) {
-    *reinterpret_cast<u32x4*>(at) = u32x4{T::pack2(f[0], f[1]), T::pack2(f[2], f[3]), T::pack2(f[4], f[5]), T::pack2(f[6], f[7])};
-  } else {
+__device__ __forceinline__ void load8(const LinRows& r, int64_t at, int d0, float* f) { lin_unpack8<kTwo>(lin_load8<kTwo>(r, at, d0), r.type, f); }
+__device__ __forceinline__ void store8(const LinRows& r, int64_t at, int d0, const float* f) {
+  if (!r.vec) {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      if (d0 + k < r.cols) at[k] = T::bits(f[k]);
+      if (d0 + k < r.cols) lin_set<kTwo>(r, at + d0 + k, f[k]);
+  } else if (r.type == 0) {
+    float* p = static_cast<float*>(r.p) + at + d0;
+    *reinterpret_cast<f32x4*>(p) = f32x4{f[0], f[1], f[2], f[3]};
+    *reinterpret_cast<f32x4*>(p + 4) = f32x4{f[4], f[5], f[6], f[7]};
+  } else {
+    u32x4 w;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = r.type == 1 ? F16::pack2(f[2 * k], f[2 * k + 1]) : BF16::pack2(f[2 * k], f[2 * k + 1]);
+    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(r.p) + at + d0) = w;
   }
 }
 
 // LPR lanes for a row.  A workgroup has p.per rows of a head (rows: batch x n).
-template <typename T, int LPR, bool BWD>
+template <int LPR, bool BWD>
 __global__ __launch_bounds__(kThreads) void gated_norm_kernel(GatedNormParams p) {
   constexpr int kRows = kThreads / LPR;
   __shared__ float red[BWD ? kThreads * 8 : 1];
@@ -45,7 +43,7 @@ __global__ __launch_bounds__(kThreads) void gated_norm_kernel(GatedNormParams p)
   const int64_t rows = (int64_t)p.B * p.N, first = (int64_t)blockIdx.x * p.per;
   float w[8], dw[8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) w[k] = p.weight ? weight_at(p, h, d0 + k, T::to_float) : 1.f, dw[k] = 0.f;
+  for (int k = 0; k < 8; ++k) w[k] = p.weight && d0 + k < cols ? lin_value(p.weight, p.w_type, h * p.w_sh + d0 + k) : 1.f, dw[k] = 0.f;
   const float inv = 1.f / cols;
   for (int i = r0; i < p.per; i += kRows) {
     const int64_t row = first + i;
@@ -56,9 +54,9 @@ __global__ __launch_bounds__(kThreads) void gated_norm_kernel(GatedNormParams p)
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] = g[k] = y[k] = 0.f;
     if (on) {
-      load8<T>(p.x, off(p.x), d0, x);
-      load8<T>(p.gate, off(p.gate), d0, g);
-      if (BWD) load8<T>(p.y, off(p.y), d0, y);
+      load8(p.x, off(p.x), d0, x);
+      load8(p.gate, off(p.gate), d0, g);
+      if (BWD) load8(p.y, off(p.y), d0, y);
     }
     float sg[8], ss = 0.f, tx = 0.f;
 #pragma unroll
@@ -80,7 +78,7 @@ __global__ __launch_bounds__(kThreads) void gated_norm_kernel(GatedNormParams p)
     if (!BWD) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) y[k] = x[k] * r * w[k] * g[k] * sg[k];
-      store8<T>(p.y, off(p.y), d0, y);
+      store8(p.y, off(p.y), d0, y);
     } else {
       const float back = r * r * tx * inv;
       float dx[8], dg[8];
@@ -91,8 +89,8 @@ __global__ __launch_bounds__(kThreads) void gated_norm_kernel(GatedNormParams p)
         dg[k] = y[k] * xr * w[k] * sg[k] * fmaf(g[k], 1.f - sg[k], 1.f);
         dw[k] = fmaf(y[k] * xr, g[k] * sg[k], dw[k]);
       }
-      store8<T>(p.dx, off(p.dx), d0, dx);
-      store8<T>(p.dgate, off(p.dgate), d0, dg);
+      store8(p.dx, off(p.dx), d0, dx);
+      store8(p.dgate, off(p.dgate), d0, dg);
     }
   }
   if (BWD && p.part) {
@@ -109,7 +107,6 @@ __global__ __launch_bounds__(kThreads) void gated_norm_kernel(GatedNormParams p)
 
 // dweight: the workgroups' sums, of a head or of all.
 constexpr int kSumThreads = 1024;
-template <typename T>
 __global__ __launch_bounds__(kSumThreads) void gated_norm_weight_kernel(GatedNormParams p, int per_head) {
   __shared__ float red[kSumThreads];
   const int tid = threadIdx.x, lane = tid & 63, q = tid >> 6, d = blockIdx.x * 64 + lane, hw = blockIdx.y;
@@ -124,8 +121,8 @@ __global__ __launch_bounds__(kSumThreads) void gated_norm_weight_kernel(GatedNor
   if (q || d >= p.x.cols) return;
   for (int i = 1; i < kSumThreads / 64; ++i) s += red[64 * i + lane];
   const int64_t at = (int64_t)hw * p.x.cols + d;
-  if (p.w_f32) static_cast<float*>(p.dweight)[at] = s;
-  else static_cast<uint16_t*>(p.dweight)[at] = T::bits(s);
+  if (p.w_type == 0) static_cast<float*>(p.dweight)[at] = s;
+  else static_cast<uint16_t*>(p.dweight)[at] = p.w_type == 1 ? F16::bits(s) : BF16::bits(s);
 }
 
 // Rows of a head per workgroup: as many workgroups as fill the chip, of at least kNormRows turns.
@@ -135,19 +132,19 @@ int rows_per(int64_t rows, int H, int at_once) {
 }
 int lanes_per(int cols) { return cols <= 64 ? 8 : cols <= 128 ? 16 : cols <= 256 ? 32 : 64; }
 
-template <typename T, bool BWD>
+template <bool BWD>
 hipError_t norm_t(GatedNormParams p, hipStream_t s) {
   const int lpr = lanes_per(p.x.cols);
   const int64_t rows = (int64_t)p.B * p.N;
   p.per = rows_per(rows, p.H, kThreads / lpr);
   const dim3 grid((unsigned)((rows + p.per - 1) / p.per), p.H), block(kThreads);
   const char* name = BWD ? "gated_norm_bwd" : "gated_norm";
-  hipError_t e = lpr == 8 ? launch_named(name, gated_norm_kernel<T, 8, BWD>, grid, block, s, p)
-                 : lpr == 16 ? launch_named(name, gated_norm_kernel<T, 16, BWD>, grid, block, s, p)
-                 : lpr == 32 ? launch_named(name, gated_norm_kernel<T, 32, BWD>, grid, block, s, p)
-                             : launch_named(name, gated_norm_kernel<T, 64, BWD>, grid, block, s, p);
+  hipError_t e = lpr == 8 ? launch_named(name, gated_norm_kernel<8, BWD>, grid, block, s, p)
+                 : lpr == 16 ? launch_named(name, gated_norm_kernel<16, BWD>, grid, block, s, p)
+                 : lpr == 32 ? launch_named(name, gated_norm_kernel<32, BWD>, grid, block, s, p)
+                             : launch_named(name, gated_norm_kernel<64, BWD>, grid, block, s, p);
   if (e != hipSuccess || !BWD || !p.part) return e;
-  return launch_named("gated_norm_weight", gated_norm_weight_kernel<T>, dim3((p.x.cols + 63) / 64, p.heads_w), dim3(kSumThreads), s, p, (int)grid.x);
+  return launch_named("gated_norm_weight", gated_norm_weight_kernel, dim3((p.x.cols + 63) / 64, p.heads_w), dim3(kSumThreads), s, p, (int)grid.x);
 }
 
 }  // namespace
@@ -157,9 +154,6 @@ int gated_norm_parts(int B, int H, int N, int cols) {
   return (int)((rows + per - 1) / per) * H;
 }
 
-hipError_t launch_gated_norm(const GatedNormParams& p, int dtype, bool bwd, hipStream_t s) {
-  if (dtype == BF16::kCode) return bwd ? norm_t<BF16, true>(p, s) : norm_t<BF16, false>(p, s);
-  return bwd ? norm_t<F16, true>(p, s) : norm_t<F16, false>(p, s);
-}
+hipError_t launch_gated_norm(const GatedNormParams& p, bool bwd, hipStream_t s) { return bwd ? norm_t<true>(p, s) : norm_t<false>(p, s); }
 
 }  // namespace pope

@@ -7,12 +7,13 @@
 
 namespace pope {
 
-// Rows (b, h, n) of `cols` 16-bit elements.
+// Rows (b, h, n) of `cols` elements.
 struct LinRows {
-  uint16_t* p;
-  int64_t s[3];
+  void* p;
+  int64_t s[3];   // elements
   int cols;
-  int vec;   // inputs: rows of whole, aligned 16-byte units; outputs: of 8-byte units
+  int type;       // pope_dtype: 0 fp32, 1 fp16, 2 bf16
+  int vec;        // rows of whole, aligned units of 8 elements (outputs of the attention: of 4)
 };
 
 // The rows of a call as segments of at most L rows of one sequence.  Padded batches: M segments for each of B sequences.
@@ -22,25 +23,37 @@ struct LinSeqs {
   int B, N, L, M, T;
 };
 
+// Expanded rows of one side, bf16: (batch, H, N, EP), columns behind E zeros; the second part, where there is one, `plane`
+// elements behind the first.
+struct LinHat {
+  uint16_t* p;
+  int64_t plane;
+  int H, EP;
+};
+
 struct LinCall {
   LinSeqs seqs;
   LinRows q, k, v, g;            // g: dO
+  LinHat qh, kh;                 // queries times the scale; keys that the mask leaves out are zeros
   const float* freqs; int64_t f_s[2]; int f_vec;
   const float* bias; int64_t bias_sh;
   const float* log_decay;        // one for each kv head, or null: no decay
   const uint8_t* mask; int64_t mask_sb;
   int Hq, Hk, G, D, R, E, Dv;    // E = D + R
   float scale;
+  int split;                     // operands as the sum of two bf16 parts; 0: one part, all rows bf16
 };
 
 // What each segment adds to the state behind it (forward), or to the gradient of the state before it (reverse):
 // (T, Hk, E, Dv) fp32, rows in the column order of apply_pope_to_qk.
 struct LinStateParams {
   LinCall c;
-  float* states;
-  int reverse, tiles;            // tiles: column tiles of the value dim (set by the launcher)
+  float* states;                 // launch_linear_states: null for the expanded rows only
+  int reverse;
+  int tiles, key_wgs;            // set by the launchers
 };
-hipError_t launch_linear_states(const LinStateParams& p, int dtype, hipStream_t s);
+hipError_t launch_linear_states(const LinStateParams& p, hipStream_t s);   // expands rows; forward: writes them
+hipError_t launch_linear_sums(const LinStateParams& p, hipStream_t s);     // from the expanded rows, which are as exact as `split` says
 
 // Those sums to the states that segments start from, in place; `first` (B, Hk, E, Dv) or null: the state before everything
 // (reverse: the gradient of the state behind it), `last` or null takes what is left at the other end.
@@ -66,11 +79,11 @@ struct LinOutParams {
 };
 // One translation unit each.
 hipError_t launch_linear_out_bf16(const LinOutParams& p, hipStream_t s);
-hipError_t launch_linear_out_f16(const LinOutParams& p, hipStream_t s);
+hipError_t launch_linear_out_split(const LinOutParams& p, hipStream_t s);
 hipError_t launch_linear_dqk_bf16(const LinOutParams& p, hipStream_t s);
-hipError_t launch_linear_dqk_f16(const LinOutParams& p, hipStream_t s);
+hipError_t launch_linear_dqk_split(const LinOutParams& p, hipStream_t s);
 hipError_t launch_linear_dv_bf16(const LinOutParams& p, hipStream_t s);
-hipError_t launch_linear_dv_f16(const LinOutParams& p, hipStream_t s);
+hipError_t launch_linear_dv_split(const LinOutParams& p, hipStream_t s);
 
 // dbias (Hb, R) from the segments' parts; dfreqs (Fb, N, R) from the rows' dphase of queries and keys.
 struct LinPhaseParams {
@@ -88,17 +101,16 @@ struct LinStepParams {
   const int* read; const int* write;   // slots of the sequences, or null: their numbers
   int64_t slot_s;
   int slots;
-  const uint16_t* gate; int64_t g_s[3]; const void* weight; int64_t w_sh; int w_f32; float eps;
+  LinRows gate; const void* weight; int64_t w_sh; int w_type; float eps;   // gate.p null: none
   int split;                     // workgroups for a (sequence, kv head): each has some of the value's columns
 };
-constexpr int kLinStepHeads = 4;   // query heads of a key head that a thread sums at once
-hipError_t launch_linear_step(const LinStepParams& p, int dtype, hipStream_t s);
+hipError_t launch_linear_step(const LinStepParams& p, hipStream_t s);
 
 // y = x rsqrt(mean x^2 + eps) w silu(gate) over rows (b, h, n), and its gradients.
 struct GatedNormParams {
   LinRows x, gate, y;            // backward: y is dy
   LinRows dx, dgate;
-  const void* weight; int64_t w_sh; int w_f32;   // (1 or H, cols), null: ones
+  const void* weight; int64_t w_sh; int w_type;   // (1 or H, cols), null: ones
   float* part;                   // backward: (workgroups, cols) sums of dweight, or null
   void* dweight;                 // (1 or H, cols) in the weight's type
   int B, H, N, heads_w;          // heads_w: rows of the weight
@@ -106,6 +118,6 @@ struct GatedNormParams {
   int per;                       // set by the launcher: rows of a head per workgroup
 };
 int gated_norm_parts(int B, int H, int N, int cols);   // workgroups of the backward
-hipError_t launch_gated_norm(const GatedNormParams& p, int dtype, bool bwd, hipStream_t s);
+hipError_t launch_gated_norm(const GatedNormParams& p, bool bwd, hipStream_t s);
 
 }  // namespace pope

@@ -5,6 +5,8 @@
 
 namespace pope {
 
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+
 // ---------------------------------------------------------------- segments
 
 struct LinSeg {
@@ -98,17 +100,147 @@ __device__ __forceinline__ float lin_turns(float b) {
   return t - __builtin_rintf(t);
 }
 
-__device__ __forceinline__ u32x4 lin_load8(const uint16_t* row, int d0, int cols, bool vec) {
-  u32x4 w = {0, 0, 0, 0};
-  if (vec) {
-    w = *reinterpret_cast<const u32x4*>(row + d0);
+// How a kernel takes its rows: kOne, bf16 rows as operands of one part; kTwo, rows of any type as the sum of two bf16 parts
+// (exactly, for 16-bit rows; 2^-17 off for fp32 ones).
+enum LinParts { kOne = 1, kTwo = 2 };
+
+// Eight elements of a row, as they are in memory.
+template <int PL>
+struct LinRaw {
+  u32x4 a;
+};
+template <>
+struct LinRaw<kTwo> {
+  u32x4 a, b;   // b: of fp32 rows
+};
+template <int PL>
+__device__ __forceinline__ LinRaw<PL> lin_zeros() { return LinRaw<PL>{}; }
+
+// `at`: elements before the row.
+template <int PL>
+__device__ __forceinline__ LinRaw<PL> lin_load8(const LinRows& r, int64_t at, int d0) {
+  LinRaw<PL> w{};
+  if constexpr (PL == kTwo) {
+    if (r.type == 0) {
+      const float* p = static_cast<const float*>(r.p) + at + d0;
+      if (r.vec) {
+        w.a = *reinterpret_cast<const u32x4*>(p);
+        w.b = *reinterpret_cast<const u32x4*>(p + 4);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (d0 + k < r.cols) w.a[k] = __float_as_uint(p[k]);
+          if (d0 + 4 + k < r.cols) w.b[k] = __float_as_uint(p[4 + k]);
+        }
+      }
+      return w;
+    }
+  }
+  const uint16_t* p = static_cast<const uint16_t*>(r.p) + at + d0;
+  if (r.vec) {
+    w.a = *reinterpret_cast<const u32x4*>(p);
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      if (d0 + k < cols) w[k >> 1] |= (uint32_t)row[d0 + k] << (16 * (k & 1));
+      if (d0 + k < r.cols) w.a[k >> 1] |= (uint32_t)p[k] << (16 * (k & 1));
   }
   return w;
 }
+template <int PL>
+__device__ __forceinline__ void lin_unpack8(const LinRaw<PL>& w, int type, float* f) {
+  if constexpr (PL == kTwo) {
+    if (type == 0) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f[k] = __uint_as_float(w.a[k]), f[4 + k] = __uint_as_float(w.b[k]);
+      return;
+    }
+    if (type == 1) return unpack8<F16>(w.a, f);
+  }
+  unpack8<BF16>(w.a, f);
+}
+// One element.
+template <int PL>
+__device__ __forceinline__ float lin_get(const LinRows& r, int64_t at) {
+  if constexpr (PL == kTwo) {
+    if (r.type == 0) return static_cast<const float*>(r.p)[at];
+    if (r.type == 1) return F16::to_float(static_cast<const uint16_t*>(r.p)[at]);
+  }
+  return BF16::to_float(static_cast<const uint16_t*>(r.p)[at]);
+}
+template <int PL>
+__device__ __forceinline__ void lin_set(const LinRows& r, int64_t at, float v) {
+  if constexpr (PL == kTwo) {
+    if (r.type == 0) {
+      static_cast<float*>(r.p)[at] = v;
+      return;
+    }
+    if (r.type == 1) {
+      static_cast<uint16_t*>(r.p)[at] = F16::bits(v);
+      return;
+    }
+  }
+  static_cast<uint16_t*>(r.p)[at] = BF16::bits(v);
+}
+// Four elements of an output row from column d on (r.vec: d a multiple of 4, whole units).
+template <int PL>
+__device__ __forceinline__ void lin_set4(const LinRows& r, int64_t at, int d, f32x4 v) {
+  if (d >= r.cols) return;
+  if (!r.vec) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (d + k < r.cols) lin_set<PL>(r, at + d + k, v[k]);
+    return;
+  }
+  if constexpr (PL == kTwo) {
+    if (r.type == 0) {
+      *reinterpret_cast<f32x4*>(static_cast<float*>(r.p) + at + d) = v;
+      return;
+    }
+    if (r.type == 1) {
+      *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(r.p) + at + d) = u32x2{F16::pack2(v[0], v[1]), F16::pack2(v[2], v[3])};
+      return;
+    }
+  }
+  *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(r.p) + at + d) = u32x2{BF16::pack2(v[0], v[1]), BF16::pack2(v[2], v[3])};
+}
+// Two elements, at an even place of an aligned row.
+template <int PL>
+__device__ __forceinline__ void lin_get2(const LinRows& r, int64_t at, float* v) {
+  if constexpr (PL == kTwo) {
+    if (r.type == 0) {
+      const f32x2 x = *reinterpret_cast<const f32x2*>(static_cast<const float*>(r.p) + at);
+      v[0] = x[0], v[1] = x[1];
+      return;
+    }
+  }
+  const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(r.p) + at);
+  if constexpr (PL == kTwo) {
+    if (r.type == 1) {
+      v[0] = F16::to_float((uint16_t)w), v[1] = F16::to_float((uint16_t)(w >> 16));
+      return;
+    }
+  }
+  v[0] = BF16::to_float((uint16_t)w), v[1] = BF16::to_float((uint16_t)(w >> 16));
+}
+template <int PL>
+__device__ __forceinline__ void lin_set2(const LinRows& r, int64_t at, float a, float b) {
+  if constexpr (PL == kTwo) {
+    if (r.type == 0) {
+      *reinterpret_cast<f32x2*>(static_cast<float*>(r.p) + at) = f32x2{a, b};
+      return;
+    }
+    if (r.type == 1) {
+      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(r.p) + at) = F16::pack2(a, b);
+      return;
+    }
+  }
+  *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(r.p) + at) = BF16::pack2(a, b);
+}
+// Values of an array of one of the types.
+__device__ __forceinline__ float lin_value(const void* p, int type, int64_t i) {
+  return type == 0 ? static_cast<const float*>(p)[i] : type == 1 ? F16::to_float(static_cast<const uint16_t*>(p)[i]) : BF16::to_float(static_cast<const uint16_t*>(p)[i]);
+}
+
 __device__ __forceinline__ void lin_angles8(const float* row, int d0, int R, bool vec, f32x4* f) {
   f[0] = f[1] = f32x4{0.f, 0.f, 0.f, 0.f};
   if (d0 >= R) return;
@@ -174,31 +306,52 @@ __device__ __forceinline__ void lin_put1(const LinTile& t, int row, int e, float
   if constexpr (PL == 2) at[t.plane] = BF16::bits(v - BF16::to_float(h));
 }
 
-// Eight columns of a plain row, from column d0 of the tile on.  Returns whether all are finite.
-template <typename T, int PL, bool PERM>
-__device__ __forceinline__ bool lin_put_plain(const LinTile& t, int row, int d0, u32x4 x, float factor = 1.f) {
-  float v[8];
-  unpack8<T>(x, v);
-  bool fin = true;
+// Whether some of eight bf16 values is not finite.
+__device__ __forceinline__ bool lin_odd8(u32x4 w) {
+  uint32_t m = 0;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) fin = fin && fabsf(v[k]) <= 3.402823466e38f, v[k] *= factor;
-  lin_put8<PL, PERM>(t, row, d0, v);
-  return fin;
+  for (int i = 0; i < 4; ++i) m |= (w[i] & 0x7fff7fffu) + 0x00800080u;   // carries into the sign where all exponent bits are set
+  return (m & 0x80008000u) != 0;
+}
+// Eight columns of a tile from e on, as parts in registers.
+template <int PL, bool PERM>
+__device__ __forceinline__ void lin_put_parts(const LinTile& t, int row, int e, const u32x4* w) {
+#pragma unroll
+  for (int l = 0; l < PL; ++l) {
+    uint16_t* at = t.p + l * t.plane + row * t.stride;
+    if constexpr (PERM) {
+      *reinterpret_cast<u32x2*>(at + lin_place<true>(e)) = u32x2{w[l][0], w[l][1]};
+      *reinterpret_cast<u32x2*>(at + lin_place<true>(e + 4)) = u32x2{w[l][2], w[l][3]};
+    } else {
+      *reinterpret_cast<u32x4*>(at + e) = w[l];
+    }
+  }
 }
 
-// Eight columns d0 .. of a row, expanded: (softplus(x) cos, softplus(x) sin) pairs of the rotated dims, then the others, all
-// times `factor`; columns e_lo .. e_lo + e_n - 1 of the expanded row are the tile's.  Rows that are not `live` are zeros.
-// turns: the bias of the keys in LDS, or null.  Returns whether all that the tile gets is finite.
-template <typename T, int PL, bool PERM>
-__device__ __forceinline__ bool lin_put_polar(const LinTile& t, int row, int d0, u32x4 x8, const f32x4* f, bool live, float factor, const float* turns,
-                                              int D, int R, int e_lo, int e_n) {
-  float x[8], a[8], b[8];
-  unpack8<T>(x8, x);
-  bool fin = true;
-  if (!live) {
+// Eight columns of a plain row, from column e of the tile on.  Returns whether some value is not finite.
+template <int PL, bool PERM>
+__device__ __forceinline__ bool lin_put_plain(const LinTile& t, int row, int e, const LinRaw<PL>& x, int type) {
+  if constexpr (PL == kOne) {
+    lin_put_parts<1, PERM>(t, row, e, &x.a);
+    return lin_odd8(x.a);
+  } else {
+    float v[8];
+    lin_unpack8<PL>(x, type, v);
+    bool odd = false;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) a[k] = b[k] = 0.f;
-  } else if (d0 < R) {
+    for (int k = 0; k < 8; ++k) odd = odd || !(fabsf(v[k]) <= 3.402823466e38f);
+    lin_put8<PL, PERM>(t, row, e, v);
+    return odd;
+  }
+}
+
+// Eight columns d0 .. of a row, expanded: a the cosine part or the value, b the sine part of rotated dims; times `factor`.
+// turns: the bias of the keys in LDS, or null.
+template <int PL>
+__device__ __forceinline__ void lin_polar8(const LinRaw<PL>& x8, int type, const f32x4* f, int d0, int R, float factor, const float* turns, float* a, float* b) {
+  float x[8];
+  lin_unpack8<PL>(x8, type, x);
+  if (d0 < R) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       float sn, cs;
@@ -207,40 +360,63 @@ __device__ __forceinline__ bool lin_put_polar(const LinTile& t, int row, int d0,
       const float m = softplus_f(x[k]) * factor;
       a[k] = rot ? m * cs : x[k] * factor;
       b[k] = rot ? m * sn : 0.f;
-      fin = fin && fabsf(a[k]) <= 3.402823466e38f && fabsf(b[k]) <= 3.402823466e38f;
     }
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) a[k] = x[k] * factor, fin = fin && fabsf(a[k]) <= 3.402823466e38f;
+    for (int k = 0; k < 8; ++k) a[k] = x[k] * factor, b[k] = 0.f;
   }
-  if (R % 8 == 0) {   // a chunk is all rotated or all not, and its columns start on a multiple of 8
+}
+// Their places in an expanded row: put8(e, eight values) where a chunk's columns start on a multiple of 8, else put1(e, value).
+template <typename F8, typename F1>
+__device__ __forceinline__ void lin_place8(int d0, int D, int R, const float* a, const float* b, F8&& put8, F1&& put1) {
+  if (R % 8 == 0) {   // a chunk is all rotated or all not; columns behind the row (D no multiple of 8) are zeros
     if (d0 < R) {
-      const int e = 2 * d0 - e_lo;
-      if ((unsigned)e < (unsigned)e_n) {
-        float w[16];
+      float w[16];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) w[2 * k] = a[k], w[2 * k + 1] = b[k];
-        lin_put8<PL, PERM>(t, row, e, w);
-        lin_put8<PL, PERM>(t, row, e + 8, w + 8);
-        return fin;
-      }
+      for (int k = 0; k < 8; ++k) w[2 * k] = a[k], w[2 * k + 1] = b[k];
+      put8(2 * d0, w);
+      put8(2 * d0 + 8, w + 8);
     } else {
-      const int e = R + d0 - e_lo;   // columns behind the row (D no multiple of 8) are zeros
-      if ((unsigned)e < (unsigned)e_n) {
-        lin_put8<PL, PERM>(t, row, e, a);
-        return fin;
-      }
+      put8(R + d0, a);
     }
-    return true;
+    return;
   }
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    const int d = d0 + k, e = (d < R ? 2 * d : R + d) - e_lo;
+    const int d = d0 + k;
     if (d >= D) break;
-    if ((unsigned)e < (unsigned)e_n) lin_put1<PL, PERM>(t, row, e, a[k]);
-    if (d < R && (unsigned)(e + 1) < (unsigned)e_n) lin_put1<PL, PERM>(t, row, e + 1, b[k]);
+    put1(d < R ? 2 * d : R + d, a[k]);
+    if (d < R) put1(2 * d + 1, b[k]);
   }
-  return fin;
+}
+
+// Expanded rows to memory.
+template <int PL>
+__device__ __forceinline__ void lin_hat_put(const LinHat& t, int64_t row, int d0, int D, int R, const float* a, const float* b) {
+  uint16_t* at = t.p + row * t.EP;
+  lin_place8(d0, D, R, a, b,
+             [&](int e, const float* v) {
+               u32x2 lo[PL], hi[PL];
+               lin_pack4<PL>(f32x4{v[0], v[1], v[2], v[3]}, lo);
+               lin_pack4<PL>(f32x4{v[4], v[5], v[6], v[7]}, hi);
+#pragma unroll
+               for (int l = 0; l < PL; ++l) *reinterpret_cast<u32x4*>(at + l * t.plane + e) = u32x4{lo[l][0], lo[l][1], hi[l][0], hi[l][1]};
+             },
+             [&](int e, float v) {
+               const uint16_t w = BF16::bits(v);
+               at[e] = w;
+               if constexpr (PL == 2) at[t.plane + e] = BF16::bits(v - BF16::to_float(w));
+             });
+}
+// The zeros behind them, by THREADS threads.
+template <int PL, int THREADS>
+__device__ __forceinline__ void lin_hat_tail(const LinHat& t, int64_t row, int thread, int D, int R) {
+  const int E = R % 8 == 0 ? R + (D + 7) / 8 * 8 : D + R;
+  uint16_t* at = t.p + row * t.EP;
+  for (int e = E + thread; e < t.EP; e += THREADS) {
+    at[e] = 0;
+    if constexpr (PL == 2) at[t.plane + e] = 0;
+  }
 }
 
 // A thread's u-th chunk of eight columns of a tile of C rows: four side by side in a row, the next rows, then the next
@@ -285,12 +461,11 @@ __device__ __forceinline__ f32x4 lin_mfma(const u32x4* a, const u32x4* b, f32x4 
 }
 
 // Tile shapes: P columns of the contraction, NT columns of the result per workgroup, NW waves of SL columns each.
-template <typename T, int P_, int NT_, int NW_>
+template <int PL_, int P_, int NT_, int NW_>
 struct LinCfg {
   static constexpr int P = P_, NT = NT_, NW = NW_, SL = NT / NW, CT = SL / 16;
   static constexpr int kThreads = 64 * NW;
-  // bf16 rows are one part, fp16 rows two, exactly
-  static constexpr int PL = T::kCode == 2 ? 1 : 2;
+  static constexpr int PL = PL_;
   static constexpr int C = PL == 1 ? 64 : 32, KS = C / 32, IT = C / 16;
   static constexpr int XS = P + 8, YS = P + 16, ZS = NT + 16, AS = C + 8;
   static constexpr int TP = (C * (P / 8) + kThreads - 1) / kThreads, TZ = (C * (NT / 8) + kThreads - 1) / kThreads;
@@ -298,23 +473,32 @@ struct LinCfg {
 
 // Rows of P / NT that a call takes: dispatch over (P, NT), P for the contraction's columns, NT for the result's.
 // Wide results go in tiles of 256 columns over eight waves; states of more than 256 rows leave room for 16 columns a wave.
-template <typename T, template <typename> class Launch, typename... A>
+template <int PL, template <typename> class Launch, typename... A>
 hipError_t lin_dispatch(int pcols, int ncols, A&&... args) {
-  const int p = pcols <= 64 ? 64 : pcols <= 128 ? 128 : pcols <= 256 ? 256 : 512;
-  const int n = ncols <= 64 ? 64 : ncols <= 128 ? 128 : 256;
-#define POPE_LIN_CASE(PP, NN, WW) return Launch<LinCfg<T, PP, NN, WW>>::go(args...)
+  const int p = pcols <= 64 ? 64 : pcols <= 96 ? 96 : pcols <= 128 ? 128 : pcols <= 256 ? 256 : 512;
+  const int n = ncols <= 64 ? 64 : ncols <= 96 ? 96 : ncols <= 128 ? 128 : 256;
+#define POPE_LIN_CASE(PP, NN, WW) return Launch<LinCfg<PL, PP, NN, WW>>::go(args...)
   if (p == 64) {
     if (n == 64) POPE_LIN_CASE(64, 64, 4);
+    if (n == 96) POPE_LIN_CASE(64, 96, 6);
     if (n == 128) POPE_LIN_CASE(64, 128, 4);
     POPE_LIN_CASE(64, 256, 8);
   }
+  if (p == 96) {
+    if (n == 64) POPE_LIN_CASE(96, 64, 4);
+    if (n == 96) POPE_LIN_CASE(96, 96, 6);
+    if (n == 128) POPE_LIN_CASE(96, 128, 4);
+    POPE_LIN_CASE(96, 256, 8);
+  }
   if (p == 128) {
     if (n == 64) POPE_LIN_CASE(128, 64, 4);
+    if (n == 96) POPE_LIN_CASE(128, 96, 6);
     if (n == 128) POPE_LIN_CASE(128, 128, 4);
     POPE_LIN_CASE(128, 256, 8);
   }
   if (p == 256) {
     if (n == 64) POPE_LIN_CASE(256, 64, 4);
+    if (n == 96) POPE_LIN_CASE(256, 96, 6);
     if (n == 128) POPE_LIN_CASE(256, 128, 4);
     POPE_LIN_CASE(256, 256, 8);
   }

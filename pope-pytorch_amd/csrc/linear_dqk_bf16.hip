@@ -3,6 +3,6 @@
 
 namespace pope {
 
-hipError_t launch_linear_dqk_bf16(const LinOutParams& p, hipStream_t s) { return launch_linear_out_t<BF16, kLinDq>(p, "linear_dqk", s); }
+hipError_t launch_linear_dqk_bf16(const LinOutParams& p, hipStream_t s) { return launch_linear_out_t<kOne, kLinDq>(p, "linear_dqk", s); }
 
 }  // namespace pope

@@ -3,6 +3,6 @@
 
 namespace pope {
 
-hipError_t launch_linear_dv_bf16(const LinOutParams& p, hipStream_t s) { return launch_linear_out_t<BF16, kLinDv>(p, "linear_dv", s); }
+hipError_t launch_linear_dv_bf16(const LinOutParams& p, hipStream_t s) { return launch_linear_out_t<kOne, kLinDv>(p, "linear_dv", s); }
 
 }  // namespace pope

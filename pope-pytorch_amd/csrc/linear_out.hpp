@@ -17,14 +17,20 @@
 // leaving its registers.
 //
 // Rounding: x, y, z, the weighted C x C products and W as an operand are bf16: one part for bf16 rows (each is off by at most 2^-9,
-// as the output is by its own rounding), the sum of two for fp16 rows (2^-17).  W itself, all sums and the powers of g are
-// fp32.
+// as the output is by its own rounding), the sum of two for fp16 and fp32 rows, and for bf16 rows whose output goes on in fp32 (2^-17;
+// C is 32 then).  W itself, all sums and the powers of g are fp32.
 #pragma once
+#include <algorithm>
+#include <type_traits>
+
 #include "linear_dev.hpp"
 
 namespace pope {
 
-template <typename T, typename K, int KIND>
+template <bool B>
+using Bool = std::integral_constant<bool, B>;
+
+template <typename K, int KIND>
 __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char* smem) {
   constexpr int kind = KIND, which = KIND == kLinDk ? 1 : 0;
   constexpr int P = K::P, NT = K::NT, CT = K::CT, PL = K::PL, C = K::C, KS = K::KS, IT = K::IT, ST = P / 32;
@@ -53,7 +59,7 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
       const int r = (int)(it / out_cols), d = (int)(it - (int64_t)r * out_cols), row = r < lo ? r : hi + r - lo;
       for (int g = 0; g < (by_query ? ng : 1); ++g) {
         const int h = by_query ? (g0 + g) * c.Hk + hk : hk;
-        out.p[(int64_t)h * out.s[1] + (int64_t)row * out.s[2] + d] = 0;
+        lin_set<PL>(out, (int64_t)h * out.s[1] + (int64_t)row * out.s[2] + d, 0.f);
         if (chain && p.dphase[which] && d < c.R) p.dphase[which][((int64_t)h * c.seqs.N + row) * c.R + d] = 0.f;
       }
     }
@@ -70,12 +76,14 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
   const LinTile Y{X.p + PL * X.plane, K::YS, C * K::YS};
   const LinTile Z{Y.p + PL * Y.plane, K::ZS, C * K::ZS};
   const LinTile A{Z.p + PL * Z.plane, K::AS, C * K::AS};
-  float* turns = reinterpret_cast<float*>(A.p + PL * A.plane);   // 256
-  int* odd = reinterpret_cast<int*>(turns + 256);                // z of this chunk that are not finite; two, by turns
+  float* later = reinterpret_cast<float*>(A.p + PL * A.plane);   // C: weights of a chunk's rows in the next state
+  float* turns = later + C;                                      // kLinDk: 256
+  int* odd = reinterpret_cast<int*>(turns + (chain ? 256 : 0));   // z of this chunk that are not finite; two, by turns
   constexpr int kTileBytes = PL * (C * (K::XS + K::YS + K::ZS + K::AS)) * 2;
   for (int i = tid; i < kTileBytes / 16; i += kThreads) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0, 0, 0, 0};
   if (tid < 2) odd[tid] = 0;
-  for (int d = tid; d < c.R; d += kThreads) turns[d] = lin_turns(c.bias[hk * c.bias_sh + d]);
+  if (kind == kLinDk)
+    for (int d = tid; d < c.R; d += kThreads) turns[d] = lin_turns(c.bias[hk * c.bias_sh + d]);
 
   const float lg = lin_log2(c, hk);
   const int a = rev ? 0 : 1;
@@ -94,134 +102,148 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
     const float* from = p.states[rev] ? p.states[rev] + ((int64_t)at * c.Hk + hk) * c.E * c.Dv
                         : p.first[rev] ? p.first[rev] + ((int64_t)seg.seq * c.Hk + hk) * c.E * c.Dv : nullptr;
     if (from && busy) {
-      const int64_t rs = chain ? 1 : c.Dv, cs = chain ? c.Dv : 1;   // transposed where the result has expanded columns
+      const bool whole = chain && c.Dv % 4 == 0 && (reinterpret_cast<uintptr_t>(from) & 15) == 0;
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
         const int col = n0 + col0 + 16 * ct + l16;
 #pragma unroll
-        for (int s = 0; s < 2 * ST; ++s)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int row = 16 * s + 4 * q4 + r;
-            if (row < pcols && col < ncols) W[ct][s][r] = from[row * rs + col * cs];
+        for (int s = 0; s < 2 * ST; ++s) {
+          const int row = 16 * s + 4 * q4;
+          if (whole) {   // transposed where the result has expanded columns
+            if (row < pcols && col < ncols) W[ct][s] = *reinterpret_cast<const f32x4*>(from + (int64_t)col * c.Dv + row);
+            continue;
           }
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (row + r < pcols && col < ncols) W[ct][s][r] = chain ? from[(int64_t)col * c.Dv + row + r] : from[(int64_t)(row + r) * c.Dv + col];
+        }
       }
     }
   }
   const float keep = lin_power(lg, C);
-  // weights of a chunk's rows in the next state, in the order of operands
-  float wz[KS][8];
-#pragma unroll
-  for (int s = 0; s < KS; ++s)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) wz[s][j] = lin_power(lg, C - a - (32 * s + 16 * (j >> 2) + 4 * q4 + (j & 3)));
+  for (int t = tid; t < C; t += kThreads) later[t] = lin_power(lg, C - a - t);
   float dbsum[CT][2];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) dbsum[ct][0] = dbsum[ct][1] = 0.f;
 
   const auto row_of = [&](int t) { return seg.row0 + (rev ? seg.len - 1 - t : t); };   // t: of the segment, in the job's order
   typedef LinItem<C, kThreads> Item;
-  const LinRows xr = kind == kLinOut ? c.q : kind == kLinDq ? c.g : kind == kLinDk ? c.v : c.k;
-  const LinRows yr = kind == kLinOut ? c.k : kind == kLinDq ? c.v : kind == kLinDk ? c.g : c.q;
-  const LinRows zr = kind == kLinOut ? c.v : kind == kLinDq ? c.k : kind == kLinDk ? c.q : c.g;
-  constexpr bool xy_polar = !chain, z_polar = chain;
-  constexpr bool x_key = kind == kLinDk || kind == kLinDv, yz_key = !x_key;   // rows that the mask may leave out
-  const auto kept = [&](int row) { return !c.mask || c.mask[(int64_t)seg.batch * c.mask_sb + row] != 0; };
-  // A thread's chunks of the tiles: read from memory ...
-  struct In { u32x4 x, y; f32x4 f[2]; bool lx, ly; };
-  struct InZ { u32x4 z; f32x4 f[2]; bool live; };
+  // x, y and z are expanded rows or plain ones, the keys' and values' rows among the latter, which the mask may leave out
+  constexpr bool x_hat = !chain, y_hat = !chain, z_hat = chain;
+  const LinRows xr = kind == kLinDq ? c.g : c.v, yr = kind == kLinDq ? c.v : c.g, zr = kind == kLinOut ? c.v : c.g;
+  const LinHat xh = kind == kLinOut ? c.qh : c.kh, yh = kind == kLinOut ? c.kh : c.qh, zh = kind == kLinDq ? c.kh : c.qh;
+  constexpr bool x_key = kind == kLinDk, y_key = kind == kLinDq, z_key = kind == kLinOut;
+  const int xcols = x_hat ? xh.EP : xr.cols, ycols = y_hat ? yh.EP : yr.cols, zcols = z_hat ? zh.EP : zr.cols;   // x and y have as many
   struct Turn { int t0, hq; bool lx, lyz; };
   const auto turn_of = [&](int it) {
     const int ch = it / ng, g = it - ch * ng;
     return Turn{ch * C, (g0 + g) * c.Hk + hk, by_query || g == 0, !by_query || g == 0};
   };
-  const auto load_xy = [&](const Turn& n, int u) {
-    const Item i(u);
-    In r;
-    r.x = r.y = u32x4{0, 0, 0, 0};
-    r.f[0] = r.f[1] = f32x4{0.f, 0.f, 0.f, 0.f};
-    r.lx = r.ly = false;
-    if (n.t0 + i.row < seg.len && i.d0 < xr.cols) {   // x and y have as many columns
-      const int row = row_of(n.t0 + i.row);
-      const bool k = kept(row);
-      r.lx = !x_key || k;
-      r.ly = !yz_key || k;
-      if (n.lx && r.lx) r.x = lin_load8(xr.p + (int64_t)seg.batch * xr.s[0] + (int64_t)(by_query ? n.hq : hk) * xr.s[1] + (int64_t)row * xr.s[2], i.d0, xr.cols, xr.vec);
-      if (n.lyz && r.ly) r.y = lin_load8(yr.p + (int64_t)seg.batch * yr.s[0] + (int64_t)(by_query ? hk : n.hq) * yr.s[1] + (int64_t)row * yr.s[2], i.d0, yr.cols, yr.vec);
-      if (xy_polar && c.R) lin_angles8(lin_angle_row(c, seg.batch, row), i.d0, c.R, c.f_vec, r.f);
+  const auto kept = [&](int row) { return !c.mask || c.mask[(int64_t)seg.batch * c.mask_sb + row] != 0; };
+  // A thread's chunks of the tiles, read from memory.  What the mask leaves out is read too, so that no load waits for it.
+  struct Part { LinRaw<PL> w; bool keep; };
+  const auto get = [&](auto hat, auto key, const LinHat& t, const LinRows& r, int h, int cols, int t0, const Item& i, int d0) {
+    Part o;
+    o.w = LinRaw<PL>{};
+    o.keep = false;
+    if (t0 + i.row < seg.len && d0 < cols) {
+      const int row = row_of(t0 + i.row);
+      if constexpr (decltype(hat)::value) {
+        const uint16_t* p = t.p + (((int64_t)seg.batch * t.H + h) * c.seqs.N + row) * t.EP + d0;
+        o.w.a = *reinterpret_cast<const u32x4*>(p);
+        if constexpr (PL == kTwo) o.w.b = *reinterpret_cast<const u32x4*>(p + t.plane);
+      } else {
+        o.w = lin_load8<PL>(r, (int64_t)seg.batch * r.s[0] + (int64_t)h * r.s[1] + (int64_t)row * r.s[2], d0);
+      }
+      o.keep = !decltype(key)::value || kept(row);
     }
-    return r;
+    return o;
   };
-  const auto load_z = [&](const Turn& n, int u) {
+  const auto get_x = [&](const Turn& n, int u) {
     const Item i(u);
-    InZ r;
-    r.z = u32x4{0, 0, 0, 0};
-    r.f[0] = r.f[1] = f32x4{0.f, 0.f, 0.f, 0.f};
-    r.live = false;
-    const int d0 = (z_polar ? 0 : n0) + i.d0;
-    if (n.t0 + i.row < seg.len && (z_polar || i.d0 < NT) && d0 < zr.cols) {
-      const int row = row_of(n.t0 + i.row);
-      r.live = !yz_key || kept(row);
-      if (r.live) r.z = lin_load8(zr.p + (int64_t)seg.batch * zr.s[0] + (int64_t)(by_query ? hk : n.hq) * zr.s[1] + (int64_t)row * zr.s[2], d0, zr.cols, zr.vec);
-      if (z_polar && c.R) lin_angles8(lin_angle_row(c, seg.batch, row), d0, c.R, c.f_vec, r.f);
-    }
-    return r;
+    return get(Bool<x_hat>{}, Bool<x_key>{}, xh, xr, by_query ? n.hq : hk, xcols, n.t0, i, i.d0);
   };
-  // ... and expanded into LDS
-  const float* xt = kind == kLinDv ? turns : nullptr;                       // keys carry the bias
-  const float* yt = kind == kLinOut ? turns : nullptr;
-  const float* zt = kind == kLinDq ? turns : nullptr;
-  const float xs = kind == kLinOut ? c.scale : 1.f, ys = kind == kLinDv ? c.scale : 1.f, zs = kind == kLinDk ? c.scale : 1.f;   // queries the scale
-  const auto put_xy = [&](const Turn& n, int u, const In& r) {
+  const auto get_y = [&](const Turn& n, int u) {
     const Item i(u);
-    if (i.d0 >= xr.cols || i.d0 >= P) return;
-    if (xy_polar) {
-      if (n.lx) lin_put_polar<T, PL, true>(X, i.row, i.d0, r.x, r.f, r.lx, xs, xt, c.D, c.R, 0, P);
-      if (n.lyz) lin_put_polar<T, PL, false>(Y, i.row, i.d0, r.y, r.f, r.ly, ys, yt, c.D, c.R, 0, P);
+    return get(Bool<y_hat>{}, Bool<y_key>{}, yh, yr, by_query ? hk : n.hq, ycols, n.t0, i, i.d0);
+  };
+  const auto get_z = [&](const Turn& n, int u) {
+    const Item i(u);
+    return get(Bool<z_hat>{}, Bool<z_key>{}, zh, zr, by_query ? hk : n.hq, i.d0 < NT ? zcols : 0, n.t0, i, n0 + i.d0);
+  };
+  // ... and put into LDS
+  const auto put = [&](auto hat, auto perm, const LinRows& r, const LinTile& t, const Item& i, Part o) {
+    constexpr bool kPerm = decltype(perm)::value;
+    if (!o.keep) o.w = LinRaw<PL>{};
+    if constexpr (!decltype(hat)::value) {
+      return lin_put_plain<PL, kPerm>(t, i.row, i.d0, o.w, r.type);
     } else {
-      if (n.lx) lin_put_plain<T, PL, true>(X, i.row, i.d0, r.x);
-      if (n.lyz) lin_put_plain<T, PL, false>(Y, i.row, i.d0, r.y);
+      if constexpr (PL == kTwo) {
+        const u32x4 both[2] = {o.w.a, o.w.b};
+        lin_put_parts<2, kPerm>(t, i.row, i.d0, both);
+      } else {
+        lin_put_parts<1, kPerm>(t, i.row, i.d0, &o.w.a);
+      }
+      return lin_odd8(o.w.a);
     }
   };
-  const auto put_z = [&](const Turn& n, int u, const InZ& r) {
+  const auto put_x = [&](int u, const Part& o) {
     const Item i(u);
-    if ((!z_polar && i.d0 >= NT) || (z_polar ? 0 : n0) + i.d0 >= zr.cols) return true;
-    if (z_polar) return lin_put_polar<T, PL, false>(Z, i.row, i.d0, r.z, r.f, r.live, zs, zt, c.D, c.R, n0, NT);
-    return lin_put_plain<T, PL, false>(Z, i.row, i.d0, r.z);
+    if (i.d0 < xcols) put(Bool<x_hat>{}, Bool<true>{}, xr, X, i, o);
+  };
+  const auto put_y = [&](int u, const Part& o) {
+    const Item i(u);
+    if (i.d0 < ycols) put(Bool<y_hat>{}, Bool<false>{}, yr, Y, i, o);
+  };
+  const auto put_z = [&](int u, const Part& o) {
+    const Item i(u);
+    return i.d0 < NT && n0 + i.d0 < zcols && put(Bool<z_hat>{}, Bool<false>{}, zr, Z, i, o);
   };
   // Narrow tiles are loaded a chunk ahead, into registers; wide ones, whose state takes those, chunk by chunk.
   constexpr bool kAhead = P <= 128 && NT <= 128;
-  In xy[kAhead ? K::TP : 1];
-  InZ zz[kAhead ? K::TZ : 1];
+  constexpr int kTX = kAhead ? K::TP : 0, kTZ = kAhead ? K::TZ : 0;
+  Part xin[kTX + 1], yin[kTX + 1], zin[kTZ + 1];
   const auto load = [&](int it) {
-    if constexpr (kAhead) {
-      const Turn n = turn_of(it);
+    const Turn n = turn_of(it);
 #pragma unroll
-      for (int u = 0; u < K::TP; ++u) xy[u] = load_xy(n, u);
-      if (n.lyz)
-#pragma unroll
-        for (int u = 0; u < K::TZ; ++u) zz[u] = load_z(n, u);
+    for (int u = 0; u < kTX; ++u) {
+      if (n.lx) xin[u] = get_x(n, u);
+      if (n.lyz) yin[u] = get_y(n, u);
     }
+    if (n.lyz)
+#pragma unroll
+      for (int u = 0; u < kTZ; ++u) zin[u] = get_z(n, u);
   };
+  const auto turns_for = [&](int cols) { return (C * ((cols + 31) / 32 * 4) + kThreads - 1) / kThreads; };
   const auto store = [&](int it) {
     const Turn n = turn_of(it);
-    bool fin = true;
+    bool some = false;
     if constexpr (kAhead) {
 #pragma unroll
-      for (int u = 0; u < K::TP; ++u) put_xy(n, u, xy[u]);
+      for (int u = 0; u < kTX; ++u) {
+        if (n.lx) put_x(u, xin[u]);
+        if (n.lyz) put_y(u, yin[u]);
+      }
       if (n.lyz)
 #pragma unroll
-        for (int u = 0; u < K::TZ; ++u) fin &= put_z(n, u, zz[u]);
+        for (int u = 0; u < kTZ; ++u) some |= put_z(u, zin[u]);
     } else {
-      const int txy = (C * ((xr.cols + 31) / 32 * 4) + kThreads - 1) / kThreads;
-#pragma unroll 1
-      for (int u = 0; u < txy; ++u) put_xy(n, u, load_xy(n, u));
-      const int tz = (C * ((min(z_polar ? 256 : NT, zr.cols) + 31) / 32 * 4) + kThreads - 1) / kThreads;
-      if (n.lyz)
-#pragma unroll 1
-        for (int u = 0; u < tz; ++u) fin &= put_z(n, u, load_z(n, u));
+      const int txy = turns_for(xcols);
+#pragma unroll 2
+      for (int u = 0; u < txy; ++u) {
+        Part x, y;
+        if (n.lx) x = get_x(n, u);
+        if (n.lyz) y = get_y(n, u);
+        if (n.lx) put_x(u, x);
+        if (n.lyz) put_y(u, y);
+      }
+      if (n.lyz) {
+        const int tz = turns_for(min(NT, zcols - n0));
+#pragma unroll 4
+        for (int u = 0; u < tz; ++u) some |= put_z(u, get_z(n, u));
+      }
     }
-    if (!fin) odd[it & 1] = 1;
+    if (some) odd[it & 1] = 1;
   };
 
   f32x4 O[CT][IT];
@@ -235,30 +257,76 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
     if (it + 1 < turns_n) load(it + 1);
     __syncthreads();
     if (!by_query || g == 0) odd_z = odd[it & 1] != 0;
-    // x . y of the rows of 16 x 16 tiles j <= i, weighted
-    constexpr int kTiles = IT * (IT + 1) / 2;
-#pragma unroll 1
-    for (int t = wave; t < kTiles; t += K::NW) {
-      const int ti = t == 0 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, tj = t - ti * (ti + 1) / 2;
-      f32x4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-      for (int k = 0; k < steps; ++k) {
-        u32x4 xa[PL], ya[PL];
+    // x . y of the rows of 16 x 16 tiles j <= i, weighted: a wave has tiles of one i
+    {
+      constexpr int kShare = K::NW / IT, kTiles = IT > kShare ? IT / kShare : 1;
+      const int ti = wave / kShare, j0 = ti < IT ? wave % kShare : K::NW;   // waves left over have none: NW > ti
+      f32x4 sc[kTiles];
 #pragma unroll
-        for (int l = 0; l < PL; ++l) {
-          xa[l] = lin_along_placed(X.p + l * X.plane, K::XS, 16 * ti, 32 * k, lane);
-          ya[l] = lin_along(Y.p + l * Y.plane, K::YS, 16 * tj, 32 * k, lane);
+      for (int j = 0; j < kTiles; ++j) sc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < ST; ++k)
+        if (k < steps) {
+          u32x4 xa[PL], ya[kTiles][PL];
+#pragma unroll
+          for (int l = 0; l < PL; ++l) {
+            xa[l] = lin_along_placed(X.p + l * X.plane, K::XS, 16 * ti, 32 * k, lane);
+#pragma unroll
+            for (int j = 0; j < kTiles; ++j)
+              if (j0 + j * kShare <= ti) ya[j][l] = lin_along(Y.p + l * Y.plane, K::YS, 16 * (j0 + j * kShare), 32 * k, lane);
+          }
+#pragma unroll
+          for (int j = 0; j < kTiles; ++j)
+            if (j0 + j * kShare <= ti) sc[j] = lin_mfma<PL, PL>(ya[j], xa, sc[j]);
         }
-        s = lin_mfma<PL, PL>(ya, xa, s);
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j) {
+        if (j0 + j * kShare > ti) continue;
+        const int i = 16 * ti + l16, jr = 16 * (j0 + j * kShare) + 4 * q4;
+        f32x4 w;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w[r] = jr + r <= i ? sc[j][r] * lin_power(lg, i - jr - r) : 0.f;
+        u32x2 wp[PL];
+        lin_pack4<PL>(w, wp);
+#pragma unroll
+        for (int l = 0; l < PL; ++l) *reinterpret_cast<u32x2*>(A.p + l * A.plane + i * K::AS + lin_place<true>(jr)) = wp[l];
       }
-      const int i = 16 * ti + l16, j0 = 16 * tj + 4 * q4;
-      f32x4 w;
+    }
+    // what the chain rule of this turn's rows reads, ahead: a lane has row 16 i + l16, and, of each 16 columns, two dims
+    const bool ends = by_query || g == ng - 1;
+    const bool pairs = out.vec && (kind == kLinDq ? c.q : c.k).vec && c.f_vec;   // two dims at a time: R, D multiples of 8
+    float cx[CT][IT][2], cf[CT][IT][2];
+    bool live[IT];
+    if constexpr (rev) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) w[r] = j0 + r <= i ? s[r] * lin_power(lg, i - j0 - r) : 0.f;
-      u32x2 wp[PL];
-      lin_pack4<PL>(w, wp);
+      for (int i = 0; i < IT; ++i) live[i] = !busy || !ends || kept(row_of(min(t0 + 16 * i + l16, seg.len - 1)));
+    }
+    if constexpr (chain) {
+      if (busy && ends) {
+        const LinRows in = kind == kLinDq ? c.q : c.k;
+        const int64_t base = (int64_t)seg.batch * in.s[0] + (int64_t)(by_query ? (g0 + g) * c.Hk + hk : hk) * in.s[1];
 #pragma unroll
-      for (int l = 0; l < PL; ++l) *reinterpret_cast<u32x2*>(A.p + l * A.plane + i * K::AS + lin_place<true>(j0)) = wp[l];
+        for (int i = 0; i < IT; ++i) {
+          const int row = row_of(min(t0 + 16 * i + l16, seg.len - 1));
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) {
+            const int d = (n0 + col0 + 16 * ct + 4 * q4) >> 1;
+            cx[ct][i][0] = cx[ct][i][1] = cf[ct][i][0] = cf[ct][i][1] = 0.f;
+            if (d >= c.R) continue;
+            const int64_t at = base + (int64_t)row * in.s[2] + d;
+            const float* fr = lin_angle_row(c, seg.batch, row) + d;
+            if (pairs) {
+              lin_get2<PL>(in, at, cx[ct][i]);
+              const f32x2 f2 = *reinterpret_cast<const f32x2*>(fr);
+              cf[ct][i][0] = f2[0], cf[ct][i][1] = f2[1];
+            } else {
+#pragma unroll
+              for (int pr = 0; pr < 2; ++pr)
+                if (d + pr < c.R) cx[ct][i][pr] = lin_get<PL>(in, at + pr), cf[ct][i][pr] = fr[pr];
+            }
+          }
+        }
+      }
     }
     // W^T x
     if (busy && (by_query || g == 0)) {
@@ -348,6 +416,7 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
         for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
           for (int s = 0; s < KS; ++s) {
+            const f32x4 w0 = *reinterpret_cast<const f32x4*>(later + 32 * s + 4 * q4), w1 = *reinterpret_cast<const f32x4*>(later + 32 * s + 16 + 4 * q4);
             float v[8];
             unpack8<BF16>(za[ct][s][0], v);
             if constexpr (PL == 2) {
@@ -357,7 +426,7 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
               for (int j = 0; j < 8; ++j) v[j] += v2[j];
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] *= wz[s][j];
+            for (int j = 0; j < 4; ++j) v[j] *= w0[j], v[4 + j] *= w1[j];
             u32x2 lo[PL], hi[PL];
             lin_pack4<PL>(f32x4{v[0], v[1], v[2], v[3]}, lo);
             lin_pack4<PL>(f32x4{v[4], v[5], v[6], v[7]}, hi);
@@ -378,58 +447,53 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
           }
       }
       // out: a lane has row 16 i + l16, columns 4 q4 .. of each tile
-      if (by_query || g == ng - 1) {
+      if (ends) {
         const int h = by_query ? (g0 + g) * c.Hk + hk : hk;
-        uint16_t* ob = out.p + (int64_t)seg.batch * out.s[0] + (int64_t)h * out.s[1];
+        const int64_t ob = (int64_t)seg.batch * out.s[0] + (int64_t)h * out.s[1];
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
           const int t = t0 + 16 * i + l16;
           if (t >= seg.len) continue;
           const int row = row_of(t);
-          uint16_t* orow = ob + (int64_t)row * out.s[2];
+          const int64_t orow = ob + (int64_t)row * out.s[2];
           if (!chain) {
-            const bool dead = kind == kLinDv && !kept(row);
+            const bool dead = rev && !live[i];
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct) {
-              const int d = n0 + col0 + 16 * ct + 4 * q4;
-              f32x4 v = O[ct][i];
-              if (dead) v = f32x4{0.f, 0.f, 0.f, 0.f};
-              if (out.vec && d < out_cols) {
-                *reinterpret_cast<u32x2*>(orow + d) = u32x2{T::pack2(v[0], v[1]), T::pack2(v[2], v[3])};
-              } else {
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                  if (d + r < out_cols) orow[d + r] = T::bits(v[r]);
-              }
-            }
+            for (int ct = 0; ct < CT; ++ct)
+              lin_set4<PL>(out, orow, n0 + col0 + 16 * ct + 4 * q4, dead ? f32x4{0.f, 0.f, 0.f, 0.f} : O[ct][i]);
           } else {
             // chain rule of the polar rows: a lane's columns are two (cosine, sine) pairs, or four other dims
-            const LinRows in = kind == kLinDq ? c.q : c.k;
-            const uint16_t* xrow = in.p + (int64_t)seg.batch * in.s[0] + (int64_t)h * in.s[1] + (int64_t)row * in.s[2];
-            const float* frow = c.R ? lin_angle_row(c, seg.batch, row) : nullptr;
             float* ph = p.dphase[which] ? p.dphase[which] + (((int64_t)seg.batch * (kind == kLinDq ? c.Hq : c.Hk) + h) * c.seqs.N + row) * c.R : nullptr;
-            const bool dead = kind == kLinDk && !kept(row);
+            const bool dead = rev && !live[i];
             const float f = kind == kLinDq ? c.scale : 1.f;
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
               const int e0 = n0 + col0 + 16 * ct + 4 * q4;
+              f32x4 v = O[ct][i] * f;
+              if (dead) v = f32x4{0.f, 0.f, 0.f, 0.f};
+              float dx[2];
 #pragma unroll
               for (int pr = 0; pr < 2; ++pr) {
                 const int e = e0 + 2 * pr;
-                const float dc = dead ? 0.f : O[ct][i][2 * pr] * f, ds = dead ? 0.f : O[ct][i][2 * pr + 1] * f;
+                const float dc = v[2 * pr], ds = v[2 * pr + 1];
                 if (e < 2 * c.R) {
                   const int d = e >> 1;
-                  const float x = T::to_float(xrow[d]);
+                  const float x = cx[ct][i][pr];
                   float sn, cs;
-                  sincos_turns(frow[d], kind == kLinDk ? turns[d] : 0.f, &sn, &cs);
-                  orow[d] = T::bits(dead ? 0.f : sigmoid_f(x) * (dc * cs + ds * sn));
+                  sincos_turns(cf[ct][i][pr], kind == kLinDk ? turns[d] : 0.f, &sn, &cs);
+                  dx[pr] = dead ? 0.f : sigmoid_f(x) * (dc * cs + ds * sn);
                   const float dth = dead ? 0.f : softplus_f(x) * (ds * cs - dc * sn);
                   dbsum[ct][pr] += dth;
                   if (ph) ph[d] = dth;
-                } else {
-                  if (e < c.E) orow[e - c.R] = T::bits(dc);
-                  if (e + 1 < c.E) orow[e + 1 - c.R] = T::bits(ds);
+                  if (!pairs) lin_set<PL>(out, orow + d, dx[pr]);
+                } else if (!pairs) {
+                  if (e < c.E) lin_set<PL>(out, orow + e - c.R, dc);
+                  if (e + 1 < c.E) lin_set<PL>(out, orow + e + 1 - c.R, ds);
                 }
+              }
+              if (pairs) {
+                if (e0 < 2 * c.R) lin_set2<PL>(out, orow + (e0 >> 1), dx[0], dx[1]);
+                else if (e0 < c.E) lin_set4<PL>(out, orow, e0 - c.R, v);
               }
             }
           }
@@ -451,22 +515,28 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
   }
 }
 
+// LDS of a workgroup, and the waves for a SIMD that registers are cut to: what LDS holds of two workgroups (160 KB for a CU).
+template <typename K, int KIND>
+constexpr int lin_out_bytes() { return K::PL * (K::C * (K::XS + K::YS + K::ZS + K::AS)) * 2 + (K::C + (KIND == kLinDq ? 256 : 0)) * 4 + 16; }
+template <typename K, int KIND>
+constexpr int lin_out_waves() { return K::NW == 4 && 2 * lin_out_bytes<K, KIND>() <= 160 * 1024 ? 2 : K::NW / 4; }
+
 // KIND kLinDq: dq and dk, in one launch.
-template <typename T, typename K, int KIND>
-__global__ __launch_bounds__(K::kThreads, 1) void linear_out_kernel(LinOutParams p) {
-  constexpr int kBytes = K::PL * (K::C * (K::XS + K::YS + K::ZS + K::AS)) * 2 + 256 * 4 + 16;
+template <typename K, int KIND>
+__global__ __launch_bounds__(K::kThreads, (lin_out_waves<K, KIND>())) void linear_out_kernel(LinOutParams p) {
+  constexpr int kBytes = lin_out_bytes<K, KIND>();
   __shared__ __attribute__((aligned(16))) char smem[kBytes];
   const int wg = blockIdx.x;
   if constexpr (KIND == kLinDq) {
     if (wg >= p.wgs) {
-      lin_out_job<T, K, kLinDk>(p, wg - p.wgs, smem);
+      lin_out_job<K, kLinDk>(p, wg - p.wgs, smem);
       return;
     }
   }
-  lin_out_job<T, K, KIND>(p, wg, smem);
+  lin_out_job<K, KIND>(p, wg, smem);
 }
 
-template <typename T, int KIND>
+template <int KIND>
 struct LinOutLaunch {
   template <typename K>
   struct Of {
@@ -477,13 +547,13 @@ struct LinOutLaunch {
       const int64_t n = segs * p.tiles * c.Hk * (KIND == kLinDv ? 1 : c.G / p.heads_per), all = n + (KIND == kLinDq ? segs * p.tiles * c.Hk : 0);
       if (all >= ((int64_t)1 << 22)) return hipErrorInvalidValue;
       p.wgs = (int)n;
-      return launch_named(name, linear_out_kernel<T, K, KIND>, dim3((unsigned)all), dim3(K::kThreads), s, p);
+      return launch_named(name, linear_out_kernel<K, KIND>, dim3((unsigned)all), dim3(K::kThreads), s, p);
     }
   };
 };
-template <typename T, int KIND>
+template <int PL, int KIND>
 hipError_t launch_linear_out_t(const LinOutParams& p, const char* name, hipStream_t s) {
-  return lin_dispatch<T, LinOutLaunch<T, KIND>::template Of>(KIND == kLinDq ? p.c.Dv : p.c.E, KIND == kLinDq ? p.c.E : p.c.Dv, p, name, s);
+  return lin_dispatch<PL, LinOutLaunch<KIND>::template Of>(KIND == kLinDq ? p.c.Dv : p.c.E, KIND == kLinDq ? p.c.E : p.c.Dv, p, name, s);
 }
 
 }  // namespace pope

@@ -3,6 +3,6 @@
 
 namespace pope {
 
-hipError_t launch_linear_out_bf16(const LinOutParams& p, hipStream_t s) { return launch_linear_out_t<BF16, kLinOut>(p, "linear_out", s); }
+hipError_t launch_linear_out_bf16(const LinOutParams& p, hipStream_t s) { return launch_linear_out_t<kOne, kLinOut>(p, "linear_out", s); }
 
 }  // namespace pope

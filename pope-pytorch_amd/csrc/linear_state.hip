@@ -1,25 +1,79 @@
-// States of the linear attention between segments, and the phases' gradients (gfx950).
+// Expanded rows, states of the linear attention between segments, and the phases' gradients (gfx950).
 //
-//   states   what the rows of a segment add to the state behind it, sum_j g^(len-1-j) k_hat_j v_j^T, or, in reverse, to the
-//            gradient of the state before it, sum_i g^(i+1) scale q_hat_i dO_i^T
+//   states   the expanded rows (q_hat times the scale, k_hat, as bf16 parts: everything after reads them, forward and backward), and
+//            what the rows of a segment add to the state behind it, sum_j g^(len-1-j) k_hat_j v_j^T; or, in reverse, to the gradient of
+//            the state before it, sum_i g^(i+1) scale q_hat_i dO_i^T.  k_hat is weighted in fp32 and goes into the products as two
+//            bf16 parts: 2^-17 of each, so that states can be handed on from call to call.
+//   sums     the same sums from the expanded rows in memory, for the backward: states that only bf16 gradients read take one part
 //   scan     S <- g^len S + sum, segment by segment; what a segment starts from goes where its sum was
 //   phase    sums of the phases' gradients over segments (bias) and heads (freqs), in a fixed order
 //
-// The sums come out as fp32 states, so each expanded row goes in as the sum of two bf16 parts, weighted in fp32 before it is
-// split: 2^-17 of each product.
+// Expanding rows where they are used instead cost more: the forward over 32,768 rows of 8 heads, D 64, R 32, took 86 us and its states
+// 46, against 44 and 65 with the rows expanded here.  So did a launch of its own for the expansion: 20 us and 10 for the
+// sums against 19 (2 x 4,096 rows of the same heads).
 #include "linear_dev.hpp"
 
 namespace pope {
 
 namespace {
 
-template <typename T, typename K>
+// ---------------------------------------------------------------- states
+
+// A workgroup's accumulators to its segment's place.
+template <typename K>
+__device__ __forceinline__ void lin_state_out(const LinStateParams& p, int at, int hk, int col0, const f32x4 (&W)[K::CT][K::P / 16]) {
+  const LinCall& c = p.c;
+  const int lane = threadIdx.x & 63, q4 = lane >> 4, l16 = lane & 15;
+  float* to = p.states + ((int64_t)at * c.Hk + hk) * c.E * c.Dv;
+#pragma unroll
+  for (int ct = 0; ct < K::CT; ++ct) {
+    const int col = col0 + 16 * ct + l16;
+#pragma unroll
+    for (int s = 0; s < K::P / 16; ++s)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = 16 * s + 4 * q4 + r;
+        if (row < c.E && col < c.Dv) to[(int64_t)row * c.Dv + col] = W[ct][s][r];
+      }
+  }
+}
+
+// The queries of a segment and head, expanded: four threads a row.
+template <int PL, int THREADS>
+__device__ __forceinline__ void lin_expand_queries(const LinCall& c, const LinSeg& seg, int hq) {
+  const int tid = threadIdx.x, per = (c.D + 7) / 8;
+  constexpr int kRows = THREADS / 4;
+  for (int r = tid >> 2; r < seg.len; r += kRows) {
+    const int row = seg.row0 + r;
+    const int64_t at = ((int64_t)seg.batch * c.Hq + hq) * c.seqs.N + row;
+    const int64_t src = (int64_t)seg.batch * c.q.s[0] + (int64_t)hq * c.q.s[1] + (int64_t)row * c.q.s[2];
+#pragma unroll 2
+    for (int u = tid & 3; u < per; u += 4) {
+      f32x4 f[2];
+      float a[8], b[8];
+      const LinRaw<PL> x = lin_load8<PL>(c.q, src, 8 * u);
+      if (c.R) lin_angles8(lin_angle_row(c, seg.batch, row), 8 * u, c.R, c.f_vec, f);
+      lin_polar8<PL>(x, c.q.type, f, 8 * u, c.R, c.scale, nullptr, a, b);
+      lin_hat_put<PL>(c.qh, at, 8 * u, c.D, c.R, a, b);
+    }
+    lin_hat_tail<PL, 4>(c.qh, at, tid & 3, c.D, c.R);
+  }
+}
+
+// p.states may be null: the expanded rows only.
+template <typename K>
 __global__ __launch_bounds__(K::kThreads, 1) void linear_state_kernel(LinStateParams p) {
   constexpr int NT = K::NT, CT = K::CT, PL = K::PL, C = K::C, KS = K::KS, ST = K::P / 32;
   __shared__ __attribute__((aligned(16))) uint16_t lds[2 * C * K::YS + PL * C * K::ZS];
   __shared__ float turns[256];
   const LinCall& c = p.c;
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), q4 = lane >> 4, l16 = lane & 15;
+  if ((int)blockIdx.x >= p.key_wgs) {
+    const int wg = blockIdx.x - p.key_wgs, at = wg / c.Hq;
+    const LinSeg seg = lin_segment(c.seqs, at);
+    if (seg.seq >= 0) lin_expand_queries<PL, K::kThreads>(c, seg, wg - at * c.Hq);
+    return;
+  }
   const int wg = blockIdx.x, tile = wg % p.tiles, rest = wg / p.tiles, hk = rest % c.Hk, at = rest / c.Hk;
   const LinSeg seg = lin_segment(c.seqs, at);
   if (seg.seq < 0) return;
@@ -39,8 +93,9 @@ __global__ __launch_bounds__(K::kThreads, 1) void linear_state_kernel(LinStatePa
   const LinRows yr = rev ? c.q : c.k, zr = rev ? c.g : c.v;
   const float* bias = rev ? nullptr : turns;
   const int ty = (C * ((c.D + 31) / 32 * 4) + K::kThreads - 1) / K::kThreads;
-  const int tz = (C * ((min(NT, c.Dv) + 31) / 32 * 4) + K::kThreads - 1) / K::kThreads;
+  const int tz = (C * ((min(NT, c.Dv - n0) + 31) / 32 * 4) + K::kThreads - 1) / K::kThreads;
   typedef LinItem<C, K::kThreads> Item;
+  const auto kept = [&](int row) { return rev || !c.mask || c.mask[(int64_t)seg.batch * c.mask_sb + row] != 0; };
   for (int t0 = 0; t0 < seg.len; t0 += C)
     for (int g = 0; g < G; ++g) {
       const int h = rev ? g * c.Hk + hk : hk;
@@ -48,27 +103,45 @@ __global__ __launch_bounds__(K::kThreads, 1) void linear_state_kernel(LinStatePa
 #pragma unroll 2
       for (int u = 0; u < ty; ++u) {
         const Item i(u);
-        if (i.d0 >= c.D) continue;
         const int row = seg.row0 + t0 + i.row;
-        u32x4 x = {0, 0, 0, 0};
+        const bool in = t0 + i.row < seg.len, keep = !rev && tile == 0 && in;
+        const int64_t to = ((int64_t)seg.batch * c.Hk + hk) * c.seqs.N + row;
+        if (keep && i.d0 < 32) lin_hat_tail<PL, 4>(c.kh, to, i.d0 / 8, c.D, c.R);
+        if (i.d0 >= c.D) continue;
+        LinRaw<PL> x{};
         f32x4 f[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-        const bool live = t0 + i.row < seg.len && (rev || !c.mask || c.mask[(int64_t)seg.batch * c.mask_sb + row]);
-        if (live) {
-          x = lin_load8(yr.p + (int64_t)seg.batch * yr.s[0] + (int64_t)h * yr.s[1] + (int64_t)row * yr.s[2], i.d0, c.D, yr.vec);
+        bool live = in;
+        if (in) {   // what the mask leaves out is read too, so that no load waits for it
+          x = lin_load8<PL>(yr, (int64_t)seg.batch * yr.s[0] + (int64_t)h * yr.s[1] + (int64_t)row * yr.s[2], i.d0);
           if (c.R) lin_angles8(lin_angle_row(c, seg.batch, row), i.d0, c.R, c.f_vec, f);
+          live = kept(row);
         }
-        const int n = rev ? t0 + i.row + 1 : seg.len - 1 - t0 - i.row;
-        lin_put_polar<T, 2, false>(Y, i.row, i.d0, x, f, live, live ? lin_power(lg, n) * (rev ? c.scale : 1.f) : 0.f, bias, c.D, c.R, 0, K::P);
+        float a[8], b[8];
+        lin_polar8<PL>(x, yr.type, f, i.d0, c.R, rev ? c.scale : 1.f, bias, a, b);
+        if (!live)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) a[k] = b[k] = 0.f;
+        if (keep) lin_hat_put<PL>(c.kh, to, i.d0, c.D, c.R, a, b);
+        if (p.states) {
+          const float w = in ? lin_power(lg, rev ? t0 + i.row + 1 : seg.len - 1 - t0 - i.row) : 0.f;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) a[k] *= w, b[k] *= w;
+          lin_place8(i.d0, c.D, c.R, a, b, [&](int e, const float* v) { lin_put8<2, false>(Y, i.row, e, v); },
+                     [&](int e, float v) { lin_put1<2, false>(Y, i.row, e, v); });
+        }
       }
+      if (!p.states) continue;
 #pragma unroll 2
       for (int u = 0; u < tz; ++u) {
         const Item i(u);
         if (i.d0 >= NT || n0 + i.d0 >= c.Dv) continue;
         const int row = seg.row0 + t0 + i.row;
-        u32x4 x = {0, 0, 0, 0};
-        if (t0 + i.row < seg.len && (rev || !c.mask || c.mask[(int64_t)seg.batch * c.mask_sb + row]))
-          x = lin_load8(zr.p + (int64_t)seg.batch * zr.s[0] + (int64_t)h * zr.s[1] + (int64_t)row * zr.s[2], n0 + i.d0, c.Dv, zr.vec);
-        lin_put_plain<T, PL, false>(Z, i.row, i.d0, x);
+        LinRaw<PL> x{};
+        if (t0 + i.row < seg.len) {
+          x = lin_load8<PL>(zr, (int64_t)seg.batch * zr.s[0] + (int64_t)h * zr.s[1] + (int64_t)row * zr.s[2], n0 + i.d0);
+          if (!kept(row)) x = LinRaw<PL>{};
+        }
+        lin_put_plain<PL, false>(Z, i.row, i.d0, x, zr.type);
       }
       __syncthreads();
       if (busy) {
@@ -93,33 +166,170 @@ __global__ __launch_bounds__(K::kThreads, 1) void linear_state_kernel(LinStatePa
           }
       }
     }
-  if (!busy) return;
-  float* to = p.states + ((int64_t)at * c.Hk + hk) * c.E * c.Dv;
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const int col = n0 + col0 + 16 * ct + l16;
-#pragma unroll
-    for (int s = 0; s < 2 * ST; ++s)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = 16 * s + 4 * q4 + r;
-        if (row < c.E && col < c.Dv) to[(int64_t)row * c.Dv + col] = W[ct][s][r];
-      }
-  }
+  if (busy && p.states) lin_state_out<K>(p, at, hk, n0 + col0, W);
 }
 
-template <typename T>
+// From the expanded rows.  EXACT: both factors as two parts (rows that are held as two).
+template <typename K, bool EXACT>
+__global__ __launch_bounds__(K::kThreads, K::P <= 128 && K::NT <= 128 ? 2 : K::NW / 4) void linear_sum_kernel(LinStateParams p) {
+  constexpr int NT = K::NT, CT = K::CT, PL = K::PL, PY = EXACT ? 2 : 1, C = K::C, KS = K::KS, ST = K::P / 32;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[PY * C * K::YS + PL * C * K::ZS];
+  __shared__ __attribute__((aligned(16))) float weight[C];
+  const LinCall& c = p.c;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), q4 = lane >> 4, l16 = lane & 15;
+  const int wg = blockIdx.x, tile = wg % p.tiles, rest = wg / p.tiles, hk = rest % c.Hk, at = rest / c.Hk;
+  const LinSeg seg = lin_segment(c.seqs, at);
+  if (seg.seq < 0) return;
+  const LinTile Y{lds, K::YS, C * K::YS}, Z{lds + PY * C * K::YS, K::ZS, C * K::ZS};
+  for (int i = tid; i < (int)sizeof(lds) / 16; i += K::kThreads) reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
+  const bool rev = p.reverse != 0;
+  const float lg = lin_log2(c, hk);
+  const int n0 = tile * NT, col0 = wave * K::SL, steps = (c.E + 31) / 32, G = rev ? c.G : 1;
+  const bool busy = n0 + col0 < c.Dv;
+  f32x4 W[CT][2 * ST];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+    for (int s = 0; s < 2 * ST; ++s) W[ct][s] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const LinHat yh = rev ? c.qh : c.kh;
+  const LinRows zr = rev ? c.g : c.v;
+  typedef LinItem<C, K::kThreads> Item;
+  const auto kept = [&](int row) { return rev || !c.mask || c.mask[(int64_t)seg.batch * c.mask_sb + row] != 0; };
+  struct InY { u32x4 w[PY]; };
+  struct InZ { LinRaw<PL> x; bool live; };   // what the mask leaves out is read too, so that no load waits for it
+  const auto get_y = [&](int it, int u) {
+    const Item i(u);
+    const int t = it / G * C + i.row, h = rev ? it % G * c.Hk + hk : hk;
+    InY r;
+#pragma unroll
+    for (int l = 0; l < PY; ++l) r.w[l] = u32x4{0, 0, 0, 0};
+    if (t < seg.len && i.d0 < yh.EP) {
+      const uint16_t* src = yh.p + (((int64_t)seg.batch * yh.H + h) * c.seqs.N + seg.row0 + t) * yh.EP + i.d0;
+#pragma unroll
+      for (int l = 0; l < PY; ++l) r.w[l] = *reinterpret_cast<const u32x4*>(src + l * yh.plane);
+    }
+    return r;
+  };
+  const auto get_z = [&](int it, int u) {
+    const Item i(u);
+    const int t = it / G * C + i.row, h = rev ? it % G * c.Hk + hk : hk, row = seg.row0 + t;
+    InZ r;
+    r.x = LinRaw<PL>{};
+    r.live = t < seg.len && i.d0 < NT && n0 + i.d0 < c.Dv;
+    if (r.live) {
+      r.x = lin_load8<PL>(zr, (int64_t)seg.batch * zr.s[0] + (int64_t)h * zr.s[1] + (int64_t)row * zr.s[2], n0 + i.d0);
+      r.live = kept(row);
+    }
+    return r;
+  };
+  const auto put_y = [&](int u, const InY& r) {
+    const Item i(u);
+    if (i.d0 < yh.EP) lin_put_parts<PY, false>(Y, i.row, i.d0, r.w);
+  };
+  const auto put_z = [&](int u, InZ r) {
+    const Item i(u);
+    if (i.d0 >= NT || n0 + i.d0 >= c.Dv) return;
+    if (!r.live) r.x = LinRaw<PL>{};
+    lin_put_plain<PL, false>(Z, i.row, i.d0, r.x, zr.type);
+  };
+  constexpr bool kAhead = K::P <= 128 && NT <= 128;
+  constexpr int kTY = kAhead ? K::TP : 0, kTZ = kAhead ? K::TZ : 0;
+  InY yin[kTY + 1];
+  InZ zin[kTZ + 1];
+  const auto load = [&](int it) {
+#pragma unroll
+    for (int u = 0; u < kTY; ++u) yin[u] = get_y(it, u);
+#pragma unroll
+    for (int u = 0; u < kTZ; ++u) zin[u] = get_z(it, u);
+  };
+  const int all = (seg.len + C - 1) / C * G;
+  load(0);
+  for (int it = 0; it < all; ++it) {
+    __syncthreads();   // nothing reads the tiles any more
+    for (int t = tid; t < C; t += K::kThreads) {
+      const int at_t = it / G * C + t;
+      weight[t] = at_t < seg.len ? lin_power(lg, rev ? at_t + 1 : seg.len - 1 - at_t) : 0.f;
+    }
+    if constexpr (kAhead) {
+#pragma unroll
+      for (int u = 0; u < kTY; ++u) put_y(u, yin[u]);
+#pragma unroll
+      for (int u = 0; u < kTZ; ++u) put_z(u, zin[u]);
+      if (it + 1 < all) load(it + 1);
+    } else {
+      const int ty = (C * (yh.EP / 8) + K::kThreads - 1) / K::kThreads;
+      const int tz = (C * ((min(NT, c.Dv - n0) + 31) / 32 * 4) + K::kThreads - 1) / K::kThreads;
+#pragma unroll 4
+      for (int u = 0; u < ty; ++u) put_y(u, get_y(it, u));
+#pragma unroll 4
+      for (int u = 0; u < tz; ++u) put_z(u, get_z(it, u));
+    }
+    __syncthreads();
+    if (busy) {
+      u32x4 za[CT][KS][PY];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const f32x4 w0 = *reinterpret_cast<const f32x4*>(weight + 32 * s + 4 * q4), w1 = *reinterpret_cast<const f32x4*>(weight + 32 * s + 16 + 4 * q4);
+          float v[8];
+          unpack8<BF16>(lin_across(Z.p, K::ZS, 32 * s, col0 + 16 * ct, lane), v);
+          if constexpr (PL == 2) {
+            float v2[8];
+            unpack8<BF16>(lin_across(Z.p + Z.plane, K::ZS, 32 * s, col0 + 16 * ct, lane), v2);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += v2[j];
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] *= w0[j], v[4 + j] *= w1[j];
+          u32x2 lo[PY], hi[PY];
+          lin_pack4<PY>(f32x4{v[0], v[1], v[2], v[3]}, lo);
+          lin_pack4<PY>(f32x4{v[4], v[5], v[6], v[7]}, hi);
+#pragma unroll
+          for (int l = 0; l < PY; ++l) za[ct][s][l] = u32x4{lo[l][0], lo[l][1], hi[l][0], hi[l][1]};
+        }
+#pragma unroll
+      for (int e = 0; e < 2 * ST; ++e)
+        if (e < 2 * steps) {
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            u32x4 ya[PY];
+#pragma unroll
+            for (int l = 0; l < PY; ++l) ya[l] = lin_across(Y.p + l * Y.plane, K::YS, 32 * s, 16 * e, lane);
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) W[ct][e] = lin_mfma<PY, PY>(ya, za[ct][s], W[ct][e]);
+          }
+        }
+    }
+  }
+  if (busy) lin_state_out<K>(p, at, hk, n0 + col0, W);
+}
+
+template <typename K>
 struct StateLaunch {
+  static hipError_t go(LinStateParams p, hipStream_t s) {
+    p.tiles = p.states ? (p.c.Dv + K::NT - 1) / K::NT : 1;
+    const int64_t keys = (int64_t)p.c.seqs.T * p.c.Hk * p.tiles, n = keys + (p.reverse ? 0 : (int64_t)p.c.seqs.T * p.c.Hq);
+    if (n >= ((int64_t)1 << 22)) return hipErrorInvalidValue;
+    p.key_wgs = (int)keys;
+    return launch_named("linear_states", linear_state_kernel<K>, dim3((unsigned)n), dim3(K::kThreads), s, p);
+  }
+};
+
+template <bool EXACT>
+struct SumLaunch {
   template <typename K>
   struct Of {
     static hipError_t go(LinStateParams p, hipStream_t s) {
       p.tiles = (p.c.Dv + K::NT - 1) / K::NT;
       const int64_t n = (int64_t)p.c.seqs.T * p.c.Hk * p.tiles;
       if (n >= ((int64_t)1 << 22)) return hipErrorInvalidValue;
-      return launch_named("linear_states", linear_state_kernel<T, K>, dim3((unsigned)n), dim3(K::kThreads), s, p);
+      return launch_named("linear_sums", linear_sum_kernel<K, EXACT>, dim3((unsigned)n), dim3(K::kThreads), s, p);
     }
   };
 };
+
+// ---------------------------------------------------------------- scan and phase
 
 constexpr int kScanAhead = 8;   // segments whose sums are loaded ahead of the sum over them
 
@@ -185,8 +395,12 @@ __global__ __launch_bounds__(256) void linear_dfreqs_kernel(LinPhaseParams p) {
 
 }  // namespace
 
-hipError_t launch_linear_states(const LinStateParams& p, int dtype, hipStream_t s) {
-  return dtype == BF16::kCode ? lin_dispatch<BF16, StateLaunch<BF16>::Of>(p.c.E, p.c.Dv, p, s) : lin_dispatch<F16, StateLaunch<F16>::Of>(p.c.E, p.c.Dv, p, s);
+hipError_t launch_linear_states(const LinStateParams& p, hipStream_t s) {
+  return p.c.split ? lin_dispatch<kTwo, StateLaunch>(p.c.E, p.c.Dv, p, s) : lin_dispatch<kOne, StateLaunch>(p.c.E, p.c.Dv, p, s);
+}
+
+hipError_t launch_linear_sums(const LinStateParams& p, hipStream_t s) {
+  return p.c.split ? lin_dispatch<kTwo, SumLaunch<true>::template Of>(p.c.E, p.c.Dv, p, s) : lin_dispatch<kOne, SumLaunch<false>::template Of>(p.c.E, p.c.Dv, p, s);
 }
 
 hipError_t launch_linear_scan(const LinScanParams& p, hipStream_t s) {

@@ -11,16 +11,14 @@ namespace pope {
 namespace {
 
 constexpr int kThreads = 256, kAhead = 8, kMaxE = 512, kMaxDv = 256;
-// Columns of a state whose rows stay in LDS for further query heads.
-constexpr int kHeldCols = 16;
 
-// GM query heads of the key head at once.  HOLD: there are more, which read the new state's columns from LDS.
-template <typename T, int GM, bool HOLD>
+// GM query heads of the key head at once.  MORE: there are others, for which a thread goes over its part of the state again: over
+// what it has written, or, where that went nowhere, over what it read.
+template <int GM, bool MORE>
 __global__ __launch_bounds__(kThreads) void linear_step_kernel(LinStepParams p) {
   __shared__ float kh[kMaxE];
   __shared__ __attribute__((aligned(16))) float qh[GM][kMaxE];
   __shared__ __attribute__((aligned(16))) float part[kThreads * 4];
-  __shared__ float held[HOLD ? kMaxE * kHeldCols : 1];
   __shared__ float out[kMaxDv];
   const LinCall& c = p.c;
   const int tid = threadIdx.x;
@@ -40,9 +38,9 @@ __global__ __launch_bounds__(kThreads) void linear_step_kernel(LinStepParams p) 
   const bool store = some && (unsigned)to < (unsigned)p.slots;
 
   const auto expand = [&](const LinRows& rows, int h, const float* bias, float factor, float* to_lds) {
-    const uint16_t* x = rows.p + (int64_t)b * rows.s[0] + (int64_t)h * rows.s[1];
+    const int64_t x = (int64_t)b * rows.s[0] + (int64_t)h * rows.s[1];
     for (int d = tid; d < c.D; d += kThreads) {
-      const float v = T::to_float(x[d]);
+      const float v = lin_get<kTwo>(rows, x + d);
       if (d < R) {
         float sn, cs;
         sincos_turns(lin_angle_row(c, b, 0)[d], bias ? lin_turns(bias[d]) : 0.f, &sn, &cs);
@@ -58,10 +56,12 @@ __global__ __launch_bounds__(kThreads) void linear_step_kernel(LinStepParams p) 
   float v[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r)
-    v[r] = on && d0 + r < Dv ? T::to_float(c.v.p[(int64_t)b * c.v.s[0] + (int64_t)hk * c.v.s[1] + d0 + r]) : 0.f;
+    v[r] = on && d0 + r < Dv ? lin_get<kTwo>(c.v, (int64_t)b * c.v.s[0] + (int64_t)hk * c.v.s[1] + d0 + r) : 0.f;
 
   for (int g0 = 0; g0 < c.G; g0 += GM) {
-    if (HOLD && g0) __syncthreads();
+    const bool again = MORE && g0 && store;   // the new state, from where it went
+    const float* in = again ? dst : src;
+    if (MORE && g0) __syncthreads();
 #pragma unroll
     for (int g = 0; g < GM; ++g)
       if (g0 + g < c.G) expand(c.q, (g0 + g) * c.Hk + hk, nullptr, c.scale, qh[g]);
@@ -77,23 +77,19 @@ __global__ __launch_bounds__(kThreads) void linear_step_kernel(LinStepParams p) 
           const int e = e0 + k * groups;
           s[k] = f32x4{0.f, 0.f, 0.f, 0.f};
           if (e >= E) continue;
-          if (HOLD && g0) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (d0 + r < c1) s[k][r] = held[e * kHeldCols + d0 - c0 + r];
-          } else if (vec) {
-            s[k] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(src + (int64_t)e * Dv + d0));
+          if (vec) {
+            s[k] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(in + (int64_t)e * Dv + d0));
           } else {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              if (d0 + r < c1) s[k][r] = src[(int64_t)e * Dv + d0 + r];
+              if (d0 + r < c1) s[k][r] = in[(int64_t)e * Dv + d0 + r];
           }
         }
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
           const int e = e0 + k * groups;
           if (e >= E) continue;
-          if (!(HOLD && g0)) {
+          if (!again) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) s[k][r] = fmaf(kh[e], v[r], decay * s[k][r]);
             if (store) {
@@ -103,10 +99,6 @@ __global__ __launch_bounds__(kThreads) void linear_step_kernel(LinStepParams p) 
                 for (int r = 0; r < 4; ++r)
                   if (d0 + r < c1) dst[(int64_t)e * Dv + d0 + r] = s[k][r];
             }
-            if (HOLD)
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (d0 + r < c1) held[e * kHeldCols + d0 - c0 + r] = s[k][r];
           }
 #pragma unroll
           for (int g = 0; g < GM; ++g)
@@ -129,9 +121,9 @@ __global__ __launch_bounds__(kThreads) void linear_step_kernel(LinStepParams p) 
         for (int r = 0; r < groups; ++r) sum += part[4 * (r * across) + tid];
         out[tid] = sum;
       }
-      uint16_t* orow = p.o.p + (int64_t)b * p.o.s[0] + (int64_t)h * p.o.s[1];
-      if (!p.gate) {
-        if (c0 + tid < c1) orow[c0 + tid] = T::bits(out[tid]);
+      const int64_t orow = (int64_t)b * p.o.s[0] + (int64_t)h * p.o.s[1];
+      if (!p.gate.p) {
+        if (c0 + tid < c1) lin_set<kTwo>(p.o, orow + c0 + tid, out[tid]);
       } else {   // the whole row is here
         __syncthreads();
         if (tid < 64) {
@@ -140,12 +132,10 @@ __global__ __launch_bounds__(kThreads) void linear_step_kernel(LinStepParams p) 
 #pragma unroll
           for (int i = 1; i < 64; i *= 2) ss += wave_shfl_xor(ss, i);
           const float r = 1.f / __builtin_sqrtf(ss / Dv + p.eps);
-          const uint16_t* gate = p.gate + (int64_t)b * p.g_s[0] + (int64_t)h * p.g_s[1];
           for (int d = tid; d < Dv; d += 64) {
-            const float w = !p.weight ? 1.f : p.w_f32 ? static_cast<const float*>(p.weight)[h * p.w_sh + d]
-                                                      : T::to_float(static_cast<const uint16_t*>(p.weight)[h * p.w_sh + d]);
-            const float x = T::to_float(gate[d]);
-            orow[d] = T::bits(some ? out[d] * r * w * x * sigmoid_f(x) : 0.f);
+            const float w = p.weight ? lin_value(p.weight, p.w_type, h * p.w_sh + d) : 1.f;
+            const float x = lin_get<kTwo>(p.gate, (int64_t)b * p.gate.s[0] + (int64_t)h * p.gate.s[1] + d);
+            lin_set<kTwo>(p.o, orow + d, some ? out[d] * r * w * x * sigmoid_f(x) : 0.f);
           }
         }
       }
@@ -153,22 +143,18 @@ __global__ __launch_bounds__(kThreads) void linear_step_kernel(LinStepParams p) 
   }
 }
 
-template <typename T>
-hipError_t step_t(const LinStepParams& p, hipStream_t s) {
+template <int GM, bool MORE>
+hipError_t launch(const LinStepParams& p, hipStream_t s) {
   const int64_t n = (int64_t)p.c.seqs.B * p.c.Hk * p.split;
   if (n >= ((int64_t)1 << 22)) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)n), block(kThreads);
-  const int G = p.c.G;
-  if (G == 1) return launch_named("linear_step", linear_step_kernel<T, 1, false>, grid, block, s, p);
-  if (G == 2) return launch_named("linear_step", linear_step_kernel<T, 2, false>, grid, block, s, p);
-  if (G <= kLinStepHeads) return launch_named("linear_step", linear_step_kernel<T, kLinStepHeads, false>, grid, block, s, p);
-  return launch_named("linear_step", linear_step_kernel<T, kLinStepHeads, true>, grid, block, s, p);
+  return launch_named("linear_step", linear_step_kernel<GM, MORE>, dim3((unsigned)n), dim3(kThreads), s, p);
 }
 
 }  // namespace
 
-hipError_t launch_linear_step(const LinStepParams& p, int dtype, hipStream_t s) {
-  return dtype == BF16::kCode ? step_t<BF16>(p, s) : step_t<F16>(p, s);
+hipError_t launch_linear_step(const LinStepParams& p, hipStream_t s) {
+  const int G = p.c.G;
+  return G == 1 ? launch<1, false>(p, s) : G == 2 ? launch<2, false>(p, s) : G <= 4 ? launch<4, false>(p, s) : launch<4, true>(p, s);
 }
 
 }  // namespace pope

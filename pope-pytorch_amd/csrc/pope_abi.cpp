@@ -1282,7 +1282,7 @@ int check_linear(const pope_linear* d) {
   if (d->D < 1 || d->D > 256 || d->Dv < 1 || d->Dv > 256)
     return fail(POPE_ERR_UNSUPPORTED, "linear attention covers head and value dims 1 to 256 (got %d, %d)", d->D, d->Dv);
   if (d->R < 0 || d->R > d->D) return fail(POPE_ERR_INVALID, "rotate dim %d must be in [0, head dim %d]", d->R, d->D);
-  if (d->dtype != POPE_F16 && d->dtype != POPE_BF16) return fail(POPE_ERR_INVALID, "linear attention takes fp16 or bf16 rows (dtype %d)", d->dtype);
+  if (d->dtype != POPE_F32 && d->dtype != POPE_F16 && d->dtype != POPE_BF16) return fail(POPE_ERR_INVALID, "unknown dtype %d", d->dtype);
   if (d->N > (1 << 28) || d->B > (1 << 20) || d->Hq > 65535)
     return fail(POPE_ERR_UNSUPPORTED, "%d sequences, %d rows, %d heads: too many", d->B, d->N, d->Hq);
   if (d->bias_sh < 0 || d->mask_sb < 0) return fail(POPE_ERR_INVALID, "negative bias / mask stride");
@@ -1294,24 +1294,33 @@ int check_linear(const pope_linear* d) {
   return rc;
 }
 
-// Rows of a segment: a multiple of 64 (a chunk) that brings the workgroups to about kLinGrid.
+// Workgroups that the chip holds at once: two for each CU, one where rows or states are wide.
 constexpr int kLinGrid = 512, kLinChunk = 64;
 
 struct LinShape {
   int L, M, T;
   bool parts;      // some sequence may have more than one segment
-  size_t states;   // bytes of the states of all segments
+  int EP, planes;  // columns of expanded rows in memory; their bf16 parts
+  size_t qh, kh, states;   // bytes of the expanded rows and of the states of all segments
 };
 
 LinShape linear_shape(const pope_linear& d, bool packed) {
   LinShape s;
   const int64_t rows = (packed ? 1 : (int64_t)d.B) * d.N;
-  const int64_t want = std::max<int64_t>(1, (rows * d.Hk + kLinGrid - 1) / kLinGrid);
+  // Rows of a segment: a multiple of 64 (a chunk) with which the heads' segments fill the chip once.  Shorter ones would only
+  // add states: at 256 + 256 columns a state is as many bytes as its head's 256 rows of q, k, v and o.
+  const bool wide = d.D + d.R > 128 || d.Dv > 128;
+  const int64_t tiles = d.D + d.R > 256 ? (d.Dv + 127) / 128 : 1, grid = wide ? kLinGrid / 2 : kLinGrid;
+  const int64_t want = std::max<int64_t>(1, (rows * d.Hk * tiles + grid - 1) / grid);
   s.L = (int)std::min<int64_t>((want + kLinChunk - 1) / kLinChunk * kLinChunk, (int64_t)(d.N + kLinChunk - 1) / kLinChunk * kLinChunk);
   s.L = std::max(s.L, kLinChunk);
   s.M = std::max(1, (d.N + s.L - 1) / s.L);
   s.T = packed ? (int)std::min<int64_t>(d.N, (int64_t)d.N / s.L + d.B) : d.B * s.M;
   s.parts = d.N > s.L;
+  s.EP = round_up(d.D + d.R, 32);
+  s.planes = d.dtype != POPE_BF16 || d.o_f32 ? 2 : 1;
+  s.qh = align_up((size_t)rows * d.Hq * s.EP * 2) * s.planes;
+  s.kh = align_up((size_t)rows * d.Hk * s.EP * 2) * s.planes;
   s.states = align_up((size_t)s.T * d.Hk * (d.D + d.R) * d.Dv * sizeof(float));
   return s;
 }
@@ -1328,23 +1337,30 @@ LinBytes linear_bwd_bytes(const pope_linear& d, const LinShape& s, bool packed, 
   return b;
 }
 
-pope::LinRows lin_rows(const void* p, const int64_t* s, int cols, int unit) {
+pope::LinRows lin_rows(const void* p, const int64_t* s, int cols, int type, int unit) {
   pope::LinRows r;
-  r.p = static_cast<uint16_t*>(const_cast<void*>(p));
+  r.p = const_cast<void*>(p);
   copy3(r.s, s);
   r.cols = cols;
-  r.vec = cols % unit == 0 && reinterpret_cast<uintptr_t>(p) % (2 * unit) == 0 && s[0] % unit == 0 && s[1] % unit == 0 && s[2] % unit == 0;
+  r.type = type;
+  const uintptr_t whole = std::min(16, unit * (type == POPE_F32 ? 4 : 2));   // bytes of an access
+  r.vec = cols % unit == 0 && reinterpret_cast<uintptr_t>(p) % whole == 0 && s[0] % unit == 0 && s[1] % unit == 0 && s[2] % unit == 0;
   return r;
 }
 
-pope::LinCall linear_call(const pope_linear& d, const LinShape& s, const void* q, const void* k, const void* v, const float* freqs,
+pope::LinHat lin_hat(const void* p, size_t bytes, const LinShape& s, int H) {
+  return pope::LinHat{static_cast<uint16_t*>(const_cast<void*>(p)), (int64_t)(bytes / s.planes / 2), H, s.EP};
+}
+
+// hats: the expanded rows, or null.
+pope::LinCall linear_call(const pope_linear& d, const LinShape& s, const void* hats, const void* q, const void* k, const void* v, const float* freqs,
                           const float* bias, const float* log_decay, const uint8_t* mask, const int32_t* cu) {
   pope::LinCall c;
   std::memset(&c, 0, sizeof c);
   c.seqs = pope::LinSeqs{cu, d.B, d.N, s.L, s.M, s.T};
-  c.q = lin_rows(q, d.q_s, d.D, 8);
-  c.k = lin_rows(k, d.k_s, d.D, 8);
-  c.v = lin_rows(v, d.v_s, d.Dv, 8);
+  c.q = lin_rows(q, d.q_s, d.D, d.dtype, 8);
+  c.k = lin_rows(k, d.k_s, d.D, d.dtype, 8);
+  c.v = lin_rows(v, d.v_s, d.Dv, d.dtype, 8);
   c.freqs = freqs;
   c.f_s[0] = d.f_s[0]; c.f_s[1] = d.f_s[1];
   c.f_vec = d.R % 8 == 0 && aligned16(freqs) && d.f_s[0] % 4 == 0 && d.f_s[1] % 4 == 0;
@@ -1353,6 +1369,11 @@ pope::LinCall linear_call(const pope_linear& d, const LinShape& s, const void* q
   c.mask = mask; c.mask_sb = d.mask_sb;
   c.Hq = d.Hq; c.Hk = d.Hk; c.G = d.Hq / d.Hk; c.D = d.D; c.R = d.R; c.E = d.D + d.R; c.Dv = d.Dv;
   c.scale = d.scale;
+  c.split = s.planes == 2;
+  if (hats) {
+    c.qh = lin_hat(hats, s.qh, s, d.Hq);
+    c.kh = lin_hat(static_cast<const char*>(hats) + s.qh, s.kh, s, d.Hk);
+  }
   return c;
 }
 
@@ -1379,7 +1400,7 @@ int check_norm(const pope_gated_norm* d) {
   if (!d) return fail(POPE_ERR_INVALID, "descriptor is NULL");
   if (d->B < 0 || d->H < 1 || d->N < 0) return fail(POPE_ERR_INVALID, "H must be >= 1 and B, N >= 0 (got %d, %d, %d)", d->H, d->B, d->N);
   if (d->cols < 1 || d->cols > 512) return fail(POPE_ERR_UNSUPPORTED, "the gated norm covers rows of 1 to 512 values (got %d)", d->cols);
-  if (d->dtype != POPE_F16 && d->dtype != POPE_BF16) return fail(POPE_ERR_INVALID, "the gated norm takes fp16 or bf16 rows (dtype %d)", d->dtype);
+  if (d->dtype != POPE_F32 && d->dtype != POPE_F16 && d->dtype != POPE_BF16) return fail(POPE_ERR_INVALID, "unknown dtype %d", d->dtype);
   if (d->weight_rows != 1 && d->weight_rows != d->H) return fail(POPE_ERR_INVALID, "weight rows %d must be 1 or %d", d->weight_rows, d->H);
   if (d->H > 65535 || (int64_t)d->B * d->N > ((int64_t)1 << 32)) return fail(POPE_ERR_UNSUPPORTED, "%d x %d rows, %d heads: too many", d->B, d->N, d->H);
   if (d->weight_sh < 0) return fail(POPE_ERR_INVALID, "negative weight stride");
@@ -1391,11 +1412,11 @@ int check_norm(const pope_gated_norm* d) {
 pope::GatedNormParams norm_params(const pope_gated_norm& d, const void* x, const void* gate, const void* weight) {
   pope::GatedNormParams p;
   std::memset(&p, 0, sizeof p);
-  p.x = lin_rows(x, d.x_s, d.cols, 8);
-  p.gate = lin_rows(gate, d.gate_s, d.cols, 8);
+  p.x = lin_rows(x, d.x_s, d.cols, d.x_f32 ? POPE_F32 : d.dtype, 8);
+  p.gate = lin_rows(gate, d.gate_s, d.cols, d.dtype, 8);
   p.weight = weight;
   p.w_sh = d.weight_rows > 1 ? d.weight_sh : 0;
-  p.w_f32 = d.weight_f32;
+  p.w_type = d.weight_f32 ? POPE_F32 : d.dtype;
   p.B = d.B; p.H = d.H; p.N = d.N; p.heads_w = d.weight_rows;
   p.eps = d.eps;
   return p;
@@ -1410,14 +1431,14 @@ int pope_linear_bytes(const pope_linear* d, int packed, int final, int want_dfre
   if (rc) return rc;
   if (!bytes) return fail(POPE_ERR_INVALID, "bytes is NULL");
   const LinShape s = linear_shape(*d, packed != 0);
-  bytes[0] = s.parts || final ? s.states : 0;
+  bytes[0] = s.qh + s.kh + (s.parts || final ? s.states : 0);
   bytes[1] = linear_bwd_bytes(*d, s, packed != 0, want_dfreqs != 0).all;
   return POPE_OK;
 }
 
 int pope_linear_fwd(const pope_linear* d, const void* q, const void* k, const void* v, const float* freqs, const float* bias,
                     const float* log_decay, const uint8_t* mask, const int32_t* cu, const float* initial, void* o, float* last,
-                    void* states, size_t states_bytes, void* stream) {
+                    void* kept, size_t kept_bytes, void* stream) {
   int rc = check_linear(d);
   if (rc) return rc;
   if (d->N == 0) return POPE_OK;
@@ -1425,31 +1446,32 @@ int pope_linear_fwd(const pope_linear* d, const void* q, const void* k, const vo
   if (!o) return fail(POPE_ERR_INVALID, "o must be non-NULL");
   const LinShape sh = linear_shape(*d, cu != nullptr);
   const bool sums = sh.parts || last;
-  if ((rc = check_ws(sums ? sh.states : 0, states, states_bytes))) return rc;
+  const size_t hats = sh.qh + sh.kh;
+  if ((rc = check_ws(hats + (sums ? sh.states : 0), kept, kept_bytes))) return rc;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const pope::LinCall c = linear_call(*d, sh, q, k, v, freqs, bias, log_decay, mask, cu);
+  float* seg_states = sums ? reinterpret_cast<float*>(static_cast<char*>(kept) + hats) : nullptr;
+  const pope::LinCall c = linear_call(*d, sh, kept, q, k, v, freqs, bias, log_decay, mask, cu);
+  const pope::LinStateParams sp{c, seg_states, 0, 0, 0};
+  hipError_t e = pope::launch_linear_states(sp, s);
+  if (e != hipSuccess) return lin_fail(e, "linear attention states launch");
   if (sums) {
-    const pope::LinStateParams sp{c, static_cast<float*>(states), 0, 0};
-    hipError_t e = pope::launch_linear_states(sp, d->dtype, s);
-    if (e != hipSuccess) return lin_fail(e, "linear attention states launch");
-    const pope::LinScanParams cp{c, static_cast<float*>(states), initial, last, 0};
+    const pope::LinScanParams cp{c, seg_states, initial, last, 0};
     if ((e = pope::launch_linear_scan(cp, s)) != hipSuccess) return lin_fail(e, "linear attention scan launch");
   }
   pope::LinOutParams p;
   std::memset(&p, 0, sizeof p);
   p.c = c;
-  p.out[0] = lin_rows(o, d->o_s, d->Dv, 4);
-  p.states[0] = sums ? static_cast<const float*>(states) : nullptr;
+  p.out[0] = lin_rows(o, d->o_s, d->Dv, d->o_f32 ? POPE_F32 : d->dtype, 4);
+  p.states[0] = seg_states;
   p.first[0] = initial;
   p.heads_per = lin_heads_per(*d, sh);
-  const hipError_t e = d->dtype == POPE_BF16 ? pope::launch_linear_out_bf16(p, s) : pope::launch_linear_out_f16(p, s);
-  if (e != hipSuccess) return lin_fail(e, "linear attention launch");
+  if ((e = c.split ? pope::launch_linear_out_split(p, s) : pope::launch_linear_out_bf16(p, s)) != hipSuccess) return lin_fail(e, "linear attention launch");
   return POPE_OK;
 }
 
 int pope_linear_bwd(const pope_linear* d, const void* dout, const float* dlast, const void* q, const void* k, const void* v,
                     const float* freqs, const float* bias, const float* log_decay, const uint8_t* mask, const int32_t* cu,
-                    const float* initial, const void* states, size_t states_bytes, void* dq, void* dk, void* dv, float* dfreqs,
+                    const float* initial, const void* kept, size_t kept_bytes, void* dq, void* dk, void* dv, float* dfreqs,
                     float* dbias, float* dinitial, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_linear(d);
   if (rc) return rc;
@@ -1460,32 +1482,34 @@ int pope_linear_bwd(const pope_linear* d, const void* dout, const float* dlast, 
   if ((rc = check_linear_ptrs(d, q, k, v, freqs, bias))) return rc;
   if (!dout || !dq || !dk || !dv) return fail(POPE_ERR_INVALID, "dout, dq, dk, dv must be non-NULL");
   const LinShape sh = linear_shape(*d, cu != nullptr);
-  if ((rc = check_ws(sh.parts ? sh.states : 0, const_cast<void*>(states), states_bytes))) return rc;
+  const size_t hats = sh.qh + sh.kh;
+  if ((rc = check_ws(hats + (sh.parts ? sh.states : 0), const_cast<void*>(kept), kept_bytes))) return rc;
   const LinBytes lb = linear_bwd_bytes(*d, sh, cu != nullptr, dfreqs != nullptr);
   if ((rc = check_ws(lb.all, workspace, workspace_bytes))) return rc;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
   float* reverse = reinterpret_cast<float*>(ws);
-  pope::LinCall c = linear_call(*d, sh, q, k, v, freqs, bias, log_decay, mask, cu);
-  c.g = lin_rows(dout, d->do_s, d->Dv, 8);
+  pope::LinCall c = linear_call(*d, sh, kept, q, k, v, freqs, bias, log_decay, mask, cu);
+  c.g = lin_rows(dout, d->do_s, d->Dv, d->o_f32 ? POPE_F32 : d->dtype, 8);
   hipError_t e;
   const bool sums = sh.parts || dinitial;
   if (sums) {
-    const pope::LinStateParams sp{c, reverse, 1, 0};
-    if ((e = pope::launch_linear_states(sp, d->dtype, s)) != hipSuccess) return lin_fail(e, "linear attention states launch");
+    // the initial states' gradient takes its queries in two parts: from the rows themselves where they are held as one
+    const pope::LinStateParams sp{c, reverse, 1, 0, 0};
+    if ((e = dinitial && !c.split ? pope::launch_linear_states(sp, s) : pope::launch_linear_sums(sp, s)) != hipSuccess) return lin_fail(e, "linear attention states launch");
     const pope::LinScanParams cp{c, reverse, dlast, dinitial, 1};
     if ((e = pope::launch_linear_scan(cp, s)) != hipSuccess) return lin_fail(e, "linear attention scan launch");
   }
   pope::LinOutParams p;
   std::memset(&p, 0, sizeof p);
   p.c = c;
-  p.states[0] = sh.parts ? static_cast<const float*>(states) : nullptr;
+  p.states[0] = sh.parts ? reinterpret_cast<const float*>(static_cast<const char*>(kept) + hats) : nullptr;
   p.first[0] = initial;
   p.states[1] = sums ? reverse : nullptr;
   p.first[1] = dlast;
   p.heads_per = lin_heads_per(*d, sh);
-  p.out[0] = lin_rows(dq, d->dq_s, d->D, 4);
-  p.out[1] = lin_rows(dk, d->dk_s, d->D, 4);
+  p.out[0] = lin_rows(dq, d->dq_s, d->D, d->dtype, 4);
+  p.out[1] = lin_rows(dk, d->dk_s, d->D, d->dtype, 4);
   if (d->R > 0) {
     if (dbias) p.dbias = reinterpret_cast<float*>(ws + lb.reverse);
     if (dfreqs) {
@@ -1493,12 +1517,11 @@ int pope_linear_bwd(const pope_linear* d, const void* dout, const float* dlast, 
       p.dphase[1] = reinterpret_cast<float*>(ws + lb.reverse + lb.dbias + lb.dq);
     }
   }
-  const bool bf16 = d->dtype == POPE_BF16;
-  if ((e = bf16 ? pope::launch_linear_dqk_bf16(p, s) : pope::launch_linear_dqk_f16(p, s)) != hipSuccess) return lin_fail(e, "linear attention launch");
+  if ((e = c.split ? pope::launch_linear_dqk_split(p, s) : pope::launch_linear_dqk_bf16(p, s)) != hipSuccess) return lin_fail(e, "linear attention launch");
   pope::LinOutParams pv = p;
-  pv.out[0] = lin_rows(dv, d->dv_s, d->Dv, 4);
+  pv.out[0] = lin_rows(dv, d->dv_s, d->Dv, d->dtype, 4);
   pv.dphase[0] = pv.dphase[1] = nullptr;
-  if ((e = bf16 ? pope::launch_linear_dv_bf16(pv, s) : pope::launch_linear_dv_f16(pv, s)) != hipSuccess) return lin_fail(e, "linear attention launch");
+  if ((e = c.split ? pope::launch_linear_dv_split(pv, s) : pope::launch_linear_dv_bf16(pv, s)) != hipSuccess) return lin_fail(e, "linear attention launch");
   if (d->R > 0 && (dbias || dfreqs)) {
     pope::LinPhaseParams ph;
     std::memset(&ph, 0, sizeof ph);
@@ -1518,8 +1541,8 @@ int pope_gated_norm_fwd(const pope_gated_norm* d, const void* x, const void* gat
   if (d->B == 0 || d->N == 0) return POPE_OK;
   if (!x || !gate || !y) return fail(POPE_ERR_INVALID, "x, gate, y must be non-NULL");
   pope::GatedNormParams p = norm_params(*d, x, gate, weight);
-  p.y = lin_rows(y, d->y_s, d->cols, 8);
-  const hipError_t e = pope::launch_gated_norm(p, d->dtype, false, reinterpret_cast<hipStream_t>(stream));
+  p.y = lin_rows(y, d->y_s, d->cols, d->dtype, 8);
+  const hipError_t e = pope::launch_gated_norm(p, false, reinterpret_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "gated norm launch");
   return POPE_OK;
 }
@@ -1544,12 +1567,12 @@ int pope_gated_norm_bwd(const pope_gated_norm* d, const void* dy, const void* x,
   if (dweight && !weight) return fail(POPE_ERR_INVALID, "dweight wanted, but there is no weight");
   if (dweight && (rc = check_ws(need, workspace, workspace_bytes))) return rc;
   pope::GatedNormParams p = norm_params(*d, x, gate, weight);
-  p.y = lin_rows(dy, d->dy_s, d->cols, 8);
-  p.dx = lin_rows(dx, d->dx_s, d->cols, 8);
-  p.dgate = lin_rows(dgate, d->dgate_s, d->cols, 8);
+  p.y = lin_rows(dy, d->dy_s, d->cols, d->dtype, 8);
+  p.dx = lin_rows(dx, d->dx_s, d->cols, p.x.type, 8);
+  p.dgate = lin_rows(dgate, d->dgate_s, d->cols, d->dtype, 8);
   p.part = dweight ? static_cast<float*>(workspace) : nullptr;
   p.dweight = dweight;
-  const hipError_t e = pope::launch_gated_norm(p, d->dtype, true, reinterpret_cast<hipStream_t>(stream));
+  const hipError_t e = pope::launch_gated_norm(p, true, reinterpret_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "gated norm backward launch");
   return POPE_OK;
 }
@@ -1567,38 +1590,26 @@ int pope_linear_step(const pope_linear* d, const void* q, const void* k, const v
   if ((norm != nullptr) != (gate != nullptr)) return fail(POPE_ERR_INVALID, "norm and gate come together");
   if (norm) {
     if ((rc = check_norm(norm))) return rc;
-    if (norm->B != d->B || norm->H != d->Hq || norm->N != 1 || norm->cols != d->Dv || norm->dtype != d->dtype)
+    if (norm->B != d->B || norm->H != d->Hq || norm->N != 1 || norm->cols != d->Dv || norm->dtype != d->dtype || norm->x_f32)
       return fail(POPE_ERR_INVALID, "the norm's rows are not the step's");
   }
   const LinShape sh = linear_shape(*d, false);
   pope::LinStepParams p;
   std::memset(&p, 0, sizeof p);
-  p.c = linear_call(*d, sh, q, k, v, freqs, bias, log_decay, nullptr, nullptr);
-  p.o = lin_rows(o, d->o_s, d->Dv, 4);
+  p.c = linear_call(*d, sh, nullptr, q, k, v, freqs, bias, log_decay, nullptr, nullptr);
+  p.o = lin_rows(o, d->o_s, d->Dv, d->o_f32 ? POPE_F32 : d->dtype, 4);
   p.from = states; p.to = states;
   p.read = from; p.write = to;
   p.slots = slots; p.slot_s = slot_s;
-  // More query heads of a key head than a thread sums at once go over columns held in LDS, 16 for each workgroup; the norm, which
-  // needs a row's columns together, is then a launch of its own.
-  const bool many = p.c.G > pope::kLinStepHeads, own = norm && many;
-  if (norm && !own) {
-    p.gate = static_cast<const uint16_t*>(gate);
-    copy3(p.g_s, norm->gate_s);
-    p.weight = weight; p.w_sh = norm->weight_rows > 1 ? norm->weight_sh : 0; p.w_f32 = norm->weight_f32; p.eps = norm->eps;
+  if (norm) {   // a row's columns together
+    p.gate = lin_rows(gate, norm->gate_s, d->Dv, d->dtype, 8);
+    p.weight = weight; p.w_sh = norm->weight_rows > 1 ? norm->weight_sh : 0; p.w_type = norm->weight_f32 ? POPE_F32 : d->dtype; p.eps = norm->eps;
     p.split = 1;
-  } else {
-    const int most = (d->Dv + 15) / 16;
-    const int64_t wgs = (int64_t)d->B * d->Hk;
-    p.split = many ? most : (int)std::min<int64_t>(most, std::max<int64_t>(1, kLinGrid / wgs));
+  } else {      // columns of few states go to several workgroups, 16 or more to each
+    p.split = (int)std::min<int64_t>((d->Dv + 15) / 16, std::max<int64_t>(1, kLinGrid / ((int64_t)d->B * d->Hk)));
   }
-  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  hipError_t e = pope::launch_linear_step(p, d->dtype, s);
+  const hipError_t e = pope::launch_linear_step(p, reinterpret_cast<hipStream_t>(stream));
   if (e != hipSuccess) return lin_fail(e, "linear attention step launch");
-  if (own) {
-    pope::GatedNormParams n = norm_params(*norm, o, gate, weight);
-    n.x = n.y = lin_rows(o, d->o_s, d->Dv, 8);
-    if ((e = pope::launch_gated_norm(n, d->dtype, false, s)) != hipSuccess) return hip_fail(e, "gated norm launch");
-  }
   return POPE_OK;
 }
 

@@ -6,14 +6,16 @@ struct LinearArgs {
   Tensor q, k, v, freqs, bias, log_decay, mask, cu, initial;
   double scale;
   bool with_state, head_first;
+  bool o_f32 = false;   // o in fp32: the gated norm goes on from it
 
   int h() const { return head_first ? 1 : 2; }
   int n() const { return head_first ? 2 : 1; }
   int64_t sequences() const { return cu.defined() ? cu.size(0) - 1 : q.size(0); }
 
   void strides(int64_t* s, const Tensor& t) const { s[0] = t.stride(0), s[1] = t.stride(h()), s[2] = t.stride(n()); }
-  Tensor rows(int64_t heads, int64_t cols) const {
-    const auto o = q.options().requires_grad(false);
+  at::ScalarType o_type() const { return o_f32 ? at::kFloat : q.scalar_type(); }
+  Tensor rows(int64_t heads, int64_t cols, at::ScalarType dtype) const {
+    const auto o = q.options().dtype(dtype).requires_grad(false);
     return head_first ? at::empty({q.size(0), heads, q.size(n()), cols}, o) : at::empty({q.size(0), q.size(n()), heads, cols}, o);
   }
 
@@ -22,7 +24,7 @@ struct LinearArgs {
   bool fits() const {
     const auto here = [&](const Tensor& t) { return !t.defined() || t.device() == q.device(); };
     const auto type = [](const Tensor& t) { return t.scalar_type() == at::kFloat || t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; };
-    if (!q.is_cuda() || q.dim() != 4 || k.dim() != 4 || v.dim() != 4 || (q.scalar_type() != at::kHalf && q.scalar_type() != at::kBFloat16) ||
+    if (!q.is_cuda() || q.dim() != 4 || k.dim() != 4 || v.dim() != 4 || !type(q) ||
         k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type())
       return false;
     for (const Tensor* t : {&k, &v, &freqs, &bias, &log_decay, &mask, &cu, &initial})
@@ -72,6 +74,7 @@ struct LinearArgs {
     d.R = freqs.defined() ? (int32_t)freqs.size(-1) : 0;
     d.Dv = (int32_t)v.size(3);
     d.dtype = dtype_code(q);
+    d.o_f32 = o_f32;
     d.scale = (float)scale;
     strides(d.q_s, q);
     strides(d.k_s, k);
@@ -97,21 +100,21 @@ const uint8_t* bytes_of(const Tensor& t) { return static_cast<const uint8_t*>(da
 const int32_t* ints_of(const Tensor& t) { return static_cast<const int32_t*>(data(t)); }
 
 struct LinearOut {
-  Tensor o, last, states;
+  Tensor o, last, kept;
 };
 
 LinearOut linear_forward(const LinearArgs& a) {   // converted operands
   pope_linear d = a.desc();
   const c10::DeviceGuard guard(a.q.device());
   LinearOut r;
-  r.o = a.rows(d.Hq, d.Dv);
+  r.o = a.rows(d.Hq, d.Dv, a.o_type());
   a.strides(d.o_s, r.o);
   if (a.with_state) r.last = a.state();
   size_t n[2] = {0, 0};
   check(pope_linear_bytes(&d, a.cu.defined(), a.with_state, 0, n), "workspace query");
-  r.states = bytes_like(a.q, n[0]);
+  r.kept = bytes_like(a.q, n[0]);
   check(pope_linear_fwd(&d, a.q.data_ptr(), a.k.data_ptr(), a.v.data_ptr(), floats(a.freqs), floats(a.bias), floats(a.log_decay), bytes_of(a.mask), ints_of(a.cu),
-                        floats(a.initial), r.o.data_ptr(), static_cast<float*>(data(r.last)), data(r.states), n[0], stream_of(a.q)),
+                        floats(a.initial), r.o.data_ptr(), static_cast<float*>(data(r.last)), data(r.kept), n[0], stream_of(a.q)),
         "linear attention");
   return r;
 }
@@ -120,22 +123,22 @@ struct LinearGrads {
   Tensor dq, dk, dv, dfreqs, dbias, dinitial;
 };
 
-LinearGrads linear_backward(const LinearArgs& a, const Tensor& dout0, const Tensor& dlast0, const Tensor& states, bool need_df, bool need_db, bool need_d0) {
+LinearGrads linear_backward(const LinearArgs& a, const Tensor& dout0, const Tensor& dlast0, const Tensor& kept, bool need_df, bool need_db, bool need_d0) {
   pope_linear d = a.desc();
   const c10::DeviceGuard guard(a.q.device());
   Tensor dout = dout0;
-  if (!dout.defined()) dout = a.rows(d.Hq, d.Dv).zero_();
-  if (dout.scalar_type() != a.q.scalar_type()) dout = dout.to(a.q.scalar_type());
+  if (!dout.defined()) dout = a.rows(d.Hq, d.Dv, a.o_type()).zero_();
+  if (dout.scalar_type() != a.o_type()) dout = dout.to(a.o_type());
   dout = unit_feature(dout);
   const Tensor dlast = dlast0.defined() ? dlast0.to(at::kFloat).contiguous() : Tensor();
-  check_device(a.q, {&dout, &dlast, &states});
+  check_device(a.q, {&dout, &dlast, &kept});
   TORCH_CHECK_VALUE(dout.dim() == 4 && dout.size(0) == a.q.size(0) && dout.size(a.h()) == d.Hq && dout.size(a.n()) == d.N && dout.size(3) == d.Dv, "dout ", dout.sizes(),
                     " does not fit the linear attention");
   a.strides(d.do_s, dout);
   LinearGrads r;
-  r.dq = a.rows(d.Hq, d.D);
-  r.dk = a.rows(d.Hk, d.D);
-  r.dv = a.rows(d.Hk, d.Dv);
+  r.dq = a.rows(d.Hq, d.D, a.q.scalar_type());
+  r.dk = a.rows(d.Hk, d.D, a.q.scalar_type());
+  r.dv = a.rows(d.Hk, d.Dv, a.q.scalar_type());
   a.strides(d.dq_s, r.dq);
   a.strides(d.dk_s, r.dk);
   a.strides(d.dv_s, r.dv);
@@ -151,7 +154,7 @@ LinearGrads linear_backward(const LinearArgs& a, const Tensor& dout0, const Tens
   check(pope_linear_bytes(&d, a.cu.defined(), 0, need_df, n), "workspace query");
   const Tensor ws = bytes_like(a.q, n[1]);
   check(pope_linear_bwd(&d, dout.data_ptr(), floats(dlast), a.q.data_ptr(), a.k.data_ptr(), a.v.data_ptr(), floats(a.freqs), floats(a.bias), floats(a.log_decay),
-                        bytes_of(a.mask), ints_of(a.cu), floats(a.initial), data(states), states.defined() ? states.nbytes() : 0, r.dq.data_ptr(), r.dk.data_ptr(),
+                        bytes_of(a.mask), ints_of(a.cu), floats(a.initial), data(kept), kept.defined() ? kept.nbytes() : 0, r.dq.data_ptr(), r.dk.data_ptr(),
                         r.dv.data_ptr(), static_cast<float*>(data(r.dfreqs)), static_cast<float*>(data(r.dbias)), static_cast<float*>(data(r.dinitial)), data(ws), n[1],
                         stream_of(a.q)),
         "linear attention backward");
@@ -163,14 +166,15 @@ using Grads6 = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
 struct LinearFn : torch::autograd::Function<LinearFn> {
   // every tensor is passed, undefined where there is none, so that inputs keep their numbers
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, OptTensor freqs, OptTensor bias, OptTensor initial,
-                               OptTensor log_decay, OptTensor mask, OptTensor cu, double scale, bool with_state, bool head_first) {
-    const LinearArgs raw{q, k, v, opt(freqs), opt(bias), opt(log_decay), opt(mask), opt(cu), opt(initial), scale, with_state, head_first};
+                               OptTensor log_decay, OptTensor mask, OptTensor cu, double scale, bool with_state, bool head_first, bool o_f32) {
+    const LinearArgs raw{q, k, v, opt(freqs), opt(bias), opt(log_decay), opt(mask), opt(cu), opt(initial), scale, with_state, head_first, o_f32};
     const LinearArgs a = raw.convert();
     const LinearOut r = linear_forward(a);
-    ctx->save_for_backward({q, k, v, raw.freqs, raw.bias, raw.initial, a.log_decay, a.mask, a.cu, r.states});
+    ctx->save_for_backward({q, k, v, raw.freqs, raw.bias, raw.initial, a.log_decay, a.mask, a.cu, r.kept});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["with_state"] = with_state;
     ctx->saved_data["head_first"] = head_first;
+    ctx->saved_data["o_f32"] = o_f32;
     // which gradients an undefined input would shift: positions of the optional inputs among the node's
     int64_t at = 3;
     for (const auto& [name, t] : {std::pair<const char*, Tensor>{"freqs", raw.freqs}, {"bias", raw.bias}, {"initial", raw.initial}}) {
@@ -184,7 +188,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list sv = ctx->get_saved_variables();
     const bool hf = ctx->saved_data["head_first"].toBool();
-    const LinearArgs raw{sv[0], sv[1], sv[2], sv[3], sv[4], sv[6], sv[7], sv[8], sv[5], ctx->saved_data["scale"].toDouble(), ctx->saved_data["with_state"].toBool(), hf};
+    const LinearArgs raw{sv[0], sv[1], sv[2], sv[3], sv[4], sv[6], sv[7], sv[8], sv[5], ctx->saved_data["scale"].toDouble(), ctx->saved_data["with_state"].toBool(), hf, ctx->saved_data["o_f32"].toBool()};
     const auto need = [&](const char* name) {
       const int64_t at = ctx->saved_data[name].toInt();
       return at >= 0 && ctx->needs_input_grad(at);
@@ -196,19 +200,19 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
       const auto front = [&](const Tensor& t) { return hf || !t.defined() ? t : t.transpose(1, 2); };
       const auto maybe = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
       const auto f32 = [](const Tensor& t) { return t.defined() ? t.to(at::kFloat) : t; };
-      const Tensor dout = grads[0].defined() ? front(grads[0]) : at::zeros({sv[0].size(0), front(sv[0]).size(1), front(sv[0]).size(2), sv[2].size(3)}, sv[0].options().requires_grad(false));
+      const Tensor dout = grads[0].defined() ? front(grads[0]) : at::zeros({sv[0].size(0), front(sv[0]).size(1), front(sv[0]).size(2), sv[2].size(3)}, sv[0].options().dtype(raw.o_type()).requires_grad(false));
       using O = OptTensor;
       std::tie(r.dq, r.dk, r.dv, r.dfreqs, r.dbias, r.dinitial) =
-          op<Grads6(const Tensor&, O, const Tensor&, const Tensor&, const Tensor&, O, O, O, O, O, O, O, double, bool, bool, bool)>("pope_amd::linear_bwd")
+          op<Grads6(const Tensor&, O, const Tensor&, const Tensor&, const Tensor&, O, O, O, O, O, O, O, double, bool, bool, bool, bool)>("pope_amd::linear_bwd")
               .call(dout, maybe(dlast), front(sv[0]), front(sv[1]), front(sv[2]), maybe(f32(sv[3])), maybe(f32(sv[4])), maybe(sv[6]), maybe(sv[7]), maybe(sv[8]),
-                    maybe(f32(sv[5])), maybe(sv[9]), raw.scale, ndf, ndb, nd0);
+                    maybe(f32(sv[5])), maybe(sv[9]), raw.scale, raw.o_f32, ndf, ndb, nd0);
       r.dq = front(r.dq), r.dk = front(r.dk), r.dv = front(r.dv);
     } else {
       r = linear_backward(raw.convert(), grads[0], dlast, sv[9], ndf, ndb, nd0);
     }
     const auto like = [](const Tensor& g, const Tensor& t, bool want) { return want ? (g.scalar_type() == t.scalar_type() ? g : g.to(t.scalar_type())) : Tensor(); };
     variable_list out{r.dq, r.dk, r.dv, like(r.dfreqs, sv[3], ndf), like(r.dbias, sv[4], ndb), like(r.dinitial, sv[5], nd0)};
-    out.resize(12);
+    out.resize(13);
     return on_ops(grads) ? out : once_differentiable(std::move(out), "linear attention");
   }
 };
@@ -216,12 +220,12 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
 // (o, last or nothing); nothing at all where the call is not as the kernels take it.
 std::optional<std::pair<Tensor, std::optional<Tensor>>> linear_eager(const Tensor& q, const Tensor& k, const Tensor& v, OptTensor freqs, OptTensor bias,
                                                                      OptTensor log_decay, OptTensor mask, OptTensor cu, OptTensor initial, double scale,
-                                                                     bool with_state, bool head_first) {
-  const LinearArgs a{q, k, v, opt(freqs), opt(bias), opt(log_decay), opt(mask), opt(cu), opt(initial), scale, with_state, head_first};
+                                                                     bool with_state, bool head_first, bool o_f32) {
+  const LinearArgs a{q, k, v, opt(freqs), opt(bias), opt(log_decay), opt(mask), opt(cu), opt(initial), scale, with_state, head_first, o_f32};
   if (!a.fits()) return std::nullopt;
   const auto maybe = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
   if (tracked({a.q, a.k, a.v, a.freqs, a.bias, a.initial})) {
-    const variable_list r = LinearFn::apply(q, k, v, freqs, bias, initial, log_decay, mask, cu, scale, with_state, head_first);
+    const variable_list r = LinearFn::apply(q, k, v, freqs, bias, initial, log_decay, mask, cu, scale, with_state, head_first, o_f32);
     return std::make_pair(r[0], with_state ? maybe(r[1]) : std::nullopt);
   }
   const LinearOut r = linear_forward(a.convert());
@@ -230,18 +234,18 @@ std::optional<std::pair<Tensor, std::optional<Tensor>>> linear_eager(const Tenso
 
 // The ops' implementations: head-first rows.  Nothing is undefined in what an op returns.
 std::tuple<Tensor, Tensor, Tensor> linear_fwd_impl(const Tensor& q, const Tensor& k, const Tensor& v, OptTensor freqs, OptTensor bias, OptTensor log_decay, OptTensor mask,
-                                                   OptTensor cu, OptTensor initial, double scale, bool with_state) {
-  const LinearArgs a{q, k, v, opt(freqs), opt(bias), opt(log_decay), opt(mask), opt(cu), opt(initial), scale, with_state, true};
+                                                   OptTensor cu, OptTensor initial, double scale, bool with_state, bool o_f32) {
+  const LinearArgs a{q, k, v, opt(freqs), opt(bias), opt(log_decay), opt(mask), opt(cu), opt(initial), scale, with_state, true, o_f32};
   check_linear_operands(a);
   const LinearOut r = linear_forward(a.convert());
-  return {r.o, r.last.defined() ? r.last : fp32_like(q, {0}), r.states.defined() ? r.states : at::empty({0}, q.options().dtype(at::kByte).requires_grad(false))};
+  return {r.o, r.last.defined() ? r.last : fp32_like(q, {0}), r.kept};
 }
 
 Grads6 linear_bwd_impl(const Tensor& dout, OptTensor dlast, const Tensor& q, const Tensor& k, const Tensor& v, OptTensor freqs, OptTensor bias, OptTensor log_decay,
-                       OptTensor mask, OptTensor cu, OptTensor initial, OptTensor states, double scale, bool need_df, bool need_db, bool need_d0) {
-  const LinearArgs a{q, k, v, opt(freqs), opt(bias), opt(log_decay), opt(mask), opt(cu), opt(initial), scale, false, true};
+                       OptTensor mask, OptTensor cu, OptTensor initial, OptTensor kept, double scale, bool o_f32, bool need_df, bool need_db, bool need_d0) {
+  const LinearArgs a{q, k, v, opt(freqs), opt(bias), opt(log_decay), opt(mask), opt(cu), opt(initial), scale, false, true, o_f32};
   check_linear_operands(a);
-  const LinearGrads r = linear_backward(a.convert(), dout, opt(dlast), opt(states), need_df, need_db, need_d0);
+  const LinearGrads r = linear_backward(a.convert(), dout, opt(dlast), opt(kept), need_df, need_db, need_d0);
   const auto some = [&](const Tensor& t) { return t.defined() ? t : fp32_like(q, {0}); };
   return {r.dq, r.dk, r.dv, some(r.dfreqs), some(r.dbias), some(r.dinitial)};
 }
@@ -296,7 +300,7 @@ struct StepArgs {
     const LinearArgs c = a.convert();
     pope_linear d = c.desc();
     const c10::DeviceGuard guard(a.q.device());
-    const Tensor o = c.rows(d.Hq, d.Dv);
+    const Tensor o = c.rows(d.Hq, d.Dv, c.o_type());
     c.strides(d.o_s, o);
     pope_gated_norm n{};
     if (gate.defined()) {
@@ -335,15 +339,17 @@ struct NormArgs {
   int h() const { return head_first ? 1 : 2; }
   int n() const { return head_first ? 2 : 1; }
   bool fits() const {
-    if (!x.is_cuda() || x.dim() != 4 || (x.scalar_type() != at::kHalf && x.scalar_type() != at::kBFloat16) || gate.device() != x.device() ||
-        gate.scalar_type() != x.scalar_type() || gate.sizes() != x.sizes() || x.size(3) < 1 || x.size(3) > 512 || x.size(h()) < 1)
+    const at::ScalarType t = gate.scalar_type();
+    if (!x.is_cuda() || x.dim() != 4 || (t != at::kFloat && t != at::kHalf && t != at::kBFloat16) || gate.device() != x.device() ||
+        (x.scalar_type() != t && x.scalar_type() != at::kFloat) || gate.sizes() != x.sizes() || x.size(3) < 1 || x.size(3) > 512 || x.size(h()) < 1)
       return false;
-    return weight_fits(weight, x, x.size(h()), x.size(3));
+    return weight_fits(weight, gate, x.size(h()), x.size(3));
   }
   void strides(int64_t* s, const Tensor& t) const { s[0] = t.stride(0), s[1] = t.stride(h()), s[2] = t.stride(n()); }
   pope_gated_norm desc() const {   // x and gate of unit feature stride
     TORCH_CHECK_VALUE(x.size(0) <= INT_MAX && x.size(1) <= INT_MAX && x.size(2) <= INT_MAX, "pope_amd gated norm: too large");
-    pope_gated_norm d = norm_desc(weight, x.size(3), eps, dtype_code(x));
+    pope_gated_norm d = norm_desc(weight, x.size(3), eps, dtype_code(gate));
+    d.x_f32 = x.scalar_type() == at::kFloat;
     d.B = (int32_t)x.size(0), d.H = (int32_t)x.size(h()), d.N = (int32_t)x.size(n());
     strides(d.x_s, x);
     strides(d.gate_s, gate);
@@ -355,7 +361,7 @@ struct NormArgs {
 Tensor norm_forward(const NormArgs& a) {
   pope_gated_norm d = a.desc();
   const c10::DeviceGuard guard(a.x.device());
-  const Tensor y = rows_like(a.x);
+  const Tensor y = rows_like(a.x, a.gate.scalar_type());
   a.strides(d.y_s, y);
   check(pope_gated_norm_fwd(&d, a.x.data_ptr(), a.gate.data_ptr(), data(a.weight), y.data_ptr(), stream_of(a.x)), "gated norm");
   return y;
@@ -364,7 +370,7 @@ Tensor norm_forward(const NormArgs& a) {
 variable_list norm_backward(const NormArgs& a, Tensor dy, bool need_dw) {
   pope_gated_norm d = a.desc();
   const c10::DeviceGuard guard(a.x.device());
-  if (dy.scalar_type() != a.x.scalar_type()) dy = dy.to(a.x.scalar_type());
+  if (dy.scalar_type() != a.gate.scalar_type()) dy = dy.to(a.gate.scalar_type());
   dy = unit_feature(dy);
   check_device(a.x, {&dy});
   TORCH_CHECK_VALUE(dy.sizes() == a.x.sizes(), "dy ", dy.sizes(), " must match x ", a.x.sizes());

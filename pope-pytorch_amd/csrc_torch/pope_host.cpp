@@ -770,8 +770,8 @@ using OptTensor = const std::optional<Tensor>&;
 
 // Rows like q's, of unit feature stride: empty_like() may put another dim last where q's rows overlap (a window that
 // slides by one element has two dims of stride 1).
-Tensor rows_like(const Tensor& q) {
-  const auto opt = q.options().requires_grad(false);
+Tensor rows_like(const Tensor& q, std::optional<at::ScalarType> dtype = std::nullopt) {
+  const auto opt = q.options().dtype(dtype.value_or(q.scalar_type())).requires_grad(false);
   const Tensor o = at::empty_like(q, opt);
   return o.stride(-1) == 1 ? o : at::empty(q.sizes(), opt);
 }

@@ -64,9 +64,9 @@ class PopeLinear(ctypes.Structure):
 
     _fields_ = [
         ("B", ctypes.c_int32), ("N", ctypes.c_int32), ("Hq", ctypes.c_int32), ("Hk", ctypes.c_int32), ("D", ctypes.c_int32),
-        ("R", ctypes.c_int32), ("Dv", ctypes.c_int32), ("dtype", ctypes.c_int32), ("scale", ctypes.c_float),
-        ("q_s", _I64x3), ("k_s", _I64x3), ("v_s", _I64x3), ("o_s", _I64x3), ("do_s", _I64x3), ("dq_s", _I64x3), ("dk_s", _I64x3),
-        ("dv_s", _I64x3), ("f_s", ctypes.c_int64 * 2), ("bias_sh", ctypes.c_int64), ("df_s", ctypes.c_int64 * 2), ("mask_sb", ctypes.c_int64),
+        ("R", ctypes.c_int32), ("Dv", ctypes.c_int32), ("dtype", ctypes.c_int32), ("o_f32", ctypes.c_int32),
+        ("scale", ctypes.c_float), ("q_s", _I64x3), ("k_s", _I64x3), ("v_s", _I64x3), ("o_s", _I64x3), ("do_s", _I64x3), ("dq_s", _I64x3),
+        ("dk_s", _I64x3), ("dv_s", _I64x3), ("f_s", ctypes.c_int64 * 2), ("bias_sh", ctypes.c_int64), ("df_s", ctypes.c_int64 * 2), ("mask_sb", ctypes.c_int64),
     ]
 
 
@@ -75,7 +75,7 @@ class PopeGatedNorm(ctypes.Structure):
 
     _fields_ = [
         ("B", ctypes.c_int32), ("H", ctypes.c_int32), ("N", ctypes.c_int32), ("cols", ctypes.c_int32), ("dtype", ctypes.c_int32),
-        ("weight_rows", ctypes.c_int32), ("weight_f32", ctypes.c_int32), ("eps", ctypes.c_float), ("x_s", _I64x3), ("gate_s", _I64x3),
+        ("x_f32", ctypes.c_int32), ("weight_rows", ctypes.c_int32), ("weight_f32", ctypes.c_int32), ("eps", ctypes.c_float), ("x_s", _I64x3), ("gate_s", _I64x3),
         ("y_s", _I64x3), ("dy_s", _I64x3), ("dx_s", _I64x3), ("dgate_s", _I64x3), ("weight_sh", ctypes.c_int64),
     ]
 

@@ -14,7 +14,7 @@ head h % heads, as in the softmax attention here.
   gated_head_norm              y = x / sqrt(mean x^2 + eps) * weight * silu(gate) over each head's row: no softmax bounds the
                                outputs, so layers of this kind norm and gate them; both calls above take ``gate``
 
-Rows are bf16 or fp16, (batch, heads, n, dim) or (batch, n, heads, dim) with ``head_dimension_at_first=False``; dim and the value
+Rows are bf16, fp16 or fp32, (batch, heads, n, dim) or (batch, n, heads, dim) with ``head_dimension_at_first=False``; dim and the value
 dim go up to 256, of any size.  A sequence goes on from a state with any split of its rows over calls: positions come from
 ``pos_emb``, ``pope(positions)``, one row of angles per row.
 
@@ -33,7 +33,7 @@ from torch.autograd import forward_ad
 
 from . import _lib
 
-_DTYPES = (torch.bfloat16, torch.float16)
+_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 _MAX_DIM, _MAX_NORM = 256, 512
 _CHUNK = 128   # rows that the CPU computation takes at once
 
@@ -61,7 +61,7 @@ def _check_rows(q: Tensor, k: Tensor, v: Tensor):
         if t.ndim != 4:
             raise ValueError(f"{name} must be 4-D, got {tuple(t.shape)}")
         if t.dtype not in _DTYPES or t.dtype != q.dtype:
-            raise TypeError(f"q, k, v must be all bfloat16 or all float16, got {name} of dtype {t.dtype}")
+            raise TypeError(f"q, k, v must be all bfloat16, all float16 or all float32, got {name} of dtype {t.dtype}")
     if k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or k.shape[3] != q.shape[3] or v.shape[:3] != k.shape[:3]:
         raise ValueError(f"incompatible q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} (batch, heads, n, dim)")
     if k.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k.shape[1]:
@@ -128,8 +128,8 @@ def _ints(name: str, t: Tensor, q: Tensor, n: int):
 def _check_norm(x: Tensor, gate: Tensor, weight: Optional[Tensor], heads: int):
     if x.ndim != 4:
         raise ValueError(f"x must be 4-D, got {tuple(x.shape)}")
-    if x.dtype not in _DTYPES or gate.dtype != x.dtype:
-        raise TypeError(f"x and gate must be both bfloat16 or both float16, got {x.dtype} and {gate.dtype}")
+    if gate.dtype not in _DTYPES or x.dtype not in (gate.dtype, torch.float32):
+        raise TypeError(f"gate must be bfloat16, float16 or float32, and x of its dtype or float32, got {gate.dtype} and {x.dtype}")
     if gate.shape != x.shape:
         raise ValueError(f"gate {tuple(gate.shape)} must match x {tuple(x.shape)}")
     _check_device(x, gate=gate, weight=weight)
@@ -140,8 +140,8 @@ def _check_norm(x: Tensor, gate: Tensor, weight: Optional[Tensor], heads: int):
     if exists(weight):
         if weight.ndim not in (1, 2) or weight.shape[-1] != x.shape[3] or (weight.ndim == 2 and weight.shape[0] not in (1, heads)):
             raise ValueError(f"weight {tuple(weight.shape)} must be ({x.shape[3]},) or (1 or {heads}, {x.shape[3]})")
-        if weight.dtype not in (x.dtype, torch.float32):
-            raise TypeError(f"weight must be {x.dtype} or float32, got {weight.dtype}")
+        if weight.dtype not in (gate.dtype, torch.float32):
+            raise TypeError(f"weight must be {gate.dtype} or float32, got {weight.dtype}")
 
 
 # ---------------------------------------------------------------- ops (tracing); eager calls take the same native calls
@@ -149,8 +149,8 @@ def _check_norm(x: Tensor, gate: Tensor, weight: Optional[Tensor], heads: int):
 
 @torch.library.custom_op("pope_amd::linear_fwd", mutates_args=(), device_types="cuda")
 def linear_fwd_op(q: Tensor, k: Tensor, v: Tensor, freqs: Optional[Tensor], bias: Optional[Tensor], log_decay: Optional[Tensor], mask: Optional[Tensor],
-                  cu_seqlens: Optional[Tensor], initial: Optional[Tensor], scale: float, with_state: bool) -> tuple[Tensor, Tensor, Tensor]:
-    return _lib.host().linear_fwd(q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial, scale, with_state)
+                  cu_seqlens: Optional[Tensor], initial: Optional[Tensor], scale: float, with_state: bool, o_f32: bool) -> tuple[Tensor, Tensor, Tensor]:
+    return _lib.host().linear_fwd(q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial, scale, with_state, o_f32)
 
 
 def _linear_state_shape(q, k, v, freqs, cu_seqlens):
@@ -158,43 +158,43 @@ def _linear_state_shape(q, k, v, freqs, cu_seqlens):
 
 
 @linear_fwd_op.register_fake
-def _(q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial, scale, with_state):
-    o = q.new_empty((*q.shape[:3], v.shape[3]))
+def _(q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial, scale, with_state, o_f32):
+    o = q.new_empty((*q.shape[:3], v.shape[3]), dtype=torch.float32 if o_f32 else q.dtype)
     last = q.new_empty(_linear_state_shape(q, k, v, freqs, cu_seqlens) if with_state else (0,), dtype=torch.float32)
-    # the states of segments: as many bytes as the library says
+    # what the backward reads: as many bytes as the library says
     n = torch.library.get_ctx().new_dynamic_size()
     return o, last, q.new_empty((n,), dtype=torch.uint8)
 
 
 @torch.library.custom_op("pope_amd::linear_bwd", mutates_args=(), device_types="cuda")
 def linear_bwd_op(dout: Tensor, dlast: Optional[Tensor], q: Tensor, k: Tensor, v: Tensor, freqs: Optional[Tensor], bias: Optional[Tensor],
-                  log_decay: Optional[Tensor], mask: Optional[Tensor], cu_seqlens: Optional[Tensor], initial: Optional[Tensor], states: Optional[Tensor],
-                  scale: float, need_dfreqs: bool, need_dbias: bool, need_dinitial: bool) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
-    return _lib.host().linear_bwd(dout, dlast, q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial, states, scale, need_dfreqs, need_dbias,
-                                  need_dinitial)
+                  log_decay: Optional[Tensor], mask: Optional[Tensor], cu_seqlens: Optional[Tensor], initial: Optional[Tensor], kept: Optional[Tensor],
+                  scale: float, o_f32: bool, need_dfreqs: bool, need_dbias: bool, need_dinitial: bool) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    return _lib.host().linear_bwd(dout, dlast, q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial, kept, scale, o_f32, need_dfreqs,
+                                  need_dbias, need_dinitial)
 
 
 @linear_bwd_op.register_fake
-def _(dout, dlast, q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial, states, scale, need_dfreqs, need_dbias, need_dinitial):
+def _(dout, dlast, q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial, kept, scale, o_f32, need_dfreqs, need_dbias, need_dinitial):
     some = lambda shape, want: q.new_empty(shape if want else (0,), dtype=torch.float32)
     return (q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape), some(freqs.shape if need_dfreqs else (0,), need_dfreqs),
             some(bias.shape if need_dbias else (0,), need_dbias), some(_linear_state_shape(q, k, v, freqs, cu_seqlens), need_dinitial))
 
 
 def _linear_setup(ctx, inputs, output):
-    q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial, ctx.scale, ctx.with_state = inputs
+    q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial, ctx.scale, ctx.with_state, ctx.o_f32 = inputs
     ctx.save_for_backward(q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial, output[2])
     ctx.set_materialize_grads(False)
 
 
-def _linear_backward(ctx, dout, dlast, dstates):
-    q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial, states = ctx.saved_tensors
+def _linear_backward(ctx, dout, dlast, dkept):
+    q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial, kept = ctx.saved_tensors
     need = ctx.needs_input_grad
     if dout is None:
-        dout = q.new_zeros((*q.shape[:3], v.shape[3]))
-    dq, dk, dv, df, db, d0 = linear_bwd_op(dout, dlast if ctx.with_state else None, q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial, states,
-                                           ctx.scale, need[3], need[4], need[8])
-    return dq, dk, dv, df if need[3] else None, db if need[4] else None, None, None, None, d0 if need[8] else None, None, None
+        dout = q.new_zeros((*q.shape[:3], v.shape[3]), dtype=torch.float32 if ctx.o_f32 else q.dtype)
+    dq, dk, dv, df, db, d0 = linear_bwd_op(dout, dlast if ctx.with_state else None, q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial, kept,
+                                           ctx.scale, ctx.o_f32, need[3], need[4], need[8])
+    return dq, dk, dv, df if need[3] else None, db if need[4] else None, None, None, None, d0 if need[8] else None, None, None, None
 
 
 linear_fwd_op.register_autograd(_linear_backward, setup_context=_linear_setup)
@@ -217,14 +217,14 @@ def gated_norm_fwd_op(x: Tensor, gate: Tensor, weight: Optional[Tensor], eps: fl
     return _lib.host().gated_norm_fwd(x, gate, weight, eps, head_first)
 
 
-def _rows_like(x):   # rows_like of csrc_torch/pope_host.cpp
-    y = torch.empty_like(x)
-    return y if y.stride(-1) == 1 else x.new_empty(x.shape)
+def _rows_like(x, dtype=None):   # rows_like of csrc_torch/pope_host.cpp
+    y = torch.empty_like(x, dtype=dtype)
+    return y if y.stride(-1) == 1 else x.new_empty(x.shape, dtype=dtype)
 
 
 @gated_norm_fwd_op.register_fake
 def _(x, gate, weight, eps, head_first):
-    return _rows_like(x if x.stride(-1) == 1 else x.contiguous())
+    return _rows_like(x if x.stride(-1) == 1 else x.contiguous(), gate.dtype)
 
 
 @torch.library.custom_op("pope_amd::gated_norm_bwd", mutates_args=(), device_types="cuda")
@@ -258,8 +258,8 @@ gated_norm_fwd_op.register_autograd(_norm_backward, setup_context=_norm_setup)
 def gated_head_norm(x: Tensor, gate: Tensor, weight: Optional[Tensor] = None, *, eps: float = 1e-5, head_dimension_at_first: bool = True) -> Tensor:
     """x / sqrt(mean x^2 + eps) * weight * silu(gate) over the last dim of x (batch, heads, n, dim), dim 1 to 512, with autograd.
 
-    ``gate`` is shaped as x; ``weight`` (dim,) or (1 or heads, dim), of x's dtype or fp32, or None.  Arithmetic is fp32, rounded
-    once.  ``head_dimension_at_first`` says which dim a weight of several heads goes with."""
+    ``gate`` is shaped as x and has the result's dtype; x has that dtype or is fp32; ``weight`` (dim,) or (1 or heads, dim), of gate's
+    dtype or fp32, or None.  Arithmetic is fp32, rounded once.  ``head_dimension_at_first`` says which dim a weight of several heads goes with."""
     if x.is_cuda and _lib.eager(x, gate, weight):
         y = _lib.host().gated_norm_eager(x, gate, weight, eps, head_dimension_at_first)
         if exists(y):
@@ -296,9 +296,12 @@ def linear_attn_with_pope(q: Tensor, k: Tensor, v: Tensor, log_decay: Optional[T
     hf = bool(head_dimension_at_first)
     if exists(norm_weight) and not exists(gate):
         raise ValueError("norm_weight given without a gate")
+    # the norm divides by the size of a row, and a short row's own rounding would come out as large as that row is small: its
+    # input, and the gradient that comes back, are fp32
+    o_f32 = exists(gate)
     out = None
     if q.is_cuda and _lib.eager(q, k, v, freqs, bias, *args):
-        out = _lib.host().linear_eager(q, k, v, freqs, bias, *args, scale, return_state, hf)
+        out = _lib.host().linear_eager(q, k, v, freqs, bias, *args, scale, return_state, hf, o_f32)
     if exists(out):
         o, last = out
     else:
@@ -324,12 +327,12 @@ def linear_attn_with_pope(q: Tensor, k: Tensor, v: Tensor, log_decay: Optional[T
             _check_state("initial_state", initial_state, shape, q)
             initial_state = initial_state.float()
         if n == 0 or B == 0:
-            o = q.new_zeros((*q.shape[:3], v.shape[3]))
+            o = q.new_zeros((*q.shape[:3], v.shape[3]), dtype=torch.float32 if o_f32 else q.dtype)
             last = initial_state.clone() if exists(initial_state) else torch.zeros(shape, device=q.device)
         elif not q.is_cuda:
-            o, last = _linear_torch(q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial_state, scale, shape)
+            o, last = _linear_torch(q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial_state, scale, shape, torch.float32 if o_f32 else q.dtype)
         else:
-            o, last, _ = linear_fwd_op(q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial_state, scale, bool(return_state))
+            o, last, _ = linear_fwd_op(q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial_state, scale, bool(return_state), o_f32)
         if not hf:
             o = o.transpose(1, 2)
     if exists(gate):
@@ -394,7 +397,7 @@ def linear_attn_step_with_pope(q: Tensor, k: Tensor, v: Tensor, log_decay: Optio
     elif not q.is_cuda:
         o = _step_torch(q, k, v, freqs, bias, log_decay, state, state_index, new_index, scale)
         if exists(gate):
-            o = _norm_torch(o, gate, norm_weight, norm_eps, True, q.dtype)
+            o = _norm_torch(o, gate, norm_weight, norm_eps, True)
         o = o.to(q.dtype)
     else:
         o = linear_step_op(q, k, v, freqs, bias, log_decay, state, state_index, new_index, gate, norm_weight, float(norm_eps), scale)
@@ -403,12 +406,12 @@ def linear_attn_step_with_pope(q: Tensor, k: Tensor, v: Tensor, log_decay: Optio
 
 # ---------------------------------------------------------------- CPU tensors: torch operators, fp32
 
-def _norm_torch(x, gate, weight, eps, head_first, dtype=None):
+def _norm_torch(x, gate, weight, eps, head_first):
     y = x.float()
     y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + eps)
     if exists(weight):
         y = y * (weight.float()[:, None, :] if weight.ndim == 2 and head_first else weight.float())
-    return (y * F.silu(gate.float())).to(x.dtype if dtype is None else dtype)
+    return (y * F.silu(gate.float())).to(gate.dtype)
 
 
 def _expand(x: Tensor, freqs: Optional[Tensor], bias: Optional[Tensor]) -> Tensor:
@@ -425,7 +428,7 @@ def _expand(x: Tensor, freqs: Optional[Tensor], bias: Optional[Tensor]) -> Tenso
     return torch.cat((pairs, x[..., R:]), -1)
 
 
-def _linear_torch(q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial, scale, shape):
+def _linear_torch(q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial, scale, shape, dtype):
     G, Hk, n = q.shape[1] // k.shape[1], k.shape[1], q.shape[2]
     qh, kh, vf = _expand(q, freqs, None) * scale, _expand(k, freqs, bias), v.float()
     if exists(mask):
@@ -439,7 +442,7 @@ def _linear_torch(q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial, sc
         parts = [(0, cu[b], max(cu[b + 1], cu[b])) for b in range(len(cu) - 1)]
     else:
         parts = [(b, 0, n) for b in range(q.shape[0])]
-    o = q.new_zeros((*q.shape[:3], v.shape[3]))
+    o = q.new_zeros((*q.shape[:3], v.shape[3]), dtype=dtype)
     last, pieces = [], []
     for s, (b, lo, hi) in enumerate(parts):
         S = initial[s] if exists(initial) else torch.zeros(shape[1:])
