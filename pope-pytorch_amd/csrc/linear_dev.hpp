@@ -203,24 +203,49 @@ __device__ __forceinline__ void lin_set4(const LinRows& r, int64_t at, int d, f3
   }
   *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(r.p) + at + d) = u32x2{BF16::pack2(v[0], v[1]), BF16::pack2(v[2], v[3])};
 }
-// Two elements, at an even place of an aligned row.
+// Two elements, as they are in memory: at an even place of an aligned row (`whole`), or one by one, the second if it is there.
 template <int PL>
-__device__ __forceinline__ void lin_get2(const LinRows& r, int64_t at, float* v) {
+struct LinPair { uint32_t w; };
+template <>
+struct LinPair<kTwo> { uint32_t w, v; };   // v: the second of fp32 rows
+template <int PL>
+__device__ __forceinline__ LinPair<PL> lin_get2(const LinRows& r, int64_t at, bool whole, bool second) {
+  LinPair<PL> o{};
   if constexpr (PL == kTwo) {
     if (r.type == 0) {
-      const f32x2 x = *reinterpret_cast<const f32x2*>(static_cast<const float*>(r.p) + at);
-      v[0] = x[0], v[1] = x[1];
-      return;
+      const uint32_t* p = static_cast<const uint32_t*>(r.p) + at;
+      if (whole) {
+        const u32x2 w = *reinterpret_cast<const u32x2*>(p);
+        o.w = w[0], o.v = w[1];
+      } else {
+        o.w = p[0];
+        if (second) o.v = p[1];
+      }
+      return o;
     }
   }
-  const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(r.p) + at);
+  const uint16_t* p = static_cast<const uint16_t*>(r.p) + at;
+  if (whole) {
+    o.w = *reinterpret_cast<const uint32_t*>(p);
+  } else {
+    o.w = p[0];
+    if (second) o.w |= (uint32_t)p[1] << 16;
+  }
+  return o;
+}
+template <int PL>
+__device__ __forceinline__ void lin_unpack2(const LinPair<PL>& p, int type, float* v) {
   if constexpr (PL == kTwo) {
-    if (r.type == 1) {
-      v[0] = F16::to_float((uint16_t)w), v[1] = F16::to_float((uint16_t)(w >> 16));
+    if (type == 0) {
+      v[0] = __uint_as_float(p.w), v[1] = __uint_as_float(p.v);
+      return;
+    }
+    if (type == 1) {
+      v[0] = F16::to_float((uint16_t)p.w), v[1] = F16::to_float((uint16_t)(p.w >> 16));
       return;
     }
   }
-  v[0] = BF16::to_float((uint16_t)w), v[1] = BF16::to_float((uint16_t)(w >> 16));
+  v[0] = BF16::to_float((uint16_t)p.w), v[1] = BF16::to_float((uint16_t)(p.w >> 16));
 }
 template <int PL>
 __device__ __forceinline__ void lin_set2(const LinRows& r, int64_t at, float a, float b) {

@@ -79,12 +79,6 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
   float* later = reinterpret_cast<float*>(A.p + PL * A.plane);   // C: weights of a chunk's rows in the next state
   float* turns = later + C;                                      // kLinDk: 256
   int* odd = reinterpret_cast<int*>(turns + (chain ? 256 : 0));   // z of this chunk that are not finite; two, by turns
-  constexpr int kTileBytes = PL * (C * (K::XS + K::YS + K::ZS + K::AS)) * 2;
-  for (int i = tid; i < kTileBytes / 16; i += kThreads) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0, 0, 0, 0};
-  if (tid < 2) odd[tid] = 0;
-  if (kind == kLinDk)
-    for (int d = tid; d < c.R; d += kThreads) turns[d] = lin_turns(c.bias[hk * c.bias_sh + d]);
-
   const float lg = lin_log2(c, hk);
   const int a = rev ? 0 : 1;
   const int chunks = (seg.len + C - 1) / C;
@@ -92,36 +86,6 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
   const bool busy = n0 + col0 < ncols;
   const int steps = (pcols + 31) / 32;
 
-  // W: accumulators of 16-row tiles 4 q4 + i x columns l16
-  f32x4 W[CT][2 * ST];
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-    for (int s = 0; s < 2 * ST; ++s) W[ct][s] = f32x4{0.f, 0.f, 0.f, 0.f};
-  {
-    const float* from = p.states[rev] ? p.states[rev] + ((int64_t)at * c.Hk + hk) * c.E * c.Dv
-                        : p.first[rev] ? p.first[rev] + ((int64_t)seg.seq * c.Hk + hk) * c.E * c.Dv : nullptr;
-    if (from && busy) {
-      const bool whole = chain && c.Dv % 4 == 0 && (reinterpret_cast<uintptr_t>(from) & 15) == 0;
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        const int col = n0 + col0 + 16 * ct + l16;
-#pragma unroll
-        for (int s = 0; s < 2 * ST; ++s) {
-          const int row = 16 * s + 4 * q4;
-          if (whole) {   // transposed where the result has expanded columns
-            if (row < pcols && col < ncols) W[ct][s] = *reinterpret_cast<const f32x4*>(from + (int64_t)col * c.Dv + row);
-            continue;
-          }
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (row + r < pcols && col < ncols) W[ct][s][r] = chain ? from[(int64_t)col * c.Dv + row + r] : from[(int64_t)(row + r) * c.Dv + col];
-        }
-      }
-    }
-  }
-  const float keep = lin_power(lg, C);
-  for (int t = tid; t < C; t += kThreads) later[t] = lin_power(lg, C - a - t);
   float dbsum[CT][2];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) dbsum[ct][0] = dbsum[ct][1] = 0.f;
@@ -139,13 +103,16 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
     const int ch = it / ng, g = it - ch * ng;
     return Turn{ch * C, (g0 + g) * c.Hk + hk, by_query || g == 0, !by_query || g == 0};
   };
-  const auto kept = [&](int row) { return !c.mask || c.mask[(int64_t)seg.batch * c.mask_sb + row] != 0; };
-  // A thread's chunks of the tiles, read from memory.  What the mask leaves out is read too, so that no load waits for it.
-  struct Part { LinRaw<PL> w; bool keep; };
+  // Loads keep what they read as it is until it is put: a conversion, or a choice by a mask's byte, would wait for the load.  What the
+  // mask leaves out is read too.
+  const uint8_t* mask = c.mask ? c.mask + (int64_t)seg.batch * c.mask_sb : nullptr;
+  const auto kept = [&](int row) { return mask ? (uint32_t)mask[row] : 1u; };
+  // A thread's chunks of the tiles, read from memory.
+  struct Part { LinRaw<PL> w; uint32_t keep; };
   const auto get = [&](auto hat, auto key, const LinHat& t, const LinRows& r, int h, int cols, int t0, const Item& i, int d0) {
     Part o;
     o.w = LinRaw<PL>{};
-    o.keep = false;
+    o.keep = 0;
     if (t0 + i.row < seg.len && d0 < cols) {
       const int row = row_of(t0 + i.row);
       if constexpr (decltype(hat)::value) {
@@ -155,7 +122,7 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
       } else {
         o.w = lin_load8<PL>(r, (int64_t)seg.batch * r.s[0] + (int64_t)h * r.s[1] + (int64_t)row * r.s[2], d0);
       }
-      o.keep = !decltype(key)::value || kept(row);
+      o.keep = decltype(key)::value ? kept(row) : 1u;
     }
     return o;
   };
@@ -172,9 +139,9 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
     return get(Bool<z_hat>{}, Bool<z_key>{}, zh, zr, by_query ? hk : n.hq, i.d0 < NT ? zcols : 0, n.t0, i, n0 + i.d0);
   };
   // ... and put into LDS
-  const auto put = [&](auto hat, auto perm, const LinRows& r, const LinTile& t, const Item& i, Part o) {
+  const auto put = [&](auto hat, auto key, auto perm, const LinRows& r, const LinTile& t, const Item& i, Part o) {
     constexpr bool kPerm = decltype(perm)::value;
-    if (!o.keep) o.w = LinRaw<PL>{};
+    if (decltype(key)::value && !o.keep) o.w = LinRaw<PL>{};
     if constexpr (!decltype(hat)::value) {
       return lin_put_plain<PL, kPerm>(t, i.row, i.d0, o.w, r.type);
     } else {
@@ -189,15 +156,15 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
   };
   const auto put_x = [&](int u, const Part& o) {
     const Item i(u);
-    if (i.d0 < xcols) put(Bool<x_hat>{}, Bool<true>{}, xr, X, i, o);
+    if (i.d0 < xcols) put(Bool<x_hat>{}, Bool<x_key>{}, Bool<true>{}, xr, X, i, o);
   };
   const auto put_y = [&](int u, const Part& o) {
     const Item i(u);
-    if (i.d0 < ycols) put(Bool<y_hat>{}, Bool<false>{}, yr, Y, i, o);
+    if (i.d0 < ycols) put(Bool<y_hat>{}, Bool<y_key>{}, Bool<false>{}, yr, Y, i, o);
   };
   const auto put_z = [&](int u, const Part& o) {
     const Item i(u);
-    return i.d0 < NT && n0 + i.d0 < zcols && put(Bool<z_hat>{}, Bool<false>{}, zr, Z, i, o);
+    return i.d0 < NT && n0 + i.d0 < zcols && put(Bool<z_hat>{}, Bool<z_key>{}, Bool<false>{}, zr, Z, i, o);
   };
   // Narrow tiles are loaded a chunk ahead, into registers; wide ones, whose state takes those, chunk by chunk.
   constexpr bool kAhead = P <= 128 && NT <= 128;
@@ -250,6 +217,42 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
   const int turns_n = chunks * ng;
   bool odd_z = false;
   load(0);
+  // W: accumulators of 16-row tiles 4 q4 + i x columns l16
+  f32x4 W[CT][2 * ST];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+    for (int s = 0; s < 2 * ST; ++s) W[ct][s] = f32x4{0.f, 0.f, 0.f, 0.f};
+  {
+    const float* from = p.states[rev] ? p.states[rev] + ((int64_t)at * c.Hk + hk) * c.E * c.Dv
+                        : p.first[rev] ? p.first[rev] + ((int64_t)seg.seq * c.Hk + hk) * c.E * c.Dv : nullptr;
+    if (from && busy) {
+      const bool whole = chain && c.Dv % 4 == 0 && (reinterpret_cast<uintptr_t>(from) & 15) == 0;
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        const int col = n0 + col0 + 16 * ct + l16;
+#pragma unroll
+        for (int s = 0; s < 2 * ST; ++s) {
+          const int row = 16 * s + 4 * q4;
+          if (whole) {   // transposed where the result has expanded columns
+            if (row < pcols && col < ncols) W[ct][s] = *reinterpret_cast<const f32x4*>(from + (int64_t)col * c.Dv + row);
+            continue;
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (row + r < pcols && col < ncols) W[ct][s][r] = chain ? from[(int64_t)col * c.Dv + row + r] : from[(int64_t)(row + r) * c.Dv + col];
+        }
+      }
+    }
+  }
+  const float keep = lin_power(lg, C);
+  for (int t = tid; t < C; t += kThreads) later[t] = lin_power(lg, C - a - t);
+  constexpr int kTileBytes = PL * (C * (K::XS + K::YS + K::ZS + K::AS)) * 2;
+  for (int i = tid; i < kTileBytes / 16; i += kThreads) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0, 0, 0, 0};
+  if (tid < 2) odd[tid] = 0;
+  if (kind == kLinDk)
+    for (int d = tid; d < c.R; d += kThreads) turns[d] = lin_turns(c.bias[hk * c.bias_sh + d]);
+
   for (int it = 0; it < turns_n; ++it) {
     const int ch = it / ng, g = it - ch * ng, t0 = ch * C;
     __syncthreads();   // nothing reads the tiles any more
@@ -295,11 +298,12 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
     // what the chain rule of this turn's rows reads, ahead: a lane has row 16 i + l16, and, of each 16 columns, two dims
     const bool ends = by_query || g == ng - 1;
     const bool pairs = out.vec && (kind == kLinDq ? c.q : c.k).vec && c.f_vec;   // two dims at a time: R, D multiples of 8
-    float cx[CT][IT][2], cf[CT][IT][2];
-    bool live[IT];
+    LinPair<PL> cx[CT][IT];
+    f32x2 cf[CT][IT];
+    uint32_t live[IT];
     if constexpr (rev) {
 #pragma unroll
-      for (int i = 0; i < IT; ++i) live[i] = !busy || !ends || kept(row_of(min(t0 + 16 * i + l16, seg.len - 1)));
+      for (int i = 0; i < IT; ++i) live[i] = busy && ends ? kept(row_of(min(t0 + 16 * i + l16, seg.len - 1))) : 1u;
     }
     if constexpr (chain) {
       if (busy && ends) {
@@ -311,18 +315,17 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct) {
             const int d = (n0 + col0 + 16 * ct + 4 * q4) >> 1;
-            cx[ct][i][0] = cx[ct][i][1] = cf[ct][i][0] = cf[ct][i][1] = 0.f;
+            cx[ct][i] = LinPair<PL>{};
+            cf[ct][i] = f32x2{0.f, 0.f};
             if (d >= c.R) continue;
             const int64_t at = base + (int64_t)row * in.s[2] + d;
             const float* fr = lin_angle_row(c, seg.batch, row) + d;
+            cx[ct][i] = lin_get2<PL>(in, at, pairs, d + 1 < c.R);
             if (pairs) {
-              lin_get2<PL>(in, at, cx[ct][i]);
-              const f32x2 f2 = *reinterpret_cast<const f32x2*>(fr);
-              cf[ct][i][0] = f2[0], cf[ct][i][1] = f2[1];
+              cf[ct][i] = *reinterpret_cast<const f32x2*>(fr);
             } else {
-#pragma unroll
-              for (int pr = 0; pr < 2; ++pr)
-                if (d + pr < c.R) cx[ct][i][pr] = lin_get<PL>(in, at + pr), cf[ct][i][pr] = fr[pr];
+              cf[ct][i][0] = fr[0];
+              if (d + 1 < c.R) cf[ct][i][1] = fr[1];
             }
           }
         }
@@ -466,19 +469,21 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
             float* ph = p.dphase[which] ? p.dphase[which] + (((int64_t)seg.batch * (kind == kLinDq ? c.Hq : c.Hk) + h) * c.seqs.N + row) * c.R : nullptr;
             const bool dead = rev && !live[i];
             const float f = kind == kLinDq ? c.scale : 1.f;
+            const int in_type = kind == kLinDq ? c.q.type : c.k.type;
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
               const int e0 = n0 + col0 + 16 * ct + 4 * q4;
               f32x4 v = O[ct][i] * f;
               if (dead) v = f32x4{0.f, 0.f, 0.f, 0.f};
-              float dx[2];
+              float dx[2], x2[2];
+              lin_unpack2<PL>(cx[ct][i], in_type, x2);
 #pragma unroll
               for (int pr = 0; pr < 2; ++pr) {
                 const int e = e0 + 2 * pr;
                 const float dc = v[2 * pr], ds = v[2 * pr + 1];
                 if (e < 2 * c.R) {
                   const int d = e >> 1;
-                  const float x = cx[ct][i][pr];
+                  const float x = x2[pr];
                   float sn, cs;
                   sincos_turns(cf[ct][i][pr], kind == kLinDk ? turns[d] : 0.f, &sn, &cs);
                   dx[pr] = dead ? 0.f : sigmoid_f(x) * (dc * cs + ds * sn);

@@ -95,7 +95,7 @@ __global__ __launch_bounds__(K::kThreads, 1) void linear_state_kernel(LinStatePa
   const int ty = (C * ((c.D + 31) / 32 * 4) + K::kThreads - 1) / K::kThreads;
   const int tz = (C * ((min(NT, c.Dv - n0) + 31) / 32 * 4) + K::kThreads - 1) / K::kThreads;
   typedef LinItem<C, K::kThreads> Item;
-  const auto kept = [&](int row) { return rev || !c.mask || c.mask[(int64_t)seg.batch * c.mask_sb + row] != 0; };
+  const auto kept = [&](int row) { return rev || !c.mask ? 1u : (uint32_t)c.mask[(int64_t)seg.batch * c.mask_sb + row]; };
   for (int t0 = 0; t0 < seg.len; t0 += C)
     for (int g = 0; g < G; ++g) {
       const int h = rev ? g * c.Hk + hk : hk;
@@ -110,7 +110,7 @@ __global__ __launch_bounds__(K::kThreads, 1) void linear_state_kernel(LinStatePa
         if (i.d0 >= c.D) continue;
         LinRaw<PL> x{};
         f32x4 f[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-        bool live = in;
+        uint32_t live = in;
         if (in) {   // what the mask leaves out is read too, so that no load waits for it
           x = lin_load8<PL>(yr, (int64_t)seg.batch * yr.s[0] + (int64_t)h * yr.s[1] + (int64_t)row * yr.s[2], i.d0);
           if (c.R) lin_angles8(lin_angle_row(c, seg.batch, row), i.d0, c.R, c.f_vec, f);
@@ -194,9 +194,9 @@ __global__ __launch_bounds__(K::kThreads, K::P <= 128 && K::NT <= 128 ? 2 : K::N
   const LinHat yh = rev ? c.qh : c.kh;
   const LinRows zr = rev ? c.g : c.v;
   typedef LinItem<C, K::kThreads> Item;
-  const auto kept = [&](int row) { return rev || !c.mask || c.mask[(int64_t)seg.batch * c.mask_sb + row] != 0; };
+  const auto kept = [&](int row) { return rev || !c.mask ? 1u : (uint32_t)c.mask[(int64_t)seg.batch * c.mask_sb + row]; };
   struct InY { u32x4 w[PY]; };
-  struct InZ { LinRaw<PL> x; bool live; };   // what the mask leaves out is read too, so that no load waits for it
+  struct InZ { LinRaw<PL> x; uint32_t live; };   // what the mask leaves out is read too, and its byte kept as it is: no load waits for it
   const auto get_y = [&](int it, int u) {
     const Item i(u);
     const int t = it / G * C + i.row, h = rev ? it % G * c.Hk + hk : hk;
@@ -215,8 +215,8 @@ __global__ __launch_bounds__(K::kThreads, K::P <= 128 && K::NT <= 128 ? 2 : K::N
     const int t = it / G * C + i.row, h = rev ? it % G * c.Hk + hk : hk, row = seg.row0 + t;
     InZ r;
     r.x = LinRaw<PL>{};
-    r.live = t < seg.len && i.d0 < NT && n0 + i.d0 < c.Dv;
-    if (r.live) {
+    r.live = 0;
+    if (t < seg.len && i.d0 < NT && n0 + i.d0 < c.Dv) {
       r.x = lin_load8<PL>(zr, (int64_t)seg.batch * zr.s[0] + (int64_t)h * zr.s[1] + (int64_t)row * zr.s[2], n0 + i.d0);
       r.live = kept(row);
     }
