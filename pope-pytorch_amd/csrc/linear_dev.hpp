@@ -104,6 +104,20 @@ __device__ __forceinline__ float lin_turns(float b) {
 // (exactly, for 16-bit rows; 2^-17 off for fp32 ones).
 enum LinParts { kOne = 1, kTwo = 2 };
 
+// Rows near each other are addressed by a base that a wave shares and a 32-bit offset in bytes (a chunk of 64 rows, row strides below
+// 2^23 elements): one register a load, the same in every chunk.
+__device__ __forceinline__ char* lin_uniform(const void* p) {
+  const uint64_t x = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+  return reinterpret_cast<char*>((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ int lin_size(int type) { return type == 0 ? 4 : 2; }
+// Base of row `row` of a (batch, head), and the bytes from row to row.
+__device__ __forceinline__ char* lin_base(const LinRows& r, int batch, int h, int64_t row) {
+  return lin_uniform(static_cast<char*>(r.p) + (batch * r.s[0] + h * r.s[1] + row * r.s[2]) * lin_size(r.type));
+}
+__device__ __forceinline__ uint32_t lin_step(const LinRows& r) { return (uint32_t)r.s[2] * lin_size(r.type); }
+
 // Eight elements of a row, as they are in memory.
 template <int PL>
 struct LinRaw {
@@ -116,35 +130,41 @@ struct LinRaw<kTwo> {
 template <int PL>
 __device__ __forceinline__ LinRaw<PL> lin_zeros() { return LinRaw<PL>{}; }
 
-// `at`: elements before the row.
+// base + off: the row.
 template <int PL>
-__device__ __forceinline__ LinRaw<PL> lin_load8(const LinRows& r, int64_t at, int d0) {
+__device__ __forceinline__ LinRaw<PL> lin_load8(const LinRows& r, const char* base, uint32_t off, int d0) {
   LinRaw<PL> w{};
   if constexpr (PL == kTwo) {
     if (r.type == 0) {
-      const float* p = static_cast<const float*>(r.p) + at + d0;
+      off += 4 * d0;
       if (r.vec) {
-        w.a = *reinterpret_cast<const u32x4*>(p);
-        w.b = *reinterpret_cast<const u32x4*>(p + 4);
+        w.a = *reinterpret_cast<const u32x4*>(base + off);
+        w.b = *reinterpret_cast<const u32x4*>(base + off + 16);
       } else {
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(base + off);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          if (d0 + k < r.cols) w.a[k] = __float_as_uint(p[k]);
-          if (d0 + 4 + k < r.cols) w.b[k] = __float_as_uint(p[4 + k]);
+          if (d0 + k < r.cols) w.a[k] = p[k];
+          if (d0 + 4 + k < r.cols) w.b[k] = p[4 + k];
         }
       }
       return w;
     }
   }
-  const uint16_t* p = static_cast<const uint16_t*>(r.p) + at + d0;
+  off += 2 * d0;
   if (r.vec) {
-    w.a = *reinterpret_cast<const u32x4*>(p);
+    w.a = *reinterpret_cast<const u32x4*>(base + off);
   } else {
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(base + off);
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       if (d0 + k < r.cols) w.a[k >> 1] |= (uint32_t)p[k] << (16 * (k & 1));
   }
   return w;
+}
+template <int PL>   // `at`: elements before the row
+__device__ __forceinline__ LinRaw<PL> lin_load8(const LinRows& r, int64_t at, int d0) {
+  return lin_load8<PL>(r, static_cast<const char*>(r.p) + at * (PL == kTwo ? lin_size(r.type) : 2), 0u, d0);
 }
 template <int PL>
 __device__ __forceinline__ void lin_unpack8(const LinRaw<PL>& w, int type, float* f) {
@@ -181,27 +201,41 @@ __device__ __forceinline__ void lin_set(const LinRows& r, int64_t at, float v) {
   }
   static_cast<uint16_t*>(r.p)[at] = BF16::bits(v);
 }
+template <int PL>
+__device__ __forceinline__ void lin_put_value(const LinRows& r, char* base, uint32_t off, int d, float v) {
+  if constexpr (PL == kTwo) {
+    if (r.type == 0) {
+      *reinterpret_cast<float*>(base + (off + 4 * d)) = v;
+      return;
+    }
+    if (r.type == 1) {
+      *reinterpret_cast<uint16_t*>(base + (off + 2 * d)) = F16::bits(v);
+      return;
+    }
+  }
+  *reinterpret_cast<uint16_t*>(base + (off + 2 * d)) = BF16::bits(v);
+}
 // Four elements of an output row from column d on (r.vec: d a multiple of 4, whole units).
 template <int PL>
-__device__ __forceinline__ void lin_set4(const LinRows& r, int64_t at, int d, f32x4 v) {
+__device__ __forceinline__ void lin_set4(const LinRows& r, char* base, uint32_t off, int d, f32x4 v) {
   if (d >= r.cols) return;
   if (!r.vec) {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (d + k < r.cols) lin_set<PL>(r, at + d + k, v[k]);
+      if (d + k < r.cols) lin_put_value<PL>(r, base, off, d + k, v[k]);
     return;
   }
   if constexpr (PL == kTwo) {
     if (r.type == 0) {
-      *reinterpret_cast<f32x4*>(static_cast<float*>(r.p) + at + d) = v;
+      *reinterpret_cast<f32x4*>(base + (off + 4 * d)) = v;
       return;
     }
     if (r.type == 1) {
-      *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(r.p) + at + d) = u32x2{F16::pack2(v[0], v[1]), F16::pack2(v[2], v[3])};
+      *reinterpret_cast<u32x2*>(base + (off + 2 * d)) = u32x2{F16::pack2(v[0], v[1]), F16::pack2(v[2], v[3])};
       return;
     }
   }
-  *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(r.p) + at + d) = u32x2{BF16::pack2(v[0], v[1]), BF16::pack2(v[2], v[3])};
+  *reinterpret_cast<u32x2*>(base + (off + 2 * d)) = u32x2{BF16::pack2(v[0], v[1]), BF16::pack2(v[2], v[3])};
 }
 // Two elements, as they are in memory: at an even place of an aligned row (`whole`), or one by one, the second if it is there.
 template <int PL>
@@ -209,11 +243,11 @@ struct LinPair { uint32_t w; };
 template <>
 struct LinPair<kTwo> { uint32_t w, v; };   // v: the second of fp32 rows
 template <int PL>
-__device__ __forceinline__ LinPair<PL> lin_get2(const LinRows& r, int64_t at, bool whole, bool second) {
+__device__ __forceinline__ LinPair<PL> lin_get2(const LinRows& r, const char* base, uint32_t off, int d, bool whole, bool second) {
   LinPair<PL> o{};
   if constexpr (PL == kTwo) {
     if (r.type == 0) {
-      const uint32_t* p = static_cast<const uint32_t*>(r.p) + at;
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(base + (off + 4 * d));
       if (whole) {
         const u32x2 w = *reinterpret_cast<const u32x2*>(p);
         o.w = w[0], o.v = w[1];
@@ -224,7 +258,7 @@ __device__ __forceinline__ LinPair<PL> lin_get2(const LinRows& r, int64_t at, bo
       return o;
     }
   }
-  const uint16_t* p = static_cast<const uint16_t*>(r.p) + at;
+  const uint16_t* p = reinterpret_cast<const uint16_t*>(base + (off + 2 * d));
   if (whole) {
     o.w = *reinterpret_cast<const uint32_t*>(p);
   } else {
@@ -248,18 +282,18 @@ __device__ __forceinline__ void lin_unpack2(const LinPair<PL>& p, int type, floa
   v[0] = BF16::to_float((uint16_t)p.w), v[1] = BF16::to_float((uint16_t)(p.w >> 16));
 }
 template <int PL>
-__device__ __forceinline__ void lin_set2(const LinRows& r, int64_t at, float a, float b) {
+__device__ __forceinline__ void lin_set2(const LinRows& r, char* base, uint32_t off, int d, float a, float b) {
   if constexpr (PL == kTwo) {
     if (r.type == 0) {
-      *reinterpret_cast<f32x2*>(static_cast<float*>(r.p) + at) = f32x2{a, b};
+      *reinterpret_cast<f32x2*>(base + (off + 4 * d)) = f32x2{a, b};
       return;
     }
     if (r.type == 1) {
-      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(r.p) + at) = F16::pack2(a, b);
+      *reinterpret_cast<uint32_t*>(base + (off + 2 * d)) = F16::pack2(a, b);
       return;
     }
   }
-  *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(r.p) + at) = BF16::pack2(a, b);
+  *reinterpret_cast<uint32_t*>(base + (off + 2 * d)) = BF16::pack2(a, b);
 }
 // Values of an array of one of the types.
 __device__ __forceinline__ float lin_value(const void* p, int type, int64_t i) {
@@ -449,8 +483,8 @@ __device__ __forceinline__ void lin_hat_tail(const LinHat& t, int64_t row, int t
 template <int C, int THREADS>
 struct LinItem {
   int row, d0;
-  __device__ __forceinline__ explicit LinItem(int u) {
-    const int t = (int)threadIdx.x + THREADS * u;
+  __device__ __forceinline__ explicit LinItem(int u, int tid = threadIdx.x) {
+    const int t = tid + THREADS * u;
     row = (t >> 2) % C;
     d0 = ((t & 3) + 4 * (t / (4 * C))) * 8;
   }

@@ -90,8 +90,13 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) dbsum[ct][0] = dbsum[ct][1] = 0.f;
 
-  const auto row_of = [&](int t) { return seg.row0 + (rev ? seg.len - 1 - t : t); };   // t: of the segment, in the job's order
+  // Rows of a chunk, t of 0 .. C - 1 in the job's order, from the chunk's base row on.
+  const auto base_row = [&](int t0) { return (int64_t)seg.row0 + (rev ? seg.len - C - t0 : t0); };   // reverse: may be in front of the first row
+  const auto place = [&](int t) { return (uint32_t)(rev ? C - 1 - t : t); };
   typedef LinItem<C, kThreads> Item;
+  // The thread's number as something new in every turn: places in memory and LDS are worked out again where they are used, instead of
+  // held in registers for the whole loop (the compiler did, and spilled the state for it).
+  int tv = tid;
   // x, y and z are expanded rows or plain ones, the keys' and values' rows among the latter, which the mask may leave out
   constexpr bool x_hat = !chain, y_hat = !chain, z_hat = chain;
   const LinRows xr = kind == kLinDq ? c.g : c.v, yr = kind == kLinDq ? c.v : c.g, zr = kind == kLinOut ? c.v : c.g;
@@ -106,37 +111,46 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
   // Loads keep what they read as it is until it is put: a conversion, or a choice by a mask's byte, would wait for the load.  What the
   // mask leaves out is read too.
   const uint8_t* mask = c.mask ? c.mask + (int64_t)seg.batch * c.mask_sb : nullptr;
-  const auto kept = [&](int row) { return mask ? (uint32_t)mask[row] : 1u; };
+  const auto mask_base = [&](int t0) { return mask ? reinterpret_cast<const uint8_t*>(lin_uniform(mask + base_row(t0))) : nullptr; };
+  const auto kept = [&](const uint8_t* m, int t) { return m ? (uint32_t)m[place(t)] : 1u; };
   // A thread's chunks of the tiles, read from memory.
   struct Part { LinRaw<PL> w; uint32_t keep; };
-  const auto get = [&](auto hat, auto key, const LinHat& t, const LinRows& r, int h, int cols, int t0, const Item& i, int d0) {
+  const auto base_of = [&](auto hat, const LinHat& t, const LinRows& r, int h, int t0) {
+    if constexpr (decltype(hat)::value) return lin_uniform(t.p + (((int64_t)seg.batch * t.H + h) * c.seqs.N + base_row(t0)) * t.EP);
+    else return lin_base(r, seg.batch, h, base_row(t0));
+  };
+  const auto get = [&](auto hat, auto key, const LinHat& t, const LinRows& r, const char* base, const uint8_t* m, int cols, int t0, const Item& i, int d0) {
     Part o;
     o.w = LinRaw<PL>{};
     o.keep = 0;
     if (t0 + i.row < seg.len && d0 < cols) {
-      const int row = row_of(t0 + i.row);
       if constexpr (decltype(hat)::value) {
-        const uint16_t* p = t.p + (((int64_t)seg.batch * t.H + h) * c.seqs.N + row) * t.EP + d0;
-        o.w.a = *reinterpret_cast<const u32x4*>(p);
-        if constexpr (PL == kTwo) o.w.b = *reinterpret_cast<const u32x4*>(p + t.plane);
+        const uint32_t off = (place(i.row) * t.EP + d0) * 2;
+        o.w.a = *reinterpret_cast<const u32x4*>(base + off);
+        if constexpr (PL == kTwo) o.w.b = *reinterpret_cast<const u32x4*>(base + 2 * t.plane + off);
       } else {
-        o.w = lin_load8<PL>(r, (int64_t)seg.batch * r.s[0] + (int64_t)h * r.s[1] + (int64_t)row * r.s[2], d0);
+        o.w = lin_load8<PL>(r, base, place(i.row) * lin_step(r), d0);
       }
-      o.keep = decltype(key)::value ? kept(row) : 1u;
+      o.keep = decltype(key)::value ? kept(m, i.row) : 1u;
     }
     return o;
   };
-  const auto get_x = [&](const Turn& n, int u) {
-    const Item i(u);
-    return get(Bool<x_hat>{}, Bool<x_key>{}, xh, xr, by_query ? n.hq : hk, xcols, n.t0, i, i.d0);
+  struct Bases { const char *x, *y, *z; const uint8_t* m; };
+  const auto bases_of = [&](const Turn& n) {
+    return Bases{base_of(Bool<x_hat>{}, xh, xr, by_query ? n.hq : hk, n.t0), base_of(Bool<y_hat>{}, yh, yr, by_query ? hk : n.hq, n.t0),
+                 base_of(Bool<z_hat>{}, zh, zr, by_query ? hk : n.hq, n.t0), mask_base(n.t0)};
   };
-  const auto get_y = [&](const Turn& n, int u) {
-    const Item i(u);
-    return get(Bool<y_hat>{}, Bool<y_key>{}, yh, yr, by_query ? hk : n.hq, ycols, n.t0, i, i.d0);
+  const auto get_x = [&](const Turn& n, const Bases& b, int u) {
+    const Item i(u, tv);
+    return get(Bool<x_hat>{}, Bool<x_key>{}, xh, xr, b.x, b.m, xcols, n.t0, i, i.d0);
   };
-  const auto get_z = [&](const Turn& n, int u) {
-    const Item i(u);
-    return get(Bool<z_hat>{}, Bool<z_key>{}, zh, zr, by_query ? hk : n.hq, i.d0 < NT ? zcols : 0, n.t0, i, n0 + i.d0);
+  const auto get_y = [&](const Turn& n, const Bases& b, int u) {
+    const Item i(u, tv);
+    return get(Bool<y_hat>{}, Bool<y_key>{}, yh, yr, b.y, b.m, ycols, n.t0, i, i.d0);
+  };
+  const auto get_z = [&](const Turn& n, const Bases& b, int u) {
+    const Item i(u, tv);
+    return get(Bool<z_hat>{}, Bool<z_key>{}, zh, zr, b.z, b.m, i.d0 < NT ? zcols : 0, n.t0, i, n0 + i.d0);
   };
   // ... and put into LDS
   const auto put = [&](auto hat, auto key, auto perm, const LinRows& r, const LinTile& t, const Item& i, Part o) {
@@ -155,15 +169,15 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
     }
   };
   const auto put_x = [&](int u, const Part& o) {
-    const Item i(u);
+    const Item i(u, tv);
     if (i.d0 < xcols) put(Bool<x_hat>{}, Bool<x_key>{}, Bool<true>{}, xr, X, i, o);
   };
   const auto put_y = [&](int u, const Part& o) {
-    const Item i(u);
+    const Item i(u, tv);
     if (i.d0 < ycols) put(Bool<y_hat>{}, Bool<y_key>{}, Bool<false>{}, yr, Y, i, o);
   };
   const auto put_z = [&](int u, const Part& o) {
-    const Item i(u);
+    const Item i(u, tv);
     return i.d0 < NT && n0 + i.d0 < zcols && put(Bool<z_hat>{}, Bool<z_key>{}, Bool<false>{}, zr, Z, i, o);
   };
   // Narrow tiles are loaded a chunk ahead, into registers; wide ones, whose state takes those, chunk by chunk.
@@ -172,14 +186,15 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
   Part xin[kTX + 1], yin[kTX + 1], zin[kTZ + 1];
   const auto load = [&](int it) {
     const Turn n = turn_of(it);
+    const Bases b = bases_of(n);
 #pragma unroll
     for (int u = 0; u < kTX; ++u) {
-      if (n.lx) xin[u] = get_x(n, u);
-      if (n.lyz) yin[u] = get_y(n, u);
+      if (n.lx) xin[u] = get_x(n, b, u);
+      if (n.lyz) yin[u] = get_y(n, b, u);
     }
     if (n.lyz)
 #pragma unroll
-      for (int u = 0; u < kTZ; ++u) zin[u] = get_z(n, u);
+      for (int u = 0; u < kTZ; ++u) zin[u] = get_z(n, b, u);
   };
   const auto turns_for = [&](int cols) { return (C * ((cols + 31) / 32 * 4) + kThreads - 1) / kThreads; };
   const auto store = [&](int it) {
@@ -195,19 +210,20 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
 #pragma unroll
         for (int u = 0; u < kTZ; ++u) some |= put_z(u, zin[u]);
     } else {
+      const Bases b = bases_of(n);
       const int txy = turns_for(xcols);
 #pragma unroll 2
       for (int u = 0; u < txy; ++u) {
         Part x, y;
-        if (n.lx) x = get_x(n, u);
-        if (n.lyz) y = get_y(n, u);
+        if (n.lx) x = get_x(n, b, u);
+        if (n.lyz) y = get_y(n, b, u);
         if (n.lx) put_x(u, x);
         if (n.lyz) put_y(u, y);
       }
       if (n.lyz) {
         const int tz = turns_for(min(NT, zcols - n0));
 #pragma unroll 4
-        for (int u = 0; u < tz; ++u) some |= put_z(u, get_z(n, u));
+        for (int u = 0; u < tz; ++u) some |= put_z(u, get_z(n, b, u));
       }
     }
     if (some) odd[it & 1] = 1;
@@ -255,6 +271,8 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
 
   for (int it = 0; it < turns_n; ++it) {
     const int ch = it / ng, g = it - ch * ng, t0 = ch * C;
+    tv = (int)opaque_u32((uint32_t)tid);
+    const int lane = tv & 63, q4 = lane >> 4, l16 = lane & 15;
     __syncthreads();   // nothing reads the tiles any more
     store(it);
     if (it + 1 < turns_n) load(it + 1);
@@ -301,26 +319,28 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
     LinPair<PL> cx[CT][IT];
     f32x2 cf[CT][IT];
     uint32_t live[IT];
+    const int h_out = by_query ? (g0 + g) * c.Hk + hk : hk;
     if constexpr (rev) {
+      const uint8_t* m = mask_base(t0);
 #pragma unroll
-      for (int i = 0; i < IT; ++i) live[i] = busy && ends ? kept(row_of(min(t0 + 16 * i + l16, seg.len - 1))) : 1u;
+      for (int i = 0; i < IT; ++i) live[i] = busy && ends && t0 + 16 * i + l16 < seg.len ? kept(m, 16 * i + l16) : 1u;
     }
     if constexpr (chain) {
       if (busy && ends) {
         const LinRows in = kind == kLinDq ? c.q : c.k;
-        const int64_t base = (int64_t)seg.batch * in.s[0] + (int64_t)(by_query ? (g0 + g) * c.Hk + hk : hk) * in.s[1];
+        const char* base = lin_base(in, seg.batch, h_out, base_row(t0));
+        const char* fbase = c.R ? lin_uniform(c.freqs + (int64_t)seg.batch * c.f_s[0] + base_row(t0) * c.f_s[1]) : nullptr;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-          const int row = row_of(min(t0 + 16 * i + l16, seg.len - 1));
+          const int t = 16 * i + l16;
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct) {
             const int d = (n0 + col0 + 16 * ct + 4 * q4) >> 1;
             cx[ct][i] = LinPair<PL>{};
             cf[ct][i] = f32x2{0.f, 0.f};
-            if (d >= c.R) continue;
-            const int64_t at = base + (int64_t)row * in.s[2] + d;
-            const float* fr = lin_angle_row(c, seg.batch, row) + d;
-            cx[ct][i] = lin_get2<PL>(in, at, pairs, d + 1 < c.R);
+            if (d >= c.R || t0 + t >= seg.len) continue;
+            cx[ct][i] = lin_get2<PL>(in, base, place(t) * lin_step(in), d, pairs, d + 1 < c.R);
+            const float* fr = reinterpret_cast<const float*>(fbase + (place(t) * (uint32_t)c.f_s[1] + d) * 4);
             if (pairs) {
               cf[ct][i] = *reinterpret_cast<const f32x2*>(fr);
             } else {
@@ -451,22 +471,22 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
       }
       // out: a lane has row 16 i + l16, columns 4 q4 .. of each tile
       if (ends) {
-        const int h = by_query ? (g0 + g) * c.Hk + hk : hk;
-        const int64_t ob = (int64_t)seg.batch * out.s[0] + (int64_t)h * out.s[1];
+        char* ob = lin_base(out, seg.batch, h_out, base_row(t0));
+        float* phase = nullptr;
+        if constexpr (chain)
+          if (p.dphase[which]) phase = p.dphase[which] + (((int64_t)seg.batch * (kind == kLinDq ? c.Hq : c.Hk) + h_out) * c.seqs.N + base_row(t0)) * c.R;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-          const int t = t0 + 16 * i + l16;
-          if (t >= seg.len) continue;
-          const int row = row_of(t);
-          const int64_t orow = ob + (int64_t)row * out.s[2];
+          const int t = 16 * i + l16;
+          if (t0 + t >= seg.len) continue;
+          const uint32_t orow = place(t) * lin_step(out);
           if (!chain) {
             const bool dead = rev && !live[i];
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct)
-              lin_set4<PL>(out, orow, n0 + col0 + 16 * ct + 4 * q4, dead ? f32x4{0.f, 0.f, 0.f, 0.f} : O[ct][i]);
+              lin_set4<PL>(out, ob, orow, n0 + col0 + 16 * ct + 4 * q4, dead ? f32x4{0.f, 0.f, 0.f, 0.f} : O[ct][i]);
           } else {
             // chain rule of the polar rows: a lane's columns are two (cosine, sine) pairs, or four other dims
-            float* ph = p.dphase[which] ? p.dphase[which] + (((int64_t)seg.batch * (kind == kLinDq ? c.Hq : c.Hk) + h) * c.seqs.N + row) * c.R : nullptr;
             const bool dead = rev && !live[i];
             const float f = kind == kLinDq ? c.scale : 1.f;
             const int in_type = kind == kLinDq ? c.q.type : c.k.type;
@@ -489,16 +509,16 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
                   dx[pr] = dead ? 0.f : sigmoid_f(x) * (dc * cs + ds * sn);
                   const float dth = dead ? 0.f : softplus_f(x) * (ds * cs - dc * sn);
                   dbsum[ct][pr] += dth;
-                  if (ph) ph[d] = dth;
-                  if (!pairs) lin_set<PL>(out, orow + d, dx[pr]);
+                  if (phase) phase[place(t) * c.R + d] = dth;
+                  if (!pairs) lin_put_value<PL>(out, ob, orow, d, dx[pr]);
                 } else if (!pairs) {
-                  if (e < c.E) lin_set<PL>(out, orow + e - c.R, dc);
-                  if (e + 1 < c.E) lin_set<PL>(out, orow + e + 1 - c.R, ds);
+                  if (e < c.E) lin_put_value<PL>(out, ob, orow, e - c.R, dc);
+                  if (e + 1 < c.E) lin_put_value<PL>(out, ob, orow, e + 1 - c.R, ds);
                 }
               }
               if (pairs) {
-                if (e0 < 2 * c.R) lin_set2<PL>(out, orow + (e0 >> 1), dx[0], dx[1]);
-                else if (e0 < c.E) lin_set4<PL>(out, orow, e0 - c.R, v);
+                if (e0 < 2 * c.R) lin_set2<PL>(out, ob, orow, e0 >> 1, dx[0], dx[1]);
+                else if (e0 < c.E) lin_set4<PL>(out, ob, orow, e0 - c.R, v);
               }
             }
           }

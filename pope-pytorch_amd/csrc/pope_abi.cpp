@@ -1274,6 +1274,8 @@ namespace {
 
 // ---------------------------------------------------------------- linear attention
 
+constexpr int64_t kLinRowStride = (int64_t)1 << 23;   // elements from row to row, less than
+
 int check_linear(const pope_linear* d) {
   if (!d) return fail(POPE_ERR_INVALID, "descriptor is NULL");
   if (d->B < 1 || d->N < 0 || d->Hq < 1 || d->Hk < 1)
@@ -1286,6 +1288,8 @@ int check_linear(const pope_linear* d) {
   if (d->N > (1 << 28) || d->B > (1 << 20) || d->Hq > 65535)
     return fail(POPE_ERR_UNSUPPORTED, "%d sequences, %d rows, %d heads: too many", d->B, d->N, d->Hq);
   if (d->bias_sh < 0 || d->mask_sb < 0) return fail(POPE_ERR_INVALID, "negative bias / mask stride");
+  for (const int64_t st : {d->q_s[2], d->k_s[2], d->v_s[2], d->o_s[2], d->f_s[1], d->do_s[2], d->dq_s[2], d->dk_s[2], d->dv_s[2]})
+    if (st >= kLinRowStride && d->N > 1) return fail(POPE_ERR_UNSUPPORTED, "a row stride of %lld elements is beyond a chunk's 32-bit offsets", (long long)st);
   int rc = check_strides("freqs", d->f_s, 2);
   if (!rc) rc = check_strides("q", d->q_s, 3);
   if (!rc) rc = check_strides("k", d->k_s, 3);
@@ -1368,6 +1372,9 @@ pope::LinCall linear_call(const pope_linear& d, const LinShape& s, const void* h
   c.log_decay = log_decay;
   c.mask = mask; c.mask_sb = d.mask_sb;
   c.Hq = d.Hq; c.Hk = d.Hk; c.G = d.Hq / d.Hk; c.D = d.D; c.R = d.R; c.E = d.D + d.R; c.Dv = d.Dv;
+  if (d.N == 1)   // strides of extents of 1 may be anything
+    for (pope::LinRows* r : {&c.q, &c.k, &c.v}) r->s[2] = 0;
+  if (d.N == 1) c.f_s[1] = 0;
   c.scale = d.scale;
   c.split = s.planes == 2;
   if (hats) {
