@@ -544,7 +544,11 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
 template <typename K, int KIND>
 constexpr int lin_out_bytes() { return K::PL * (K::C * (K::XS + K::YS + K::ZS + K::AS)) * 2 + (K::C + (KIND == kLinDq ? 256 : 0)) * 4 + 16; }
 template <typename K, int KIND>
-constexpr int lin_out_waves() { return K::NW == 4 && 2 * lin_out_bytes<K, KIND>() <= 160 * 1024 ? 2 : K::NW / 4; }
+constexpr int lin_out_waves() {
+  if (2 * lin_out_bytes<K, KIND>() > 160 * 1024) return (K::NW + 3) / 4;
+  // six waves start on the same SIMD in each workgroup: two on two SIMDs, so two workgroups take four places there
+  return K::NW == 4 ? 2 : K::NW == 6 ? 4 : 2;
+}
 
 // KIND kLinDq: dq and dk, in one launch.
 template <typename K, int KIND>
@@ -578,7 +582,7 @@ struct LinOutLaunch {
 };
 template <int PL, int KIND>
 hipError_t launch_linear_out_t(const LinOutParams& p, const char* name, hipStream_t s) {
-  return lin_dispatch<PL, LinOutLaunch<KIND>::template Of>(KIND == kLinDq ? p.c.Dv : p.c.E, KIND == kLinDq ? p.c.E : p.c.Dv, p, name, s);
+  return lin_dispatch<PL, LinOutLaunch<KIND>::template Of>(KIND == kLinDq ? p.c.Dv : p.c.E, KIND == kLinDq ? (p.c.E > 64 && p.c.E <= 96 ? 128 : p.c.E) : p.c.Dv, p, name, s);
 }
 
 }  // namespace pope
