@@ -130,29 +130,29 @@ struct LinRaw<kTwo> {
 template <int PL>
 __device__ __forceinline__ LinRaw<PL> lin_zeros() { return LinRaw<PL>{}; }
 
-// base + off: the row.
+// base + off: the row.  whole: r.vec, known before.
 template <int PL>
-__device__ __forceinline__ LinRaw<PL> lin_load8(const LinRows& r, const char* base, uint32_t off, int d0) {
+__device__ __forceinline__ LinRaw<PL> lin_load8(const LinRows& r, const char* base, uint32_t off, int d0, bool whole) {
   LinRaw<PL> w{};
   if constexpr (PL == kTwo) {
+    if (whole) {   // both loads, one of them twice for 16-bit rows: no branch
+      off += d0 * lin_size(r.type);
+      w.a = *reinterpret_cast<const u32x4*>(base + off);
+      w.b = *reinterpret_cast<const u32x4*>(base + (off + (r.type == 0 ? 16 : 0)));
+      return w;
+    }
     if (r.type == 0) {
-      off += 4 * d0;
-      if (r.vec) {
-        w.a = *reinterpret_cast<const u32x4*>(base + off);
-        w.b = *reinterpret_cast<const u32x4*>(base + off + 16);
-      } else {
-        const uint32_t* p = reinterpret_cast<const uint32_t*>(base + off);
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(base + (off + 4 * d0));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (d0 + k < r.cols) w.a[k] = p[k];
-          if (d0 + 4 + k < r.cols) w.b[k] = p[4 + k];
-        }
+      for (int k = 0; k < 4; ++k) {
+        if (d0 + k < r.cols) w.a[k] = p[k];
+        if (d0 + 4 + k < r.cols) w.b[k] = p[4 + k];
       }
       return w;
     }
   }
   off += 2 * d0;
-  if (r.vec) {
+  if (whole) {
     w.a = *reinterpret_cast<const u32x4*>(base + off);
   } else {
     const uint16_t* p = reinterpret_cast<const uint16_t*>(base + off);
@@ -164,7 +164,7 @@ __device__ __forceinline__ LinRaw<PL> lin_load8(const LinRows& r, const char* ba
 }
 template <int PL>   // `at`: elements before the row
 __device__ __forceinline__ LinRaw<PL> lin_load8(const LinRows& r, int64_t at, int d0) {
-  return lin_load8<PL>(r, static_cast<const char*>(r.p) + at * (PL == kTwo ? lin_size(r.type) : 2), 0u, d0);
+  return lin_load8<PL>(r, static_cast<const char*>(r.p) + at * (PL == kTwo ? lin_size(r.type) : 2), 0u, d0, r.vec);
 }
 template <int PL>
 __device__ __forceinline__ void lin_unpack8(const LinRaw<PL>& w, int type, float* f) {
@@ -237,35 +237,26 @@ __device__ __forceinline__ void lin_set4(const LinRows& r, char* base, uint32_t 
   }
   *reinterpret_cast<u32x2*>(base + (off + 2 * d)) = u32x2{BF16::pack2(v[0], v[1]), BF16::pack2(v[2], v[3])};
 }
-// Two elements, as they are in memory: at an even place of an aligned row (`whole`), or one by one, the second if it is there.
+// Two elements at an even place of an aligned row, as they are in memory.
 template <int PL>
 struct LinPair { uint32_t w; };
 template <>
 struct LinPair<kTwo> { uint32_t w, v; };   // v: the second of fp32 rows
 template <int PL>
-__device__ __forceinline__ LinPair<PL> lin_get2(const LinRows& r, const char* base, uint32_t off, int d, bool whole, bool second) {
-  LinPair<PL> o{};
-  if constexpr (PL == kTwo) {
-    if (r.type == 0) {
-      const uint32_t* p = reinterpret_cast<const uint32_t*>(base + (off + 4 * d));
-      if (whole) {
-        const u32x2 w = *reinterpret_cast<const u32x2*>(p);
-        o.w = w[0], o.v = w[1];
-      } else {
-        o.w = p[0];
-        if (second) o.v = p[1];
-      }
-      return o;
-    }
-  }
-  const uint16_t* p = reinterpret_cast<const uint16_t*>(base + (off + 2 * d));
-  if (whole) {
-    o.w = *reinterpret_cast<const uint32_t*>(p);
-  } else {
-    o.w = p[0];
-    if (second) o.w |= (uint32_t)p[1] << 16;
-  }
+__device__ __forceinline__ LinPair<PL> lin_get2(const LinRows& r, const char* base, uint32_t off, int d) {
+  LinPair<PL> o;
+  off += d * lin_size(r.type);
+  o.w = *reinterpret_cast<const uint32_t*>(base + off);
+  if constexpr (PL == kTwo) o.v = *reinterpret_cast<const uint32_t*>(base + (off + (r.type == 0 ? 4 : 0)));
   return o;
+}
+template <int PL>
+__device__ __forceinline__ float lin_get1(const LinRows& r, const char* base, uint32_t off, int d) {
+  if constexpr (PL == kTwo) {
+    if (r.type == 0) return *reinterpret_cast<const float*>(base + (off + 4 * d));
+    if (r.type == 1) return F16::to_float(*reinterpret_cast<const uint16_t*>(base + (off + 2 * d)));
+  }
+  return BF16::to_float(*reinterpret_cast<const uint16_t*>(base + (off + 2 * d)));
 }
 template <int PL>
 __device__ __forceinline__ void lin_unpack2(const LinPair<PL>& p, int type, float* v) {

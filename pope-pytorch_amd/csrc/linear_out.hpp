@@ -108,8 +108,9 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
     const int ch = it / ng, g = it - ch * ng;
     return Turn{ch * C, (g0 + g) * c.Hk + hk, by_query || g == 0, !by_query || g == 0};
   };
-  // Loads keep what they read as it is until it is put: a conversion, or a choice by a mask's byte, would wait for the load.  What the
-  // mask leaves out is read too.
+  // Loads keep what they read as it is until it is put, and nothing decides whether they happen: a conversion, a choice by a mask's
+  // byte or a branch around a load would wait for it.  Rows behind the segment are the last one's again, and what they and the mask's
+  // rows gave becomes zeros on the way into LDS.  Plain rows that are not whole 16-byte units take another way, branches and all.
   const uint8_t* mask = c.mask ? c.mask + (int64_t)seg.batch * c.mask_sb : nullptr;
   const auto mask_base = [&](int t0) { return mask ? reinterpret_cast<const uint8_t*>(lin_uniform(mask + base_row(t0))) : nullptr; };
   const auto kept = [&](const uint8_t* m, int t) { return m ? (uint32_t)m[place(t)] : 1u; };
@@ -119,20 +120,18 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
     if constexpr (decltype(hat)::value) return lin_uniform(t.p + (((int64_t)seg.batch * t.H + h) * c.seqs.N + base_row(t0)) * t.EP);
     else return lin_base(r, seg.batch, h, base_row(t0));
   };
-  const auto get = [&](auto hat, auto key, const LinHat& t, const LinRows& r, const char* base, const uint8_t* m, int cols, int t0, const Item& i, int d0) {
+  const auto get = [&](auto hat, auto key, auto whole, const LinHat& t, const LinRows& r, const char* base, const uint8_t* m, int cols, int t0, const Item& i, int d0) {
     Part o;
-    o.w = LinRaw<PL>{};
-    o.keep = 0;
-    if (t0 + i.row < seg.len && d0 < cols) {
-      if constexpr (decltype(hat)::value) {
-        const uint32_t off = (place(i.row) * t.EP + d0) * 2;
-        o.w.a = *reinterpret_cast<const u32x4*>(base + off);
-        if constexpr (PL == kTwo) o.w.b = *reinterpret_cast<const u32x4*>(base + 2 * t.plane + off);
-      } else {
-        o.w = lin_load8<PL>(r, base, place(i.row) * lin_step(r), d0);
-      }
-      o.keep = decltype(key)::value ? kept(m, i.row) : 1u;
+    const int at = min(i.row, seg.len - 1 - t0);
+    d0 = min(d0, (cols - 1) & ~7);
+    if constexpr (decltype(hat)::value) {
+      const uint32_t off = (place(at) * t.EP + d0) * 2;
+      o.w.a = *reinterpret_cast<const u32x4*>(base + off);
+      if constexpr (PL == kTwo) o.w.b = *reinterpret_cast<const u32x4*>(base + 2 * t.plane + off);
+    } else {
+      o.w = lin_load8<PL>(r, base, place(at) * lin_step(r), d0, decltype(whole)::value);
     }
+    if constexpr (decltype(key)::value) o.keep = kept(m, at);
     return o;
   };
   struct Bases { const char *x, *y, *z; const uint8_t* m; };
@@ -140,22 +139,22 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
     return Bases{base_of(Bool<x_hat>{}, xh, xr, by_query ? n.hq : hk, n.t0), base_of(Bool<y_hat>{}, yh, yr, by_query ? hk : n.hq, n.t0),
                  base_of(Bool<z_hat>{}, zh, zr, by_query ? hk : n.hq, n.t0), mask_base(n.t0)};
   };
-  const auto get_x = [&](const Turn& n, const Bases& b, int u) {
+  const auto get_x = [&](auto whole, const Turn& n, const Bases& b, int u) {
     const Item i(u, tv);
-    return get(Bool<x_hat>{}, Bool<x_key>{}, xh, xr, b.x, b.m, xcols, n.t0, i, i.d0);
+    return get(Bool<x_hat>{}, Bool<x_key>{}, whole, xh, xr, b.x, b.m, xcols, n.t0, i, i.d0);
   };
-  const auto get_y = [&](const Turn& n, const Bases& b, int u) {
+  const auto get_y = [&](auto whole, const Turn& n, const Bases& b, int u) {
     const Item i(u, tv);
-    return get(Bool<y_hat>{}, Bool<y_key>{}, yh, yr, b.y, b.m, ycols, n.t0, i, i.d0);
+    return get(Bool<y_hat>{}, Bool<y_key>{}, whole, yh, yr, b.y, b.m, ycols, n.t0, i, i.d0);
   };
-  const auto get_z = [&](const Turn& n, const Bases& b, int u) {
+  const auto get_z = [&](auto whole, const Turn& n, const Bases& b, int u) {
     const Item i(u, tv);
-    return get(Bool<z_hat>{}, Bool<z_key>{}, zh, zr, b.z, b.m, i.d0 < NT ? zcols : 0, n.t0, i, n0 + i.d0);
+    return get(Bool<z_hat>{}, Bool<z_key>{}, whole, zh, zr, b.z, b.m, zcols, n.t0, i, n0 + i.d0);
   };
   // ... and put into LDS
-  const auto put = [&](auto hat, auto key, auto perm, const LinRows& r, const LinTile& t, const Item& i, Part o) {
+  const auto put = [&](auto hat, auto key, auto perm, const LinRows& r, const LinTile& t, int t0, const Item& i, Part o) {
     constexpr bool kPerm = decltype(perm)::value;
-    if (decltype(key)::value && !o.keep) o.w = LinRaw<PL>{};
+    if (t0 + i.row >= seg.len || (decltype(key)::value && !o.keep)) o.w = LinRaw<PL>{};
     if constexpr (!decltype(hat)::value) {
       return lin_put_plain<PL, kPerm>(t, i.row, i.d0, o.w, r.type);
     } else {
@@ -168,63 +167,77 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
       return lin_odd8(o.w.a);
     }
   };
-  const auto put_x = [&](int u, const Part& o) {
+  const auto put_x = [&](const Turn& n, int u, const Part& o) {
     const Item i(u, tv);
-    if (i.d0 < xcols) put(Bool<x_hat>{}, Bool<x_key>{}, Bool<true>{}, xr, X, i, o);
+    if (i.d0 < xcols) put(Bool<x_hat>{}, Bool<x_key>{}, Bool<true>{}, xr, X, n.t0, i, o);
   };
-  const auto put_y = [&](int u, const Part& o) {
+  const auto put_y = [&](const Turn& n, int u, const Part& o) {
     const Item i(u, tv);
-    if (i.d0 < ycols) put(Bool<y_hat>{}, Bool<y_key>{}, Bool<false>{}, yr, Y, i, o);
+    if (i.d0 < ycols) put(Bool<y_hat>{}, Bool<y_key>{}, Bool<false>{}, yr, Y, n.t0, i, o);
   };
-  const auto put_z = [&](int u, const Part& o) {
+  const auto put_z = [&](const Turn& n, int u, const Part& o) {
     const Item i(u, tv);
-    return i.d0 < NT && n0 + i.d0 < zcols && put(Bool<z_hat>{}, Bool<z_key>{}, Bool<false>{}, zr, Z, i, o);
+    return i.d0 < NT && n0 + i.d0 < zcols && put(Bool<z_hat>{}, Bool<z_key>{}, Bool<false>{}, zr, Z, n.t0, i, o);
   };
+  const bool whole_rows = (x_hat || xr.vec) && (y_hat || yr.vec) && (z_hat || zr.vec);
   // Narrow tiles are loaded a chunk ahead, into registers; wide ones, whose state takes those, chunk by chunk.
   constexpr bool kAhead = P <= 128 && NT <= 128;
   constexpr int kTX = kAhead ? K::TP : 0, kTZ = kAhead ? K::TZ : 0;
   Part xin[kTX + 1], yin[kTX + 1], zin[kTZ + 1];
-  const auto load = [&](int it) {
+  const auto load_as = [&](auto whole, int it) {
     const Turn n = turn_of(it);
     const Bases b = bases_of(n);
+    if (n.lx)
 #pragma unroll
-    for (int u = 0; u < kTX; ++u) {
-      if (n.lx) xin[u] = get_x(n, b, u);
-      if (n.lyz) yin[u] = get_y(n, b, u);
+      for (int u = 0; u < kTX; ++u) xin[u] = get_x(whole, n, b, u);
+    if (n.lyz) {
+#pragma unroll
+      for (int u = 0; u < kTX; ++u) yin[u] = get_y(whole, n, b, u);
+#pragma unroll
+      for (int u = 0; u < kTZ; ++u) zin[u] = get_z(whole, n, b, u);
     }
-    if (n.lyz)
-#pragma unroll
-      for (int u = 0; u < kTZ; ++u) zin[u] = get_z(n, b, u);
+  };
+  const auto load = [&](int it) {
+    if constexpr (kAhead) {
+      if (whole_rows) load_as(Bool<true>{}, it);
+      else load_as(Bool<false>{}, it);
+    }
   };
   const auto turns_for = [&](int cols) { return (C * ((cols + 31) / 32 * 4) + kThreads - 1) / kThreads; };
+  const auto store_as = [&](auto whole, const Turn& n) {   // loaded here
+    const Bases b = bases_of(n);
+    bool some = false;
+    const int txy = turns_for(xcols);
+#pragma unroll 2
+    for (int u = 0; u < txy; ++u) {
+      Part x, y;
+      if (n.lx) x = get_x(whole, n, b, u);
+      if (n.lyz) y = get_y(whole, n, b, u);
+      if (n.lx) put_x(n, u, x);
+      if (n.lyz) put_y(n, u, y);
+    }
+    if (n.lyz) {
+      const int tz = turns_for(min(NT, zcols - n0));
+#pragma unroll 4
+      for (int u = 0; u < tz; ++u) some |= put_z(n, u, get_z(whole, n, b, u));
+    }
+    return some;
+  };
   const auto store = [&](int it) {
     const Turn n = turn_of(it);
     bool some = false;
     if constexpr (kAhead) {
+      if (n.lx)
 #pragma unroll
-      for (int u = 0; u < kTX; ++u) {
-        if (n.lx) put_x(u, xin[u]);
-        if (n.lyz) put_y(u, yin[u]);
-      }
-      if (n.lyz)
-#pragma unroll
-        for (int u = 0; u < kTZ; ++u) some |= put_z(u, zin[u]);
-    } else {
-      const Bases b = bases_of(n);
-      const int txy = turns_for(xcols);
-#pragma unroll 2
-      for (int u = 0; u < txy; ++u) {
-        Part x, y;
-        if (n.lx) x = get_x(n, b, u);
-        if (n.lyz) y = get_y(n, b, u);
-        if (n.lx) put_x(u, x);
-        if (n.lyz) put_y(u, y);
-      }
+        for (int u = 0; u < kTX; ++u) put_x(n, u, xin[u]);
       if (n.lyz) {
-        const int tz = turns_for(min(NT, zcols - n0));
-#pragma unroll 4
-        for (int u = 0; u < tz; ++u) some |= put_z(u, get_z(n, b, u));
+#pragma unroll
+        for (int u = 0; u < kTX; ++u) put_y(n, u, yin[u]);
+#pragma unroll
+        for (int u = 0; u < kTZ; ++u) some |= put_z(n, u, zin[u]);
       }
+    } else {
+      some = whole_rows ? store_as(Bool<true>{}, n) : store_as(Bool<false>{}, n);
     }
     if (some) odd[it & 1] = 1;
   };
@@ -315,7 +328,7 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
     }
     // what the chain rule of this turn's rows reads, ahead: a lane has row 16 i + l16, and, of each 16 columns, two dims
     const bool ends = by_query || g == ng - 1;
-    const bool pairs = out.vec && (kind == kLinDq ? c.q : c.k).vec && c.f_vec;   // two dims at a time: R, D multiples of 8
+    const bool pairs = out.vec && (kind == kLinDq ? c.q : c.k).vec && (c.f_vec || !c.R);   // two dims at a time: R, D multiples of 8
     LinPair<PL> cx[CT][IT];
     f32x2 cf[CT][IT];
     uint32_t live[IT];
@@ -323,30 +336,21 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
     if constexpr (rev) {
       const uint8_t* m = mask_base(t0);
 #pragma unroll
-      for (int i = 0; i < IT; ++i) live[i] = busy && ends && t0 + 16 * i + l16 < seg.len ? kept(m, 16 * i + l16) : 1u;
+      for (int i = 0; i < IT; ++i) live[i] = kept(m, min(16 * i + l16, seg.len - 1 - t0));
     }
+    const LinRows in = kind == kLinDq ? c.q : c.k;   // chain
+    const char* in_base = chain ? lin_base(in, seg.batch, h_out, base_row(t0)) : nullptr;
+    const char* f_base = chain && c.R ? lin_uniform(c.freqs + (int64_t)seg.batch * c.f_s[0] + base_row(t0) * c.f_s[1]) : nullptr;
     if constexpr (chain) {
-      if (busy && ends) {
-        const LinRows in = kind == kLinDq ? c.q : c.k;
-        const char* base = lin_base(in, seg.batch, h_out, base_row(t0));
-        const char* fbase = c.R ? lin_uniform(c.freqs + (int64_t)seg.batch * c.f_s[0] + base_row(t0) * c.f_s[1]) : nullptr;
+      if (pairs && c.R) {
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-          const int t = 16 * i + l16;
+          const uint32_t at = place(min(16 * i + l16, seg.len - 1 - t0));
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct) {
-            const int d = (n0 + col0 + 16 * ct + 4 * q4) >> 1;
-            cx[ct][i] = LinPair<PL>{};
-            cf[ct][i] = f32x2{0.f, 0.f};
-            if (d >= c.R || t0 + t >= seg.len) continue;
-            cx[ct][i] = lin_get2<PL>(in, base, place(t) * lin_step(in), d, pairs, d + 1 < c.R);
-            const float* fr = reinterpret_cast<const float*>(fbase + (place(t) * (uint32_t)c.f_s[1] + d) * 4);
-            if (pairs) {
-              cf[ct][i] = *reinterpret_cast<const f32x2*>(fr);
-            } else {
-              cf[ct][i][0] = fr[0];
-              if (d + 1 < c.R) cf[ct][i][1] = fr[1];
-            }
+            const int d = min((n0 + col0 + 16 * ct + 4 * q4) >> 1, c.R - 2);
+            cx[ct][i] = lin_get2<PL>(in, in_base, at * lin_step(in), d);
+            cf[ct][i] = *reinterpret_cast<const f32x2*>(f_base + (at * (uint32_t)c.f_s[1] + d) * 4);
           }
         }
       }
@@ -489,14 +493,23 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
             // chain rule of the polar rows: a lane's columns are two (cosine, sine) pairs, or four other dims
             const bool dead = rev && !live[i];
             const float f = kind == kLinDq ? c.scale : 1.f;
-            const int in_type = kind == kLinDq ? c.q.type : c.k.type;
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
               const int e0 = n0 + col0 + 16 * ct + 4 * q4;
               f32x4 v = O[ct][i] * f;
               if (dead) v = f32x4{0.f, 0.f, 0.f, 0.f};
               float dx[2], x2[2];
-              lin_unpack2<PL>(cx[ct][i], in_type, x2);
+              f32x2 f2 = cf[ct][i];
+              if (pairs) {
+                lin_unpack2<PL>(cx[ct][i], in.type, x2);
+              } else {
+#pragma unroll
+                for (int pr = 0; pr < 2; ++pr) {
+                  const int d = min((e0 >> 1) + pr, c.R - 1);
+                  x2[pr] = c.R ? lin_get1<PL>(in, in_base, place(t) * lin_step(in), d) : 0.f;
+                  f2[pr] = c.R ? *reinterpret_cast<const float*>(f_base + (place(t) * (uint32_t)c.f_s[1] + d) * 4) : 0.f;
+                }
+              }
 #pragma unroll
               for (int pr = 0; pr < 2; ++pr) {
                 const int e = e0 + 2 * pr;
@@ -505,7 +518,7 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
                   const int d = e >> 1;
                   const float x = x2[pr];
                   float sn, cs;
-                  sincos_turns(cf[ct][i][pr], kind == kLinDk ? turns[d] : 0.f, &sn, &cs);
+                  sincos_turns(f2[pr], kind == kLinDk ? turns[d] : 0.f, &sn, &cs);
                   dx[pr] = dead ? 0.f : sigmoid_f(x) * (dc * cs + ds * sn);
                   const float dth = dead ? 0.f : softplus_f(x) * (ds * cs - dc * sn);
                   dbsum[ct][pr] += dth;
@@ -582,7 +595,7 @@ struct LinOutLaunch {
 };
 template <int PL, int KIND>
 hipError_t launch_linear_out_t(const LinOutParams& p, const char* name, hipStream_t s) {
-  return lin_dispatch<PL, LinOutLaunch<KIND>::template Of>(KIND == kLinDq ? p.c.Dv : p.c.E, KIND == kLinDq ? (p.c.E > 64 && p.c.E <= 96 ? 128 : p.c.E) : p.c.Dv, p, name, s);
+  return lin_dispatch<PL, LinOutLaunch<KIND>::template Of>(KIND == kLinDq ? p.c.Dv : p.c.E, KIND == kLinDq ? p.c.E : p.c.Dv, p, name, s);
 }
 
 }  // namespace pope
