@@ -360,6 +360,7 @@ int pope_paged_attn(const pope_paged* desc, const void* q, const float* freqs, c
  * contiguous; `initial` NULL: zeros.  Products take bf16 rows as they are; fp16 and fp32 rows, and bf16 rows with o_f32, as the sum of two
  * bf16 parts (2^-17 of each factor).  Calls that need 2^22 workgroups or more return POPE_ERR_UNSUPPORTED.
  */
+#define POPE_LINEAR_ROW_STRIDE (1 << 22)  /* row strides are below this many elements, where there are rows */
 typedef struct pope_linear {
   int32_t B, N, Hq, Hk;      /* sequences; rows per sequence (packed: in all); heads */
   int32_t D, R, Dv;          /* 1 <= D <= 256, 0 <= R <= D, 1 <= Dv <= 256, any values */

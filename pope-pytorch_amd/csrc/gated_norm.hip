@@ -14,21 +14,48 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kNormGrid = 2048, kNormRows = 4;   // workgroups that fill the chip; the least turns of one
 
-__device__ __forceinline__ void load8(const LinRows& r, int64_t at, int d0, float* f) { lin_unpack8<kTwo>(lin_load8<kTwo>(r, at, d0), r.type, f); }
+// Eight elements from column d0 on; r.vec: whole aligned units of 8, or of 4 (2), or none (0).
+__device__ __forceinline__ void load8(const LinRows& r, int64_t at, int d0, float* f) {
+  LinRaw<kTwo> w{};
+  if (r.vec == 2) {
+    const char* p = static_cast<const char*>(r.p) + (at + d0) * lin_size(r.type);
+    const bool second = d0 + 4 < r.cols;
+    if (r.type == 0) {
+      w.a = *reinterpret_cast<const u32x4*>(p);
+      if (second) w.b = *reinterpret_cast<const u32x4*>(p + 16);
+    } else {
+      const u32x2 lo = *reinterpret_cast<const u32x2*>(p);
+      u32x2 hi = {0, 0};
+      if (second) hi = *reinterpret_cast<const u32x2*>(p + 8);
+      w.a = u32x4{lo[0], lo[1], hi[0], hi[1]};
+    }
+  } else {
+    w = lin_load8<kTwo>(r, at, d0);
+  }
+  lin_unpack8<kTwo>(w, r.type, f);
+}
 __device__ __forceinline__ void store8(const LinRows& r, int64_t at, int d0, const float* f) {
   if (!r.vec) {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       if (d0 + k < r.cols) lin_set<kTwo>(r, at + d0 + k, f[k]);
-  } else if (r.type == 0) {
-    float* p = static_cast<float*>(r.p) + at + d0;
+    return;
+  }
+  const bool second = r.vec == 1 || d0 + 4 < r.cols;
+  char* p = static_cast<char*>(r.p) + (at + d0) * lin_size(r.type);
+  if (r.type == 0) {
     *reinterpret_cast<f32x4*>(p) = f32x4{f[0], f[1], f[2], f[3]};
-    *reinterpret_cast<f32x4*>(p + 4) = f32x4{f[4], f[5], f[6], f[7]};
-  } else {
-    u32x4 w;
+    if (second) *reinterpret_cast<f32x4*>(p + 16) = f32x4{f[4], f[5], f[6], f[7]};
+    return;
+  }
+  u32x4 w;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] = r.type == 1 ? F16::pack2(f[2 * k], f[2 * k + 1]) : BF16::pack2(f[2 * k], f[2 * k + 1]);
-    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(r.p) + at + d0) = w;
+  for (int k = 0; k < 4; ++k) w[k] = r.type == 1 ? F16::pack2(f[2 * k], f[2 * k + 1]) : BF16::pack2(f[2 * k], f[2 * k + 1]);
+  if (r.vec == 1) {
+    *reinterpret_cast<u32x4*>(p) = w;
+  } else {
+    *reinterpret_cast<u32x2*>(p) = u32x2{w[0], w[1]};
+    if (second) *reinterpret_cast<u32x2*>(p + 8) = u32x2{w[2], w[3]};
   }
 }
 

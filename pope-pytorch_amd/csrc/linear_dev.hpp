@@ -523,32 +523,30 @@ struct LinCfg {
 
 // Rows of P / NT that a call takes: dispatch over (P, NT), P for the contraction's columns, NT for the result's.
 // Wide results go in tiles of 256 columns over eight waves; states of more than 256 rows leave room for 16 columns a wave.
+// 65 to 96 columns run as 128 over four waves: six waves of 16 columns have nothing to skip, but a CU takes one such workgroup, not
+// two (two waves on two of the SIMDs each time), and dq and dk of 2 x 8 heads x 4,096 rows of 64 + 32 columns took 70 us against 61.
 template <int PL, template <typename> class Launch, typename... A>
 hipError_t lin_dispatch(int pcols, int ncols, A&&... args) {
   const int p = pcols <= 64 ? 64 : pcols <= 96 ? 96 : pcols <= 128 ? 128 : pcols <= 256 ? 256 : 512;
-  const int n = ncols <= 64 ? 64 : ncols <= 96 ? 96 : ncols <= 128 ? 128 : 256;
+  const int n = ncols <= 64 ? 64 : ncols <= 128 ? 128 : 256;
 #define POPE_LIN_CASE(PP, NN, WW) return Launch<LinCfg<PL, PP, NN, WW>>::go(args...)
   if (p == 64) {
     if (n == 64) POPE_LIN_CASE(64, 64, 4);
-    if (n == 96) POPE_LIN_CASE(64, 96, 6);
     if (n == 128) POPE_LIN_CASE(64, 128, 4);
     POPE_LIN_CASE(64, 256, 8);
   }
   if (p == 96) {
     if (n == 64) POPE_LIN_CASE(96, 64, 4);
-    if (n == 96) POPE_LIN_CASE(96, 96, 6);
     if (n == 128) POPE_LIN_CASE(96, 128, 4);
     POPE_LIN_CASE(96, 256, 8);
   }
   if (p == 128) {
     if (n == 64) POPE_LIN_CASE(128, 64, 4);
-    if (n == 96) POPE_LIN_CASE(128, 96, 6);
     if (n == 128) POPE_LIN_CASE(128, 128, 4);
     POPE_LIN_CASE(128, 256, 8);
   }
   if (p == 256) {
     if (n == 64) POPE_LIN_CASE(256, 64, 4);
-    if (n == 96) POPE_LIN_CASE(256, 96, 6);
     if (n == 128) POPE_LIN_CASE(256, 128, 4);
     POPE_LIN_CASE(256, 256, 8);
   }

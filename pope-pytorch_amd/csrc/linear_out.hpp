@@ -284,7 +284,9 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
 
   for (int it = 0; it < turns_n; ++it) {
     const int ch = it / ng, g = it - ch * ng, t0 = ch * C;
-    tv = (int)opaque_u32((uint32_t)tid);
+    // places are worked out anew each turn: kept across turns, they leave the chains and the two-part products no registers (dq and
+    // dk of 256 columns: 399 us with spills, 194 without); one-part outputs and dv have the room, and save 5 to 8 us in 70
+    if constexpr (chain || PL == kTwo) tv = (int)opaque_u32((uint32_t)tid);
     const int lane = tv & 63, q4 = lane >> 4, l16 = lane & 15;
     __syncthreads();   // nothing reads the tiles any more
     store(it);
@@ -294,7 +296,7 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
     // x . y of the rows of 16 x 16 tiles j <= i, weighted: a wave has tiles of one i
     {
       constexpr int kShare = K::NW / IT, kTiles = IT > kShare ? IT / kShare : 1;
-      const int ti = wave / kShare, j0 = ti < IT ? wave % kShare : K::NW;   // waves left over have none: NW > ti
+      const int ti = wave / kShare, j0 = wave % kShare;
       f32x4 sc[kTiles];
 #pragma unroll
       for (int j = 0; j < kTiles; ++j) sc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -559,8 +561,7 @@ constexpr int lin_out_bytes() { return K::PL * (K::C * (K::XS + K::YS + K::ZS + 
 template <typename K, int KIND>
 constexpr int lin_out_waves() {
   if (2 * lin_out_bytes<K, KIND>() > 160 * 1024) return (K::NW + 3) / 4;
-  // six waves start on the same SIMD in each workgroup: two on two SIMDs, so two workgroups take four places there
-  return K::NW == 4 ? 2 : K::NW == 6 ? 4 : 2;
+  return 2;
 }
 
 // KIND kLinDq: dq and dk, in one launch.

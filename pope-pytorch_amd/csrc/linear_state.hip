@@ -11,6 +11,8 @@
 // Expanding rows where they are used instead cost more: the forward over 32,768 rows of 8 heads, D 64, R 32, took 86 us and its states
 // 46, against 44 and 65 with the rows expanded here.  So did a launch of its own for the expansion: 20 us and 10 for the
 // sums against 19 (2 x 4,096 rows of the same heads).
+#include <type_traits>
+
 #include "linear_dev.hpp"
 
 namespace pope {
@@ -38,25 +40,71 @@ __device__ __forceinline__ void lin_state_out(const LinStateParams& p, int at, i
   }
 }
 
-// The queries of a segment and head, expanded: four threads a row.
-template <int PL, int THREADS>
+// A chunk of a row and its angles, as they are in memory.  FAST: whole units; then nothing decides whether the loads happen (a
+// branch around a load waits for it), and places past the end are moved to the last ones.
+template <int PL>
+struct LinIn {
+  LinRaw<PL> x;
+  f32x4 f[2];
+};
+template <int PL, bool FAST>
+__device__ __forceinline__ LinIn<PL> lin_in(const LinCall& c, const LinRows& r, const char* base, const char* f_base, uint32_t at, int d0) {
+  LinIn<PL> o;
+  o.f[0] = o.f[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  o.x = lin_load8<PL>(r, base, at * lin_step(r), FAST ? min(d0, c.D - 8) : d0, FAST);
+  if (!c.R) return o;
+  const float* fr = reinterpret_cast<const float*>(f_base + (uint32_t)(at * (uint32_t)c.f_s[1] * 4));
+  if constexpr (FAST) {
+    const int d = min(d0, c.R - 8);
+    o.f[0] = *reinterpret_cast<const f32x4*>(fr + d);
+    o.f[1] = *reinterpret_cast<const f32x4*>(fr + d + 4);
+  } else {
+    lin_angles8(fr, d0, c.R, false, o.f);
+  }
+  return o;
+}
+__device__ __forceinline__ bool lin_fast(const LinCall& c, const LinRows& r) { return r.vec && (c.f_vec || !c.R); }
+__device__ __forceinline__ char* lin_angle_base(const LinCall& c, int batch, int64_t row) {
+  return c.R ? lin_uniform(c.freqs + (int64_t)batch * c.f_s[0] + row * c.f_s[1]) : nullptr;
+}
+
+// The queries of a segment and head, expanded: four threads a row, two rows and two chunks of each at once.
+template <int PL, int THREADS, bool FAST>
 __device__ __forceinline__ void lin_expand_queries(const LinCall& c, const LinSeg& seg, int hq) {
   const int tid = threadIdx.x, per = (c.D + 7) / 8;
   constexpr int kRows = THREADS / 4;
-  for (int r = tid >> 2; r < seg.len; r += kRows) {
-    const int row = seg.row0 + r;
-    const int64_t at = ((int64_t)seg.batch * c.Hq + hq) * c.seqs.N + row;
-    const int64_t src = (int64_t)seg.batch * c.q.s[0] + (int64_t)hq * c.q.s[1] + (int64_t)row * c.q.s[2];
-#pragma unroll 2
-    for (int u = tid & 3; u < per; u += 4) {
-      f32x4 f[2];
-      float a[8], b[8];
-      const LinRaw<PL> x = lin_load8<PL>(c.q, src, 8 * u);
-      if (c.R) lin_angles8(lin_angle_row(c, seg.batch, row), 8 * u, c.R, c.f_vec, f);
-      lin_polar8<PL>(x, c.q.type, f, 8 * u, c.R, c.scale, nullptr, a, b);
-      lin_hat_put<PL>(c.qh, at, 8 * u, c.D, c.R, a, b);
+  for (int r0 = 0; r0 < seg.len; r0 += 2 * kRows) {
+    const char* base = lin_base(c.q, seg.batch, hq, seg.row0 + r0);
+    const char* f_base = lin_angle_base(c, seg.batch, seg.row0 + r0);
+    const int64_t to = ((int64_t)seg.batch * c.Hq + hq) * c.seqs.N + seg.row0 + r0;
+    const int left = seg.len - r0;
+    for (int u0 = tid & 3; u0 - (tid & 3) < per; u0 += 8) {
+      LinIn<PL> in[2][2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int r = (tid >> 2) + j * kRows, u = u0 + 4 * k;
+          if (FAST || (r < left && u < per)) in[j][k] = lin_in<PL, FAST>(c, c.q, base, f_base, min(r, left - 1), 8 * u);
+        }
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int r = (tid >> 2) + j * kRows, u = u0 + 4 * k;
+          if (r < left && u < per) {
+            float a[8], b[8];
+            lin_polar8<PL>(in[j][k].x, c.q.type, in[j][k].f, 8 * u, c.R, c.scale, nullptr, a, b);
+            lin_hat_put<PL>(c.qh, to + r, 8 * u, c.D, c.R, a, b);
+          }
+          __builtin_amdgcn_sched_barrier(0);   // one expansion at a time: side by side they take all registers
+        }
     }
-    lin_hat_tail<PL, 4>(c.qh, at, tid & 3, c.D, c.R);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int r = (tid >> 2) + j * kRows;
+      if (r < left) lin_hat_tail<PL, 4>(c.qh, to + r, tid & 3, c.D, c.R);
+    }
   }
 }
 
@@ -71,7 +119,9 @@ __global__ __launch_bounds__(K::kThreads, 1) void linear_state_kernel(LinStatePa
   if ((int)blockIdx.x >= p.key_wgs) {
     const int wg = blockIdx.x - p.key_wgs, at = wg / c.Hq;
     const LinSeg seg = lin_segment(c.seqs, at);
-    if (seg.seq >= 0) lin_expand_queries<PL, K::kThreads>(c, seg, wg - at * c.Hq);
+    if (seg.seq < 0) return;
+    if (lin_fast(c, c.q)) lin_expand_queries<PL, K::kThreads, true>(c, seg, wg - at * c.Hq);
+    else lin_expand_queries<PL, K::kThreads, false>(c, seg, wg - at * c.Hq);
     return;
   }
   const int wg = blockIdx.x, tile = wg % p.tiles, rest = wg / p.tiles, hk = rest % c.Hk, at = rest / c.Hk;
@@ -95,53 +145,91 @@ __global__ __launch_bounds__(K::kThreads, 1) void linear_state_kernel(LinStatePa
   const int ty = (C * ((c.D + 31) / 32 * 4) + K::kThreads - 1) / K::kThreads;
   const int tz = (C * ((min(NT, c.Dv - n0) + 31) / 32 * 4) + K::kThreads - 1) / K::kThreads;
   typedef LinItem<C, K::kThreads> Item;
-  const auto kept = [&](int row) { return rev || !c.mask ? 1u : (uint32_t)c.mask[(int64_t)seg.batch * c.mask_sb + row]; };
-  for (int t0 = 0; t0 < seg.len; t0 += C)
-    for (int g = 0; g < G; ++g) {
-      const int h = rev ? g * c.Hk + hk : hk;
-      __syncthreads();   // nothing reads the tiles any more
-#pragma unroll 2
-      for (int u = 0; u < ty; ++u) {
-        const Item i(u);
-        const int row = seg.row0 + t0 + i.row;
-        const bool in = t0 + i.row < seg.len, keep = !rev && tile == 0 && in;
-        const int64_t to = ((int64_t)seg.batch * c.Hk + hk) * c.seqs.N + row;
-        if (keep && i.d0 < 32) lin_hat_tail<PL, 4>(c.kh, to, i.d0 / 8, c.D, c.R);
-        if (i.d0 >= c.D) continue;
-        LinRaw<PL> x{};
-        f32x4 f[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-        uint32_t live = in;
-        if (in) {   // what the mask leaves out is read too, so that no load waits for it
-          x = lin_load8<PL>(yr, (int64_t)seg.batch * yr.s[0] + (int64_t)h * yr.s[1] + (int64_t)row * yr.s[2], i.d0);
-          if (c.R) lin_angles8(lin_angle_row(c, seg.batch, row), i.d0, c.R, c.f_vec, f);
-          live = kept(row);
-        }
-        float a[8], b[8];
-        lin_polar8<PL>(x, yr.type, f, i.d0, c.R, rev ? c.scale : 1.f, bias, a, b);
-        if (!live)
+  const uint8_t* mask = rev || !c.mask ? nullptr : c.mask + (int64_t)seg.batch * c.mask_sb + seg.row0;
+  // a turn's chunks of a tile, two at once
+  const auto turn_y = [&](auto fast, int t0, int h, int u0) {
+    constexpr bool kFast = decltype(fast)::value;
+    const char* base = lin_base(yr, seg.batch, h, seg.row0 + t0);
+    const char* f_base = lin_angle_base(c, seg.batch, seg.row0 + t0);
+    const int left = seg.len - t0;
+    LinIn<PL> in[2];
+    uint32_t live[2];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) a[k] = b[k] = 0.f;
+    for (int k = 0; k < 2; ++k) {
+      const Item i(u0 + k);
+      const int at = min(i.row, left - 1);
+      if (kFast || i.d0 < c.D) in[k] = lin_in<PL, kFast>(c, yr, base, f_base, at, i.d0);
+      live[k] = mask ? (uint32_t)mask[t0 + at] : 1u;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const Item i(u0 + k);
+      const bool there = i.row < left, keep = !rev && tile == 0 && there;
+      const int64_t to = ((int64_t)seg.batch * c.Hk + hk) * c.seqs.N + seg.row0 + t0 + i.row;
+      if (keep && i.d0 < 32) lin_hat_tail<PL, 4>(c.kh, to, i.d0 / 8, c.D, c.R);
+      if (i.d0 < c.D) {
+        float a[8], b[8];
+        lin_polar8<PL>(in[k].x, yr.type, in[k].f, i.d0, c.R, rev ? c.scale : 1.f, bias, a, b);
+        if (!there || !live[k])
+#pragma unroll
+          for (int j = 0; j < 8; ++j) a[j] = b[j] = 0.f;
         if (keep) lin_hat_put<PL>(c.kh, to, i.d0, c.D, c.R, a, b);
         if (p.states) {
-          const float w = in ? lin_power(lg, rev ? t0 + i.row + 1 : seg.len - 1 - t0 - i.row) : 0.f;
+          const float w = there ? lin_power(lg, rev ? t0 + i.row + 1 : left - 1 - i.row) : 0.f;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) a[k] *= w, b[k] *= w;
+          for (int j = 0; j < 8; ++j) a[j] *= w, b[j] *= w;
           lin_place8(i.d0, c.D, c.R, a, b, [&](int e, const float* v) { lin_put8<2, false>(Y, i.row, e, v); },
                      [&](int e, float v) { lin_put1<2, false>(Y, i.row, e, v); });
         }
       }
-      if (!p.states) continue;
-#pragma unroll 2
-      for (int u = 0; u < tz; ++u) {
-        const Item i(u);
-        if (i.d0 >= NT || n0 + i.d0 >= c.Dv) continue;
-        const int row = seg.row0 + t0 + i.row;
-        LinRaw<PL> x{};
-        if (t0 + i.row < seg.len) {
-          x = lin_load8<PL>(zr, (int64_t)seg.batch * zr.s[0] + (int64_t)h * zr.s[1] + (int64_t)row * zr.s[2], n0 + i.d0);
-          if (!kept(row)) x = LinRaw<PL>{};
+      __builtin_amdgcn_sched_barrier(0);   // one expansion at a time: side by side they take all registers
+    }
+  };
+  constexpr int kZ = 2;   // chunks of values that are loaded in front of the keys'
+  LinRaw<PL> zin[kZ];
+  uint32_t zlive[kZ];
+  const auto get_z = [&](auto fast, int t0, int h, int u, LinRaw<PL>& x, uint32_t& live) {
+    constexpr bool kFast = decltype(fast)::value;
+    const char* base = lin_base(zr, seg.batch, h, seg.row0 + t0);
+    const Item i(u);
+    const int at = min(i.row, seg.len - t0 - 1), d0 = n0 + i.d0;
+    x = LinRaw<PL>{};
+    if (kFast || (i.d0 < NT && d0 < c.Dv)) x = lin_load8<PL>(zr, base, at * lin_step(zr), kFast ? min(d0, c.Dv - 8) : d0, kFast);
+    live = mask ? (uint32_t)mask[t0 + at] : 1u;
+  };
+  const auto put_z = [&](int t0, int u, LinRaw<PL> x, uint32_t live) {
+    const Item i(u);
+    if (i.d0 >= NT || n0 + i.d0 >= c.Dv) return;
+    if (i.row >= seg.len - t0 || !live) x = LinRaw<PL>{};
+    lin_put_plain<PL, false>(Z, i.row, i.d0, x, zr.type);
+  };
+  const bool fast_y = lin_fast(c, yr), fast_z = zr.vec;
+  for (int t0 = 0; t0 < seg.len; t0 += C)
+    for (int g = 0; g < G; ++g) {
+      const int h = rev ? g * c.Hk + hk : hk;
+      if (p.states) {
+#pragma unroll
+        for (int u = 0; u < kZ; ++u) {
+          if (fast_z) get_z(std::true_type{}, t0, h, u, zin[u], zlive[u]);
+          else get_z(std::false_type{}, t0, h, u, zin[u], zlive[u]);
         }
-        lin_put_plain<PL, false>(Z, i.row, i.d0, x, zr.type);
+      }
+      __syncthreads();   // nothing reads the tiles any more
+#pragma unroll 1
+      for (int u = 0; u < ty; u += 2) {
+        if (fast_y) turn_y(std::true_type{}, t0, h, u);
+        else turn_y(std::false_type{}, t0, h, u);
+      }
+      if (!p.states) continue;
+#pragma unroll
+      for (int u = 0; u < kZ; ++u) put_z(t0, u, zin[u], zlive[u]);
+#pragma unroll 2
+      for (int u = kZ; u < tz; ++u) {
+        LinRaw<PL> x;
+        uint32_t live;
+        if (fast_z) get_z(std::true_type{}, t0, h, u, x, live);
+        else get_z(std::false_type{}, t0, h, u, x, live);
+        put_z(t0, u, x, live);
       }
       __syncthreads();
       if (busy) {
@@ -194,44 +282,46 @@ __global__ __launch_bounds__(K::kThreads, K::P <= 128 && K::NT <= 128 ? 2 : K::N
   const LinHat yh = rev ? c.qh : c.kh;
   const LinRows zr = rev ? c.g : c.v;
   typedef LinItem<C, K::kThreads> Item;
-  const auto kept = [&](int row) { return rev || !c.mask ? 1u : (uint32_t)c.mask[(int64_t)seg.batch * c.mask_sb + row]; };
+  const uint8_t* mask = rev || !c.mask ? nullptr : c.mask + (int64_t)seg.batch * c.mask_sb + seg.row0;
   struct InY { u32x4 w[PY]; };
-  struct InZ { LinRaw<PL> x; uint32_t live; };   // what the mask leaves out is read too, and its byte kept as it is: no load waits for it
+  struct InZ { LinRaw<PL> x; uint32_t live; };
+  // loads that nothing decides about (a branch around a load waits for it): rows behind the segment are the last one's again, what
+  // the mask leaves out is read too, and becomes zeros on the way into LDS
   const auto get_y = [&](int it, int u) {
     const Item i(u);
-    const int t = it / G * C + i.row, h = rev ? it % G * c.Hk + hk : hk;
+    const int t0 = it / G * C, h = rev ? it % G * c.Hk + hk : hk, at = min(i.row, seg.len - 1 - t0);
+    const char* base = lin_uniform(yh.p + (((int64_t)seg.batch * yh.H + h) * c.seqs.N + seg.row0 + t0) * yh.EP);
     InY r;
 #pragma unroll
-    for (int l = 0; l < PY; ++l) r.w[l] = u32x4{0, 0, 0, 0};
-    if (t < seg.len && i.d0 < yh.EP) {
-      const uint16_t* src = yh.p + (((int64_t)seg.batch * yh.H + h) * c.seqs.N + seg.row0 + t) * yh.EP + i.d0;
-#pragma unroll
-      for (int l = 0; l < PY; ++l) r.w[l] = *reinterpret_cast<const u32x4*>(src + l * yh.plane);
-    }
+    for (int l = 0; l < PY; ++l) r.w[l] = *reinterpret_cast<const u32x4*>(base + l * 2 * yh.plane + (uint32_t)((at * yh.EP + min(i.d0, yh.EP - 8)) * 2));
     return r;
   };
-  const auto get_z = [&](int it, int u) {
+  const auto get_z = [&](auto fast, int it, int u) {
+    constexpr bool kFast = decltype(fast)::value;
     const Item i(u);
-    const int t = it / G * C + i.row, h = rev ? it % G * c.Hk + hk : hk, row = seg.row0 + t;
+    const int t0 = it / G * C, h = rev ? it % G * c.Hk + hk : hk, at = min(i.row, seg.len - 1 - t0), d0 = n0 + i.d0;
+    const char* base = lin_base(zr, seg.batch, h, seg.row0 + t0);
     InZ r;
     r.x = LinRaw<PL>{};
-    r.live = 0;
-    if (t < seg.len && i.d0 < NT && n0 + i.d0 < c.Dv) {
-      r.x = lin_load8<PL>(zr, (int64_t)seg.batch * zr.s[0] + (int64_t)h * zr.s[1] + (int64_t)row * zr.s[2], n0 + i.d0);
-      r.live = kept(row);
-    }
+    if (kFast || d0 < c.Dv) r.x = lin_load8<PL>(zr, base, at * lin_step(zr), kFast ? min(d0, c.Dv - 8) : d0, kFast);
+    r.live = mask ? (uint32_t)mask[t0 + at] : 1u;
     return r;
   };
-  const auto put_y = [&](int u, const InY& r) {
+  const auto put_y = [&](int it, int u, InY r) {
     const Item i(u);
-    if (i.d0 < yh.EP) lin_put_parts<PY, false>(Y, i.row, i.d0, r.w);
+    if (i.d0 >= yh.EP) return;
+    if (it / G * C + i.row >= seg.len)
+#pragma unroll
+      for (int l = 0; l < PY; ++l) r.w[l] = u32x4{0, 0, 0, 0};
+    lin_put_parts<PY, false>(Y, i.row, i.d0, r.w);
   };
-  const auto put_z = [&](int u, InZ r) {
+  const auto put_z = [&](int it, int u, InZ r) {
     const Item i(u);
     if (i.d0 >= NT || n0 + i.d0 >= c.Dv) return;
-    if (!r.live) r.x = LinRaw<PL>{};
+    if (it / G * C + i.row >= seg.len || !r.live) r.x = LinRaw<PL>{};
     lin_put_plain<PL, false>(Z, i.row, i.d0, r.x, zr.type);
   };
+  const bool fast = zr.vec;
   constexpr bool kAhead = K::P <= 128 && NT <= 128;
   constexpr int kTY = kAhead ? K::TP : 0, kTZ = kAhead ? K::TZ : 0;
   InY yin[kTY + 1];
@@ -240,7 +330,10 @@ __global__ __launch_bounds__(K::kThreads, K::P <= 128 && K::NT <= 128 ? 2 : K::N
 #pragma unroll
     for (int u = 0; u < kTY; ++u) yin[u] = get_y(it, u);
 #pragma unroll
-    for (int u = 0; u < kTZ; ++u) zin[u] = get_z(it, u);
+    for (int u = 0; u < kTZ; ++u) {
+      if (fast) zin[u] = get_z(std::true_type{}, it, u);
+      else zin[u] = get_z(std::false_type{}, it, u);
+    }
   };
   const int all = (seg.len + C - 1) / C * G;
   load(0);
@@ -252,17 +345,17 @@ __global__ __launch_bounds__(K::kThreads, K::P <= 128 && K::NT <= 128 ? 2 : K::N
     }
     if constexpr (kAhead) {
 #pragma unroll
-      for (int u = 0; u < kTY; ++u) put_y(u, yin[u]);
+      for (int u = 0; u < kTY; ++u) put_y(it, u, yin[u]);
 #pragma unroll
-      for (int u = 0; u < kTZ; ++u) put_z(u, zin[u]);
+      for (int u = 0; u < kTZ; ++u) put_z(it, u, zin[u]);
       if (it + 1 < all) load(it + 1);
     } else {
       const int ty = (C * (yh.EP / 8) + K::kThreads - 1) / K::kThreads;
       const int tz = (C * ((min(NT, c.Dv - n0) + 31) / 32 * 4) + K::kThreads - 1) / K::kThreads;
 #pragma unroll 4
-      for (int u = 0; u < ty; ++u) put_y(u, get_y(it, u));
+      for (int u = 0; u < ty; ++u) put_y(it, u, get_y(it, u));
 #pragma unroll 4
-      for (int u = 0; u < tz; ++u) put_z(u, get_z(it, u));
+      for (int u = 0; u < tz; ++u) put_z(it, u, fast ? get_z(std::true_type{}, it, u) : get_z(std::false_type{}, it, u));
     }
     __syncthreads();
     if (busy) {

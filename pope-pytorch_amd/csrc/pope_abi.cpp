@@ -1274,8 +1274,6 @@ namespace {
 
 // ---------------------------------------------------------------- linear attention
 
-constexpr int64_t kLinRowStride = (int64_t)1 << 23;   // elements from row to row, less than
-
 int check_linear(const pope_linear* d) {
   if (!d) return fail(POPE_ERR_INVALID, "descriptor is NULL");
   if (d->B < 1 || d->N < 0 || d->Hq < 1 || d->Hk < 1)
@@ -1289,7 +1287,7 @@ int check_linear(const pope_linear* d) {
     return fail(POPE_ERR_UNSUPPORTED, "%d sequences, %d rows, %d heads: too many", d->B, d->N, d->Hq);
   if (d->bias_sh < 0 || d->mask_sb < 0) return fail(POPE_ERR_INVALID, "negative bias / mask stride");
   for (const int64_t st : {d->q_s[2], d->k_s[2], d->v_s[2], d->o_s[2], d->f_s[1], d->do_s[2], d->dq_s[2], d->dk_s[2], d->dv_s[2]})
-    if (st >= kLinRowStride && d->N > 1) return fail(POPE_ERR_UNSUPPORTED, "a row stride of %lld elements is beyond a chunk's 32-bit offsets", (long long)st);
+    if (st >= POPE_LINEAR_ROW_STRIDE && d->N > 1) return fail(POPE_ERR_UNSUPPORTED, "a row stride of %lld elements is beyond a chunk's 32-bit offsets", (long long)st);
   int rc = check_strides("freqs", d->f_s, 2);
   if (!rc) rc = check_strides("q", d->q_s, 3);
   if (!rc) rc = check_strides("k", d->k_s, 3);
@@ -1416,11 +1414,18 @@ int check_norm(const pope_gated_norm* d) {
   return rc;
 }
 
+// Rows of the norm: whole units of 8, or (2) of 4.
+pope::LinRows norm_rows(const void* p, const int64_t* s, int cols, int type) {
+  pope::LinRows r = lin_rows(p, s, cols, type, 8);
+  if (!r.vec && lin_rows(p, s, cols, type, 4).vec) r.vec = 2;
+  return r;
+}
+
 pope::GatedNormParams norm_params(const pope_gated_norm& d, const void* x, const void* gate, const void* weight) {
   pope::GatedNormParams p;
   std::memset(&p, 0, sizeof p);
-  p.x = lin_rows(x, d.x_s, d.cols, d.x_f32 ? POPE_F32 : d.dtype, 8);
-  p.gate = lin_rows(gate, d.gate_s, d.cols, d.dtype, 8);
+  p.x = norm_rows(x, d.x_s, d.cols, d.x_f32 ? POPE_F32 : d.dtype);
+  p.gate = norm_rows(gate, d.gate_s, d.cols, d.dtype);
   p.weight = weight;
   p.w_sh = d.weight_rows > 1 ? d.weight_sh : 0;
   p.w_type = d.weight_f32 ? POPE_F32 : d.dtype;
@@ -1448,7 +1453,7 @@ int pope_linear_fwd(const pope_linear* d, const void* q, const void* k, const vo
                     void* kept, size_t kept_bytes, void* stream) {
   int rc = check_linear(d);
   if (rc) return rc;
-  if (d->N == 0) return POPE_OK;
+  if (d->N == 0) return last ? fail(POPE_ERR_INVALID, "no rows: the states are those given") : POPE_OK;
   if ((rc = check_linear_ptrs(d, q, k, v, freqs, bias))) return rc;
   if (!o) return fail(POPE_ERR_INVALID, "o must be non-NULL");
   const LinShape sh = linear_shape(*d, cu != nullptr);
@@ -1548,7 +1553,7 @@ int pope_gated_norm_fwd(const pope_gated_norm* d, const void* x, const void* gat
   if (d->B == 0 || d->N == 0) return POPE_OK;
   if (!x || !gate || !y) return fail(POPE_ERR_INVALID, "x, gate, y must be non-NULL");
   pope::GatedNormParams p = norm_params(*d, x, gate, weight);
-  p.y = lin_rows(y, d->y_s, d->cols, d->dtype, 8);
+  p.y = norm_rows(y, d->y_s, d->cols, d->dtype);
   const hipError_t e = pope::launch_gated_norm(p, false, reinterpret_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "gated norm launch");
   return POPE_OK;
@@ -1574,9 +1579,9 @@ int pope_gated_norm_bwd(const pope_gated_norm* d, const void* dy, const void* x,
   if (dweight && !weight) return fail(POPE_ERR_INVALID, "dweight wanted, but there is no weight");
   if (dweight && (rc = check_ws(need, workspace, workspace_bytes))) return rc;
   pope::GatedNormParams p = norm_params(*d, x, gate, weight);
-  p.y = lin_rows(dy, d->dy_s, d->cols, d->dtype, 8);
-  p.dx = lin_rows(dx, d->dx_s, d->cols, p.x.type, 8);
-  p.dgate = lin_rows(dgate, d->dgate_s, d->cols, d->dtype, 8);
+  p.y = norm_rows(dy, d->dy_s, d->cols, d->dtype);
+  p.dx = norm_rows(dx, d->dx_s, d->cols, p.x.type);
+  p.dgate = norm_rows(dgate, d->dgate_s, d->cols, d->dtype);
   p.part = dweight ? static_cast<float*>(workspace) : nullptr;
   p.dweight = dweight;
   const hipError_t e = pope::launch_gated_norm(p, true, reinterpret_cast<hipStream_t>(stream));

@@ -51,12 +51,15 @@ struct LinearArgs {
   }
   static bool tracked(const Tensor& t) { return t.defined() && ((t.requires_grad() && at::GradMode::is_enabled()) || t._fw_grad(0).defined()); }
 
-  // Unit feature strides, fp32 angles and states.
+  // Rows as the kernels address them: unit feature stride, and not so far apart that a chunk's offsets pass 32 bits.
+  static Tensor near_rows(const Tensor& t, int n) { return t.stride(-1) == 1 && t.stride(n) < POPE_LINEAR_ROW_STRIDE ? t : t.contiguous(); }
+
+  // Rows near each other, fp32 angles and states.
   LinearArgs convert() const {
     LinearArgs a = *this;
-    for (Tensor* t : {&a.q, &a.k, &a.v}) *t = unit_feature(*t);
-    for (Tensor* t : {&a.freqs, &a.bias})
-      if (t->defined()) *t = unit_feature(t->to(at::kFloat));
+    for (Tensor* t : {&a.q, &a.k, &a.v}) *t = near_rows(*t, n());
+    if (a.freqs.defined()) a.freqs = near_rows(a.freqs.to(at::kFloat), -2);
+    if (a.bias.defined()) a.bias = unit_feature(a.bias.to(at::kFloat));
     if (a.mask.defined() && a.mask.stride(1) != 1) a.mask = a.mask.contiguous();
     if (a.initial.defined()) a.initial = a.initial.to(at::kFloat).contiguous();
     return a;
@@ -129,7 +132,7 @@ LinearGrads linear_backward(const LinearArgs& a, const Tensor& dout0, const Tens
   Tensor dout = dout0;
   if (!dout.defined()) dout = a.rows(d.Hq, d.Dv, a.o_type()).zero_();
   if (dout.scalar_type() != a.o_type()) dout = dout.to(a.o_type());
-  dout = unit_feature(dout);
+  dout = LinearArgs::near_rows(dout, dout.dim() == 4 ? a.n() : 0);
   const Tensor dlast = dlast0.defined() ? dlast0.to(at::kFloat).contiguous() : Tensor();
   check_device(a.q, {&dout, &dlast, &kept});
   TORCH_CHECK_VALUE(dout.dim() == 4 && dout.size(0) == a.q.size(0) && dout.size(a.h()) == d.Hq && dout.size(a.n()) == d.N && dout.size(3) == d.Dv, "dout ", dout.sizes(),
@@ -320,7 +323,9 @@ std::optional<Tensor> linear_step_eager(const Tensor& q, const Tensor& k, const 
                                         OptTensor from, OptTensor to, OptTensor gate, OptTensor weight, double eps, double scale, bool head_first) {
   const StepArgs s{{q, k, v, opt(freqs), opt(bias), opt(log_decay), Tensor(), Tensor(), Tensor(), scale, false, head_first}, state, opt(from), opt(to), opt(gate), opt(weight), eps};
   if (!s.fits()) return std::nullopt;
-  return s.run();
+  const Tensor o = s.run();
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+  return o;
 }
 
 Tensor linear_step_impl(const Tensor& q, const Tensor& k, const Tensor& v, OptTensor freqs, OptTensor bias, OptTensor log_decay, const Tensor& state, OptTensor from, OptTensor to,
@@ -381,7 +386,8 @@ variable_list norm_backward(const NormArgs& a, Tensor dy, bool need_dw) {
   Tensor dw, ws;
   size_t n = 0;
   if (need_dw) {
-    dw = at::zeros(a.weight.sizes(), a.weight.options().requires_grad(false));
+    const auto o = a.weight.options().requires_grad(false);
+    dw = a.x.numel() ? at::empty(a.weight.sizes(), o) : at::zeros(a.weight.sizes(), o);
     check(pope_gated_norm_bytes(&d, &n), "workspace query");
     ws = bytes_like(a.x, n);
   }

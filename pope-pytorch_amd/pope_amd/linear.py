@@ -135,7 +135,7 @@ def _check_norm(x: Tensor, gate: Tensor, weight: Optional[Tensor], heads: int):
     _check_device(x, gate=gate, weight=weight)
     if not 1 <= x.shape[3] <= _MAX_NORM:
         raise ValueError(f"rows must have 1 to {_MAX_NORM} values, got {x.shape[3]}")
-    if x.shape[1] < 1 or x.shape[2] < 1 and heads < 1:
+    if heads < 1:
         raise ValueError(f"x {tuple(x.shape)} has no heads")
     if exists(weight):
         if weight.ndim not in (1, 2) or weight.shape[-1] != x.shape[3] or (weight.ndim == 2 and weight.shape[0] not in (1, heads)):
