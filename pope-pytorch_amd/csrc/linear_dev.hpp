@@ -101,7 +101,7 @@ __device__ __forceinline__ float lin_turns(float b) {
 }
 
 // How a kernel takes its rows: kOne, bf16 rows as operands of one part; kTwo, rows of any type as the sum of two bf16 parts
-// (exactly, for 16-bit rows; 2^-17 off for fp32 ones).
+// (exactly, for 16-bit rows; 2^-16 off for fp32 ones).
 enum LinParts { kOne = 1, kTwo = 2 };
 
 // Rows near each other are addressed by a base that a wave shares and a 32-bit offset in bytes (a chunk of 64 rows, row strides below

@@ -16,8 +16,8 @@
 // chunk.  W's accumulators are in the order in which a product reads an operand, so W goes from one to the next without
 // leaving its registers.
 //
-// Rounding: x, y, z, the weighted C x C products and W as an operand are bf16: one part for bf16 rows (each is off by at most 2^-9,
-// as the output is by its own rounding), the sum of two for fp16 and fp32 rows, and for bf16 rows whose output goes on in fp32 (2^-17;
+// Rounding: x, y, z, the weighted C x C products and W as an operand are bf16: one part for bf16 rows (each is off by at most 2^-8,
+// as the output is by its own rounding), the sum of two for fp16 and fp32 rows, and for bf16 rows whose output goes on in fp32 (2^-16;
 // C is 32 then).  W itself, all sums and the powers of g are fp32.
 #pragma once
 #include <algorithm>

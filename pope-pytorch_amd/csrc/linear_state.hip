@@ -3,7 +3,7 @@
 //   states   the expanded rows (q_hat times the scale, k_hat, as bf16 parts: everything after reads them, forward and backward), and
 //            what the rows of a segment add to the state behind it, sum_j g^(len-1-j) k_hat_j v_j^T; or, in reverse, to the gradient of
 //            the state before it, sum_i g^(i+1) scale q_hat_i dO_i^T.  k_hat is weighted in fp32 and goes into the products as two
-//            bf16 parts: 2^-17 of each, so that states can be handed on from call to call.
+//            bf16 parts: 2^-16 of each, so that states can be handed on from call to call.
 //   sums     the same sums from the expanded rows in memory, for the backward: states that only bf16 gradients read take one part
 //   scan     S <- g^len S + sum, segment by segment; what a segment starts from goes where its sum was
 //   phase    sums of the phases' gradients over segments (bias) and heads (freqs), in a fixed order
