@@ -285,8 +285,8 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
   for (int it = 0; it < turns_n; ++it) {
     const int ch = it / ng, g = it - ch * ng, t0 = ch * C;
     // places are worked out anew each turn: kept across turns, they leave the chains and the two-part products no registers (dq and
-    // dk of 256 columns: 399 us with spills, 194 without); one-part outputs and dv have the room, and save 5 to 8 us in 70
-    if constexpr (chain || PL == kTwo) tv = (int)opaque_u32((uint32_t)tid);
+    // dk of 256 columns: 399 us with spills, 194 without), nor outputs with two tiles a wave; the others have the room, and save 5 to 8 us in 70
+    if constexpr (chain || PL == kTwo || CT > 1) tv = (int)opaque_u32((uint32_t)tid);
     const int lane = tv & 63, q4 = lane >> 4, l16 = lane & 15;
     __syncthreads();   // nothing reads the tiles any more
     store(it);
