@@ -365,6 +365,7 @@ typedef struct pope_linear {
   int32_t B, N, Hq, Hk;      /* sequences; rows per sequence (packed: in all); heads */
   int32_t D, R, Dv;          /* 1 <= D <= 256, 0 <= R <= D, 1 <= Dv <= 256, any values */
   int32_t dtype;             /* enum pope_dtype of rows */
+  int32_t bias_dtype;        /* of the bias and its gradient */
   int32_t o_f32;             /* o and its gradient in fp32, whatever dtype is */
   float scale;
   int64_t q_s[3], k_s[3], v_s[3], o_s[3];      /* (b, h, n) element strides, unit feature stride, any alignment */
@@ -381,15 +382,15 @@ int pope_linear_bytes(const pope_linear* desc, int packed, int final, int want_d
 
 /* o (dtype, o_s), every row; `last` NULL or the states behind the sequences. */
 int pope_linear_fwd(const pope_linear* desc, const void* q, const void* k, const void* v, const float* freqs,
-                    const float* bias, const float* log_decay, const uint8_t* mask, const int32_t* cu_seqlens,
+                    const void* bias, const float* log_decay, const uint8_t* mask, const int32_t* cu_seqlens,
                     const float* initial, void* o, float* last, void* kept, size_t kept_bytes, void* stream);
 
-/* Gradients of o's `dout` and the final states' `dlast` (NULL: zeros): dq, dk, dv (dtype); dfreqs (fp32, df_s), dbias (fp32, rows of
+/* Gradients of o's `dout` and the final states' `dlast` (NULL: zeros): dq, dk, dv (dtype); dfreqs (fp32, df_s), dbias (bias_dtype, rows of
  * R) and dinitial (fp32) or NULL.  All are written, not accumulated into, in a fixed order. */
 int pope_linear_bwd(const pope_linear* desc, const void* dout, const float* dlast, const void* q, const void* k,
-                    const void* v, const float* freqs, const float* bias, const float* log_decay,
+                    const void* v, const float* freqs, const void* bias, const float* log_decay,
                     const uint8_t* mask, const int32_t* cu_seqlens, const float* initial, const void* kept,
-                    size_t kept_bytes, void* dq, void* dk, void* dv, float* dfreqs, float* dbias, float* dinitial,
+                    size_t kept_bytes, void* dq, void* dk, void* dv, float* dfreqs, void* dbias, float* dinitial,
                     void* workspace, size_t workspace_bytes, void* stream);
 
 /*
@@ -420,7 +421,7 @@ int pope_gated_norm_bwd(const pope_gated_norm* desc, const void* dy, const void*
  * cols = Dv; NULL: none) and `gate`, o is the gated norm of the output.
  */
 int pope_linear_step(const pope_linear* desc, const void* q, const void* k, const void* v, const float* freqs,
-                     const float* bias, const float* log_decay, float* states, int32_t slots, int64_t slot_s,
+                     const void* bias, const float* log_decay, float* states, int32_t slots, int64_t slot_s,
                      const int32_t* from, const int32_t* to, const pope_gated_norm* norm, const void* gate,
                      const void* weight, void* o, void* stream);
 

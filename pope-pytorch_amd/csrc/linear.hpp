@@ -36,7 +36,7 @@ struct LinCall {
   LinRows q, k, v, g;            // g: dO
   LinHat qh, kh;                 // queries times the scale; keys that the mask leaves out are zeros
   const float* freqs; int64_t f_s[2]; int f_vec;
-  const float* bias; int64_t bias_sh;
+  const void* bias; int bias_type; int64_t bias_sh;   // pope_dtype
   const float* log_decay;        // one for each kv head, or null: no decay
   const uint8_t* mask; int64_t mask_sb;
   int Hq, Hk, G, D, R, E, Dv;    // E = D + R
@@ -88,7 +88,7 @@ hipError_t launch_linear_dv_split(const LinOutParams& p, hipStream_t s);
 // dbias (Hb, R) from the segments' parts; dfreqs (Fb, N, R) from the rows' dphase of queries and keys.
 struct LinPhaseParams {
   LinCall c;
-  const float* part; float* dbias; int Hb;
+  const float* part; void* dbias; int Hb;   // dbias in the bias's type
   const float* dphase_q; const float* dphase_k; float* dfreqs; int64_t df_s[2]; int Fb;
 };
 hipError_t launch_linear_phase(const LinPhaseParams& p, hipStream_t s);

@@ -290,6 +290,7 @@ __device__ __forceinline__ void lin_set2(const LinRows& r, char* base, uint32_t 
 __device__ __forceinline__ float lin_value(const void* p, int type, int64_t i) {
   return type == 0 ? static_cast<const float*>(p)[i] : type == 1 ? F16::to_float(static_cast<const uint16_t*>(p)[i]) : BF16::to_float(static_cast<const uint16_t*>(p)[i]);
 }
+__device__ __forceinline__ float lin_bias(const LinCall& c, int hk, int d) { return lin_value(c.bias, c.bias_type, hk * c.bias_sh + d); }
 
 __device__ __forceinline__ void lin_angles8(const float* row, int d0, int R, bool vec, f32x4* f) {
   f[0] = f[1] = f32x4{0.f, 0.f, 0.f, 0.f};

@@ -280,7 +280,7 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
   for (int i = tid; i < kTileBytes / 16; i += kThreads) reinterpret_cast<u32x4*>(smem)[i] = u32x4{0, 0, 0, 0};
   if (tid < 2) odd[tid] = 0;
   if (kind == kLinDk)
-    for (int d = tid; d < c.R; d += kThreads) turns[d] = lin_turns(c.bias[hk * c.bias_sh + d]);
+    for (int d = tid; d < c.R; d += kThreads) turns[d] = lin_turns(lin_bias(c, hk, d));
 
   for (int it = 0; it < turns_n; ++it) {
     const int ch = it / ng, g = it - ch * ng, t0 = ch * C;

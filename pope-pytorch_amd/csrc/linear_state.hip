@@ -131,7 +131,7 @@ __global__ __launch_bounds__(K::kThreads, 1) void linear_state_kernel(LinStatePa
   for (int i = tid; i < (int)sizeof(lds) / 16; i += K::kThreads) reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
   const bool rev = p.reverse != 0;
   if (!rev)
-    for (int d = tid; d < c.R; d += K::kThreads) turns[d] = lin_turns(c.bias[hk * c.bias_sh + d]);
+    for (int d = tid; d < c.R; d += K::kThreads) turns[d] = lin_turns(lin_bias(c, hk, d));
   const float lg = lin_log2(c, hk);
   const int n0 = tile * NT, col0 = wave * K::SL, steps = (c.E + 31) / 32, G = rev ? c.G : 1;
   const bool busy = n0 + col0 < c.Dv;
@@ -468,7 +468,12 @@ __global__ __launch_bounds__(256) void linear_dbias_kernel(LinPhaseParams p) {
       for (int s = q; s < c.seqs.T; s += 4) sum += p.part[((int64_t)s * c.Hk + h) * c.R + d];
   red[q][threadIdx.x & 63] = sum;
   __syncthreads();
-  if (q == 0 && d < c.R) p.dbias[(int64_t)h0 * c.R + d] = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+  if (q == 0 && d < c.R) {
+    const float v = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+    const int64_t at = (int64_t)h0 * c.R + d;
+    if (c.bias_type == 0) static_cast<float*>(p.dbias)[at] = v;
+    else static_cast<uint16_t*>(p.dbias)[at] = c.bias_type == 1 ? F16::bits(v) : BF16::bits(v);
+  }
 }
 
 // A thread per (table batch, row, dim).

@@ -37,13 +37,13 @@ __global__ __launch_bounds__(kThreads) void linear_step_kernel(LinStepParams p) 
   float* dst = p.to + (int64_t)to * p.slot_s + (int64_t)hk * E * Dv;
   const bool store = some && (unsigned)to < (unsigned)p.slots;
 
-  const auto expand = [&](const LinRows& rows, int h, const float* bias, float factor, float* to_lds) {
+  const auto expand = [&](const LinRows& rows, int h, bool key, float factor, float* to_lds) {
     const int64_t x = (int64_t)b * rows.s[0] + (int64_t)h * rows.s[1];
     for (int d = tid; d < c.D; d += kThreads) {
       const float v = lin_get<kTwo>(rows, x + d);
       if (d < R) {
         float sn, cs;
-        sincos_turns(lin_angle_row(c, b, 0)[d], bias ? lin_turns(bias[d]) : 0.f, &sn, &cs);
+        sincos_turns(lin_angle_row(c, b, 0)[d], key ? lin_turns(lin_bias(c, hk, d)) : 0.f, &sn, &cs);
         const float m = softplus_f(v) * factor;
         to_lds[2 * d] = m * cs;
         to_lds[2 * d + 1] = m * sn;
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(kThreads) void linear_step_kernel(LinStepParams p) 
       }
     }
   };
-  expand(c.k, hk, R ? c.bias + hk * c.bias_sh : nullptr, 1.f, kh);
+  expand(c.k, hk, true, 1.f, kh);
   float v[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r)
@@ -64,7 +64,7 @@ __global__ __launch_bounds__(kThreads) void linear_step_kernel(LinStepParams p) 
     if (MORE && g0) __syncthreads();
 #pragma unroll
     for (int g = 0; g < GM; ++g)
-      if (g0 + g < c.G) expand(c.q, (g0 + g) * c.Hk + hk, nullptr, c.scale, qh[g]);
+      if (g0 + g < c.G) expand(c.q, (g0 + g) * c.Hk + hk, false, c.scale, qh[g]);
     __syncthreads();
     f32x4 o[GM];
 #pragma unroll

@@ -1283,6 +1283,7 @@ int check_linear(const pope_linear* d) {
     return fail(POPE_ERR_UNSUPPORTED, "linear attention covers head and value dims 1 to 256 (got %d, %d)", d->D, d->Dv);
   if (d->R < 0 || d->R > d->D) return fail(POPE_ERR_INVALID, "rotate dim %d must be in [0, head dim %d]", d->R, d->D);
   if (d->dtype != POPE_F32 && d->dtype != POPE_F16 && d->dtype != POPE_BF16) return fail(POPE_ERR_INVALID, "unknown dtype %d", d->dtype);
+  if (d->bias_dtype != POPE_F32 && d->bias_dtype != POPE_F16 && d->bias_dtype != POPE_BF16) return fail(POPE_ERR_INVALID, "unknown bias dtype %d", d->bias_dtype);
   if (d->N > (1 << 28) || d->B > (1 << 20) || d->Hq > 65535)
     return fail(POPE_ERR_UNSUPPORTED, "%d sequences, %d rows, %d heads: too many", d->B, d->N, d->Hq);
   if (d->bias_sh < 0 || d->mask_sb < 0) return fail(POPE_ERR_INVALID, "negative bias / mask stride");
@@ -1356,7 +1357,7 @@ pope::LinHat lin_hat(const void* p, size_t bytes, const LinShape& s, int H) {
 
 // hats: the expanded rows, or null.
 pope::LinCall linear_call(const pope_linear& d, const LinShape& s, const void* hats, const void* q, const void* k, const void* v, const float* freqs,
-                          const float* bias, const float* log_decay, const uint8_t* mask, const int32_t* cu) {
+                          const void* bias, const float* log_decay, const uint8_t* mask, const int32_t* cu) {
   pope::LinCall c;
   std::memset(&c, 0, sizeof c);
   c.seqs = pope::LinSeqs{cu, d.B, d.N, s.L, s.M, s.T};
@@ -1366,7 +1367,7 @@ pope::LinCall linear_call(const pope_linear& d, const LinShape& s, const void* h
   c.freqs = freqs;
   c.f_s[0] = d.f_s[0]; c.f_s[1] = d.f_s[1];
   c.f_vec = d.R % 8 == 0 && aligned16(freqs) && d.f_s[0] % 4 == 0 && d.f_s[1] % 4 == 0;
-  c.bias = bias; c.bias_sh = d.bias_sh;
+  c.bias = bias; c.bias_type = d.bias_dtype; c.bias_sh = d.bias_sh;
   c.log_decay = log_decay;
   c.mask = mask; c.mask_sb = d.mask_sb;
   c.Hq = d.Hq; c.Hk = d.Hk; c.G = d.Hq / d.Hk; c.D = d.D; c.R = d.R; c.E = d.D + d.R; c.Dv = d.Dv;
@@ -1382,7 +1383,7 @@ pope::LinCall linear_call(const pope_linear& d, const LinShape& s, const void* h
   return c;
 }
 
-int check_linear_ptrs(const pope_linear* d, const void* q, const void* k, const void* v, const float* freqs, const float* bias) {
+int check_linear_ptrs(const pope_linear* d, const void* q, const void* k, const void* v, const float* freqs, const void* bias) {
   if (!q || !k || !v) return fail(POPE_ERR_INVALID, "q, k, v must be non-NULL");
   if (d->R > 0 && (!freqs || !bias)) return fail(POPE_ERR_INVALID, "rotate dim %d > 0 needs freqs and bias", d->R);
   return POPE_OK;
@@ -1448,7 +1449,7 @@ int pope_linear_bytes(const pope_linear* d, int packed, int final, int want_dfre
   return POPE_OK;
 }
 
-int pope_linear_fwd(const pope_linear* d, const void* q, const void* k, const void* v, const float* freqs, const float* bias,
+int pope_linear_fwd(const pope_linear* d, const void* q, const void* k, const void* v, const float* freqs, const void* bias,
                     const float* log_decay, const uint8_t* mask, const int32_t* cu, const float* initial, void* o, float* last,
                     void* kept, size_t kept_bytes, void* stream) {
   int rc = check_linear(d);
@@ -1482,9 +1483,9 @@ int pope_linear_fwd(const pope_linear* d, const void* q, const void* k, const vo
 }
 
 int pope_linear_bwd(const pope_linear* d, const void* dout, const float* dlast, const void* q, const void* k, const void* v,
-                    const float* freqs, const float* bias, const float* log_decay, const uint8_t* mask, const int32_t* cu,
+                    const float* freqs, const void* bias, const float* log_decay, const uint8_t* mask, const int32_t* cu,
                     const float* initial, const void* kept, size_t kept_bytes, void* dq, void* dk, void* dv, float* dfreqs,
-                    float* dbias, float* dinitial, void* workspace, size_t workspace_bytes, void* stream) {
+                    void* dbias, float* dinitial, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_linear(d);
   if (rc) return rc;
   for (const int64_t* st : {d->do_s, d->dq_s, d->dk_s, d->dv_s})
@@ -1589,7 +1590,7 @@ int pope_gated_norm_bwd(const pope_gated_norm* d, const void* dy, const void* x,
   return POPE_OK;
 }
 
-int pope_linear_step(const pope_linear* d, const void* q, const void* k, const void* v, const float* freqs, const float* bias,
+int pope_linear_step(const pope_linear* d, const void* q, const void* k, const void* v, const float* freqs, const void* bias,
                      const float* log_decay, float* states, int32_t slots, int64_t slot_s, const int32_t* from, const int32_t* to,
                      const pope_gated_norm* norm, const void* gate, const void* weight, void* o, void* stream) {
   int rc = check_linear(d);

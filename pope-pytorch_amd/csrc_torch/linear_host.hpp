@@ -54,12 +54,12 @@ struct LinearArgs {
   // Rows as the kernels address them: unit feature stride, and not so far apart that a chunk's offsets pass 32 bits.
   static Tensor near_rows(const Tensor& t, int n) { return t.stride(-1) == 1 && t.stride(n) < POPE_LINEAR_ROW_STRIDE ? t : t.contiguous(); }
 
-  // Rows near each other, fp32 angles and states.
+  // Rows near each other, fp32 angles and states; the bias is read as it is.
   LinearArgs convert() const {
     LinearArgs a = *this;
     for (Tensor* t : {&a.q, &a.k, &a.v}) *t = near_rows(*t, n());
     if (a.freqs.defined()) a.freqs = near_rows(a.freqs.to(at::kFloat), -2);
-    if (a.bias.defined()) a.bias = unit_feature(a.bias.to(at::kFloat));
+    if (a.bias.defined()) a.bias = unit_feature(a.bias);
     if (a.mask.defined() && a.mask.stride(1) != 1) a.mask = a.mask.contiguous();
     if (a.initial.defined()) a.initial = a.initial.to(at::kFloat).contiguous();
     return a;
@@ -85,6 +85,7 @@ struct LinearArgs {
     if (freqs.defined()) {
       d.f_s[0] = freqs.dim() == 3 && freqs.size(0) > 1 ? freqs.stride(0) : 0;
       d.f_s[1] = freqs.stride(-2);
+      d.bias_dtype = dtype_code(bias);
       d.bias_sh = bias.size(0) > 1 ? bias.stride(0) : 0;
     }
     if (mask.defined()) d.mask_sb = mask.stride(0);
@@ -116,7 +117,7 @@ LinearOut linear_forward(const LinearArgs& a) {   // converted operands
   size_t n[2] = {0, 0};
   check(pope_linear_bytes(&d, a.cu.defined(), a.with_state, 0, n), "workspace query");
   r.kept = bytes_like(a.q, n[0]);
-  check(pope_linear_fwd(&d, a.q.data_ptr(), a.k.data_ptr(), a.v.data_ptr(), floats(a.freqs), floats(a.bias), floats(a.log_decay), bytes_of(a.mask), ints_of(a.cu),
+  check(pope_linear_fwd(&d, a.q.data_ptr(), a.k.data_ptr(), a.v.data_ptr(), floats(a.freqs), data(a.bias), floats(a.log_decay), bytes_of(a.mask), ints_of(a.cu),
                         floats(a.initial), r.o.data_ptr(), static_cast<float*>(data(r.last)), data(r.kept), n[0], stream_of(a.q)),
         "linear attention");
   return r;
@@ -150,15 +151,15 @@ LinearGrads linear_backward(const LinearArgs& a, const Tensor& dout0, const Tens
     d.df_s[0] = a.freqs.dim() == 3 && a.freqs.size(0) > 1 ? r.dfreqs.stride(0) : 0;
     d.df_s[1] = r.dfreqs.stride(-2);
   }
-  if (need_db) r.dbias = fp32_like(a.q, a.bias.sizes());
+  if (need_db) r.dbias = at::empty(a.bias.sizes(), a.bias.options().requires_grad(false));
   if (need_d0) r.dinitial = fp32_like(a.q, {d.B, d.Hk, d.D + d.R, d.Dv});
   TORCH_CHECK_VALUE(!dlast.defined() || dlast.numel() == (int64_t)d.B * d.Hk * (d.D + d.R) * d.Dv, "the states' gradient ", dlast.sizes(), " does not fit");
   size_t n[2] = {0, 0};
   check(pope_linear_bytes(&d, a.cu.defined(), 0, need_df, n), "workspace query");
   const Tensor ws = bytes_like(a.q, n[1]);
-  check(pope_linear_bwd(&d, dout.data_ptr(), floats(dlast), a.q.data_ptr(), a.k.data_ptr(), a.v.data_ptr(), floats(a.freqs), floats(a.bias), floats(a.log_decay),
+  check(pope_linear_bwd(&d, dout.data_ptr(), floats(dlast), a.q.data_ptr(), a.k.data_ptr(), a.v.data_ptr(), floats(a.freqs), data(a.bias), floats(a.log_decay),
                         bytes_of(a.mask), ints_of(a.cu), floats(a.initial), data(kept), kept.defined() ? kept.nbytes() : 0, r.dq.data_ptr(), r.dk.data_ptr(),
-                        r.dv.data_ptr(), static_cast<float*>(data(r.dfreqs)), static_cast<float*>(data(r.dbias)), static_cast<float*>(data(r.dinitial)), data(ws), n[1],
+                        r.dv.data_ptr(), static_cast<float*>(data(r.dfreqs)), data(r.dbias), static_cast<float*>(data(r.dinitial)), data(ws), n[1],
                         stream_of(a.q)),
         "linear attention backward");
   return r;
@@ -207,14 +208,14 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
       using O = OptTensor;
       std::tie(r.dq, r.dk, r.dv, r.dfreqs, r.dbias, r.dinitial) =
           op<Grads6(const Tensor&, O, const Tensor&, const Tensor&, const Tensor&, O, O, O, O, O, O, O, double, bool, bool, bool, bool)>("pope_amd::linear_bwd")
-              .call(dout, maybe(dlast), front(sv[0]), front(sv[1]), front(sv[2]), maybe(f32(sv[3])), maybe(f32(sv[4])), maybe(sv[6]), maybe(sv[7]), maybe(sv[8]),
+              .call(dout, maybe(dlast), front(sv[0]), front(sv[1]), front(sv[2]), maybe(f32(sv[3])), maybe(sv[4]), maybe(sv[6]), maybe(sv[7]), maybe(sv[8]),
                     maybe(f32(sv[5])), maybe(sv[9]), raw.scale, raw.o_f32, ndf, ndb, nd0);
       r.dq = front(r.dq), r.dk = front(r.dk), r.dv = front(r.dv);
     } else {
       r = linear_backward(raw.convert(), grads[0], dlast, sv[9], ndf, ndb, nd0);
     }
     const auto like = [](const Tensor& g, const Tensor& t, bool want) { return want ? (g.scalar_type() == t.scalar_type() ? g : g.to(t.scalar_type())) : Tensor(); };
-    variable_list out{r.dq, r.dk, r.dv, like(r.dfreqs, sv[3], ndf), like(r.dbias, sv[4], ndb), like(r.dinitial, sv[5], nd0)};
+    variable_list out{r.dq, r.dk, r.dv, like(r.dfreqs, sv[3], ndf), ndb ? r.dbias : Tensor(), like(r.dinitial, sv[5], nd0)};
     out.resize(13);
     return on_ops(grads) ? out : once_differentiable(std::move(out), "linear attention");
   }
@@ -312,7 +313,7 @@ struct StepArgs {
       c.strides(n.gate_s, gate);
     }
     const int64_t slot = state.size(0) > 1 ? state.stride(0) : state.size(1) * state.size(2) * state.size(3);
-    check(pope_linear_step(&d, c.q.data_ptr(), c.k.data_ptr(), c.v.data_ptr(), floats(c.freqs), floats(c.bias), floats(c.log_decay), static_cast<float*>(state.data_ptr()),
+    check(pope_linear_step(&d, c.q.data_ptr(), c.k.data_ptr(), c.v.data_ptr(), floats(c.freqs), data(c.bias), floats(c.log_decay), static_cast<float*>(state.data_ptr()),
                            (int32_t)state.size(0), slot, ints_of(from), ints_of(to), gate.defined() ? &n : nullptr, data(gate), data(weight), o.data_ptr(), stream_of(a.q)),
           "linear attention step");
     return o;

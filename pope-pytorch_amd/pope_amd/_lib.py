@@ -64,7 +64,7 @@ class PopeLinear(ctypes.Structure):
 
     _fields_ = [
         ("B", ctypes.c_int32), ("N", ctypes.c_int32), ("Hq", ctypes.c_int32), ("Hk", ctypes.c_int32), ("D", ctypes.c_int32),
-        ("R", ctypes.c_int32), ("Dv", ctypes.c_int32), ("dtype", ctypes.c_int32), ("o_f32", ctypes.c_int32),
+        ("R", ctypes.c_int32), ("Dv", ctypes.c_int32), ("dtype", ctypes.c_int32), ("bias_dtype", ctypes.c_int32), ("o_f32", ctypes.c_int32),
         ("scale", ctypes.c_float), ("q_s", _I64x3), ("k_s", _I64x3), ("v_s", _I64x3), ("o_s", _I64x3), ("do_s", _I64x3), ("dq_s", _I64x3),
         ("dk_s", _I64x3), ("dv_s", _I64x3), ("f_s", ctypes.c_int64 * 2), ("bias_sh", ctypes.c_int64), ("df_s", ctypes.c_int64 * 2), ("mask_sb", ctypes.c_int64),
     ]

@@ -71,7 +71,7 @@ def _check_rows(q: Tensor, k: Tensor, v: Tensor):
 
 
 def _check_pos_emb(pos_emb, q: Tensor, heads: int):
-    """freqs (n, R) or (1 or batch, n, R) and bias (1 or heads, R) in fp32; None, None without rotation."""
+    """freqs (n, R) or (1 or batch, n, R) and bias (1 or heads, R); None, None without rotation."""
     if not exists(pos_emb):
         return None, None
     freqs, bias = pos_emb
@@ -90,7 +90,7 @@ def _check_pos_emb(pos_emb, q: Tensor, heads: int):
     if bias.ndim != 2 or bias.shape[1] != R or bias.shape[0] not in (1, heads):
         raise ValueError(f"bias {tuple(bias.shape)} must be (1 or {heads}, {R})")
     _check_device(q, freqs=freqs, bias=bias)
-    return freqs.float(), bias.float()
+    return freqs.float(), bias if bias.dtype in _DTYPES else bias.float()
 
 
 def _check_decay(log_decay: Optional[Tensor], q: Tensor, heads: int):
@@ -178,7 +178,7 @@ def linear_bwd_op(dout: Tensor, dlast: Optional[Tensor], q: Tensor, k: Tensor, v
 def _(dout, dlast, q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial, kept, scale, o_f32, need_dfreqs, need_dbias, need_dinitial):
     some = lambda shape, want: q.new_empty(shape if want else (0,), dtype=torch.float32)
     return (q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape), some(freqs.shape if need_dfreqs else (0,), need_dfreqs),
-            some(bias.shape if need_dbias else (0,), need_dbias), some(_linear_state_shape(q, k, v, freqs, cu_seqlens), need_dinitial))
+            q.new_empty(bias.shape, dtype=bias.dtype) if need_dbias else some((0,), False), some(_linear_state_shape(q, k, v, freqs, cu_seqlens), need_dinitial))
 
 
 def _linear_setup(ctx, inputs, output):
