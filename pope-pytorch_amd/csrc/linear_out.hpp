@@ -180,31 +180,32 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
     return i.d0 < NT && n0 + i.d0 < zcols && put(Bool<z_hat>{}, Bool<z_key>{}, Bool<false>{}, zr, Z, n.t0, i, o);
   };
   const bool whole_rows = (x_hat || xr.vec) && (y_hat || yr.vec) && (z_hat || zr.vec);
-  // Narrow tiles are loaded a chunk ahead, into registers; wide ones, whose state takes those, chunk by chunk.
+  // Narrow tiles are loaded a chunk ahead, into registers; wide ones, whose state takes those, when the chunk's turn
+  // begins: x and z at once, then y in the registers that these leave; where eight waves have a chain's wide state, two at a time (dq and
+  // dk of 256 columns: 222 us against 194).
   constexpr bool kAhead = P <= 128 && NT <= 128;
-  constexpr int kTX = kAhead ? K::TP : 0, kTZ = kAhead ? K::TZ : 0;
-  Part xin[kTX + 1], yin[kTX + 1], zin[kTZ + 1];
-  const auto load_as = [&](auto whole, int it) {
+  constexpr bool kFew = chain && P > 128 && K::NW == 8;
+  constexpr int kTX = K::TP, kTZ = K::TZ;
+  Part xin[kTX], yin[kTX], zin[kTZ];
+  const auto load_as = [&](auto whole, int it, bool xz, bool y) {
     const Turn n = turn_of(it);
     const Bases b = bases_of(n);
-    if (n.lx)
+    if (xz && n.lx)
 #pragma unroll
       for (int u = 0; u < kTX; ++u) xin[u] = get_x(whole, n, b, u);
-    if (n.lyz) {
-#pragma unroll
-      for (int u = 0; u < kTX; ++u) yin[u] = get_y(whole, n, b, u);
+    if (xz && n.lyz)
 #pragma unroll
       for (int u = 0; u < kTZ; ++u) zin[u] = get_z(whole, n, b, u);
-    }
+    if (y && n.lyz)
+#pragma unroll
+      for (int u = 0; u < kTX; ++u) yin[u] = get_y(whole, n, b, u);
   };
-  const auto load = [&](int it) {
-    if constexpr (kAhead) {
-      if (whole_rows) load_as(Bool<true>{}, it);
-      else load_as(Bool<false>{}, it);
-    }
+  const auto load = [&](int it, bool xz, bool y) {
+    if (whole_rows) load_as(Bool<true>{}, it, xz, y);
+    else load_as(Bool<false>{}, it, xz, y);
   };
   const auto turns_for = [&](int cols) { return (C * ((cols + 31) / 32 * 4) + kThreads - 1) / kThreads; };
-  const auto store_as = [&](auto whole, const Turn& n) {   // loaded here
+  const auto store_few = [&](auto whole, const Turn& n) {
     const Bases b = bases_of(n);
     bool some = false;
     const int txy = turns_for(xcols);
@@ -226,26 +227,31 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
   const auto store = [&](int it) {
     const Turn n = turn_of(it);
     bool some = false;
-    if constexpr (kAhead) {
-      if (n.lx)
-#pragma unroll
-        for (int u = 0; u < kTX; ++u) put_x(n, u, xin[u]);
-      if (n.lyz) {
-#pragma unroll
-        for (int u = 0; u < kTX; ++u) put_y(n, u, yin[u]);
-#pragma unroll
-        for (int u = 0; u < kTZ; ++u) some |= put_z(n, u, zin[u]);
-      }
-    } else {
-      some = whole_rows ? store_as(Bool<true>{}, n) : store_as(Bool<false>{}, n);
+    if constexpr (kFew) {
+      some = whole_rows ? store_few(Bool<true>{}, n) : store_few(Bool<false>{}, n);
+      if (some) odd[it & 1] = 1;
+      return;
     }
+    if (n.lx)
+#pragma unroll
+      for (int u = 0; u < kTX; ++u) put_x(n, u, xin[u]);
+    if (n.lyz)
+#pragma unroll
+      for (int u = 0; u < kTZ; ++u) some |= put_z(n, u, zin[u]);
+    if constexpr (!kAhead) load(it, false, true);
+    if (n.lyz)
+#pragma unroll
+      for (int u = 0; u < kTX; ++u) put_y(n, u, yin[u]);
     if (some) odd[it & 1] = 1;
   };
 
+  // A row alone: the norm behind it leaves of its gradient what is at right angles to the row itself, so dO . v is a sum that all but
+  // cancels, 500 times and more.  That product, and the row's own direction, are in fp32 then.
+  const bool lone = PL == kTwo && seg.len == 1;
   f32x4 O[CT][IT];
   const int turns_n = chunks * ng;
   bool odd_z = false;
-  load(0);
+  if constexpr (kAhead) load(0, true, true);
   // W: accumulators of 16-row tiles 4 q4 + i x columns l16
   f32x4 W[CT][2 * ST];
 #pragma unroll
@@ -285,14 +291,15 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
   for (int it = 0; it < turns_n; ++it) {
     const int ch = it / ng, g = it - ch * ng, t0 = ch * C;
     // places are worked out anew each turn: kept across turns, they leave the chains and the two-part products no registers (dq and
-    // dk of 256 columns: 399 us with spills, 194 without), nor outputs with two tiles a wave; the others have the room, and save 5 to 8 us in 70
-    if constexpr (chain || PL == kTwo || CT > 1) tv = (int)opaque_u32((uint32_t)tid);
+    // dk of 256 columns: 399 us with spills, 194 without), nor wide states and outputs with two tiles a wave; the others have the room, and save 5 to 8 us in 70
+    if constexpr (chain || PL == kTwo || CT > 1 || P > 128) tv = (int)opaque_u32((uint32_t)tid);
     const int lane = tv & 63, q4 = lane >> 4, l16 = lane & 15;
+    if constexpr (!kAhead && !kFew) load(it, true, false);
     __syncthreads();   // nothing reads the tiles any more
     store(it);
-    if (it + 1 < turns_n) load(it + 1);
+    if (kAhead && it + 1 < turns_n) load(it + 1, true, true);
     __syncthreads();
-    if (!by_query || g == 0) odd_z = odd[it & 1] != 0;
+    if (!by_query || g == 0) odd_z = odd[it & 1] != 0 || lone;
     // x . y of the rows of 16 x 16 tiles j <= i, weighted: a wave has tiles of one i
     {
       constexpr int kShare = K::NW / IT, kTiles = IT > kShare ? IT / kShare : 1;
@@ -315,6 +322,16 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
           for (int j = 0; j < kTiles; ++j)
             if (j0 + j * kShare <= ti) sc[j] = lin_mfma<PL, PL>(ya[j], xa, sc[j]);
         }
+      if (chain && lone && wave == 0) {
+        const int64_t row = base_row(0) + place(0);
+        const int hq = turn_of(it).hq;
+        float dot = 0.f;
+        for (int d = lane; d < c.Dv; d += 64)
+          dot += lin_get<PL>(c.g, seg.batch * c.g.s[0] + hq * c.g.s[1] + row * c.g.s[2] + d) * lin_get<PL>(c.v, seg.batch * c.v.s[0] + hk * c.v.s[1] + row * c.v.s[2] + d);
+#pragma unroll
+        for (int m = 1; m < 64; m *= 2) dot += wave_shfl_xor(dot, m);
+        if (lane == 0) sc[0][0] = kept(mask_base(0), 0) ? dot : 0.f;
+      }
 #pragma unroll
       for (int j = 0; j < kTiles; ++j) {
         if (j0 + j * kShare > ti) continue;
@@ -419,7 +436,7 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
 #pragma unroll
         for (int i = 0; i < IT; ++i)
 #pragma unroll 1
-          for (int j = 0; j <= 16 * i + l16; ++j) {
+          for (int j = 0; j <= 16 * i + l16 && !(lone && j); ++j) {
             float w = 0.f;
             for (int l = 0; l < PL; ++l) w += BF16::to_float(A.p[l * A.plane + (16 * i + l16) * K::AS + lin_place<true>(j)]);
 #pragma unroll
