@@ -75,7 +75,7 @@ struct LinOutParams {
   float* dbias;                  // kLinDk: (T, Hk, R), or null
   float* dphase[2];              // (b, h, n, R) of the kind's rows, or null
   int heads_per;                 // query heads of a key head per workgroup (kLinOut, kLinDq)
-  int tiles, wgs;                // set by the launchers
+  int tiles, first_wgs;          // set by the launchers
 };
 // One translation unit each.
 hipError_t launch_linear_out_bf16(const LinOutParams& p, hipStream_t s);

@@ -581,19 +581,19 @@ constexpr int lin_out_waves() {
   return 2;
 }
 
-// KIND kLinDq: dq and dk, in one launch.
+// KIND kLinDq: dk and dq, in one launch; dk first, whose workgroups take all query heads of a key head and so the longest.
 template <typename K, int KIND>
 __global__ __launch_bounds__(K::kThreads, (lin_out_waves<K, KIND>())) void linear_out_kernel(LinOutParams p) {
   constexpr int kBytes = lin_out_bytes<K, KIND>();
   __shared__ __attribute__((aligned(16))) char smem[kBytes];
   const int wg = blockIdx.x;
   if constexpr (KIND == kLinDq) {
-    if (wg >= p.wgs) {
-      lin_out_job<K, kLinDk>(p, wg - p.wgs, smem);
+    if (wg < p.first_wgs) {
+      lin_out_job<K, kLinDk>(p, wg, smem);
       return;
     }
   }
-  lin_out_job<K, KIND>(p, wg, smem);
+  lin_out_job<K, KIND>(p, wg - p.first_wgs, smem);
 }
 
 template <int KIND>
@@ -604,9 +604,9 @@ struct LinOutLaunch {
       const LinCall& c = p.c;
       const int64_t segs = c.seqs.T + (c.seqs.cu ? 1 : 0);
       p.tiles = ((KIND == kLinDq ? c.E : c.Dv) + K::NT - 1) / K::NT;
-      const int64_t n = segs * p.tiles * c.Hk * (KIND == kLinDv ? 1 : c.G / p.heads_per), all = n + (KIND == kLinDq ? segs * p.tiles * c.Hk : 0);
+      const int64_t n = segs * p.tiles * c.Hk, first = KIND == kLinDq ? n : 0, all = first + n * (KIND == kLinDv ? 1 : c.G / p.heads_per);
       if (all >= ((int64_t)1 << 22)) return hipErrorInvalidValue;
-      p.wgs = (int)n;
+      p.first_wgs = (int)first;
       return launch_named(name, linear_out_kernel<K, KIND>, dim3((unsigned)all), dim3(K::kThreads), s, p);
     }
   };

@@ -1297,12 +1297,13 @@ int check_linear(const pope_linear* d) {
   return rc;
 }
 
-// Workgroups that the chip holds at once: two for each CU, one where rows or states are wide.
+// Workgroups that the chip holds at once: two for each CU, half of that where rows or states are wide.
 constexpr int kLinGrid = 512, kLinChunk = 64;
 
 struct LinShape {
   int L, M, T;
   bool parts;      // some sequence may have more than one segment
+  int grid;        // workgroups that the chip holds at once
   int EP, planes;  // columns of expanded rows in memory; their bf16 parts
   size_t qh, kh, states;   // bytes of the expanded rows and of the states of all segments
 };
@@ -1320,6 +1321,7 @@ LinShape linear_shape(const pope_linear& d, bool packed) {
   s.M = std::max(1, (d.N + s.L - 1) / s.L);
   s.T = packed ? (int)std::min<int64_t>(d.N, (int64_t)d.N / s.L + d.B) : d.B * s.M;
   s.parts = d.N > s.L;
+  s.grid = (int)grid;
   s.EP = round_up(d.D + d.R, 32);
   s.planes = d.dtype != POPE_BF16 || d.o_f32 ? 2 : 1;
   s.qh = align_up((size_t)rows * d.Hq * s.EP * 2) * s.planes;
@@ -1389,12 +1391,21 @@ int check_linear_ptrs(const pope_linear* d, const void* q, const void* k, const 
   return POPE_OK;
 }
 
-// Query heads of a key head per workgroup: all, where that fills the chip, or as many as divide them.
-int lin_heads_per(const pope_linear& d, const LinShape& s) {
-  const int G = d.Hq / d.Hk;
-  for (int n = G; n > 1; --n)
-    if (G % n == 0 && (int64_t)s.T * d.Hk * (G / n) >= kLinGrid) return n;
-  return 1;
+// Query heads of a key head per workgroup.  A workgroup of n heads takes as long as its state's load (about two turns) and n turns for
+// each chunk; the chip holds a grid's worth at once, and the backward's other workgroups, dk's, take all G heads of a key head and go
+// first.  16 heads on 4, 2,999 rows of 128 + 64 columns in two parts: 1, 2 and 4 heads take 83, 78 and 63 us forward, 124, 113 and 120
+// us for dq and dk.
+int lin_heads_per(const pope_linear& d, const LinShape& s, bool backward) {
+  const int64_t G = d.Hq / d.Hk, jobs = (int64_t)s.T * d.Hk, chunks = s.L / (s.planes == 2 ? 32 : 64), grid = s.grid;
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int64_t n = 1; n <= G; ++n) {
+    if (G % n) continue;
+    const int64_t turns = 2 + chunks * n, count = jobs * (G / n);
+    const int64_t cost = backward ? (count * turns + jobs * (2 + chunks * G)) * 2 / grid + turns : 2 * ((count + grid - 1) / grid) * turns;
+    if (cost < least) least = cost, best = (int)n;
+  }
+  return best;
 }
 
 int lin_fail(hipError_t e, const char* what) {
@@ -1477,7 +1488,7 @@ int pope_linear_fwd(const pope_linear* d, const void* q, const void* k, const vo
   p.out[0] = lin_rows(o, d->o_s, d->Dv, d->o_f32 ? POPE_F32 : d->dtype, 4);
   p.states[0] = seg_states;
   p.first[0] = initial;
-  p.heads_per = lin_heads_per(*d, sh);
+  p.heads_per = lin_heads_per(*d, sh, false);
   if ((e = c.split ? pope::launch_linear_out_split(p, s) : pope::launch_linear_out_bf16(p, s)) != hipSuccess) return lin_fail(e, "linear attention launch");
   return POPE_OK;
 }
@@ -1520,7 +1531,7 @@ int pope_linear_bwd(const pope_linear* d, const void* dout, const float* dlast, 
   p.first[0] = initial;
   p.states[1] = sums ? reverse : nullptr;
   p.first[1] = dlast;
-  p.heads_per = lin_heads_per(*d, sh);
+  p.heads_per = lin_heads_per(*d, sh, true);
   p.out[0] = lin_rows(dq, d->dq_s, d->D, d->dtype, 4);
   p.out[1] = lin_rows(dk, d->dk_s, d->D, d->dtype, 4);
   if (d->R > 0) {
