@@ -11,6 +11,7 @@
 // Expanding rows where they are used instead cost more: the forward over 32,768 rows of 8 heads, D 64, R 32, took 86 us and its states
 // 46, against 44 and 65 with the rows expanded here.  So did a launch of its own for the expansion: 20 us and 10 for the
 // sums against 19 (2 x 4,096 rows of the same heads).
+#include <algorithm>
 #include <type_traits>
 
 #include "linear_dev.hpp"
@@ -493,12 +494,21 @@ __global__ __launch_bounds__(256) void linear_dfreqs_kernel(LinPhaseParams p) {
 
 }  // namespace
 
+// Columns of values for a workgroup: narrower tiles, whose expanded rows are read or made again, where wide ones leave CUs without work.
+int sum_cols(const LinCall& c) {
+  int n = c.Dv <= 64 ? 64 : c.Dv <= 128 ? 128 : 256;
+  while (n > 64 && (int64_t)c.seqs.T * c.Hk * ((c.Dv + n - 1) / n) < 256) n /= 2;
+  return std::min(n, c.Dv);
+}
+
 hipError_t launch_linear_states(const LinStateParams& p, hipStream_t s) {
-  return p.c.split ? lin_dispatch<kTwo, StateLaunch>(p.c.E, p.c.Dv, p, s) : lin_dispatch<kOne, StateLaunch>(p.c.E, p.c.Dv, p, s);
+  const int n = sum_cols(p.c);
+  return p.c.split ? lin_dispatch<kTwo, StateLaunch>(p.c.E, n, p, s) : lin_dispatch<kOne, StateLaunch>(p.c.E, n, p, s);
 }
 
 hipError_t launch_linear_sums(const LinStateParams& p, hipStream_t s) {
-  return p.c.split ? lin_dispatch<kTwo, SumLaunch<true>::template Of>(p.c.E, p.c.Dv, p, s) : lin_dispatch<kOne, SumLaunch<false>::template Of>(p.c.E, p.c.Dv, p, s);
+  const int n = sum_cols(p.c);
+  return p.c.split ? lin_dispatch<kTwo, SumLaunch<true>::template Of>(p.c.E, n, p, s) : lin_dispatch<kOne, SumLaunch<false>::template Of>(p.c.E, n, p, s);
 }
 
 hipError_t launch_linear_scan(const LinScanParams& p, hipStream_t s) {
