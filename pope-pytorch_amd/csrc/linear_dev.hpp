@@ -105,11 +105,11 @@ __device__ __forceinline__ float lin_turns(float b) {
 enum LinParts { kOne = 1, kTwo = 2 };
 
 // Rows near each other are addressed by a base that a wave shares and a 32-bit offset in bytes (a chunk of 64 rows, row strides below
-// 2^23 elements): one register a load, the same in every chunk.
+// 2^22 elements): one register a load, the same in every chunk.
 __device__ __forceinline__ char* lin_uniform(const void* p) {
   const uint64_t x = reinterpret_cast<uint64_t>(p);
   const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
-  return reinterpret_cast<char*>((uint64_t)hi << 32 | lo);
+  return (char*)(__attribute__((address_space(1))) char*)((uint64_t)hi << 32 | lo);   // global memory: else loads would ask LDS too
 }
 __device__ __forceinline__ int lin_size(int type) { return type == 0 ? 4 : 2; }
 // Base of row `row` of a (batch, head), and the bytes from row to row.
