@@ -4,6 +4,7 @@
 // Bound by HBM: a state is read and written once (8 E Dv bytes for each sequence and kv head), everything else is a few
 // rows.  A workgroup has a state, or, where there are few of them, some of its columns; a thread four columns of every n-th row,
 // eight rows in flight.  States, sums and the expanded rows are fp32.
+// 200 sequences of 8 kv heads, D 128, R 64, Dv 128: 72 us, 4.5 TB/s (a copy of 1 GiB: 4.9); 64 of 16 heads, D 64, R 64, gated: 17.5, 3.9 TB/s.
 #include "linear_dev.hpp"
 
 namespace pope {

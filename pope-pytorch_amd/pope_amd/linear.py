@@ -20,7 +20,8 @@ dim go up to 256, of any size.  A sequence goes on from a state with any split o
 
 No counterpart in the reference, whose attention is the softmax's (PoPE_pytorch/attention.py:75-145).  GPU tensors run the HIP
 kernels (csrc/linear_*.hip, csrc/gated_norm.hip), CPU tensors the torch computation below.  Calls do not synchronise or read
-lengths on the host, and can be captured into graphs; gradients are summed in a fixed order.
+lengths on the host, and can be captured into graphs (a backward pass while no eager autograd graph of the same leaves
+lives); gradients are summed in a fixed order.
 """
 from __future__ import annotations
 
