@@ -122,6 +122,7 @@ def test_no_rows():
     o, last = linear_attn_with_pope(q, kv, kv, return_state=True)
     assert last.shape == (2, 2, 8, 8) and not last.any()
     assert gated_head_norm(q, q).shape == q.shape
+    assert linear_attn_with_pope(q, kv, kv, gate=q).shape == q.shape
 
 
 def test_refusals():

@@ -30,6 +30,7 @@ SHAPES = {
     "wide_rows": dict(N=100, D=200, R=101, Dv=19, Hq=2, Hk=1),
     "many_segments": dict(Hq=1, Hk=1, N=1000, R=64, initial=True),
     "longer_segments": dict(B=2, Hq=16, Hk=16, N=1100, D=32, R=16, Dv=32),
+    "heads_share_wide_rows": dict(B=40, Hq=24, Hk=8, N=64, D=130, R=6, Dv=20),
     "heads_share_rows": dict(B=9, Hq=24, Hk=8, N=500, D=32, R=16, Dv=32, mask="random"),
 }
 
@@ -52,6 +53,13 @@ def test_packed(cuda, lens, lead, tail, dtype):
     for n in ("o", "d_q", "d_k", "d_v"):
         assert not got[n][:, :, outside].any(), n
     assert not got["d_freqs"][outside].any()
+
+
+@TYPES
+def test_packed_with_a_mask(cuda, dtype):
+    case = Case(cuda, lens=[100, 3, 0, 61], lead=1, tail=2, Hq=4, Hk=2, dtype=dtype, initial=True, mask="random")
+    case.mask[0, 101:104] = False   # nothing is left of the second sequence
+    compare(run(pope_amd, case), case)
 
 
 def test_decreasing_bounds_stay_in_range(cuda):
@@ -256,6 +264,34 @@ def test_gated_gradients(cuda, dtype):
     for n, a, b in zip(x, got, want):
         own = half(dtype) if a.dtype == dtype else 0.0
         assert a.dtype == x[n].dtype and (a.double() - b).norm() <= (own + 2e-3) * b.norm(), (n, ((a.double() - b).norm() / b.norm()).item())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("lens", [None, [1] * 9])
+def test_gated_gradients_of_rows_alone(cuda, dtype, lens):
+    """Of a sequence of one row o is a multiple of v, and the norm's gradient at right angles to it but for eps: what is left of
+    dO . v is `small` of its terms.  dO and the sum are fp32 (16 roundings of 2^-24 together), so d_q and d_k, multiples of it, are off by
+    2^-20 / small, and by half a step; a row's k_hat and q_hat are expanded to 2^-16."""
+    case = Case(cuda, B=1 if lens else 3, N=1, lens=lens, Hq=4, Hk=2, D=16, R=8, Dv=16, dtype=dtype)
+    gate = torch.randn_like(case.do)
+    x = {n: t.clone().requires_grad_() for n, t in {**{n: case.leaves()[n] for n in "qkv"}, "gate": gate}.items()}
+    y = linear_attn_with_pope(x["q"], x["k"], x["v"], case.ld, case.emb(), gate=x["gate"], **case.kw())
+    got = torch.autograd.grad(y, list(x.values()), case.do)
+    e = {n: t.detach().double().requires_grad_() for n, t in x.items()}
+    o, _ = L.attend64(L.expand64(e["q"], case.freqs, None, case.R), L.expand64(e["k"], case.freqs, case.bias, case.R), e["v"], case.decay64(), case.scale, None, case.zero, case.seqs)
+    o.retain_grad()
+    (L.norm64(o, e["gate"], None, 1e-5) * case.do.double()).sum().backward()
+    dov = o.grad.unflatten(1, (2, 2)) * e["v"][:, None]
+    small = (dov.sum(-1).abs() / dov.abs().sum(-1)).flatten(1, 2)[..., None]   # (batch, query heads, n, 1)
+    of = {"q": small, "k": small.unflatten(1, (2, 2)).amin(1)}
+    for n, t in zip(x, got):
+        want, own = e[n].grad, half(dtype)
+        if n in of:
+            err, lim = (t.double() - want).abs(), own + 2.0 ** -14 + 2.0 ** -20 / of[n]
+            size = want.norm(dim=-1, keepdim=True) if n == "q" else want.norm(dim=-1, keepdim=True) * 4
+            assert (err <= lim * size + 2.0 ** -24).all(), (n, (err / (lim * size + 2.0 ** -24)).max().item())
+        else:
+            assert ((t.double() - want).norm() <= (own + 1e-4) * want.norm()), n
 
 
 # ---------------------------------------------------------------- single tokens
