@@ -127,8 +127,12 @@ template <>
 struct LinRaw<kTwo> {
   u32x4 a, b;   // b: of fp32 rows
 };
-template <int PL>
-__device__ __forceinline__ LinRaw<PL> lin_zeros() { return LinRaw<PL>{}; }
+// softplus and its derivative, of one exponential.
+__device__ __forceinline__ void lin_soft(float x, float* soft, float* slope) {
+  const float e = __builtin_amdgcn_exp2f(-fabsf(x) * kLog2e), r = __builtin_amdgcn_rcpf(1.f + e);
+  *soft = fmaf(__builtin_amdgcn_logf(1.f + e), kLn2, fmaxf(x, 0.f));
+  *slope = x >= 0.f ? r : e * r;
+}
 
 // base + off: the row.  whole: r.vec, known before.
 template <int PL>

@@ -87,7 +87,10 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
   const float lg = lin_log2(c, hk);
   const int a = rev ? 0 : 1;
   const int chunks = (seg.len + C - 1) / C;
-  const int col0 = wave * K::SL;                    // the wave's columns in the tile
+  // The wave's columns in the tile: 16 and, where it has two tiles, 16 half of the tile further on, so that the rotated columns, which
+  // come first and take the chain rule, fall to all waves (dq and dk of 16 heads on 4, 128 + 64 columns: 112 us with 32 columns in a row, 109 so).
+  constexpr int kStep = 16 * K::NW;
+  const int col0 = 16 * wave;
   const bool busy = n0 + col0 < ncols;
   const int steps = (pcols + 31) / 32;
 
@@ -270,7 +273,7 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
       const bool whole = chain && c.Dv % 4 == 0 && (reinterpret_cast<uintptr_t>(from) & 15) == 0;
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        const int col = n0 + col0 + 16 * ct + l16;
+        const int col = n0 + col0 + kStep * ct + l16;
 #pragma unroll
         for (int s = 0; s < 2 * ST; ++s) {
           const int row = 16 * s + 4 * q4;
@@ -372,7 +375,7 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
           const uint32_t at = place(min(16 * i + l16, seg.len - 1 - t0));
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct) {
-            const int d = min((n0 + col0 + 16 * ct + 4 * q4) >> 1, c.R - 2);
+            const int d = min((n0 + col0 + kStep * ct + 4 * q4) >> 1, c.R - 2);
             cx[ct][i] = lin_get2<PL>(in, in_base, at * lin_step(in), d);
             cf[ct][i] = *reinterpret_cast<const f32x2*>(f_base + (at * (uint32_t)c.f_s[1] + d) * 4);
           }
@@ -422,7 +425,7 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
 #pragma unroll
         for (int s = 0; s < KS; ++s)
 #pragma unroll
-          for (int l = 0; l < PL; ++l) za[ct][s][l] = lin_across(Z.p + l * Z.plane, K::ZS, 32 * s, col0 + 16 * ct, lane);
+          for (int l = 0; l < PL; ++l) za[ct][s][l] = lin_across(Z.p + l * Z.plane, K::ZS, 32 * s, col0 + kStep * ct, lane);
       if (!odd_z) {
 #pragma unroll
         for (int i = 0; i < IT; ++i)
@@ -448,9 +451,9 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
             for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
-                float z = BF16::to_float(Z.p[j * K::ZS + col0 + 16 * ct + 4 * q4 + r]);
+                float z = BF16::to_float(Z.p[j * K::ZS + col0 + kStep * ct + 4 * q4 + r]);
                 if constexpr (PL == 2)
-                  if (fabsf(z) <= 3.402823466e38f) z += BF16::to_float(Z.p[Z.plane + j * K::ZS + col0 + 16 * ct + 4 * q4 + r]);
+                  if (fabsf(z) <= 3.402823466e38f) z += BF16::to_float(Z.p[Z.plane + j * K::ZS + col0 + kStep * ct + 4 * q4 + r]);
                 O[ct][i][r] += w * z;
               }
           }
@@ -512,14 +515,14 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
             const bool dead = rev && !live[i];
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct)
-              lin_set4<PL>(out, ob, orow, n0 + col0 + 16 * ct + 4 * q4, dead ? f32x4{0.f, 0.f, 0.f, 0.f} : O[ct][i]);
+              lin_set4<PL>(out, ob, orow, n0 + col0 + kStep * ct + 4 * q4, dead ? f32x4{0.f, 0.f, 0.f, 0.f} : O[ct][i]);
           } else {
             // chain rule of the polar rows: a lane's columns are two (cosine, sine) pairs, or four other dims
             const bool dead = rev && !live[i];
             const float f = kind == kLinDq ? c.scale : 1.f;
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
-              const int e0 = n0 + col0 + 16 * ct + 4 * q4;
+              const int e0 = n0 + col0 + kStep * ct + 4 * q4;
               f32x4 v = O[ct][i] * f;
               if (dead) v = f32x4{0.f, 0.f, 0.f, 0.f};
               float dx[2], x2[2];
@@ -543,8 +546,10 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
                   const float x = x2[pr];
                   float sn, cs;
                   sincos_turns(f2[pr], kind == kLinDk ? turns[d] : 0.f, &sn, &cs);
-                  dx[pr] = dead ? 0.f : sigmoid_f(x) * (dc * cs + ds * sn);
-                  const float dth = dead ? 0.f : softplus_f(x) * (ds * cs - dc * sn);
+                  float soft, slope;
+                  lin_soft(x, &soft, &slope);
+                  dx[pr] = dead ? 0.f : slope * (dc * cs + ds * sn);
+                  const float dth = dead ? 0.f : soft * (ds * cs - dc * sn);
                   dbsum[ct][pr] += dth;
                   if (phase) phase[place(t) * c.R + d] = dth;
                   if (!pairs) lin_put_value<PL>(out, ob, orow, d, dx[pr]);
@@ -571,7 +576,7 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
         float v = dbsum[ct][pr];
 #pragma unroll
         for (int i = 1; i < 16; i *= 2) v += wave_shfl_xor(v, i);
-        const int e = n0 + col0 + 16 * ct + 4 * q4 + 2 * pr;
+        const int e = n0 + col0 + kStep * ct + 4 * q4 + 2 * pr;
         if (l16 == 0 && e < 2 * c.R) p.dbias[((int64_t)at * c.Hk + hk) * c.R + (e >> 1)] = v;
       }
   }
