@@ -50,7 +50,7 @@ struct LinStateParams {
   LinCall c;
   float* states;                 // launch_linear_states: null for the expanded rows only
   int reverse;
-  int tiles, key_wgs;            // set by the launchers
+  int tiles, key_wgs, q_parts;   // set by the launchers
 };
 hipError_t launch_linear_states(const LinStateParams& p, hipStream_t s);   // expands rows; forward: writes them
 hipError_t launch_linear_sums(const LinStateParams& p, hipStream_t s);     // from the expanded rows, which are as exact as `split` says
