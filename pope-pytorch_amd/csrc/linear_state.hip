@@ -71,7 +71,8 @@ __device__ __forceinline__ char* lin_angle_base(const LinCall& c, int batch, int
 }
 
 // The queries of a segment and head, expanded: four threads a row, two rows and two chunks of each at once.  A workgroup has every
-// parts-th 64 columns, so that queries are small pieces behind the keys' long ones (256 columns, 2 x 2,048 rows: 94 us whole, 86 so).
+// parts-th 64 columns: where one workgroup fills a CU, queries are small pieces behind the keys' long ones (D 256, R 256, 2 x 2,048 rows:
+// 94 us whole, 86 so; with four waves, 16 heads on 4 of D 128, R 64, 27.5 whole, 30 so).
 template <int PL, int THREADS, bool FAST>
 __device__ __forceinline__ void lin_expand_queries(const LinCall& c, const LinSeg& seg, int hq, int part, int parts) {
   const int tid = threadIdx.x, per = (c.D + 7) / 8;
@@ -406,7 +407,7 @@ struct StateLaunch {
   static hipError_t go(LinStateParams p, hipStream_t s) {
     p.tiles = p.states ? (p.c.Dv + K::NT - 1) / K::NT : 1;
     const int64_t keys = (int64_t)p.c.seqs.T * p.c.Hk * p.tiles, heads = p.reverse ? 0 : (int64_t)p.c.seqs.T * p.c.Hq;
-    p.q_parts = (p.c.D + 63) / 64;
+    p.q_parts = K::NW == 8 ? (p.c.D + 63) / 64 : 1;
     const int64_t n = keys + heads * p.q_parts;
     if (n >= ((int64_t)1 << 22)) return hipErrorInvalidValue;
     p.key_wgs = (int)keys;
