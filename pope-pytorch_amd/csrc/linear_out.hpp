@@ -17,8 +17,8 @@
 // leaving its registers.
 //
 // Rounding: x, y, z, the weighted C x C products and W as an operand are bf16: one part for bf16 rows (each is off by at most 2^-8,
-// as the output is by its own rounding), the sum of two for fp16 and fp32 rows, and for bf16 rows whose output goes on in fp32 (2^-16;
-// C is 32 then).  W itself, all sums and the powers of g are fp32.
+// as the output is by its own rounding), the sum of two for fp16 and fp32 rows, for bf16 rows whose output goes on in fp32, and for
+// a few bf16 rows (2^-16; C is 32 then).  W itself, all sums and the powers of g are fp32.
 //
 // What bounds it: waits.  32,768 rows of 8 heads, D 64, R 32, bf16: 45-48 us for the outputs (6.4 GFLOP, 167 MB, 3.5 TB/s); 2 x 4,096 of
 // them: outputs 19, dq and dk 62, dv 19.  D 256, R 256 (2 x 2,048 rows): 77, 200 and 77, where a segment's state is 512 KB, its load a

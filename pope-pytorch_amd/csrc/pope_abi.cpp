@@ -1323,7 +1323,11 @@ LinShape linear_shape(const pope_linear& d, bool packed) {
   s.parts = d.N > s.L;
   s.grid = (int)grid;
   s.EP = round_up(d.D + d.R, 32);
-  s.planes = d.dtype != POPE_BF16 || d.o_f32 ? 2 : 1;
+  // Two parts also for bf16 sequences of up to one chunk of them, while that takes no second round of the chip: a few rows have few
+  // roundings to even out, and the time is the same (8 heads, D 64, R 32, forward and backward: 1 row 35 us as two parts, 36 as one; 16
+  // rows 32 and 32; 64 rows 50 and 37).
+  const bool few = d.N <= 32 && (int64_t)d.B * d.Hk <= kLinGrid / 2;
+  s.planes = d.dtype != POPE_BF16 || d.o_f32 || few ? 2 : 1;
   s.qh = align_up((size_t)rows * d.Hq * s.EP * 2) * s.planes;
   s.kh = align_up((size_t)rows * d.Hk * s.EP * 2) * s.planes;
   s.states = align_up((size_t)s.T * d.Hk * (d.D + d.R) * d.Dv * sizeof(float));
