@@ -370,7 +370,7 @@ typedef struct pope_linear {
   float scale;
   int64_t q_s[3], k_s[3], v_s[3], o_s[3];      /* (b, h, n) element strides, unit feature stride, any alignment */
   int64_t do_s[3], dq_s[3], dk_s[3], dv_s[3];
-  int64_t f_s[2], bias_sh;   /* freqs (b, n): a row of angles per row; bias (1 or Hk, R) */
+  int64_t f_s[2], bias_sh;   /* freqs (b, n): a row of angles per row; bias (1 or Hk, R): a stride of 0 is one row, with one row of gradients */
   int64_t df_s[2];           /* of dfreqs: f_s, or a batch stride of 0 where the table is one for all */
   int64_t mask_sb;
 } pope_linear;

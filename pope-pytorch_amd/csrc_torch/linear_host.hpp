@@ -151,13 +151,21 @@ LinearGrads linear_backward(const LinearArgs& a, const Tensor& dout0, const Tens
     d.df_s[0] = a.freqs.dim() == 3 && a.freqs.size(0) > 1 ? r.dfreqs.stride(0) : 0;
     d.df_s[1] = r.dfreqs.stride(-2);
   }
-  if (need_db) r.dbias = at::empty(a.bias.sizes(), a.bias.options().requires_grad(false));
+  // the library takes a stride of 0 for one bias row, and so for one gradient row: a row that a view repeats for the heads is copied
+  Tensor bias = a.bias;
+  if (need_db) {
+    r.dbias = at::empty(bias.sizes(), bias.options().requires_grad(false));
+    if (bias.size(0) > 1 && bias.stride(0) == 0) {
+      bias = bias.contiguous();
+      d.bias_sh = bias.stride(0);
+    }
+  }
   if (need_d0) r.dinitial = fp32_like(a.q, {d.B, d.Hk, d.D + d.R, d.Dv});
   TORCH_CHECK_VALUE(!dlast.defined() || dlast.numel() == (int64_t)d.B * d.Hk * (d.D + d.R) * d.Dv, "the states' gradient ", dlast.sizes(), " does not fit");
   size_t n[2] = {0, 0};
   check(pope_linear_bytes(&d, a.cu.defined(), 0, need_df, n), "workspace query");
   const Tensor ws = bytes_like(a.q, n[1]);
-  check(pope_linear_bwd(&d, dout.data_ptr(), floats(dlast), a.q.data_ptr(), a.k.data_ptr(), a.v.data_ptr(), floats(a.freqs), data(a.bias), floats(a.log_decay),
+  check(pope_linear_bwd(&d, dout.data_ptr(), floats(dlast), a.q.data_ptr(), a.k.data_ptr(), a.v.data_ptr(), floats(a.freqs), data(bias), floats(a.log_decay),
                         bytes_of(a.mask), ints_of(a.cu), floats(a.initial), data(kept), kept.defined() ? kept.nbytes() : 0, r.dq.data_ptr(), r.dk.data_ptr(),
                         r.dv.data_ptr(), static_cast<float*>(data(r.dfreqs)), data(r.dbias), static_cast<float*>(data(r.dinitial)), data(ws), n[1],
                         stream_of(a.q)),

@@ -1,0 +1,45 @@
+"""Inputs of the linear attention, its step and the gated norm that few calls have, against 64-bit formulas (bounds: linear_common)."""
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+import linear_common as L
+import pope_amd
+from linear_common import Case, check, half, run
+from pope_amd import gated_head_norm, linear_attn_step_with_pope, linear_attn_with_pope
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+TYPES = pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=["bf16", "fp16", "fp32"])
+
+
+# ---------------------------------------------------------------- broadcast inputs
+
+@pytest.mark.parametrize("bias_dtype", [F32, BF16])
+def test_gradients_of_expanded_angles_and_biases(cuda, bias_dtype):
+    """One bias for all heads and one table for all batches, as views that repeat them: a gradient row for each row of the views."""
+    case = Case(cuda, B=3, Hq=6, Hk=3, N=150, D=32, R=16, Dv=24, dtype=F16, bias_heads=1)
+    one_bias, table = case.bias.to(bias_dtype), case.freqs
+    case.freqs = table.expand(3, -1, -1)
+    case.bias = one_bias.float().expand(3, -1)
+    val, tol = case.exact()
+    case.bias = one_bias.expand(3, -1)
+    got = run(pope_amd, case)
+    for n in val:
+        own = half(bias_dtype) * val[n].abs() if n == "d_bias" and bias_dtype != F32 else 0.0
+        check(got[n], val[n], case.bound(n, val[n], tol[n]) + own, n)
+    # through the expand: the rows' sum
+    b = one_bias.clone().requires_grad_()
+    o, last = linear_attn_with_pope(case.q, case.k, case.v, case.ld, (table, b.expand(3, -1)), return_state=True)
+    g, = torch.autograd.grad([o, last], b, [case.do, case.ds])
+    own = 0.0 if bias_dtype == F32 else 2 * half(bias_dtype) * val["d_bias"].abs().sum(0, keepdim=True) * 1.01
+    check(g, val["d_bias"].sum(0, keepdim=True), case.bound("d_bias", val["d_bias"].sum(0, keepdim=True), tol["d_bias"].sum(0, keepdim=True)) + own, "bias")
+    # the op, as traced programs call it
+    x = {n: t.detach().requires_grad_() for n, t in case.leaves().items()}
+    o, last, _ = torch.ops.pope_amd.linear_fwd(x["q"], x["k"], x["v"], x["freqs"], x["bias"], case.ld, None, None, None, case.scale, True, False)
+    g = dict(zip(x, torch.autograd.grad([o, last], list(x.values()), [case.do, case.ds])))
+    for n in x:
+        assert torch.equal(g[n], got["d_" + n]), n
