@@ -237,6 +237,13 @@ def strides3(t) -> tuple:
     return (s[0], s[1], s[2])
 
 
+def bias_rows(bias):
+    """A bias whose gradient is wanted, in rows side by side.  The library writes the gradient's rows as far apart as the bias's rows
+    are: past the end of a gradient with rows side by side where the bias is part of wider rows, and into its first row only where a view
+    repeats one row for the heads."""
+    return bias if bias.is_contiguous() else bias.contiguous()
+
+
 def workspace_bytes(op: int, desc: PopeDesc) -> int:
     n = ctypes.c_size_t(0)
     check(lib().pope_workspace_bytes(op, ctypes.byref(desc), ctypes.byref(n)), "workspace query")

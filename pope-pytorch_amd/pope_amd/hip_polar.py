@@ -77,6 +77,8 @@ def polar_bwd_op(gq: Tensor, gk: Tensor, q: Tensor, k: Tensor, freqs: Tensor, bi
                  need_dbias: bool, complex_out: bool = False) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     q, k = _rows4(q), _rows4(k)
     gq, gk = gq.float().contiguous(), gk.float().contiguous()
+    if need_dbias:
+        bias = _lib.bias_rows(bias)
     d = _desc(q, k, freqs, bias, complex_out)
     d.flags |= _lib.deterministic_flag()   # torch.use_deterministic_algorithms(True): no fp32 atomics
     dq, dk = torch.empty_like(q), torch.empty_like(k)
@@ -153,6 +155,8 @@ def fits(q: Tensor, k: Tensor, freqs: Tensor, bias: Tensor, to_magnitude, return
 def polar(q: Tensor, k: Tensor, freqs: Tensor, bias: Tensor, return_complex: bool = False) -> tuple[Tensor, Tensor]:
     D, R = q.shape[-1], freqs.shape[-1]
     plan = pad_plan(D, R)
+    if bias.requires_grad and torch.is_grad_enabled():
+        bias = _lib.bias_rows(bias)
     eager = _lib.eager(q, k, freqs, bias)
     if plan is not None and eager and not return_complex:
         return _lib.host().polar_padded(q, k, freqs, bias, plan.R, plan.R8, plan.Dp)

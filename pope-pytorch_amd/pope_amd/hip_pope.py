@@ -89,6 +89,8 @@ def sim_bwd_op(dsim: Tensor, q: Tensor, k: Tensor, freqs: Tensor, bias: Tensor, 
                need_dbias: bool, split: bool = False) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     L = _lib.lib()
     q, k, dsim = _aligned(q), _aligned(k), _aligned(dsim.float())
+    if need_dbias:
+        bias = _lib.bias_rows(bias)
     d = _desc(q, k, freqs, bias, split)
     d.flags |= _lib.deterministic_flag()   # torch.use_deterministic_algorithms(True): no fp32 atomics
     # the library clears dfreqs / dbias before accumulating into them
@@ -144,6 +146,8 @@ def _prep(q, k, freqs, bias):
         bias = bias.unsqueeze(0)
     if bias.stride(-1) != 1:
         bias = bias.contiguous()
+    if bias.requires_grad and torch.is_grad_enabled():
+        bias = _lib.bias_rows(bias)
     return freqs, bias
 
 

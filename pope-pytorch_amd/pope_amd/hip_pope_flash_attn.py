@@ -108,6 +108,8 @@ def _prep_pope(freqs: Optional[Tensor], bias: Optional[Tensor]):
         bias = bias.unsqueeze(0)
     if bias.stride(-1) != 1:
         bias = bias.contiguous()
+    if bias.requires_grad and torch.is_grad_enabled():
+        bias = _lib.bias_rows(bias)
     return freqs, bias
 
 
@@ -404,6 +406,8 @@ def _bwd_impl(do, q, k, v, o, lse, freqs, bias, mask, causal, softmax_scale, nee
         do = do.to(q.dtype)
     if not lse.is_contiguous():
         lse = lse.contiguous()
+    if need_dbias and not bias.is_contiguous():   # the forward's preparation is for the rows as they were
+        bias, fwd_ws = _lib.bias_rows(bias), None
     _check_views(q, k, v, mask, lse)
     if o.shape != q.shape or do.shape != q.shape:
         raise ValueError(f"o {tuple(o.shape)} and do {tuple(do.shape)} must match q {tuple(q.shape)}")
