@@ -3,18 +3,10 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "linear_rows.hpp"
 #include "pope_kernels.hpp"
 
 namespace pope {
-
-// Rows (b, h, n) of `cols` elements.
-struct LinRows {
-  void* p;
-  int64_t s[3];   // elements
-  int cols;
-  int type;       // pope_dtype: 0 fp32, 1 fp16, 2 bf16
-  int vec;        // rows of whole, aligned units of 8 elements (outputs of the attention: of 4)
-};
 
 // The rows of a call as segments of at most L rows of one sequence.  Padded batches: M segments for each of B sequences.
 // Packed rows: a sequence's segments follow those of the sequences before it; T is the most that N rows can have.

@@ -111,12 +111,10 @@ __device__ __forceinline__ char* lin_uniform(const void* p) {
   const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
   return (char*)(__attribute__((address_space(1))) char*)((uint64_t)hi << 32 | lo);   // global memory: else loads would ask LDS too
 }
-__device__ __forceinline__ int lin_size(int type) { return type == 0 ? 4 : 2; }
-// Base of row `row` of a (batch, head), and the bytes from row to row.
+// Base of row `row` of a (batch, head).
 __device__ __forceinline__ char* lin_base(const LinRows& r, int batch, int h, int64_t row) {
   return lin_uniform(static_cast<char*>(r.p) + (batch * r.s[0] + h * r.s[1] + row * r.s[2]) * lin_size(r.type));
 }
-__device__ __forceinline__ uint32_t lin_step(const LinRows& r) { return (uint32_t)r.s[2] * lin_size(r.type); }
 
 // Eight elements of a row, as they are in memory.
 template <int PL>

@@ -1346,17 +1346,6 @@ LinBytes linear_bwd_bytes(const pope_linear& d, const LinShape& s, bool packed, 
   return b;
 }
 
-pope::LinRows lin_rows(const void* p, const int64_t* s, int cols, int type, int unit) {
-  pope::LinRows r;
-  r.p = const_cast<void*>(p);
-  copy3(r.s, s);
-  r.cols = cols;
-  r.type = type;
-  const uintptr_t whole = std::min(16, unit * (type == POPE_F32 ? 4 : 2));   // bytes of an access
-  r.vec = cols % unit == 0 && reinterpret_cast<uintptr_t>(p) % whole == 0 && s[0] % unit == 0 && s[1] % unit == 0 && s[2] % unit == 0;
-  return r;
-}
-
 pope::LinHat lin_hat(const void* p, size_t bytes, const LinShape& s, int H) {
   return pope::LinHat{static_cast<uint16_t*>(const_cast<void*>(p)), (int64_t)(bytes / s.planes / 2), H, s.EP};
 }
@@ -1367,9 +1356,9 @@ pope::LinCall linear_call(const pope_linear& d, const LinShape& s, const void* h
   pope::LinCall c;
   std::memset(&c, 0, sizeof c);
   c.seqs = pope::LinSeqs{cu, d.B, d.N, s.L, s.M, s.T};
-  c.q = lin_rows(q, d.q_s, d.D, d.dtype, 8);
-  c.k = lin_rows(k, d.k_s, d.D, d.dtype, 8);
-  c.v = lin_rows(v, d.v_s, d.Dv, d.dtype, 8);
+  c.q = pope::lin_rows(q, d.q_s, d.N, d.D, d.dtype, 8);
+  c.k = pope::lin_rows(k, d.k_s, d.N, d.D, d.dtype, 8);
+  c.v = pope::lin_rows(v, d.v_s, d.N, d.Dv, d.dtype, 8);
   c.freqs = freqs;
   c.f_s[0] = d.f_s[0]; c.f_s[1] = d.f_s[1];
   c.f_vec = d.R % 8 == 0 && aligned16(freqs) && d.f_s[0] % 4 == 0 && d.f_s[1] % 4 == 0;
@@ -1377,9 +1366,7 @@ pope::LinCall linear_call(const pope_linear& d, const LinShape& s, const void* h
   c.log_decay = log_decay;
   c.mask = mask; c.mask_sb = d.mask_sb;
   c.Hq = d.Hq; c.Hk = d.Hk; c.G = d.Hq / d.Hk; c.D = d.D; c.R = d.R; c.E = d.D + d.R; c.Dv = d.Dv;
-  if (d.N == 1)   // strides of extents of 1 may be anything
-    for (pope::LinRows* r : {&c.q, &c.k, &c.v}) r->s[2] = 0;
-  if (d.N == 1) c.f_s[1] = 0;
+  if (d.N == 1) c.f_s[1] = 0;   // as lin_rows
   c.scale = d.scale;
   c.split = s.planes == 2;
   if (hats) {
@@ -1431,17 +1418,17 @@ int check_norm(const pope_gated_norm* d) {
 }
 
 // Rows of the norm: whole units of 8, or (2) of 4.
-pope::LinRows norm_rows(const void* p, const int64_t* s, int cols, int type) {
-  pope::LinRows r = lin_rows(p, s, cols, type, 8);
-  if (!r.vec && lin_rows(p, s, cols, type, 4).vec) r.vec = 2;
+pope::LinRows norm_rows(const void* p, const int64_t* s, int n, int cols, int type) {
+  pope::LinRows r = pope::lin_rows(p, s, n, cols, type, 8);
+  if (!r.vec && pope::lin_rows(p, s, n, cols, type, 4).vec) r.vec = 2;
   return r;
 }
 
 pope::GatedNormParams norm_params(const pope_gated_norm& d, const void* x, const void* gate, const void* weight) {
   pope::GatedNormParams p;
   std::memset(&p, 0, sizeof p);
-  p.x = norm_rows(x, d.x_s, d.cols, d.x_f32 ? POPE_F32 : d.dtype);
-  p.gate = norm_rows(gate, d.gate_s, d.cols, d.dtype);
+  p.x = norm_rows(x, d.x_s, d.N, d.cols, d.x_f32 ? POPE_F32 : d.dtype);
+  p.gate = norm_rows(gate, d.gate_s, d.N, d.cols, d.dtype);
   p.weight = weight;
   p.w_sh = d.weight_rows > 1 ? d.weight_sh : 0;
   p.w_type = d.weight_f32 ? POPE_F32 : d.dtype;
@@ -1489,7 +1476,7 @@ int pope_linear_fwd(const pope_linear* d, const void* q, const void* k, const vo
   pope::LinOutParams p;
   std::memset(&p, 0, sizeof p);
   p.c = c;
-  p.out[0] = lin_rows(o, d->o_s, d->Dv, d->o_f32 ? POPE_F32 : d->dtype, 4);
+  p.out[0] = pope::lin_rows(o, d->o_s, d->N, d->Dv, d->o_f32 ? POPE_F32 : d->dtype, 4);
   p.states[0] = seg_states;
   p.first[0] = initial;
   p.heads_per = lin_heads_per(*d, sh, false);
@@ -1518,7 +1505,7 @@ int pope_linear_bwd(const pope_linear* d, const void* dout, const float* dlast, 
   char* ws = static_cast<char*>(workspace);
   float* reverse = reinterpret_cast<float*>(ws);
   pope::LinCall c = linear_call(*d, sh, kept, q, k, v, freqs, bias, log_decay, mask, cu);
-  c.g = lin_rows(dout, d->do_s, d->Dv, d->o_f32 ? POPE_F32 : d->dtype, 8);
+  c.g = pope::lin_rows(dout, d->do_s, d->N, d->Dv, d->o_f32 ? POPE_F32 : d->dtype, 8);
   hipError_t e;
   const bool sums = sh.parts || dinitial;
   if (sums) {
@@ -1536,8 +1523,8 @@ int pope_linear_bwd(const pope_linear* d, const void* dout, const float* dlast, 
   p.states[1] = sums ? reverse : nullptr;
   p.first[1] = dlast;
   p.heads_per = lin_heads_per(*d, sh, true);
-  p.out[0] = lin_rows(dq, d->dq_s, d->D, d->dtype, 4);
-  p.out[1] = lin_rows(dk, d->dk_s, d->D, d->dtype, 4);
+  p.out[0] = pope::lin_rows(dq, d->dq_s, d->N, d->D, d->dtype, 4);
+  p.out[1] = pope::lin_rows(dk, d->dk_s, d->N, d->D, d->dtype, 4);
   if (d->R > 0) {
     if (dbias) p.dbias = reinterpret_cast<float*>(ws + lb.reverse);
     if (dfreqs) {
@@ -1547,7 +1534,7 @@ int pope_linear_bwd(const pope_linear* d, const void* dout, const float* dlast, 
   }
   if ((e = c.split ? pope::launch_linear_dqk_split(p, s) : pope::launch_linear_dqk_bf16(p, s)) != hipSuccess) return lin_fail(e, "linear attention launch");
   pope::LinOutParams pv = p;
-  pv.out[0] = lin_rows(dv, d->dv_s, d->Dv, d->dtype, 4);
+  pv.out[0] = pope::lin_rows(dv, d->dv_s, d->N, d->Dv, d->dtype, 4);
   pv.dphase[0] = pv.dphase[1] = nullptr;
   if ((e = c.split ? pope::launch_linear_dv_split(pv, s) : pope::launch_linear_dv_bf16(pv, s)) != hipSuccess) return lin_fail(e, "linear attention launch");
   if (d->R > 0 && (dbias || dfreqs)) {
@@ -1569,7 +1556,7 @@ int pope_gated_norm_fwd(const pope_gated_norm* d, const void* x, const void* gat
   if (d->B == 0 || d->N == 0) return POPE_OK;
   if (!x || !gate || !y) return fail(POPE_ERR_INVALID, "x, gate, y must be non-NULL");
   pope::GatedNormParams p = norm_params(*d, x, gate, weight);
-  p.y = norm_rows(y, d->y_s, d->cols, d->dtype);
+  p.y = norm_rows(y, d->y_s, d->N, d->cols, d->dtype);
   const hipError_t e = pope::launch_gated_norm(p, false, reinterpret_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "gated norm launch");
   return POPE_OK;
@@ -1595,9 +1582,9 @@ int pope_gated_norm_bwd(const pope_gated_norm* d, const void* dy, const void* x,
   if (dweight && !weight) return fail(POPE_ERR_INVALID, "dweight wanted, but there is no weight");
   if (dweight && (rc = check_ws(need, workspace, workspace_bytes))) return rc;
   pope::GatedNormParams p = norm_params(*d, x, gate, weight);
-  p.y = norm_rows(dy, d->dy_s, d->cols, d->dtype);
-  p.dx = norm_rows(dx, d->dx_s, d->cols, p.x.type);
-  p.dgate = norm_rows(dgate, d->dgate_s, d->cols, d->dtype);
+  p.y = norm_rows(dy, d->dy_s, d->N, d->cols, d->dtype);
+  p.dx = norm_rows(dx, d->dx_s, d->N, d->cols, p.x.type);
+  p.dgate = norm_rows(dgate, d->dgate_s, d->N, d->cols, d->dtype);
   p.part = dweight ? static_cast<float*>(workspace) : nullptr;
   p.dweight = dweight;
   const hipError_t e = pope::launch_gated_norm(p, true, reinterpret_cast<hipStream_t>(stream));
@@ -1625,12 +1612,12 @@ int pope_linear_step(const pope_linear* d, const void* q, const void* k, const v
   pope::LinStepParams p;
   std::memset(&p, 0, sizeof p);
   p.c = linear_call(*d, sh, nullptr, q, k, v, freqs, bias, log_decay, nullptr, nullptr);
-  p.o = lin_rows(o, d->o_s, d->Dv, d->o_f32 ? POPE_F32 : d->dtype, 4);
+  p.o = pope::lin_rows(o, d->o_s, d->N, d->Dv, d->o_f32 ? POPE_F32 : d->dtype, 4);
   p.from = states; p.to = states;
   p.read = from; p.write = to;
   p.slots = slots; p.slot_s = slot_s;
   if (norm) {   // a row's columns together
-    p.gate = lin_rows(gate, norm->gate_s, d->Dv, d->dtype, 8);
+    p.gate = pope::lin_rows(gate, norm->gate_s, 1, d->Dv, d->dtype, 8);
     p.weight = weight; p.w_sh = norm->weight_rows > 1 ? norm->weight_sh : 0; p.w_type = norm->weight_f32 ? POPE_F32 : d->dtype; p.eps = norm->eps;
     p.split = 1;
   } else {      // columns of few states go to several workgroups, 16 or more to each

@@ -43,3 +43,24 @@ def test_gradients_of_expanded_angles_and_biases(cuda, bias_dtype):
     g = dict(zip(x, torch.autograd.grad([o, last], list(x.values()), [case.do, case.ds])))
     for n in x:
         assert torch.equal(g[n], got["d_" + n]), n
+
+
+# ---------------------------------------------------------------- one row, at any stride
+
+@TYPES
+def test_one_row_of_any_stride(cuda, dtype):
+    """The row dim of one row may have any stride: nothing reads or writes by it."""
+    for gated in (False, True):
+        case = Case(cuda, B=2, Hq=4, Hk=2, N=1, D=48, R=16, Dv=40, dtype=dtype, initial=True)
+        gate = torch.randn(2, 4, 1, 40, generator=torch.Generator().manual_seed(2)).to(cuda, dtype)
+
+        def call(turn):
+            x = {n: turn(t).detach().requires_grad_() for n, t in dict(case.leaves(), gate=gate).items()}
+            o, last = linear_attn_with_pope(x["q"], x["k"], x["v"], case.ld, (x["freqs"], x["bias"]), initial_state=x["s0"], return_state=True, gate=x["gate"] if gated else None)
+            used = [t for n, t in x.items() if gated or n != "gate"]
+            return [o, last, *torch.autograd.grad([o, last], used, [turn(case.do.to(o.dtype)), case.ds])]
+
+        far = lambda t: t.as_strided(t.shape, (*t.stride()[:2], 2 ** 33 + 1, t.stride(3)), t.storage_offset()) if t.ndim == 4 and t.shape[2] == 1 else t
+        assert far(case.do).stride(2) > 2 ** 33
+        for a, b in zip(call(lambda t: t), call(far)):
+            assert torch.equal(a, b)
