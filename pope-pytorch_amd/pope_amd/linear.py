@@ -432,10 +432,12 @@ def _expand(x: Tensor, freqs: Optional[Tensor], bias: Optional[Tensor]) -> Tenso
 
 def _linear_torch(q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial, scale, shape, dtype):
     G, Hk, n = q.shape[1] // k.shape[1], k.shape[1], q.shape[2]
+    gone = ~mask[:, None, :, None] if exists(mask) else None
+    if exists(gone):   # before the expansion: its derivatives of what is not finite would make a gradient of 0 NaN
+        k, v = k.masked_fill(gone, 0.0), v.masked_fill(gone, 0.0)
     qh, kh, vf = _expand(q, freqs, None) * scale, _expand(k, freqs, bias), v.float()
-    if exists(mask):
-        gone = ~mask[:, None, :, None]
-        kh, vf = kh.masked_fill(gone, 0.0), vf.masked_fill(gone, 0.0)
+    if exists(gone):   # and behind it: the magnitude of 0 is log 2
+        kh = kh.masked_fill(gone, 0.0)
     ld = log_decay.double() if exists(log_decay) else torch.zeros(Hk, dtype=torch.float64)
     # g^p; g^0 is 1 whatever g is
     power = lambda p: torch.where(p == 0, 1.0, (ld.view(-1, *([1] * p.ndim)) * p.clamp_min(1)).exp()).float()
