@@ -358,7 +358,7 @@ int pope_paged_attn(const pope_paged* desc, const void* q, const float* freqs, c
  * sequence b owning rows cu_seqlens[b] <= r < cu_seqlens[b + 1]; outputs and gradients of rows outside every sequence are 0.
  * cu_seqlens that decrease leave unspecified values (never an access out of bounds).  States are fp32 (B, Hk, D + R, Dv),
  * contiguous; `initial` NULL: zeros.  Products take bf16 rows as they are; fp16 and fp32 rows, bf16 rows with o_f32, and a few bf16
- * rows, as the sum of two bf16 parts (2^-16 of each factor).  Calls that need 2^22 workgroups or more return POPE_ERR_UNSUPPORTED.
+ * rows, as the sum of two bf16 parts (2^-16 of each factor; finite fp32 values above the largest bf16 count as that).  Calls that need 2^22 workgroups or more return POPE_ERR_UNSUPPORTED.
  */
 #define POPE_LINEAR_ROW_STRIDE (1 << 22)  /* row strides are below this many elements, where there are rows */
 typedef struct pope_linear {

@@ -6,6 +6,7 @@
 namespace pope {
 
 typedef __attribute__((ext_vector_type(2))) float f32x2;
+constexpr float kF32Max = 3.402823466e38f, kBf16Max = 3.3895313892515355e38f;
 
 // ---------------------------------------------------------------- segments
 
@@ -180,6 +181,23 @@ __device__ __forceinline__ void lin_unpack8(const LinRaw<PL>& w, int type, float
   }
   unpack8<BF16>(w.a, f);
 }
+// An fp32 value of rows that become bf16 parts: finite ones above the largest bf16 (by 2^-8 of it at most) count as that.  Their first
+// part would round to infinity, and 0 x infinity of a row behind would be NaN.
+__device__ __forceinline__ float lin_part(uint32_t w) {
+  const float v = __uint_as_float(w);
+  return fabsf(v) <= kF32Max ? __builtin_amdgcn_fmed3f(v, -kBf16Max, kBf16Max) : v;
+}
+template <int PL>
+__device__ __forceinline__ void lin_row8(const LinRaw<PL>& w, int type, float* f) {
+  if constexpr (PL == kTwo) {
+    if (type == 0) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f[k] = lin_part(w.a[k]), f[4 + k] = lin_part(w.b[k]);
+      return;
+    }
+  }
+  lin_unpack8<PL>(w, type, f);
+}
 // One element.
 template <int PL>
 __device__ __forceinline__ float lin_get(const LinRows& r, int64_t at) {
@@ -255,7 +273,7 @@ __device__ __forceinline__ LinPair<PL> lin_get2(const LinRows& r, const char* ba
 template <int PL>
 __device__ __forceinline__ float lin_get1(const LinRows& r, const char* base, uint32_t off, int d) {
   if constexpr (PL == kTwo) {
-    if (r.type == 0) return *reinterpret_cast<const float*>(base + (off + 4 * d));
+    if (r.type == 0) return lin_part(*reinterpret_cast<const uint32_t*>(base + (off + 4 * d)));
     if (r.type == 1) return F16::to_float(*reinterpret_cast<const uint16_t*>(base + (off + 2 * d)));
   }
   return BF16::to_float(*reinterpret_cast<const uint16_t*>(base + (off + 2 * d)));
@@ -264,7 +282,7 @@ template <int PL>
 __device__ __forceinline__ void lin_unpack2(const LinPair<PL>& p, int type, float* v) {
   if constexpr (PL == kTwo) {
     if (type == 0) {
-      v[0] = __uint_as_float(p.w), v[1] = __uint_as_float(p.v);
+      v[0] = lin_part(p.w), v[1] = lin_part(p.v);
       return;
     }
     if (type == 1) {
@@ -389,10 +407,10 @@ __device__ __forceinline__ bool lin_put_plain(const LinTile& t, int row, int e, 
     return lin_odd8(x.a);
   } else {
     float v[8];
-    lin_unpack8<PL>(x, type, v);
+    lin_row8<PL>(x, type, v);
     bool odd = false;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) odd = odd || !(fabsf(v[k]) <= 3.402823466e38f);
+    for (int k = 0; k < 8; ++k) odd = odd || !(fabsf(v[k]) <= kF32Max);
     lin_put8<PL, PERM>(t, row, e, v);
     return odd;
   }
@@ -403,7 +421,7 @@ __device__ __forceinline__ bool lin_put_plain(const LinTile& t, int row, int e, 
 template <int PL>
 __device__ __forceinline__ void lin_polar8(const LinRaw<PL>& x8, int type, const f32x4* f, int d0, int R, float factor, const float* turns, float* a, float* b) {
   float x[8];
-  lin_unpack8<PL>(x8, type, x);
+  lin_row8<PL>(x8, type, x);
   if (d0 < R) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {

@@ -453,7 +453,7 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
               for (int r = 0; r < 4; ++r) {
                 float z = BF16::to_float(Z.p[j * K::ZS + col0 + kStep * ct + 4 * q4 + r]);
                 if constexpr (PL == 2)
-                  if (fabsf(z) <= 3.402823466e38f) z += BF16::to_float(Z.p[Z.plane + j * K::ZS + col0 + kStep * ct + 4 * q4 + r]);
+                  if (fabsf(z) <= kF32Max) z += BF16::to_float(Z.p[Z.plane + j * K::ZS + col0 + kStep * ct + 4 * q4 + r]);
                 O[ct][i][r] += w * z;
               }
           }

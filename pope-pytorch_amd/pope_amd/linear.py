@@ -290,7 +290,8 @@ def linear_attn_with_pope(q: Tensor, k: Tensor, v: Tensor, log_decay: Optional[T
 
     ``gate`` (as o): o is ``gated_head_norm(o, gate, norm_weight, eps=norm_eps)``.
 
-    A value that is not finite reaches the rows from its own on, where sums through a state may turn infinities into NaN.  GPU calls
+    A value that is not finite reaches the rows from its own on, where sums through a state may turn infinities into NaN; on the GPU,
+    finite fp32 values above 3.3895e38, the largest bf16, count as that.  GPU calls
     that would need 2^22 workgroups (about one for each 64 rows or more of each head) raise."""
     args = (log_decay, mask, cu_seqlens, initial_state)
     freqs, bias = pos_emb if exists(pos_emb) else (None, None)

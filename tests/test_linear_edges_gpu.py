@@ -64,3 +64,27 @@ def test_one_row_of_any_stride(cuda, dtype):
         assert far(case.do).stride(2) > 2 ** 33
         for a, b in zip(call(lambda t: t), call(far)):
             assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------- values next to the largest
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("name,column", [("q", 20), ("q", 3), ("k", 20), ("k", 3), ("v", 20), ("do", 20)])
+def test_fp32_values_next_to_the_largest(cuda, name, column, sign):
+    """The largest fp32 value in a row: every output is finite and the formula's of the largest bf16, as which it counts (2^-8 below); the
+    bounds of rows that do not depend on it are as small as ever.  The other operands are small, so that the formula is finite."""
+    most = torch.finfo(BF16).max
+    for at in (0, 37, 140, 209):
+        case = Case(cuda, B=2, N=210, D=32, R=16, Dv=40, dtype=F32, seed=at)
+        for n in ("q", "k", "v", "do"):
+            if n != name:
+                setattr(case, n, getattr(case, n) * 2.0 ** -8)
+        case.ds = case.ds * 2.0 ** -8
+        t = getattr(case, name)
+        t[0, 0, at, column] = sign * most
+        val, tol = case.exact()
+        t[0, 0, at, column] = sign * torch.finfo(F32).max
+        got = run(pope_amd, case)
+        for n in val:
+            assert val[n].isfinite().all() and got[n].isfinite().all(), (n, at)
+            check(got[n], val[n], case.bound(n, val[n], tol[n]), f"{n} {at}")
