@@ -102,7 +102,23 @@ __global__ __launch_bounds__(kThreads) void gated_norm_kernel(GatedNormParams p)
       ss += wave_shfl_xor(ss, m);
       if (BWD) tx += wave_shfl_xor(tx, m);
     }
-    const float r = 1.f / __builtin_sqrtf(fmaf(ss, inv, p.eps));
+    float scale = 1.f, eps = p.eps;
+    if (!(ss <= kF32Max)) {   // the same of the row at a smaller scale; infinities and NaN stay what they are
+      POPE_COLD_PATH();
+      scale = kNormDown, eps = ss = tx = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        x[k] *= scale;
+        ss = fmaf(x[k], x[k], ss);
+        if (BWD) tx = fmaf(t[k], x[k], tx);
+      }
+#pragma unroll
+      for (int m = 1; m < LPR; m *= 2) {
+        ss += wave_shfl_xor(ss, m);
+        if (BWD) tx += wave_shfl_xor(tx, m);
+      }
+    }
+    const float r = 1.f / __builtin_sqrtf(fmaf(ss, inv, eps));
     if (!on) continue;
     if (!BWD) {
 #pragma unroll
@@ -114,7 +130,7 @@ __global__ __launch_bounds__(kThreads) void gated_norm_kernel(GatedNormParams p)
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const float xr = x[k] * r;
-        dx[k] = r * (t[k] - x[k] * back);
+        dx[k] = r * scale * (t[k] - x[k] * back);
         dg[k] = y[k] * xr * w[k] * sg[k] * fmaf(g[k], 1.f - sg[k], 1.f);
         dw[k] = fmaf(y[k] * xr, g[k] * sg[k], dw[k]);
       }

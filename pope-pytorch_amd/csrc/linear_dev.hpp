@@ -8,6 +8,10 @@ namespace pope {
 typedef __attribute__((ext_vector_type(2))) float f32x2;
 constexpr float kF32Max = 3.402823466e38f, kBf16Max = 3.3895313892515355e38f;
 
+// The norm of a row whose squares pass fp32's range is that of the row times 2^-100: its largest value, 2^59 at least (of up to 512),
+// is between 2^-41 and 2^28 then, and the eps that goes with it, times 2^-200, nothing beside that.
+constexpr float kNormDown = 0x1p-100f;
+
 // ---------------------------------------------------------------- segments
 
 struct LinSeg {

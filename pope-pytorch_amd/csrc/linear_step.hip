@@ -128,15 +128,20 @@ __global__ __launch_bounds__(kThreads) void linear_step_kernel(LinStepParams p) 
       } else {   // the whole row is here
         __syncthreads();
         if (tid < 64) {
-          float ss = 0.f;
-          for (int d = tid; d < Dv; d += 64) ss += out[d] * out[d];
+          const auto squares = [&](float scale) {
+            float ss = 0.f;
+            for (int d = tid; d < Dv; d += 64) ss += (scale * out[d]) * (scale * out[d]);
 #pragma unroll
-          for (int i = 1; i < 64; i *= 2) ss += wave_shfl_xor(ss, i);
-          const float r = 1.f / __builtin_sqrtf(ss / Dv + p.eps);
+            for (int i = 1; i < 64; i *= 2) ss += wave_shfl_xor(ss, i);
+            return ss;
+          };
+          float down = 1.f, eps = p.eps, ss = squares(1.f);
+          if (!(ss <= kF32Max)) down = kNormDown, eps = 0.f, ss = squares(kNormDown);
+          const float r = 1.f / __builtin_sqrtf(ss / Dv + eps);
           for (int d = tid; d < Dv; d += 64) {
             const float w = p.weight ? lin_value(p.weight, p.w_type, h * p.w_sh + d) : 1.f;
             const float x = lin_get<kTwo>(p.gate, (int64_t)b * p.gate.s[0] + (int64_t)h * p.gate.s[1] + d);
-            lin_set<kTwo>(p.o, orow + d, some ? out[d] * r * w * x * sigmoid_f(x) : 0.f);
+            lin_set<kTwo>(p.o, orow + d, some ? down * out[d] * r * w * x * sigmoid_f(x) : 0.f);
           }
         }
       }

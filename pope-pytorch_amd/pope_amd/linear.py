@@ -36,6 +36,7 @@ from . import _lib
 
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 _MAX_DIM, _MAX_NORM = 256, 512
+_NORM_DOWN = 2.0 ** -100   # kNormDown of csrc/linear_dev.hpp
 _CHUNK = 128   # rows that the CPU computation takes at once
 
 
@@ -411,7 +412,10 @@ def linear_attn_step_with_pope(q: Tensor, k: Tensor, v: Tensor, log_decay: Optio
 
 def _norm_torch(x, gate, weight, eps, head_first):
     y = x.float()
-    y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + eps)
+    with torch.no_grad():   # rows whose squares pass fp32's range, at a smaller scale
+        scale = torch.where(y.square().sum(-1, keepdim=True).isfinite(), 1.0, _NORM_DOWN)
+    y = y * scale
+    y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + eps * scale * scale)
     if exists(weight):
         y = y * (weight.float()[:, None, :] if weight.ndim == 2 and head_first else weight.float())
     return (y * F.silu(gate.float())).to(gate.dtype)

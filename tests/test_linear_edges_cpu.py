@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import pope_amd
-from linear_common import Case, run
+from linear_common import Case, check, norm64, run
 
 CPU = torch.device("cpu")
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -32,3 +32,20 @@ def test_masked_rows_reach_no_gradient(dtype, value):
     for n in clean:
         assert torch.equal(got[n], clean[n]), n
     assert not got["d_k"][0].any() and not got["d_v"][0].any()
+
+
+@pytest.mark.parametrize("size", [1.0, 1e20, 1e37])
+def test_norm_of_large_rows(size):
+    """Rows whose squares pass fp32's range: fp32 arithmetic on them all the same."""
+    g = torch.Generator().manual_seed(3)
+    x, gate, dy = (torch.randn(2, 3, 5, 33, generator=g) for _ in range(3))
+    x[:, :, ::2] *= size
+    w = torch.randn(3, 33, generator=g)
+    leaves = [t.requires_grad_() for t in (x, gate, w)]
+    y = pope_amd.gated_head_norm(x, gate, w)
+    e = [t.detach().double().requires_grad_() for t in leaves]
+    want = norm64(*e, 1e-5)
+    check(y.detach(), want.detach(), 1e-5 * want.detach().abs() + 1e-7, "y")
+    for n, a, b in zip(("dx", "dgate", "dweight"), torch.autograd.grad(y, leaves, dy), torch.autograd.grad(want, e, dy.double())):
+        scale = b.abs().amax(-1, keepdim=True) if n == "dx" else 1.0
+        check(a, b, 1e-4 * scale + 1e-5 * b.abs(), n)

@@ -88,3 +88,51 @@ def test_fp32_values_next_to_the_largest(cuda, name, column, sign):
         for n in val:
             assert val[n].isfinite().all() and got[n].isfinite().all(), (n, at)
             check(got[n], val[n], case.bound(n, val[n], tol[n]), f"{n} {at}")
+
+
+@pytest.mark.parametrize("size", [1e18, 1e20, 1e30, 1e37])
+@pytest.mark.parametrize("dim", [7, 64, 200, 512])
+@pytest.mark.parametrize("x_dtype,dtype", [(F32, F32), (F32, BF16), (F32, F16), (BF16, BF16)])
+def test_norm_of_large_rows(cuda, dim, size, x_dtype, dtype):
+    """Rows whose squares pass fp32's range, among ordinary ones: fp32 arithmetic and one rounding, as for all (512 2^-24 of the sum of
+    squares), above 2^-126, where fp32 and bf16 lose bits."""
+    g = torch.Generator().manual_seed(dim)
+    x, gate, dy = (torch.randn(2, 3, 9, dim, generator=g).to(cuda) for _ in range(3))
+    x[:, :, ::2] *= size
+    x[0, 0, 1, :3] = torch.finfo(BF16).max
+    x, gate, dy = x.to(x_dtype), gate.to(dtype), dy.to(dtype)
+    w = torch.randn(3, dim, generator=g).to(cuda)
+    leaves = [t.requires_grad_() for t in (x, gate, w)]
+    y = gated_head_norm(x, gate, w)
+    got = torch.autograd.grad(y, leaves, dy)
+    e = [t.detach().double().requires_grad_() for t in leaves]
+    want = L.norm64(*e, 1e-5)
+    grads = torch.autograd.grad(want, e, dy.double())
+    u, small = half(dtype), 2.0 ** -126 + (2.0 ** -25 if dtype == F16 else 0)
+    check(y.detach(), want.detach(), (u + 1e-4) * want.detach().abs() + small, "y")
+    with torch.no_grad():
+        a = (dy.double() * e[2][:, None, :] * F.silu(e[1])).abs()
+        rms = (e[0].square().mean(-1, keepdim=True) + 1e-5).sqrt()
+        mags = [(a + e[0].abs() / rms * (a * e[0].abs() / rms).mean(-1, keepdim=True)) / rms, (dy.double() * e[2][:, None, :] * e[0] / rms).abs() * 1.1,
+                (dy.double() * e[0] / rms * F.silu(e[1])).abs().sum((0, 2))]
+    for n, t, got_t, want_t, mag in zip(("dx", "dgate", "dweight"), leaves, got, grads, mags):
+        assert got_t.dtype == t.dtype
+        check(got_t, want_t, half(t.dtype) * want_t.abs() + 1e-4 * mag + small, n)
+
+
+@TYPES
+def test_gated_step_of_large_states(cuda, dtype):
+    case = Case(cuda, B=3, Hq=4, Hk=2, N=1, D=40, R=16, Dv=72, dtype=dtype, initial=True)
+    gate, w = torch.randn(3, 4, 1, 72, device=cuda).to(dtype), torch.rand(72, device=cuda) + 0.5
+    for size in (1.0, 2.0 ** 66, 2.0 ** 110):
+        state = case.s0 * size
+        y = linear_attn_step_with_pope(case.q, case.k, case.v, case.ld, case.emb(), state.clone(), gate=gate, norm_weight=w)
+        o, _ = L.attend64(L.expand64(case.q, case.freqs, None, 16), L.expand64(case.k, case.freqs, case.bias, 16), case.v.double(), case.decay64(), case.scale, None,
+                          state.double(), case.seqs)
+        a, _ = L.attend64(L.expand64(case.q, case.freqs, None, 16).abs() + 0.05, L.expand64(case.k, case.freqs, case.bias, 16).abs() + 0.05, case.v.double().abs(),
+                          case.decay64(), case.scale, None, state.double().abs(), case.seqs)
+        # fp32 sums (2e-5 of absolute values, as in linear_common), relative to a row's size, and the output's rounding
+        rms = (o.square().mean(-1, keepdim=True) + 1e-5).sqrt()
+        want = L.norm64(o, gate, w, 1e-5)
+        e = 2e-5 * a / rms
+        check(y, want, 2 * (e * (w * F.silu(gate.double())).abs() + want.abs() * e.square().mean(-1, keepdim=True).sqrt()) + (half(dtype) + 1e-4) * want.abs() + 2.0 ** -25, size)
