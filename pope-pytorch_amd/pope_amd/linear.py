@@ -337,6 +337,11 @@ def linear_attn_with_pope(q: Tensor, k: Tensor, v: Tensor, log_decay: Optional[T
             o, last = _linear_torch(q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial_state, scale, shape, torch.float32 if o_f32 else q.dtype)
         else:
             o, last, _ = linear_fwd_op(q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial_state, scale, bool(return_state), o_f32)
+        if not o.requires_grad and (n == 0 or B == 0 or not q.is_cuda):
+            for t in (q, k, v, freqs, bias):   # gradients of zeros, for a batch without rows, or with rows of no sequence
+                if _tracked(t):
+                    none = t.flatten()[:0].sum(dtype=torch.float32)
+                    o, last = o + none.to(o.dtype), last + none
         if not hf:
             o = o.transpose(1, 2)
     if exists(gate):

@@ -49,3 +49,21 @@ def test_norm_of_large_rows(size):
     for n, a, b in zip(("dx", "dgate", "dweight"), torch.autograd.grad(y, leaves, dy), torch.autograd.grad(want, e, dy.double())):
         scale = b.abs().amax(-1, keepdim=True) if n == "dx" else 1.0
         check(a, b, 1e-4 * scale + 1e-5 * b.abs(), n)
+
+
+def no_rows_have_gradients(device):
+    for shape, cu in (((2, 4, 0), None), ((0, 4, 5), None), ((1, 4, 0), (0, 0)), ((1, 4, 3), (2, 2))):   # the last: rows of no sequence
+        cu = None if cu is None else torch.tensor(cu, dtype=torch.int32, device=device)
+        x = {n: torch.randn(*s, device=device).requires_grad_() for n, s in dict(q=(*shape, 8), k=(shape[0], 2, shape[2], 8), v=(shape[0], 2, shape[2], 5), freqs=(shape[2], 4), bias=(2, 4),
+                                                                                 s0=(shape[0], 2, 12, 5), gate=(*shape, 5), w=(5,)).items()}
+        for gated in (False, True):
+            o, last = pope_amd.linear_attn_with_pope(x["q"], x["k"], x["v"], None, (x["freqs"], x["bias"]), initial_state=x["s0"], return_state=True, cu_seqlens=cu,
+                                                     gate=x["gate"] if gated else None, norm_weight=x["w"] if gated else None)
+            used = list(x) if gated else list(x)[:6]
+            g = dict(zip(used, torch.autograd.grad([o.sum() + last.sum()], [x[n] for n in used])))
+            for n in used:
+                assert g[n].shape == x[n].shape and g[n].dtype == x[n].dtype and bool((g[n] == (1 if n == "s0" else 0)).all()), n
+
+
+def test_no_rows_have_gradients():
+    no_rows_have_gradients(CPU)

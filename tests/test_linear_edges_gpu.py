@@ -136,3 +136,8 @@ def test_gated_step_of_large_states(cuda, dtype):
         want = L.norm64(o, gate, w, 1e-5)
         e = 2e-5 * a / rms
         check(y, want, 2 * (e * (w * F.silu(gate.double())).abs() + want.abs() * e.square().mean(-1, keepdim=True).sqrt()) + (half(dtype) + 1e-4) * want.abs() + 2.0 ** -25, size)
+
+
+def test_no_rows_have_gradients(cuda):
+    from test_linear_edges_cpu import no_rows_have_gradients
+    no_rows_have_gradients(cuda)
