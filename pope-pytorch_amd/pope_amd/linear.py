@@ -289,7 +289,7 @@ def linear_attn_with_pope(q: Tensor, k: Tensor, v: Tensor, log_decay: Optional[T
     fp32.  Packed calls have batch 1 and ``cu_seqlens`` (sequences + 1 ascending numbers): rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1
     belong to sequence b; rows outside every sequence give 0.
 
-    ``gate`` (as o): o is ``gated_head_norm(o, gate, norm_weight, eps=norm_eps)``.
+    ``gate`` (shaped as o; bf16, fp16 or fp32, which the result then has): o is ``gated_head_norm(o, gate, norm_weight, eps=norm_eps)``.
 
     A value that is not finite reaches the rows from its own on, where sums through a state may turn infinities into NaN; on the GPU,
     finite fp32 values above 3.3895e38, the largest bf16, count as that.  GPU calls
@@ -300,6 +300,12 @@ def linear_attn_with_pope(q: Tensor, k: Tensor, v: Tensor, log_decay: Optional[T
     hf = bool(head_dimension_at_first)
     if exists(norm_weight) and not exists(gate):
         raise ValueError("norm_weight given without a gate")
+    if exists(gate) and q.ndim == 4 and v.ndim == 4:   # before anything is launched
+        want = (*q.shape[:3], v.shape[3])
+        if tuple(gate.shape) != want:
+            raise ValueError(f"gate {tuple(gate.shape)} must match the output {want}")
+        _check_device(q, gate=gate)
+        _check_norm(gate, gate, norm_weight, q.shape[1 if hf else 2])
     # the norm divides by the size of a row, and a short row's own rounding would come out as large as that row is small: its
     # input, and the gradient that comes back, are fp32
     o_f32 = exists(gate)
@@ -360,7 +366,7 @@ def linear_attn_step_with_pope(q: Tensor, k: Tensor, v: Tensor, log_decay: Optio
     can go on from a prompt that they share.  No slot may be written by two sequences of a call, or written by one and read by
     another: what they then hold is unspecified.  A sequence whose ``state_index`` is no slot has no token: its output is 0 and nothing
     is written; a ``new_index`` that is no slot is not written.  ``pos_emb``: (freqs, bias) of the new rows, freqs (1, rotate dim) or (batch,
-    1, rotate dim); the other arguments as in ``linear_attn_with_pope``.  No gradient is defined."""
+    1, rotate dim); ``gate`` has the rows' dtype; the other arguments as in ``linear_attn_with_pope``.  No gradient is defined."""
     freqs, bias = pos_emb if exists(pos_emb) else (None, None)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     hf = bool(head_dimension_at_first)

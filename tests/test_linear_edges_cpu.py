@@ -67,3 +67,24 @@ def no_rows_have_gradients(device):
 
 def test_no_rows_have_gradients():
     no_rows_have_gradients(CPU)
+
+
+def test_gates_are_refused_before_the_attention(monkeypatch):
+    case = Case(CPU, N=6, D=8, R=4, Dv=5)
+    call = lambda **kw: pope_amd.linear_attn_with_pope(case.q, case.k, case.v, case.ld, case.emb(), **kw)
+    gate = torch.randn(1, 2, 6, 5)
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):   # of any of the types, whatever the rows'
+        assert call(gate=gate.to(dtype), norm_weight=torch.ones(5)).dtype == dtype
+
+    def computed(*a):
+        raise AssertionError("the attention ran")
+
+    monkeypatch.setattr(pope_amd.linear, "_linear_torch", computed)
+    with pytest.raises(AssertionError):
+        call(gate=gate)
+    for kind, match, kw in ((ValueError, "gate", dict(gate=gate[..., :4])), (ValueError, "gate", dict(gate=gate.transpose(1, 2))), (ValueError, "gate", dict(gate=gate[0])),
+                            (TypeError, "gate", dict(gate=gate.double())), (ValueError, "weight", dict(gate=gate, norm_weight=torch.ones(4))),
+                            (TypeError, "weight", dict(gate=gate, norm_weight=torch.ones(5, dtype=torch.float16))),
+                            (RuntimeError, "meta", dict(gate=gate.to("meta"))), (RuntimeError, "meta", dict(gate=gate, norm_weight=torch.ones(5, device="meta")))):
+        with pytest.raises(kind, match=match):
+            call(**kw)
