@@ -72,6 +72,11 @@ def _check_rows(q: Tensor, k: Tensor, v: Tensor):
         raise ValueError(f"dim and value dim must be 1 to {_MAX_DIM}, got {q.shape[3]} and {v.shape[3]}")
 
 
+def _default_scale(q: Tensor) -> float:
+    dim = q.shape[-1] if q.ndim else 0
+    return dim ** -0.5 if dim else 1.0   # no dim: refused with the rows
+
+
 def _check_pos_emb(pos_emb, q: Tensor, heads: int):
     """freqs (n, R) or (1 or batch, n, R) and bias (1 or heads, R); None, None without rotation."""
     if not exists(pos_emb):
@@ -296,7 +301,7 @@ def linear_attn_with_pope(q: Tensor, k: Tensor, v: Tensor, log_decay: Optional[T
     that would need 2^22 workgroups (about one for each 64 rows or more of each head) raise."""
     args = (log_decay, mask, cu_seqlens, initial_state)
     freqs, bias = pos_emb if exists(pos_emb) else (None, None)
-    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    scale = _default_scale(q) if scale is None else float(scale)
     hf = bool(head_dimension_at_first)
     if exists(norm_weight) and not exists(gate):
         raise ValueError("norm_weight given without a gate")
@@ -368,7 +373,7 @@ def linear_attn_step_with_pope(q: Tensor, k: Tensor, v: Tensor, log_decay: Optio
     is written; a ``new_index`` that is no slot is not written.  ``pos_emb``: (freqs, bias) of the new rows, freqs (1, rotate dim) or (batch,
     1, rotate dim); ``gate`` has the rows' dtype; the other arguments as in ``linear_attn_with_pope``.  No gradient is defined."""
     freqs, bias = pos_emb if exists(pos_emb) else (None, None)
-    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    scale = _default_scale(q) if scale is None else float(scale)
     hf = bool(head_dimension_at_first)
     if q.is_cuda and _lib.eager(q, k, v, freqs, bias, log_decay, state, state_index, new_index, gate, norm_weight):
         o = _lib.host().linear_step_eager(q, k, v, freqs, bias, log_decay, state, state_index, new_index, gate, norm_weight, norm_eps, scale, hf)

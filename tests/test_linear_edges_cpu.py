@@ -88,3 +88,11 @@ def test_gates_are_refused_before_the_attention(monkeypatch):
                             (RuntimeError, "meta", dict(gate=gate.to("meta"))), (RuntimeError, "meta", dict(gate=gate, norm_weight=torch.ones(5, device="meta")))):
         with pytest.raises(kind, match=match):
             call(**kw)
+
+
+def test_rows_without_a_dim_are_refused():
+    for call in (lambda *a: pope_amd.linear_attn_with_pope(*a), lambda *a: pope_amd.linear_attn_step_with_pope(*a, None, None, torch.zeros(1, 2, 1, 1))):
+        with pytest.raises(ValueError, match="1 to 256"):
+            call(*(torch.zeros(1, 2, 1, 0) for _ in range(3)))
+        with pytest.raises(ValueError, match="4-D"):
+            call(*(torch.zeros(()) for _ in range(3)))
