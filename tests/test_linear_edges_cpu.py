@@ -96,3 +96,15 @@ def test_rows_without_a_dim_are_refused():
             call(*(torch.zeros(1, 2, 1, 0) for _ in range(3)))
         with pytest.raises(ValueError, match="4-D"):
             call(*(torch.zeros(()) for _ in range(3)))
+
+
+def test_exact_operands_give_the_formula():
+    """linear_rounded without roundings is the formula of linear_common; with those of one part it is off by what bf16 takes."""
+    from linear_rounded import outputs
+    for shape in (dict(B=2, N=70, mask="random", batch_freqs=True), dict(Hq=4, Hk=2, N=50, D=24, R=10, Dv=9, initial=True, bias_heads=1), dict(N=40, D=12, R=0, Dv=8)):
+        case = Case(CPU, dtype=torch.bfloat16, **shape)
+        val, _ = case.exact()
+        for n, y in outputs(case, 0, own=False).items():
+            assert (y - val[n]).norm() <= 1e-12 * val[n].norm(), n
+        for n, y in outputs(case, 1).items():
+            assert 1e-3 * val[n].norm() <= (y - val[n]).norm() <= 6e-3 * val[n].norm(), n
