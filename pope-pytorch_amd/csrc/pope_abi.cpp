@@ -1323,10 +1323,11 @@ LinShape linear_shape(const pope_linear& d, bool packed) {
   s.parts = d.N > s.L;
   s.grid = (int)grid;
   s.EP = round_up(d.D + d.R, 32);
-  // Two parts also for bf16 sequences of up to one chunk of them, while that takes no second round of the chip: a few rows have few
-  // roundings to even out, and the time is the same (8 heads, D 64, R 32, forward and backward: 1 row 35 us as two parts, 36 as one; 16
-  // rows 32 and 32; 64 rows 50 and 37).
-  const bool few = d.N <= 32 && (int64_t)d.B * d.Hk <= kLinGrid / 2;
+  // Two parts also for calls of up to one chunk of bf16 rows a sequence, whatever the batch: a few rows have few roundings to even
+  // out, and the time is about the same.  us as two parts and as one, forward, forward and backward: one sequence of 8 heads, D 64, R 32, 1
+  // row - 35, - 36; 64 rows - 50, - 37.  32 rows of 256 sequences of 16 heads, D 64, R 32: 77 279, 90 295; of 256 x 8, D 128, R 64: 150 405,
+  // 158 413; of 64 x 16, D 256, R 128: 179 526, 164 527; 1 row of those 159 479, 154 441.
+  const bool few = d.N <= 32;
   s.planes = d.dtype != POPE_BF16 || d.o_f32 || few ? 2 : 1;
   s.qh = align_up((size_t)rows * d.Hq * s.EP * 2) * s.planes;
   s.kh = align_up((size_t)rows * d.Hk * s.EP * 2) * s.planes;

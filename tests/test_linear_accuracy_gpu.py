@@ -69,6 +69,16 @@ def test_few_bf16_rows_in_two_parts(cuda, rows, packed):
         check(got[n], val[n], (rel + 2e-5) * tol[n] * (1 + own) + own * val[n].abs() + 1e-30, n)
 
 
+@pytest.mark.parametrize("shape", [dict(B=40, Hq=8, Hk=8), dict(B=9, Hq=64, Hk=32, D=24, R=8, Dv=20)])
+def test_few_bf16_rows_are_as_exact_in_large_batches(cuda, shape):
+    case = Case(cuda, N=17, dtype=BF16, **shape)
+    got = run(pope_amd, case)
+    val, tol = case.exact()
+    for n in ("o", "d_q", "d_k", "d_v"):
+        own = half(BF16)
+        check(got[n], val[n], (6 * 2.0 ** -16 + 2e-5) * tol[n] * (1 + own) + own * val[n].abs() + 1e-30, n)
+
+
 def test_gated_bf16_gradients_in_two_parts(cuda):
     """bf16 rows under a gate: what gradients are off by beyond their own rounding.  Operands of two parts leave 6e-6 of the sums' norms;
     the norm behind them raises that in rows that are short beside their terms, by 100 in the worst one: 1e-3 over all allows
