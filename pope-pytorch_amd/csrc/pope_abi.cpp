@@ -1274,7 +1274,7 @@ namespace {
 
 // ---------------------------------------------------------------- linear attention
 
-int check_linear(const pope_linear* d) {
+int check_linear(const pope_linear* d, bool packed) {
   if (!d) return fail(POPE_ERR_INVALID, "descriptor is NULL");
   if (d->B < 1 || d->N < 0 || d->Hq < 1 || d->Hk < 1)
     return fail(POPE_ERR_INVALID, "B, Hq, Hk must be >= 1 and N >= 0 (got %d, %d, %d, %d)", d->B, d->Hq, d->Hk, d->N);
@@ -1286,6 +1286,8 @@ int check_linear(const pope_linear* d) {
   if (d->bias_dtype != POPE_F32 && d->bias_dtype != POPE_F16 && d->bias_dtype != POPE_BF16) return fail(POPE_ERR_INVALID, "unknown bias dtype %d", d->bias_dtype);
   if (d->N > (1 << 28) || d->B > (1 << 20) || d->Hq > 65535)
     return fail(POPE_ERR_UNSUPPORTED, "%d sequences, %d rows, %d heads: too many", d->B, d->N, d->Hq);
+  // byte counts, and the segments' number in 32 bits, stay in range
+  if ((int64_t)(packed ? 1 : d->B) * d->N > ((int64_t)1 << 40) / d->Hq) return fail(POPE_ERR_UNSUPPORTED, "%d x %d rows of %d heads: too many", d->B, d->N, d->Hq);
   if (d->bias_sh < 0 || d->mask_sb < 0) return fail(POPE_ERR_INVALID, "negative bias / mask stride");
   for (const int64_t st : {d->q_s[2], d->k_s[2], d->v_s[2], d->o_s[2], d->f_s[1], d->do_s[2], d->dq_s[2], d->dk_s[2], d->dv_s[2]})
     if (st >= POPE_LINEAR_ROW_STRIDE && d->N > 1) return fail(POPE_ERR_UNSUPPORTED, "a row stride of %lld elements is beyond a chunk's 32-bit offsets", (long long)st);
@@ -1443,7 +1445,7 @@ pope::GatedNormParams norm_params(const pope_gated_norm& d, const void* x, const
 extern "C" {
 
 int pope_linear_bytes(const pope_linear* d, int packed, int final, int want_dfreqs, size_t bytes[2]) {
-  const int rc = check_linear(d);
+  const int rc = check_linear(d, packed != 0);
   if (rc) return rc;
   if (!bytes) return fail(POPE_ERR_INVALID, "bytes is NULL");
   const LinShape s = linear_shape(*d, packed != 0);
@@ -1455,7 +1457,7 @@ int pope_linear_bytes(const pope_linear* d, int packed, int final, int want_dfre
 int pope_linear_fwd(const pope_linear* d, const void* q, const void* k, const void* v, const float* freqs, const void* bias,
                     const float* log_decay, const uint8_t* mask, const int32_t* cu, const float* initial, void* o, float* last,
                     void* kept, size_t kept_bytes, void* stream) {
-  int rc = check_linear(d);
+  int rc = check_linear(d, cu != nullptr);
   if (rc) return rc;
   if (d->N == 0) return last ? fail(POPE_ERR_INVALID, "no rows: the states are those given") : POPE_OK;
   if ((rc = check_linear_ptrs(d, q, k, v, freqs, bias))) return rc;
@@ -1489,7 +1491,7 @@ int pope_linear_bwd(const pope_linear* d, const void* dout, const float* dlast, 
                     const float* freqs, const void* bias, const float* log_decay, const uint8_t* mask, const int32_t* cu,
                     const float* initial, const void* kept, size_t kept_bytes, void* dq, void* dk, void* dv, float* dfreqs,
                     void* dbias, float* dinitial, void* workspace, size_t workspace_bytes, void* stream) {
-  int rc = check_linear(d);
+  int rc = check_linear(d, cu != nullptr);
   if (rc) return rc;
   for (const int64_t* st : {d->do_s, d->dq_s, d->dk_s, d->dv_s})
     if ((rc = check_strides("gradient", st, 3))) return rc;
@@ -1596,7 +1598,7 @@ int pope_gated_norm_bwd(const pope_gated_norm* d, const void* dy, const void* x,
 int pope_linear_step(const pope_linear* d, const void* q, const void* k, const void* v, const float* freqs, const void* bias,
                      const float* log_decay, float* states, int32_t slots, int64_t slot_s, const int32_t* from, const int32_t* to,
                      const pope_gated_norm* norm, const void* gate, const void* weight, void* o, void* stream) {
-  int rc = check_linear(d);
+  int rc = check_linear(d, false);
   if (rc) return rc;
   if (d->N != 1) return fail(POPE_ERR_INVALID, "a step takes one row for each sequence (N = %d)", d->N);
   if ((rc = check_linear_ptrs(d, q, k, v, freqs, bias))) return rc;

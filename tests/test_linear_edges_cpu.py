@@ -108,3 +108,18 @@ def test_exact_operands_give_the_formula():
             assert (y - val[n]).norm() <= 1e-12 * val[n].norm(), n
         for n, y in outputs(case, 1).items():
             assert 1e-3 * val[n].norm() <= (y - val[n]).norm() <= 6e-3 * val[n].norm(), n
+
+
+def test_abi_refuses_rows_beyond_its_counts():
+    """Their bytes and segments would pass the integers that hold them: a query answered with what was left of those."""
+    import ctypes
+
+    from pope_amd import _lib
+    from test_linear_cpu import _desc
+    size = (ctypes.c_size_t * 2)()
+    ask = lambda packed, **kw: _lib.lib().pope_linear_bytes(ctypes.byref(_desc(**kw)), packed, 1, 1, size)
+    assert ask(0, B=1 << 20, N=1 << 28, Hq=32768, Hk=32768) != 0
+    assert ask(0, B=1 << 20, N=1 << 20, Hq=2, Hk=1) != 0
+    assert ask(0, B=1 << 20, N=1 << 19, Hq=2, Hk=1) == 0 and size[0] >= 3 * (1 << 39) * 96 * 2
+    assert ask(1, B=1 << 16, N=1 << 20, Hq=64, Hk=64) == 0   # sequences of packed rows are not rows
+    assert ask(1, B=1, N=1 << 28, Hq=4, Hk=4) == 0 and size[0] >= 8 * (1 << 28) * 96 * 2
