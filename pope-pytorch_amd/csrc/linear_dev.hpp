@@ -17,8 +17,9 @@ constexpr float kNormDown = 0x1p-100f;
 struct LinSeg {
   int seq, batch;   // seq < 0: none
   int row0, len;    // rows row0 .. row0 + len - 1 of the batch entry
-  int m;            // which of the sequence's
+  int m;            // which of the sequence's; where there is none: how many segments there are
 };
+constexpr int kLinNone = 0x7fffffff;   // behind every segment
 
 __device__ __forceinline__ int lin_bound(const LinSeqs& q, int i) { return min(max(q.cu[i], 0), q.N); }
 
@@ -76,6 +77,7 @@ __device__ __forceinline__ LinSeg lin_segment(const LinSeqs& q, int at) {
     }
     before += __builtin_amdgcn_readlane(upto, 63);
   }
+  g.m = before;
   return g;
 }
 

@@ -55,26 +55,28 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
   const int pcols = kind == kLinOut || kind == kLinDv ? c.E : c.Dv;          // of the contraction
   const int n0 = tile * NT;
   constexpr bool chain = kind == kLinDq || kind == kLinDk;
-  const int out_cols = out.cols;
 
-  if (c.seqs.cu && at == c.seqs.T) {   // rows outside every sequence: zeros
-    if (tile) return;
+  // packed calls have a workgroup more than there can be segments
+  const LinSeg seg = lin_segment(c.seqs, c.seqs.cu && at == c.seqs.T ? kLinNone : at);
+  if (seg.seq < 0) {
+    if (kind == kLinDk && p.dbias && at < c.seqs.T)
+      for (int d = tid; d < c.R; d += kThreads) p.dbias[((int64_t)at * c.Hk + hk) * c.R + d] = 0.f;
+    // Rows outside every sequence become zeros, a row a wave, by all workgroups without a segment (200 rows in a buffer of 32,768, 8
+    // heads, D 64, bf16: one workgroup a head took 1,879 us for the call, all of them 71).
+    const int total = (unsigned)seg.m < (unsigned)c.seqs.T ? seg.m : c.seqs.T;   // bounds that descend may have any
+    const int workers = (c.seqs.T + 1 - total) * tiles, worker = (at - total) * tiles + tile;
     const int lo = lin_bound(c.seqs, 0), hi = lin_bound(c.seqs, c.seqs.B);
-    for (int64_t it = tid; it < (int64_t)(lo + c.seqs.N - hi) * out_cols; it += kThreads) {
-      const int r = (int)(it / out_cols), d = (int)(it - (int64_t)r * out_cols), row = r < lo ? r : hi + r - lo;
+    for (int64_t r = worker * K::NW + wave; r < lo + c.seqs.N - hi; r += workers * K::NW) {
+      const int64_t row = r < lo ? r : hi + r - lo;
       for (int g = 0; g < (by_query ? ng : 1); ++g) {
         const int h = by_query ? (g0 + g) * c.Hk + hk : hk;
-        lin_set<PL>(out, (int64_t)h * out.s[1] + (int64_t)row * out.s[2] + d, 0.f);
-        if (chain && p.dphase[which] && d < c.R) p.dphase[which][((int64_t)h * c.seqs.N + row) * c.R + d] = 0.f;
+        lin_set4<PL>(out, lin_base(out, 0, h, row), 0u, 4 * lane, f32x4{0.f, 0.f, 0.f, 0.f});
+        if (chain && p.dphase[which])
+          for (int d = lane; d < c.R; d += 64) p.dphase[which][((int64_t)h * c.seqs.N + row) * c.R + d] = 0.f;
       }
     }
     return;
   }
-  const LinSeg seg = lin_segment(c.seqs, at);
-  if (kind == kLinDk && p.dbias && seg.seq < 0) {
-    for (int d = tid; d < c.R; d += kThreads) p.dbias[((int64_t)at * c.Hk + hk) * c.R + d] = 0.f;
-  }
-  if (seg.seq < 0) return;
 
   uint16_t* lds = reinterpret_cast<uint16_t*>(smem);
   const LinTile X{lds, K::XS, C * K::XS};

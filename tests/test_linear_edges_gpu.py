@@ -141,3 +141,22 @@ def test_gated_step_of_large_states(cuda, dtype):
 def test_no_rows_have_gradients(cuda):
     from test_linear_edges_cpu import no_rows_have_gradients
     no_rows_have_gradients(cuda)
+
+
+# ---------------------------------------------------------------- buffers that are mostly empty
+
+@TYPES
+@pytest.mark.parametrize("lens,lead,tail", [([60, 40], 1500, 3400), ([0, 0], 0, 4097), ([1], 4100, 0), ([3] * 70, 5, 1), ([2500], 700, 900)])
+def test_rows_of_no_sequence_are_zeros(cuda, lens, lead, tail, dtype):
+    """Every output and gradient row outside every sequence is written, over memory that held NaN, with shared and single heads, wide and odd rows."""
+    for kw in (dict(Hq=4, Hk=2, D=40, R=20, Dv=48), dict(Hq=1, Hk=1, D=130, R=65, Dv=250), dict(Hq=6, Hk=2, D=9, R=3, Dv=7)):
+        case = Case(cuda, lens=lens, lead=lead, tail=tail, dtype=dtype, initial=True, **kw)
+        stale = [torch.full((n,), math.nan, device=cuda) for n in (1 << 16, 1 << 18, 1 << 20, 1 << 22) for _ in range(4)]
+        del stale
+        got = run(pope_amd, case, head_first=False)
+        outside = torch.ones(case.q.shape[2], dtype=torch.bool, device=cuda)
+        outside[lead:lead + sum(lens)] = False
+        for n in ("o", "d_q", "d_k", "d_v"):
+            assert torch.equal(got[n][:, :, outside], torch.zeros_like(got[n][:, :, outside])), n
+        assert not got["d_freqs"][outside].any()
+        L.compare(got, case)
