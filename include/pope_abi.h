@@ -350,15 +350,17 @@ int pope_paged_attn(const pope_paged* desc, const void* q, const float* freqs, c
 /*
  * Linear attention of PoPE rows with a decay for each head.  No counterpart in the reference.
  *
- * With q_hat, k_hat the rows of pope_polar_fwd (D + R columns, (cos, sin) pairs interleaved, unrounded), g = exp(log_decay) of
+ * With q_hat, k_hat the rows of pope_polar_fwd (D + R columns, (cos, sin) pairs interleaved), g = exp(log_decay) of
  * the kv head (NULL: 1) and S its state of (D + R, Dv):
  *   S_i = g S_(i-1) + k_hat_i v_i^T,   o_i = scale S_i^T q_hat_i
  * over the rows i of a sequence; query head h reads kv head h % Hk.  Rows whose mask byte (B, N) is 0 have no key and no value
  * (their query still has an output).  Padded batches: B sequences of N rows; packed (cu_seqlens given): N rows in one batch entry,
  * sequence b owning rows cu_seqlens[b] <= r < cu_seqlens[b + 1]; outputs and gradients of rows outside every sequence are 0.
  * cu_seqlens that decrease leave unspecified values (never an access out of bounds).  States are fp32 (B, Hk, D + R, Dv),
- * contiguous; `initial` NULL: zeros.  Products take bf16 rows as they are; fp16 and fp32 rows, bf16 rows with o_f32, and a few bf16
- * rows, as the sum of two bf16 parts (2^-16 of each factor; finite fp32 values above the largest bf16 count as that).  Calls that need 2^22 workgroups or more return POPE_ERR_UNSUPPORTED.
+ * contiguous; `initial` NULL: zeros.  Operands of products are bf16: of bf16 rows one part (q_hat times scale, k_hat, the weighted
+ * x . y and states each rounded); of fp16 and fp32 rows, bf16 rows with o_f32, and bf16 calls of N <= 32, the sum of two parts (2^-16 of
+ * each factor; finite fp32 values above the largest bf16 count as that).  Calls that need 2^22 workgroups or more, or whose rows
+ * times Hq pass 2^40, return POPE_ERR_UNSUPPORTED.
  */
 #define POPE_LINEAR_ROW_STRIDE (1 << 22)  /* row strides are below this many elements, where there are rows */
 typedef struct pope_linear {

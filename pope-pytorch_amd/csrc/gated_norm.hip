@@ -3,8 +3,8 @@
 //
 // Bound by HBM (three rows of 16-bit values forward, five backward) or the launch.  A row is 8 columns for each of 8 to 64 lanes;
 // all arithmetic is fp32, rounded once.
-// 48,000 rows of 128 with fp32 x: 14 us (3.5 TB/s) and 22 back (3.9); 96,000 rows of 100 in fp16, in units of four: 16 us, 3.6 TB/s
-// (element by element 34); 65,536 rows of 64: 11 and 16, which is latency: four turns of a workgroup, each waiting for its rows.
+// 48,000 rows of 128 with fp32 x: 14 us (3.5 TB/s) and 21 back (3.9); 96,000 rows of 100 in fp16, in units of four: 16 us, 3.6 TB/s
+// (element by element 34); 65,536 rows of 64: 11 and 17, which is latency: four turns of a workgroup, each waiting for its rows.
 #include <algorithm>
 
 #include "linear_dev.hpp"

@@ -18,10 +18,10 @@
 //
 // Rounding: x, y, z, the weighted C x C products and W as an operand are bf16: one part for bf16 rows (each is off by at most 2^-8,
 // as the output is by its own rounding), the sum of two for fp16 and fp32 rows, for bf16 rows whose output goes on in fp32, and for
-// a few bf16 rows (2^-16; C is 32 then).  W itself, all sums and the powers of g are fp32.
+// calls of up to 32 bf16 rows (2^-16; C is 32 then).  W itself, all sums and the powers of g are fp32.
 //
 // What bounds it: waits.  32,768 rows of 8 heads, D 64, R 32, bf16: 45-48 us for the outputs (6.4 GFLOP, 167 MB, 3.5 TB/s); 2 x 4,096 of
-// them: outputs 19, dq and dk 62, dv 19.  D 256, R 256 (2 x 2,048 rows): 77, 200 and 77, where a segment's state is 512 KB, its load a
+// them: outputs 19, dq and dk 62, dv 20.  D 256, R 256 (2 x 2,048 rows): 80, 213 and 80, where a segment's state is 512 KB, its load a
 // burst of 15 us, and one workgroup has a CU.  A chunk's tiles come a chunk ahead where registers allow; two workgroups a CU cover for
 // each other where LDS allows.
 #pragma once
@@ -256,7 +256,7 @@ __device__ __forceinline__ void lin_out_job(const LinOutParams& p, int wg, char*
   };
 
   // A row alone: the norm behind it leaves of its gradient what is at right angles to the row itself, so dO . v is a sum that all but
-  // cancels, 500 times and more.  That product, and the row's own direction, are in fp32 then.
+  // cancels, 500 times and more.  Its sum is over fp32 values then, not their parts; it goes on as two parts, as the row that it multiplies.
   const bool lone = PL == kTwo && seg.len == 1;
   f32x4 O[CT][IT];
   const int turns_n = chunks * ng;

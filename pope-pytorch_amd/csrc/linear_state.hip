@@ -8,7 +8,7 @@
 //   scan     S <- g^len S + sum, segment by segment; what a segment starts from goes where its sum was
 //   phase    sums of the phases' gradients over segments (bias) and heads (freqs), in a fixed order
 //
-// Bound by memory, and by the sines and exponentials of the expansion: 32,768 rows of 8 heads, D 64, R 32, bf16, take 59-64 us (189 MB to and
+// Bound by memory, and by the sines and exponentials of the expansion: 32,768 rows of 8 heads, D 64, R 32, bf16, take 54-64 us (189 MB to and
 // from HBM, 3 TB/s), the sums from expanded rows (2 x 4,096 of them) 11, a scan of 134 MB of states 28 (4.8 TB/s).
 // Expanding rows where they are used instead cost more: the forward over those 32,768 rows took 86 us and its states 46, against 45 and
 // 64 with the rows expanded here.  So did a launch of its own for the expansion: 20 us and 10 for the sums against 19 (2 x 4,096 rows).

@@ -1,6 +1,6 @@
 """Linear attention of PoPE rows with a decay for each head, its single-token step, and the gated norm behind it.
 
-With q_hat, k_hat the rows of ``apply_pope_to_qk`` (unrounded), g = exp(log_decay) of a kv head and S its state, a matrix of
+With q_hat, k_hat the rows of ``apply_pope_to_qk``, g = exp(log_decay) of a kv head and S its state, a matrix of
 (dim + rotate_dim, value dim) in fp32 whose rows have the column order of ``apply_pope_to_qk``:
 
   S_i = g S_(i-1) + k_hat_i v_i^T        o_i = scale S_i^T q_hat_i
@@ -17,6 +17,15 @@ head h % heads, as in the softmax attention here.
 Rows are bf16, fp16 or fp32, (batch, heads, n, dim) or (batch, n, heads, dim) with ``head_dimension_at_first=False``; dim and the value
 dim go up to 256, of any size.  A sequence goes on from a state with any split of its rows over calls: positions come from
 ``pos_emb``, ``pope(positions)``, one row of angles per row.
+
+Precision on the GPU.  States, sums, powers of g and the norm are fp32; softplus, sine and cosine are off by up to 1e-6, whatever their
+value.  A step is fp32 throughout, from rows as they are.  Prompts and training run on bf16 matrix instructions.  bf16 rows are one
+bf16 part: q_hat (times the scale), k_hat, the weighted q_hat . k_hat (backward: dO . v) and a state on its way into a product are each
+rounded to bf16, which leaves outputs and gradients off by 0.003 to 0.004 in the 2-norm; their own rounding is 0.0017 of that.  fp16 and fp32
+rows are the sum of two bf16 parts, as are bf16 rows under a gate and calls of up to 32 bf16 rows a sequence (packed: in all): 16 significant
+bits, fp32 rows too, the product of the second parts left out; outputs are off by 1e-5, and by their own rounding.  The states that a call returns
+have keys of two parts whatever the rows.  How rows are cut into segments depends on the call's batch, heads and length, and with that the last
+bits of a sequence's results; the same call gives the same bits.
 
 No counterpart in the reference, whose attention is the softmax's (PoPE_pytorch/attention.py:75-145).  GPU tensors run the HIP
 kernels (csrc/linear_*.hip, csrc/gated_norm.hip), CPU tensors the torch computation below.  Calls do not synchronise or read
