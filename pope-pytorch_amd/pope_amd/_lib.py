@@ -12,6 +12,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libpope_hip.so")
 ABI_VERSION = 3
@@ -210,6 +211,13 @@ def eager(*ts) -> bool:
     operator-recording checkpointing), no functorch transform and no tensor subclass, each of which works on
     the ops."""
     return not torch.compiler.is_compiling() and host().untraced() and all(type(t) in _PLAIN for t in ts)
+
+
+def refuse_tangents(what: str, *ts) -> None:
+    """The ops have no forward-mode derivative.  A functorch transform or a mode would have them drop their inputs' tangents without
+    a word: the result's would be 0."""
+    if not torch.compiler.is_compiling() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise RuntimeError(f"pope_amd {what}: no forward-mode derivative is defined")
 
 
 def last_error() -> str:

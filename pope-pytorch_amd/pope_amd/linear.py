@@ -285,6 +285,7 @@ def gated_head_norm(x: Tensor, gate: Tensor, weight: Optional[Tensor] = None, *,
         weight = weight.contiguous()
     if not x.is_cuda:
         return _norm_torch(x, gate, weight, eps, head_dimension_at_first)
+    _lib.refuse_tangents("gated norm", x, gate, weight)
     return gated_norm_fwd_op(x, gate, weight, float(eps), bool(head_dimension_at_first))
 
 
@@ -356,6 +357,7 @@ def linear_attn_with_pope(q: Tensor, k: Tensor, v: Tensor, log_decay: Optional[T
         elif not q.is_cuda:
             o, last = _linear_torch(q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial_state, scale, shape, torch.float32 if o_f32 else q.dtype)
         else:
+            _lib.refuse_tangents("linear attention", q, k, v, freqs, bias, initial_state)
             o, last, _ = linear_fwd_op(q, k, v, freqs, bias, log_decay, mask, cu_seqlens, initial_state, scale, bool(return_state), o_f32)
         if not o.requires_grad and (n == 0 or B == 0 or not q.is_cuda):
             for t in (q, k, v, freqs, bias):   # gradients of zeros, for a batch without rows, or with rows of no sequence

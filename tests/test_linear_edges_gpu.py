@@ -160,3 +160,24 @@ def test_rows_of_no_sequence_are_zeros(cuda, lens, lead, tail, dtype):
             assert torch.equal(got[n][:, :, outside], torch.zeros_like(got[n][:, :, outside])), n
         assert not got["d_freqs"][outside].any()
         L.compare(got, case)
+
+
+# ---------------------------------------------------------------- forward-mode derivatives
+
+def test_tangents_are_refused_under_transforms(cuda):
+    """There is no forward-mode derivative: torch's would be 0, without a word."""
+    case = Case(cuda, B=2, N=70, initial=True, dtype=F32)
+    ones = {n: torch.ones_like(t) for n, t in case.leaves().items()}
+    for name in case.leaves():
+        def f(t):
+            x = dict(case.leaves(), **{name: t})
+            return linear_attn_with_pope(x["q"], x["k"], x["v"], case.ld, (x["freqs"], x["bias"]), initial_state=x["s0"])
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            torch.func.jvp(f, (case.leaves()[name],), (ones[name],))
+        assert torch.equal(torch.func.vmap(f, in_dims=0)(case.leaves()[name][None])[0], f(case.leaves()[name]))   # other transforms are as they were
+    gate, w = torch.randn_like(case.do), torch.rand(64, device=cuda)
+    for i in range(3):
+        args = [case.do, gate, w]
+        f = lambda t: gated_head_norm(*args[:i], t, *args[i + 1:])
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            torch.func.jvp(f, (args[i],), (torch.ones_like(args[i]),))
