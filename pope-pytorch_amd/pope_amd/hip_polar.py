@@ -167,6 +167,7 @@ def polar(q: Tensor, k: Tensor, freqs: Tensor, bias: Tensor, return_complex: boo
     if eager:   # the same forward / backward without the custom-op dispatch
         qh, kh = _lib.host().polar(q, k, freqs, bias, return_complex)
     else:
+        _lib.refuse_tangents("polar transform", q, k, freqs, bias)
         qh, kh = polar_fwd_op(q, k, freqs, bias, return_complex)
     if return_complex:
         W = q.shape[-1]

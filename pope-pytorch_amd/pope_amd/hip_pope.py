@@ -193,5 +193,6 @@ def hip_compute_qk_similarity(q, k, freqs, bias, rotate_dim=None, allow_tf32=Tru
     if eager:   # the same forward / backward without the custom-op dispatch
         sim = _lib.host().sim(qf, kf, freqs, bias, bool(allow_tf32))
     else:
+        _lib.refuse_tangents("similarity", qf, kf, freqs, bias)
         sim = sim_fwd_op(qf, kf, freqs, bias, bool(allow_tf32))
     return sim.to(out_dtype) if out_dtype != torch.float32 else sim

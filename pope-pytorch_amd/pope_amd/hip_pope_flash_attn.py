@@ -516,6 +516,7 @@ def _flash(q, k, v, freqs, bias, mask, causal, scale) -> Tensor:
     """The native call layer (csrc_torch/pope_host.cpp), or the ops above, with the same forward / backward,
     where tracing, a dispatch mode or a transform works on the call."""
     if not _lib.eager(q, k, v, freqs, bias, mask):
+        _lib.refuse_tangents("flash attention", q, k, v, freqs, bias)
         return flash_fwd_op(q, k, v, freqs, bias, mask, causal, scale)[0]
     if exists(freqs) and freqs.shape[-1] > q.shape[-1]:
         raise AssertionError(f"rotate dim {freqs.shape[-1]} exceeds head dim {q.shape[-1]}")
